@@ -346,6 +346,125 @@ int omni_hidream_attend_ws(const void* q, const void* k, const void* v, void* ou
 /* Workspace bytes omni_hidream_attend_ws needs at most on the current device. */
 int64_t omni_hidream_workspace_bytes(void);
 
+/* ------------------------------------- serving over an 8-bit block cache */
+
+/* A Qwen3 step over a paged cache held in 8 bits: the step's row tables from
+ * the request lengths, the rotary with the quantized cache write, causal
+ * attention of whole prompts over their own bf16 rows, and decode attention
+ * over the cache. No counterpart in the reference, whose 8-bit cache has one
+ * scale per slot and head (lm_rope above).
+ *
+ * Cache layout: blocks of 16 tokens (a page of `page` tokens, a multiple of 16,
+ * is page / 16 blocks; slot x lies in block x / 16). kv holds [blocks][2 hk][2048]
+ * bytes: K heads as [16 tokens][128 dims], then V heads as [128 dims][16 tokens].
+ * kv_scale holds [blocks][2 hk] exponents e (biased, 1..254): byte b of a head
+ * stands for value(b) * 2^(e - 127). Formats: FP8 E4M3 (OCP), or signed integers
+ * in -127..127. e is the smallest exponent that brings the block's largest
+ * finite magnitude to at most 448 or 127. */
+#define OMNI_ATTN_Q8_E4M3 0
+#define OMNI_ATTN_Q8_INT8 1
+
+/* The step's row tables, built on the device (the engines' `Rows` without the
+ * host loop and the upload): sequence s has first[s] tokens in the cache and
+ * gets count[s] new rows; count[s] < 0 says that the request is done. Its pages
+ * are the entries of line lines[s] (s where lines is NULL) of the block table
+ * [num_lines][table_ld], first ones first. With ring > 0 position p lives at
+ * index p % ring.
+ *
+ * Written: pos, slots and seq of every new row, sequences in order (slot =
+ * page id * page + index % page); row_indptr [nseq + 1], the rows of each
+ * sequence; indptr [nseq + 1] and pages, its page ids up to its last new token,
+ * as omni_qwen3_attend and omni_qwen3_attend_q8 read them. Rows past the last
+ * get pos, slots and seq -1 (up to row_cap); pages past the last stay as they
+ * were.
+ *
+ * Pages come from the free queue: entries head, head + 1, .. (modulo num_pages)
+ * of free_pages [num_pages], num_pages being the pool's pages, with free_state =
+ * {head, free entries}. New pages are taken in sequence order and written to the
+ * table; the pages of a done request go to the queue's end and can be taken from
+ * the next step on. With free_pages NULL nothing is taken or returned: the table
+ * already holds every page that the step needs.
+ *
+ * status int32[5] = {code, rows, pages, head, free entries}: &status[3] is the
+ * next call's free_state (so two status buffers take turns: free_state must not
+ * lie in status). code 0: done. Otherwise nothing is taken, all rows are -1,
+ * row_indptr and indptr are zeros, and code says why: */
+#define OMNI_ATTN_TABLES_BAD 1       /* negative first, position past int32, line or free_state out of range */
+#define OMNI_ATTN_TABLES_ROWS 2      /* more rows than row_cap */
+#define OMNI_ATTN_TABLES_PAGES 3     /* more pages than page_cap */
+#define OMNI_ATTN_TABLES_LINE 4      /* a sequence needs more than table_ld pages */
+#define OMNI_ATTN_TABLES_EXHAUSTED 5 /* fewer free pages than the step needs */
+/* The lowest that applies. Sequences of a call have different lines (a done
+ * request's line is free from the next call on), and the table's and the
+ * queue's page ids are the caller's to keep in the pool. */
+int omni_attn_step_tables(const int32_t* first, const int32_t* count, const int32_t* lines, int nseq, int page, int ring,
+                          int32_t* table, int64_t table_ld, int num_lines, int32_t* free_pages, int num_pages,
+                          const int32_t* free_state, int row_cap, int page_cap, int32_t* pos, int32_t* slots,
+                          int32_t* seq, int32_t* row_indptr, int32_t* indptr, int32_t* pages, int32_t* status,
+                          void* stream);
+
+/* omni_qwen3_rope's RMSNorm and rotary (angles in 64 bits) over qkv rows
+ * [(hq + 2 hk)][128] of stride ld, with K and V written to the 8-bit cache: q to
+ * q_out rows [hq][128] of stride q_ld, the turned k to k_out rows [hk][128] of
+ * stride k_ld (NULL: not written), and the bf16 values of k and v, quantized, to
+ * slot slots[n]. A row with slots[n] < 0 is skipped: nothing of it is written.
+ * In place: q_out = qkv and k_out = qkv + hq * 128 with q_ld = k_ld = ld.
+ *
+ * Within a call the rows of one block of 16 slots stand within 16 consecutive
+ * rows (rows of a sequence do), in any order; of rows with one slot the last
+ * counts; a block whose rows stand further apart is left unspecified. The
+ * block's other tokens stay, re-rounded if the exponent grows; but rows that
+ * hold its first slot start it anew (the other tokens become zeros). So a ring
+ * that wraps inside a block is not served.
+ *
+ * NaN and infinities do not count for the exponent. E4M3 stores both as NaN;
+ * integers store NaN as 0 and infinities as +-127. Row strides are multiples of
+ * 8 elements. */
+int omni_qwen3_rope_q8(const void* qkv, int64_t ld, const void* q_norm, const void* k_norm, const int32_t* pos,
+                       const int32_t* slots, void* q_out, int64_t q_ld, void* k_out, int64_t k_ld, void* kv,
+                       void* kv_scale, int format, int rows, int hq, int hk, float eps, float theta, void* stream);
+
+/* The plan for omni_qwen3_attend_q8: hq / hk from 1 to 16, page a multiple of
+ * 16, chunk_hint a multiple of 64 (<= 0 picks from the shape). */
+int omni_attn_decode_plan_init_q8(int rows, int hq, int hk, int page, int max_len, int chunk_hint,
+                                  omni_attn_decode_plan* plan);
+
+/* omni_qwen3_attend over the 8-bit cache: row n of sequence s = ragged ? seq[n] :
+ * n sees keys 0..pos[n]; a row with pos[n] < 0 stores zeros (seq[n] is not
+ * read). q rows [hq][128] of stride q_stride (a multiple of 8). P is carried in
+ * 16 bits or more. Tokens past pos[n] may hold anything. */
+int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const void* kv_scale, int format,
+                         const int32_t* pos, const int32_t* seq, int ragged, const int32_t* indptr, const int32_t* pages,
+                         int page, void* out, int hq, int hk, float scale, const omni_attn_decode_plan* plan,
+                         void* workspace, void* stream);
+
+/* Work list for causal attention of whole prompts that lie packed, one behind
+ * the other, in the rows of one call. */
+typedef struct omni_attn_prompt_plan {
+  int32_t nseq, rows, hq, hk; /* rows: the sum of the lengths */
+  int32_t tiles;      /* query tiles (each runs once per kv head) */
+  int32_t tile_rows;  /* packed (position, head) rows per tile */
+  int32_t workgroups; /* workgroups of a run that takes one per item */
+  int32_t exact_p;    /* as in omni_attn_prefill_plan */
+  int64_t work_bytes; /* bytes of the int32 work list the caller uploads */
+} omni_attn_prompt_plan;
+
+/* Host: lengths (zero allowed) to a work list of the form
+ * omni_attn_prefill_plan_init writes (an item's first field is the first row of
+ * its sequence). hq / hk in {1, 2, 4, 8}. OMNI_ATTN_EWORKSPACE with
+ * plan->work_bytes set when work_h is too small. */
+int omni_attn_prompt_plan_init(int nseq, const int32_t* lens_h, int hq, int hk, int32_t* work_h, int64_t work_cap,
+                               omni_attn_prompt_plan* plan);
+
+/* Row n of a prompt that starts at row b sees rows b..n of k and v. q rows
+ * [hq][128], k and v rows [hk][128], at strides that are multiples of 8 elements
+ * (k and v at most 2^22): parts of one qkv row, or buffers of their own. out
+ * rows [hq][128]; rows past the plan's are left as they were. A row's bits
+ * depend on its own prompt alone. */
+int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64_t q_stride, const void* k,
+                         int64_t k_stride, const void* v, int64_t v_stride, void* out, float scale, const int32_t* work,
+                         void* stream);
+
 /* ------------------------------------------------------- host row builder */
 
 /* The engines' `Rows` (crates/omni-qwen3-tts/src/model.rs:266-303,

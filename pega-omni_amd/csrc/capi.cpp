@@ -107,6 +107,42 @@ int pick_chunk_fp8(int rows, int heads, int max_len) {
   return 256;
 }
 
+// The work list of the tiles `tl` (first two fields of an item, rows, keys the last row sees) x hk
+// heads, into work_h (header, then items). Returns the workgroups of a run that takes one per item.
+// Item order: tiles by the keys they see, most first (a tile's time grows
+// with its key tiles, whatever its row count), each followed by its hk kv
+// heads. Workgroup i runs on XCD i % 8 and item k goes to XCD k % 8, so each
+// XCD's workgroups run longest first and the grid ends on short tiles; and
+// as hk is a power of two, an XCD always sees the same kv heads (h = x mod
+// hk for hk <= 8, h = x mod 8 beyond), so its L2 holds their K/V.
+int32_t write_work_list(std::vector<std::array<int32_t, 4>>& tl, int hk, int32_t* work_h) {
+  const int64_t items = (int64_t)tl.size() * hk;
+  std::stable_sort(tl.begin(), tl.end(), [](const auto& x, const auto& y) {
+    if (x[3] != y[3]) return x[3] > y[3];
+    if (x[0] != y[0]) return x[0] < y[0];
+    return x[1] < y[1];
+  });
+  int32_t* hdr = work_h;
+  for (int k = 0; k < omni::kPrefillWorkHeader; ++k) hdr[k] = 0;
+  int32_t* body = work_h + omni::kPrefillWorkHeader;
+  int64_t at = 0;
+  for (int x = 0; x < omni::kXcds; ++x) {
+    hdr[x] = (int32_t)at;
+    for (int64_t k = x; k < items; k += omni::kXcds, ++at) {
+      const auto& t = tl[k / hk];
+      int32_t* it = body + 4 * at;
+      it[0] = t[0];
+      it[1] = t[1];
+      it[2] = t[2];
+      it[3] = (int32_t)(k % hk);
+    }
+  }
+  hdr[omni::kXcds] = (int32_t)items;
+  int32_t widest = 0;
+  for (int x = 0; x < omni::kXcds; ++x) widest = std::max(widest, hdr[x + 1] - hdr[x]);
+  return widest * omni::kXcds;
+}
+
 int decode_common(const void* qkv, const void* kv, const int32_t* pos, const int32_t* seq, int ragged,
                   const int32_t* indptr, const int32_t* pages, int page, void* out, int hq, int hk, float scale,
                   int context, int len_mode, const omni_attn_decode_plan* plan, void* workspace, void* stream,
@@ -367,36 +403,7 @@ int omni_attn_prefill_plan_init(int rows, int hq, int hk, int page, const int32_
   plan->exact_p = 0;
   if (!work_h || need > work_cap)
     return fail(OMNI_ATTN_EWORKSPACE, "prefill_plan: work list needs %lld int32", (long long)need);
-  // Item order: tiles by the keys they see, most first (a tile's time grows
-  // with its key tiles, whatever its row count), each followed by its hk kv
-  // heads. Workgroup i runs on XCD i % 8 and item k goes to XCD k % 8, so each
-  // XCD's workgroups run longest first and the grid ends on short tiles; and
-  // as hk is a power of two, an XCD always sees the same kv heads (h = x mod
-  // hk for hk <= 8, h = x mod 8 beyond), so its L2 holds their K/V.
-  std::stable_sort(tl.begin(), tl.end(), [](const auto& x, const auto& y) {
-    if (x[3] != y[3]) return x[3] > y[3];
-    if (x[0] != y[0]) return x[0] < y[0];
-    return x[1] < y[1];
-  });
-  int32_t* hdr = work_h;
-  for (int k = 0; k < omni::kPrefillWorkHeader; ++k) hdr[k] = 0;
-  int32_t* body = work_h + omni::kPrefillWorkHeader;
-  int64_t at = 0;
-  for (int x = 0; x < omni::kXcds; ++x) {
-    hdr[x] = (int32_t)at;
-    for (int64_t k = x; k < items; k += omni::kXcds, ++at) {
-      const auto& t = tl[k / hk];
-      int32_t* it = body + 4 * at;
-      it[0] = t[0];
-      it[1] = t[1];
-      it[2] = t[2];
-      it[3] = (int32_t)(k % hk);
-    }
-  }
-  hdr[omni::kXcds] = (int32_t)items;
-  int32_t widest = 0;
-  for (int x = 0; x < omni::kXcds; ++x) widest = std::max(widest, hdr[x + 1] - hdr[x]);
-  plan->workgroups = widest * omni::kXcds;
+  plan->workgroups = write_work_list(tl, hk, work_h);
   return ok();
 }
 
@@ -748,6 +755,290 @@ int omni_qwen3_attend_dense(const void* qkv, const void* kv, int per, int base, 
     return fail(OMNI_ATTN_EINVAL, "qwen3_attend_dense: plan max_len=%d below base + per=%d", plan->max_len, base + per);
   return decode_common(qkv, kv, nullptr, nullptr, 0, nullptr, nullptr, 1, out, hq, hk, scale, 0, 2, plan, workspace,
                        stream, 0, per, base, span);
+}
+
+// ---------------------------------------------------- serving over the 8-bit cache
+
+namespace {
+
+// Split size of a decode bucket over the 8-bit cache.
+int pick_chunk_q8(int rows, int hk, int max_len) {
+  const long long units = (long long)rows * hk;
+  int chunk = 1024;
+  while (chunk > 128 && units * (((long long)max_len + chunk - 1) / chunk) < 1024) chunk /= 2;
+  return chunk;
+}
+
+int q8_format(int format, const char* who) {
+  if (format != OMNI_ATTN_Q8_E4M3 && format != OMNI_ATTN_Q8_INT8)
+    return fail(OMNI_ATTN_EINVAL, "%s: format=%d", who, format);
+  return 0;
+}
+
+bool row_stride_ok(int64_t stride, int heads) {
+  return stride >= (int64_t)heads * OMNI_ATTN_HEAD_DIM && stride % 8 == 0;
+}
+
+}  // namespace
+
+int omni_attn_step_tables(const int32_t* first, const int32_t* count, const int32_t* lines, int nseq, int page, int ring,
+                          int32_t* table, int64_t table_ld, int num_lines, int32_t* free_pages, int num_pages,
+                          const int32_t* free_state, int row_cap, int page_cap, int32_t* pos, int32_t* slots,
+                          int32_t* seq, int32_t* row_indptr, int32_t* indptr, int32_t* pages, int32_t* status,
+                          void* stream) {
+  if (nseq < 0 || page <= 0 || ring < 0 || table_ld < 0 || num_lines < 0 || row_cap < 0 || page_cap < 0)
+    return fail(OMNI_ATTN_EINVAL, "step_tables: nseq=%d page=%d ring=%d table_ld=%lld num_lines=%d row_cap=%d page_cap=%d",
+                nseq, page, ring, (long long)table_ld, num_lines, row_cap, page_cap);
+  if (nseq > 0 && (!first || !count || !table)) return fail(OMNI_ATTN_EINVAL, "step_tables: null first, count or table");
+  if (!row_indptr || !indptr || !status || (row_cap > 0 && (!pos || !slots || !seq)) || (page_cap > 0 && !pages))
+    return fail(OMNI_ATTN_EINVAL, "step_tables: null output");
+  if (free_pages) {
+    if (!free_state) return fail(OMNI_ATTN_EINVAL, "step_tables: free pages without their state");
+    if (num_pages <= 0 || (int64_t)num_pages * page > (int64_t)INT_MAX + 1)
+      return fail(OMNI_ATTN_EINVAL, "step_tables: %d pages of %d tokens: slots are int32", num_pages, page);
+    // Every workgroup reads the state while one writes the status.
+    if (free_state + 2 > status && free_state < status + 5)
+      return fail(OMNI_ATTN_EINVAL, "step_tables: free_state lies in status (two status buffers take turns)");
+  }
+  omni::TablesArgs a{};
+  a.first = first;
+  a.count = count;
+  a.lines = lines;
+  a.nseq = nseq;
+  a.pd = omni::make_page_div(page);
+  a.ring = ring;
+  a.table = table;
+  a.table_ld = table_ld;
+  a.num_lines = num_lines;
+  a.free_pages = free_pages;
+  a.num_pages = num_pages;
+  a.free_state = free_state;
+  a.row_cap = row_cap;
+  a.page_cap = page_cap;
+  a.pos = pos;
+  a.slots = slots;
+  a.seq = seq;
+  a.row_indptr = row_indptr;
+  a.indptr = indptr;
+  a.pages = pages;
+  a.status = status;
+  if (omni::launch_tables(a, as_stream(stream)) != 0)
+    return fail(OMNI_ATTN_ELAUNCH, "step_tables: launch failed: %s", hipGetErrorString(omni::g_launch_status));
+  return ok();
+}
+
+int omni_qwen3_rope_q8(const void* qkv, int64_t ld, const void* q_norm, const void* k_norm, const int32_t* pos,
+                       const int32_t* slots, void* q_out, int64_t q_ld, void* k_out, int64_t k_ld, void* kv,
+                       void* kv_scale, int format, int rows, int hq, int hk, float eps, float theta, void* stream) {
+  const char* who = "qwen3_rope_q8";
+  if (rows < 0) return fail(OMNI_ATTN_EINVAL, "%s: rows=%d", who, rows);
+  if (hq <= 0 || hk <= 0) return fail(OMNI_ATTN_EINVAL, "%s: hq=%d hk=%d", who, hq, hk);
+  if (int rc = q8_format(format, who)) return rc;
+  if ((int64_t)hk + (hq + 15) / 16 > 65535) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many heads", who);
+  if (rows == 0) return ok();
+  if (int rc = norm_rope_checks(q_norm, k_norm, eps, theta, who)) return rc;
+  if (!qkv || !pos || !slots || !q_out || !kv || !kv_scale) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(kv))
+    return fail(OMNI_ATTN_EINVAL, "%s: qkv, q_out, k_out and kv must be 16-byte aligned", who);
+  if (!row_stride_ok(ld, hq + 2 * hk) || !row_stride_ok(q_ld, hq) || (k_out && !row_stride_ok(k_ld, hk)))
+    return fail(OMNI_ATTN_EINVAL, "%s: row strides %lld / %lld / %lld: multiples of 8 that hold a row", who, (long long)ld,
+                (long long)q_ld, (long long)k_ld);
+  omni::RopeQ8Args a{};
+  a.qkv = static_cast<const omni::bf16_t*>(qkv);
+  a.ld = ld;
+  a.q_norm = static_cast<const omni::bf16_t*>(q_norm);
+  a.k_norm = static_cast<const omni::bf16_t*>(k_norm);
+  a.pos = pos;
+  a.slots = slots;
+  a.q = static_cast<omni::bf16_t*>(q_out);
+  a.q_ld = q_ld;
+  a.k = static_cast<omni::bf16_t*>(k_out);
+  a.k_ld = k_ld;
+  a.kv = static_cast<uint8_t*>(kv);
+  a.kv_scale = static_cast<uint8_t*>(kv_scale);
+  a.format = format;
+  a.rows = rows;
+  a.hq = hq;
+  a.hk = hk;
+  a.eps = eps;
+  a.inv_theta64 = std::pow((double)theta, -1.0 / 64.0);
+  if (omni::launch_rope_q8(a, as_stream(stream)) != 0)
+    return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));
+  return ok();
+}
+
+static int q8_shape(int hq, int hk, int page, const char* who) {
+  if (hk <= 0 || hq <= 0 || hq % hk != 0) return fail(OMNI_ATTN_EINVAL, "%s: hq=%d is not a multiple of hk=%d", who, hq, hk);
+  if (hq / hk > 16) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: hq/hk=%d above 16", who, hq / hk);
+  if (hk > 65535) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: hk=%d", who, hk);
+  if (page <= 0) return fail(OMNI_ATTN_EINVAL, "%s: page=%d", who, page);
+  if (page % 16 != 0) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: page=%d is not a multiple of a 16-token block", who, page);
+  return 0;
+}
+
+int omni_attn_decode_plan_init_q8(int rows, int hq, int hk, int page, int max_len, int chunk_hint,
+                                  omni_attn_decode_plan* plan) {
+  if (!plan) return fail(OMNI_ATTN_EINVAL, "decode_plan_q8: null plan");
+  std::memset(plan, 0, sizeof *plan);
+  if (rows < 0 || rows > 65535) return fail(OMNI_ATTN_EINVAL, "decode_plan_q8: rows=%d outside [0, 65535]", rows);
+  if (int rc = q8_shape(hq, hk, page, "decode_plan_q8")) return rc;
+  if ((int64_t)rows * hq > INT_MAX) return fail(OMNI_ATTN_EUNSUPPORTED, "decode_plan_q8: rows * hq passes 2^31");
+  if (max_len <= 0) return fail(OMNI_ATTN_EINVAL, "decode_plan_q8: max_len=%d", max_len);
+  const int chunk = chunk_hint > 0 ? chunk_hint : pick_chunk_q8(rows, hk, max_len);
+  if (chunk % 64 != 0) return fail(OMNI_ATTN_EINVAL, "decode_plan_q8: chunk=%d is not a multiple of 64", chunk);
+  plan->rows = rows;
+  plan->hq = hq;
+  plan->hk = hk;
+  plan->page = page;
+  plan->max_len = max_len;
+  plan->chunk = chunk;
+  plan->splits = (int32_t)(((int64_t)max_len + chunk - 1) / chunk);
+  plan->workspace_bytes =
+      plan->splits > 1 ? (int64_t)rows * hq * plan->splits * (OMNI_ATTN_HEAD_DIM + 1) * (int64_t)sizeof(float) : 0;
+  return ok();
+}
+
+int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const void* kv_scale, int format,
+                         const int32_t* pos, const int32_t* seq, int ragged, const int32_t* indptr, const int32_t* pages,
+                         int page, void* out, int hq, int hk, float scale, const omni_attn_decode_plan* plan,
+                         void* workspace, void* stream) {
+  const char* who = "qwen3_attend_q8";
+  if (!plan) return fail(OMNI_ATTN_EINVAL, "%s: null plan", who);
+  if (int rc = q8_format(format, who)) return rc;
+  if (int rc = q8_shape(hq, hk, page, who)) return rc;
+  if (plan->hq != hq || plan->hk != hk || plan->page != page)
+    return fail(OMNI_ATTN_EINVAL, "%s: plan was made for hq=%d hk=%d page=%d, called with hq=%d hk=%d page=%d", who,
+                plan->hq, plan->hk, plan->page, hq, hk, page);
+  if (plan->rows < 0 || plan->rows > 65535 || (int64_t)plan->rows * hq > INT_MAX || plan->max_len <= 0 ||
+      plan->chunk <= 0 || plan->chunk % 64 != 0 || plan->group_heads != 0 ||
+      plan->splits != ((int64_t)plan->max_len + plan->chunk - 1) / plan->chunk ||
+      (plan->splits > 1 &&
+       plan->workspace_bytes < (int64_t)plan->rows * hq * plan->splits * (OMNI_ATTN_HEAD_DIM + 1) * (int64_t)sizeof(float)))
+    return fail(OMNI_ATTN_EINVAL, "%s: plan is not self-consistent (rows=%d max_len=%d chunk=%d splits=%d group_heads=%d)",
+                who, plan->rows, plan->max_len, plan->chunk, plan->splits, plan->group_heads);
+  if (plan->rows == 0) return ok();
+  if (!q || !kv || !kv_scale || !pos || !indptr || !pages || !out || (ragged && !seq))
+    return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (!aligned16(q) || !aligned16(kv) || !aligned16(out))
+    return fail(OMNI_ATTN_EINVAL, "%s: q, kv and out must be 16-byte aligned", who);
+  if (!row_stride_ok(q_stride, hq))
+    return fail(OMNI_ATTN_EINVAL, "%s: q_stride=%lld: a multiple of 8 that holds a row", who, (long long)q_stride);
+  if (!std::isfinite(scale)) return fail(OMNI_ATTN_EINVAL, "%s: non-finite scale", who);
+  if (plan->splits > 1 && !workspace)
+    return fail(OMNI_ATTN_EWORKSPACE, "%s: plan needs %lld workspace bytes", who, (long long)plan->workspace_bytes);
+  if (!aligned16(workspace)) return fail(OMNI_ATTN_EINVAL, "%s: workspace must be 16-byte aligned", who);
+  omni::DecodeQ8Args a{};
+  a.q = static_cast<const omni::bf16_t*>(q);
+  a.q_stride = q_stride;
+  a.kv = static_cast<const uint8_t*>(kv);
+  a.kv_scale = static_cast<const uint8_t*>(kv_scale);
+  a.pos = pos;
+  a.seq = seq;
+  a.indptr = indptr;
+  a.pages = pages;
+  a.out = static_cast<omni::bf16_t*>(out);
+  a.ws_o = static_cast<float*>(workspace);
+  a.ws_lse = a.ws_o ? a.ws_o + (int64_t)plan->rows * hq * plan->splits * OMNI_ATTN_HEAD_DIM : nullptr;
+  a.format = format;
+  a.hq = hq;
+  a.hk = hk;
+  a.ragged = ragged ? 1 : 0;
+  a.pd = omni::make_page_div(page / 16);
+  a.chunk = plan->chunk;
+  a.splits = plan->splits;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  if (omni::launch_decode_q8(a, plan->rows, as_stream(stream)) != 0)
+    return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));
+  return ok();
+}
+
+int omni_attn_prompt_plan_init(int nseq, const int32_t* lens_h, int hq, int hk, int32_t* work_h, int64_t work_cap,
+                               omni_attn_prompt_plan* plan) {
+  if (!plan) return fail(OMNI_ATTN_EINVAL, "prompt_plan: null plan");
+  std::memset(plan, 0, sizeof *plan);
+  if (nseq < 0 || (nseq > 0 && !lens_h)) return fail(OMNI_ATTN_EINVAL, "prompt_plan: nseq=%d, null lengths", nseq);
+  if (hk <= 0 || hq <= 0 || hq % hk != 0)
+    return fail(OMNI_ATTN_EINVAL, "prompt_plan: hq=%d is not a multiple of hk=%d", hq, hk);
+  const int G = hq / hk;
+  if (G != 1 && G != 2 && G != 4 && G != 8)
+    return fail(OMNI_ATTN_EUNSUPPORTED, "prompt_plan: hq/hk=%d not in {1,2,4,8}", G);
+  const int per_tile = omni::kTiledRows / G;
+  int64_t rows = 0, tiles = 0;
+  for (int s = 0; s < nseq; ++s) {
+    if (lens_h[s] < 0) return fail(OMNI_ATTN_EINVAL, "prompt_plan: length %d of sequence %d", lens_h[s], s);
+    rows += lens_h[s];
+    tiles += ((int64_t)lens_h[s] + per_tile - 1) / per_tile;
+  }
+  const int64_t items = tiles * hk;
+  if (rows > INT_MAX || items > (INT_MAX - omni::kPrefillWorkHeader) / 4)
+    return fail(OMNI_ATTN_EUNSUPPORTED, "prompt_plan: too many rows or tiles");
+  plan->nseq = nseq;
+  plan->rows = (int32_t)rows;
+  plan->hq = hq;
+  plan->hk = hk;
+  plan->tiles = (int32_t)tiles;
+  plan->tile_rows = omni::kTiledRows;
+  const int64_t need = omni::kPrefillWorkHeader + 4 * items;
+  plan->work_bytes = need * (int64_t)sizeof(int32_t);
+  if (!work_h || need > work_cap)
+    return fail(OMNI_ATTN_EWORKSPACE, "prompt_plan: work list needs %lld int32", (long long)need);
+  // Tiles of each sequence: (its first row, the tile's first row, rows, keys the last row sees).
+  std::vector<std::array<int32_t, 4>> tl;
+  tl.reserve((size_t)tiles);
+  for (int32_t s = 0, at = 0; s < nseq; at += lens_h[s++])
+    for (int32_t f = 0; f < lens_h[s]; f += per_tile) {
+      const int32_t nq = std::min(per_tile, lens_h[s] - f);
+      tl.push_back({at, at + f, nq, f + nq});
+    }
+  plan->workgroups = write_work_list(tl, hk, work_h);
+  return ok();
+}
+
+int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64_t q_stride, const void* k,
+                         int64_t k_stride, const void* v, int64_t v_stride, void* out, float scale, const int32_t* work,
+                         void* stream) {
+  if (!plan) return fail(OMNI_ATTN_EINVAL, "prompt_run: null plan");
+  const int G = plan->hk > 0 && plan->hq > 0 && plan->hq % plan->hk == 0 ? plan->hq / plan->hk : 0;
+  const int64_t items = (int64_t)plan->tiles * (plan->hk > 0 ? plan->hk : 0);
+  if (plan->tiles < 0 || plan->rows < 0 || (G != 1 && G != 2 && G != 4 && G != 8) || plan->tile_rows != omni::kTiledRows ||
+      plan->workgroups != (items + omni::kXcds - 1) / omni::kXcds * omni::kXcds ||
+      plan->work_bytes != (omni::kPrefillWorkHeader + 4 * items) * (int64_t)sizeof(int32_t) ||
+      (plan->exact_p != 0 && plan->exact_p != 1))
+    return fail(OMNI_ATTN_EINVAL,
+                "prompt_run: plan is not one prompt_plan_init made (rows=%d tiles=%d hq=%d hk=%d tile_rows=%d workgroups=%d "
+                "exact_p=%d)",
+                plan->rows, plan->tiles, plan->hq, plan->hk, plan->tile_rows, plan->workgroups, plan->exact_p);
+  if (plan->tiles == 0) return ok();
+  if (!q || !k || !v || !out || !work) return fail(OMNI_ATTN_EINVAL, "prompt_run: null device pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return fail(OMNI_ATTN_EINVAL, "prompt_run: q, k, v and out must be 16-byte aligned");
+  // A key tile is addressed with 32-bit byte offsets from its first row.
+  if (!row_stride_ok(q_stride, plan->hq) || !row_stride_ok(k_stride, plan->hk) || !row_stride_ok(v_stride, plan->hk) ||
+      k_stride > omni::kMostPromptStride || v_stride > omni::kMostPromptStride)
+    return fail(OMNI_ATTN_EINVAL, "prompt_run: row strides %lld / %lld / %lld: multiples of 8 that hold a row, k and v at most %lld",
+                (long long)q_stride, (long long)k_stride, (long long)v_stride, (long long)omni::kMostPromptStride);
+  if (!std::isfinite(scale)) return fail(OMNI_ATTN_EINVAL, "prompt_run: non-finite scale");
+  omni::TiledArgs a{};
+  a.q = static_cast<const omni::bf16_t*>(q);
+  a.q_stride = q_stride;
+  a.k = static_cast<const omni::bf16_t*>(k);
+  a.v = static_cast<const omni::bf16_t*>(v);
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.work = work;
+  a.causal = 1;
+  a.out = static_cast<omni::bf16_t*>(out);
+  a.hq = plan->hq;
+  a.hk = plan->hk;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.exact_p = plan->exact_p;
+  const int resident = resident_tiled_groups();
+  a.quarters = omni::tiled_quarters(items, resident);
+  a.halved = omni::prefill_halves(items, resident);
+  const int rc = omni::launch_prompt(a, (int)items, as_stream(stream));
+  if (rc == -2) return fail(OMNI_ATTN_EUNSUPPORTED, "prompt_run: shape not implemented");
+  if (rc != 0) return fail(OMNI_ATTN_ELAUNCH, "prompt_run: launch failed: %s", hipGetErrorString(omni::g_launch_status));
+  return ok();
 }
 
 // ------------------------------------------------------ head-64 ring attentions

@@ -104,6 +104,8 @@ struct TiledArgs {
   int quarters;
   // Prefill with P carried as two bf16 terms (hi + lo) through P.V.
   int exact_p;
+  // packed prompts (mode 2): elements between rows of k and of v
+  int64_t k_stride, v_stride;
 };
 
 // Packed (position, head) query rows per MFMA tile: one 8-wave workgroup, one per CU.
@@ -117,6 +119,9 @@ constexpr int64_t kSegmentBytes = (int64_t)kTiledRows * (128 + 2) * 4;
 constexpr int kPrefillWorkHeader = 16;
 constexpr int kXcds = 8;
 int launch_prefill(const TiledArgs& a, int items, hipStream_t stream);
+// Packed prompts: items are (sequence's first row, first row, rows, kv head).
+constexpr int64_t kMostPromptStride = 1LL << 22;  // elements: 128 rows stay below 2^30 bytes
+int launch_prompt(const TiledArgs& a, int items, hipStream_t stream);
 
 // Rotary embedding + K/V scatter (the step before attention).
 struct RopeArgs {
@@ -164,5 +169,75 @@ bool tiled_quarters(long long items, int resident);
 int prefill_halves(long long items, int resident);
 // Items launch_dit should run as row halves when no split is used (0: none).
 int dit_halves(const TiledArgs& a, int batch, int resident);
+
+// Row tables of a step, built on the GPU (tables.hip).
+struct TablesArgs {
+  const int32_t* first;  // [nseq] positions in the cache before the step
+  const int32_t* count;  // [nseq] new rows; negative: the request is done
+  const int32_t* lines;  // [nseq] table line of each sequence, or null (line s)
+  int nseq;
+  PageDiv pd;
+  int ring;  // > 0: position p lives at index p % ring
+  int32_t* table;  // [num_lines][table_ld] page ids
+  int64_t table_ld;
+  int num_lines;
+  int32_t* free_pages;  // queue of num_pages entries, or null: every page is in the table
+  int num_pages;
+  const int32_t* free_state;  // {first free entry, free entries}
+  int row_cap, page_cap;
+  int32_t *pos, *slots, *seq;   // [row_cap]
+  int32_t *row_indptr, *indptr; // [nseq + 1]
+  int32_t* pages;               // [page_cap]
+  int32_t* status;              // {code, rows, pages, first free entry, free entries}
+};
+int launch_tables(const TablesArgs& a, hipStream_t stream);
+
+// The 8-bit block cache (q8.hip): blocks of 16 tokens, [2 hk heads][2048]
+// bytes (K heads [16 tokens][128 dims], V heads [128 dims][16 tokens]) and one
+// biased power-of-two exponent per (block, head).
+constexpr int kQ8Block = 16;
+constexpr int kQ8HeadBytes = kQ8Block * 128;
+constexpr int kQ8E4m3 = 0, kQ8Int8 = 1;
+
+struct RopeQ8Args {
+  const bf16_t* qkv;
+  int64_t ld;
+  const bf16_t* q_norm;
+  const bf16_t* k_norm;
+  const int32_t* pos;
+  const int32_t* slots;  // negative: the row is skipped
+  bf16_t* q;
+  int64_t q_ld;
+  bf16_t* k;  // may be null
+  int64_t k_ld;
+  uint8_t* kv;
+  uint8_t* kv_scale;
+  int format;
+  int rows, hq, hk;
+  float eps;
+  double inv_theta64;  // theta^(-1/64): pair i turns by pos * inv_theta64^i
+};
+int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream);
+
+struct DecodeQ8Args {
+  const bf16_t* q;
+  int64_t q_stride;
+  const uint8_t* kv;
+  const uint8_t* kv_scale;
+  const int32_t* pos;  // negative: the row stores zeros
+  const int32_t* seq;
+  const int32_t* indptr;
+  const int32_t* pages;
+  bf16_t* out;
+  float* ws_o;    // [rows][hq][splits][128]
+  float* ws_lse;  // [rows][hq][splits]
+  int format;
+  int hq, hk;
+  int ragged;
+  PageDiv pd;  // blocks per page
+  int chunk, splits;
+  float scale_log2;
+};
+int launch_decode_q8(const DecodeQ8Args& a, int rows, hipStream_t stream);
 
 }  // namespace omni

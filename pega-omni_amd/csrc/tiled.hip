@@ -152,11 +152,14 @@ static_assert(kDmas == 8, "one DMA per K-step of the S stage");
 
 // Key sources: dense K and V; paged with pages that are multiples of the 16
 // rows a wave loads (a wave's rows of a tile lie in one page); any other page.
-constexpr int kDense = 0, kPagedWave = 1, kPagedLane = 2;
+// And packed: K and V rows of prompts that lie one behind the other, each row
+// of a prompt seeing its own prompt's rows up to itself.
+constexpr int kDense = 0, kPagedWave = 1, kPagedLane = 2, kPacked = 3;
 
 template <int G, int SRC, int FORM = kWhole, bool EXACT = false>
 __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items, int ntiles) {
-  constexpr bool PAGED = SRC != kDense;
+  constexpr bool LISTED = SRC != kDense;  // items come from a work list
+  constexpr bool PAGED = SRC == kPagedWave || SRC == kPagedLane;
   constexpr int PARTS = FORM == kQuarters ? 4 : FORM == kHalves ? 2 : 1;
   // DiT, XCD-aware order: workgroup id i runs on XCD i % 8; give each XCD a
   // contiguous block of work items so the tiles sharing one K/V head (and
@@ -171,8 +174,8 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   // DiT row halves: the last `halved` items, in the same order as the split
   // chunks.
   int idx, chunk = -1, part = -1;
-  int4 item{};  // prefill: sequence, first row, rows, kv head
-  if constexpr (PAGED) {
+  int4 item{};  // prefill: sequence (packed: its first row), first row, rows, kv head
+  if constexpr (LISTED) {
     // XCD x's items are those from header entry x to entry x + 1. The plan puts
     // its range at x (items / 8) + min(x, items % 8), so the item is read there
     // beside the header, in one round trip, and once more only if the list's
@@ -228,9 +231,9 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       idx /= PARTS;
     }
   }
-  const int tile = PAGED ? 0 : idx % ntiles;
-  const int kvh = PAGED ? item.w : (idx / ntiles) % a.hk;
-  const int b = PAGED ? 0 : idx / (ntiles * a.hk);
+  const int tile = LISTED ? 0 : idx % ntiles;
+  const int kvh = LISTED ? item.w : (idx / ntiles) % a.hk;
+  const int b = LISTED ? 0 : idx / (ntiles * a.hk);
   constexpr int kPos = kBM / G;  // positions per tile
   constexpr int kPartPos = kPos / PARTS;  // and per part
   // This workgroup's rows end at position `ends` of the tile; a part past a
@@ -253,6 +256,17 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     t.kbase = a.kv + (int64_t)kvh * kHead;
     t.vbase = a.kv + (int64_t)(a.hk + kvh) * kHead;
     t.qpos0 = 0;
+  } else if constexpr (SRC == kPacked) {
+    const int begin = item.x, first = item.y;
+    t.nq = item.z;
+    if (no_rows(t.nq)) return;
+    t.q = a.q + (int64_t)first * a.q_stride;
+    t.out = a.out + (int64_t)first * a.hq * kHead;
+    t.qpos0 = first - begin;
+    t.last = t.qpos0 + ends(t.nq);
+    t.len = t.last;
+    t.kbase = a.k + begin * a.k_stride + (int64_t)kvh * kHead;
+    t.vbase = a.v + begin * a.v_stride + (int64_t)kvh * kHead;
   } else {
     const int q0 = tile * kPos;
     t.nq = min(kPos, a.q_len - q0);
@@ -295,6 +309,8 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   int lim;  // keys this row sees
   if constexpr (PAGED)
     lim = row_ok ? t.pos[p] + 1 : 0;
+  else if constexpr (SRC == kPacked)
+    lim = row_ok ? t.qpos0 + p + 1 : 0;
   else
     lim = row_ok ? (a.causal ? min(t.len, t.qpos0 + p + 1) : t.len) : 0;
 
@@ -329,7 +345,8 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   // block (dense: from the tile's first key): constants for every tile.
   uint32_t koff[kRowsPerWave / 4], voff[kRowsPerWave / 4];
   {
-    const int64_t stride = PAGED ? t.per_slot : t.kv_stride;
+    const int64_t stride = PAGED ? t.per_slot : SRC == kPacked ? a.k_stride : t.kv_stride;
+    const int64_t vstride = SRC == kPacked ? a.v_stride : stride;
 #pragma unroll
     for (int i = 0; i < kRowsPerWave / 4; ++i) {
       const int wrow = 4 * i + (lane >> 4);  // row within the wave's block
@@ -339,7 +356,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       const int vc = (((cs >> 2) ^ (row & 3)) << 2) | (cs & 3);
       const int64_t r0 = PAGED ? wrow : row;
       koff[i] = (uint32_t)(r0 * stride + 8 * kc);
-      voff[i] = (uint32_t)(r0 * stride + 8 * vc);
+      voff[i] = (uint32_t)(r0 * vstride + 8 * vc);
     }
   }
   // Page ids of this wave's rows (kPagedWave): lane l holds the id of tile
@@ -362,8 +379,14 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     const int n0 = st * kBN;
     const int first = PAGED ? n0 + kRowsPerWave * wave_u : n0;  // key of this lane's row 0
     const int rows = st < s_hi ? min(max(t.last - first, 0), PAGED ? kRowsPerWave : kBN) : 0;
+    const bool whole = rows == (PAGED ? kRowsPerWave : kBN);
+    if constexpr (SRC == kPacked) {
+      k_rsrc = buffer_rsrc(t.kbase + n0 * a.k_stride, whole ? -1 : (int)(rows * 2 * a.k_stride));
+      v_rsrc = buffer_rsrc(t.vbase + n0 * a.v_stride, whole ? -1 : (int)(rows * 2 * a.v_stride));
+      return;
+    }
     const int64_t stride_bytes = 2 * (PAGED ? t.per_slot : t.kv_stride);
-    const int bytes = rows == (PAGED ? kRowsPerWave : kBN) ? -1 : (int)(rows * stride_bytes);
+    const int bytes = whole ? -1 : (int)(rows * stride_bytes);
     int64_t off;
     if constexpr (PAGED) {
       const int at = st - s_lo;
@@ -889,15 +912,16 @@ void launch_g(const TiledArgs& a, int grid, int items, int ntiles, hipStream_t s
     tiled_attn<G, SRC, FORM><<<grid, kThreads, 0, stream>>>(a, items, ntiles);
 }
 
-template <bool PAGED>
+template <int SRC>  // kDense, kPacked, or kPagedWave for any page size
 int launch_tiled(const TiledArgs& a, int items, int ntiles, hipStream_t stream) {
+  constexpr bool LISTED = SRC != kDense;
   if (items <= 0) return 0;
   // Pages that are no multiple of a wave's rows keep whole tiles.
-  const bool lane_pages = PAGED && a.pd.page % kRowsPerWave != 0;
-  const bool parts = !lane_pages && (PAGED || a.split_k == 0);
+  const bool lane_pages = SRC == kPagedWave && a.pd.page % kRowsPerWave != 0;
+  const bool parts = !lane_pages && (LISTED || a.split_k == 0);
   const int form = parts && a.quarters ? kQuarters : parts && a.halved > 0 ? kHalves : kWhole;
   int grid = ((items + 7) >> 3) << 3;
-  if (PAGED)
+  if (LISTED)
     grid *= form == kQuarters ? 4 : form == kHalves ? 2 : 1;  // an XCD's items, each as so many workgroups
   else if (form == kQuarters)
     grid = ((items * 4 + 7) >> 3) << 3;
@@ -909,13 +933,13 @@ int launch_tiled(const TiledArgs& a, int items, int ntiles, hipStream_t stream) 
 #define OMNI_CASE(G)                                                                       \
   case G:                                                                                  \
     if (lane_pages)                                                                        \
-      launch_g<G, PAGED ? kPagedLane : kDense, kWhole>(a, grid, items, ntiles, stream);    \
+      launch_g<G, SRC == kPagedWave ? kPagedLane : SRC, kWhole>(a, grid, items, ntiles, stream); \
     else if (form == kQuarters)                                                            \
-      launch_g<G, PAGED ? kPagedWave : kDense, kQuarters>(a, grid, items, ntiles, stream); \
+      launch_g<G, SRC, kQuarters>(a, grid, items, ntiles, stream);                         \
     else if (form == kHalves)                                                              \
-      launch_g<G, PAGED ? kPagedWave : kDense, kHalves>(a, grid, items, ntiles, stream);   \
+      launch_g<G, SRC, kHalves>(a, grid, items, ntiles, stream);                           \
     else                                                                                   \
-      launch_g<G, PAGED ? kPagedWave : kDense, kWhole>(a, grid, items, ntiles, stream);    \
+      launch_g<G, SRC, kWhole>(a, grid, items, ntiles, stream);                            \
     break;
     OMNI_CASE(1)
     OMNI_CASE(2)
@@ -925,7 +949,7 @@ int launch_tiled(const TiledArgs& a, int items, int ntiles, hipStream_t stream) 
     default: return -2;
   }
   if (check_launch() != 0) return -3;
-  if (!PAGED && a.split_k > 0) {
+  if (!LISTED && a.split_k > 0) {
     dit_combine<<<dim3(items - a.split_from, kBM / kCombineRows), 256, 0, stream>>>(a, ntiles);
     return check_launch();
   }
@@ -933,7 +957,11 @@ int launch_tiled(const TiledArgs& a, int items, int ntiles, hipStream_t stream) 
 }
 
 int launch_prefill(const TiledArgs& a, int items, hipStream_t stream) {
-  return launch_tiled<true>(a, items, 0, stream);
+  return launch_tiled<kPagedWave>(a, items, 0, stream);
+}
+
+int launch_prompt(const TiledArgs& a, int items, hipStream_t stream) {
+  return launch_tiled<kPacked>(a, items, 0, stream);
 }
 
 int launch_dit(const TiledArgs& a, int batch, hipStream_t stream) {
@@ -943,7 +971,7 @@ int launch_dit(const TiledArgs& a, int batch, hipStream_t stream) {
   const long long items = (long long)ntiles * a.hk * batch;
   if (items > (1LL << 30)) return -2;
   if (a.halved < 0 || a.halved > items || a.halved > (1 << 29)) return -2;
-  return launch_tiled<false>(a, (int)items, ntiles, stream);
+  return launch_tiled<kDense>(a, (int)items, ntiles, stream);
 }
 
 // Calls whose tiles fill at most a quarter of the CUs run each as four

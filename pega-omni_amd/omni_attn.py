@@ -58,6 +58,12 @@ EXPORTS = (
     "omni_lm_rope_attend_fp8",
     "omni_lm_rope",
     "omni_hidream_qk_rope",
+    "omni_attn_step_tables",
+    "omni_qwen3_rope_q8",
+    "omni_attn_decode_plan_init_q8",
+    "omni_qwen3_attend_q8",
+    "omni_attn_prompt_plan_init",
+    "omni_attn_prompt_run",
     "omni_attn_rows_new",
     "omni_attn_rows_free",
     "omni_attn_rows_clear",
@@ -103,6 +109,20 @@ class PrefillPlan(ctypes.Structure):
     ]
 
 
+class PromptPlan(ctypes.Structure):
+    _fields_ = [
+        ("nseq", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("hq", ctypes.c_int32),
+        ("hk", ctypes.c_int32),
+        ("tiles", ctypes.c_int32),
+        ("tile_rows", ctypes.c_int32),
+        ("workgroups", ctypes.c_int32),
+        ("exact_p", ctypes.c_int32),
+        ("work_bytes", ctypes.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -119,6 +139,7 @@ def load(path: str | None = None):
     P, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
     dplan = ctypes.POINTER(DecodePlan)
     pplan = ctypes.POINTER(PrefillPlan)
+    qplan = ctypes.POINTER(PromptPlan)
     sig = {
         "omni_attn_decode_plan_init": [i32, i32, i32, i32, i32, i32, dplan],
         "omni_attn_decode_plan_init_fp8": [i32, i32, i32, i32, i32, dplan],
@@ -152,6 +173,12 @@ def load(path: str | None = None):
         "omni_attn_last_error": [],
     }
     sig.update({
+        "omni_attn_step_tables": [P, P, P, i32, i32, i32, P, i64, i32, P, i32, P, i32, i32, P, P, P, P, P, P, P, P],
+        "omni_qwen3_rope_q8": [P, i64, P, P, P, P, P, i64, P, i64, P, P, i32, i32, i32, i32, f32, f32, P],
+        "omni_attn_decode_plan_init_q8": [i32, i32, i32, i32, i32, i32, dplan],
+        "omni_qwen3_attend_q8": [P, i64, P, P, i32, P, P, i32, P, P, i32, P, i32, i32, f32, dplan, P, P],
+        "omni_attn_prompt_plan_init": [i32, P, i32, i32, P, i64, qplan],
+        "omni_attn_prompt_run": [qplan, P, i64, P, i64, P, i64, P, f32, P, P],
         "omni_attn_rows_new": [i32, i32],
         "omni_attn_rows_free": [P],
         "omni_attn_rows_clear": [P],
@@ -519,6 +546,167 @@ def hidream_attend_ws(q, k, v, out, q_len, kv_len_at, q_stride, causal, scale_lo
                                          int(causal), float(scale_log2), hq, hk, batch, int(q_bstride),
                                          int(kv_bstride), int(out_bstride), _ptr(workspace), nbytes,
                                          _stream(stream)))
+    return out
+
+
+# ------------------------------------------ serving over an 8-bit block cache
+TABLES_OK, TABLES_BAD, TABLES_ROWS, TABLES_PAGES, TABLES_LINE, TABLES_EXHAUSTED = range(6)
+_Q8_FORMATS = {_torch.float8_e4m3fn: 0, _torch.int8: 1}
+_Q8_SCALES = (_torch.uint8, _torch.float8_e8m0fnu)
+
+
+def _here(t, name):
+    """The device the call launches on holds t (the stream is the current device's)."""
+    if not t.is_cuda or t.get_device() != _torch.cuda.current_device():
+        raise OmniAttnError(EINVAL, f"{name} must lie on the current device")
+
+
+def _i32_here(t, name, least):
+    if t.dtype != _torch.int32 or not t.is_contiguous() or t.numel() < least:
+        raise OmniAttnError(EINVAL, f"{name} must be a contiguous int32 tensor of at least {least}")
+    _here(t, name)
+    return t.data_ptr()
+
+
+def _rows_here(t, name, rows, heads):
+    """Pointer and row stride of at least `rows` bf16 rows of heads x 128."""
+    if t.dtype != _torch.bfloat16 or t.dim() != 2 or t.shape[0] < rows or t.shape[1] != heads * HEAD_DIM:
+        raise OmniAttnError(EINVAL, f"{name} must be bf16 rows [{rows}][{heads * HEAD_DIM}]")
+    if t.stride(1) != 1:
+        raise OmniAttnError(EINVAL, f"{name}: the elements of a row must be adjacent")
+    _here(t, name)
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * HEAD_DIM
+
+
+def _q8_cache(kv, kv_scale, hk):
+    """Pointers of a cache and its exponents, and its format."""
+    if kv.dtype not in _Q8_FORMATS or kv.dim() != 3 or kv.shape[1] != 2 * hk or kv.shape[2] != 16 * HEAD_DIM:
+        raise OmniAttnError(EINVAL, f"kv must be float8_e4m3fn or int8 [blocks][{2 * hk}][2048]")
+    if kv_scale.dtype not in _Q8_SCALES or kv_scale.shape != kv.shape[:2]:
+        raise OmniAttnError(EINVAL, f"kv_scale must be uint8 or float8_e8m0fnu [{kv.shape[0]}][{2 * hk}]")
+    if not kv.is_contiguous() or not kv_scale.is_contiguous():
+        raise OmniAttnError(EINVAL, "kv and kv_scale must be contiguous")
+    _here(kv, "kv"), _here(kv_scale, "kv_scale")
+    return kv.data_ptr(), kv_scale.data_ptr(), _Q8_FORMATS[kv.dtype]
+
+
+def q8_cache(pages, page, hk, dtype=_torch.float8_e4m3fn, device="cuda"):
+    """A zeroed 8-bit cache of `pages` pages: (kv [blocks][2 hk][2048], kv_scale [blocks][2 hk] exponents)."""
+    if page <= 0 or page % 16 or dtype not in _Q8_FORMATS or pages < 0 or hk <= 0:
+        raise OmniAttnError(EINVAL, f"q8_cache: pages={pages} page={page} hk={hk} dtype={dtype}")
+    blocks = pages * (page // 16)
+    kv = _torch.zeros(blocks, 2 * hk, 16 * HEAD_DIM, dtype=_torch.uint8, device=device).view(dtype)
+    return kv, _torch.full((blocks, 2 * hk), 1, dtype=_torch.uint8, device=device).view(_torch.float8_e8m0fnu)
+
+
+def step_tables(first, count, lines, table, free_pages, free_state, pos, slots, seq, row_indptr, indptr, pages, status,
+                page=16, ring=0, stream=None):
+    """The step's row tables on the GPU from the request lengths: ``pos``,
+    ``slots``, ``seq``, ``row_indptr``, ``indptr`` and ``pages`` of every new row
+    and sequence, pages taken from the free queue (free_pages, free_state =
+    [head, free entries]) into ``table`` [lines][pages per line], pages of done
+    requests (count < 0) given back. lines None: line s; free_pages None: the
+    table holds every page. ``status`` = [code, rows, pages, head, free entries];
+    ``status[3:5]`` is the next call's free_state, with another status."""
+    n = first.numel()
+    if table.dtype != _torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise OmniAttnError(EINVAL, "table must be a contiguous int32 tensor [lines][pages]")
+    _here(table, "table")
+    rows = pos.numel()
+    _check(load().omni_attn_step_tables(
+        _i32_here(first, "first", 0), _i32_here(count, "count", n),
+        None if lines is None else _i32_here(lines, "lines", n), n, page, ring, table.data_ptr(), table.shape[1],
+        table.shape[0], None if free_pages is None else _i32_here(free_pages, "free_pages", 1),
+        0 if free_pages is None else free_pages.numel(),
+        None if free_state is None else _i32_here(free_state, "free_state", 2), rows, pages.numel(),
+        _i32_here(pos, "pos", 0), _i32_here(slots, "slots", rows), _i32_here(seq, "seq", rows),
+        _i32_here(row_indptr, "row_indptr", n + 1), _i32_here(indptr, "indptr", n + 1), _i32_here(pages, "pages", 0),
+        _i32_here(status, "status", 5), _stream(stream)))
+    return status
+
+
+def qwen3_rope_q8(qkv, q_norm, k_norm, pos, slots, q_out, k_out, kv, kv_scale, hq, hk, eps, theta, stream=None):
+    """``qwen3_rope`` with the quantized cache write: q to ``q_out`` rows, the
+    turned k to ``k_out`` rows (None: not written), K and V to slot ``slots[n]``
+    of the 8-bit cache. Rows may be strided; rows with a negative slot are
+    skipped."""
+    rows = pos.numel()
+    for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        _bf16_dev(t, n), _here(t, n)
+        if t.numel() != HEAD_DIM:
+            raise OmniAttnError(EINVAL, f"{n} must have {HEAD_DIM} elements")
+    src, ld = _rows_here(qkv, "qkv", rows, hq + 2 * hk)
+    q, q_ld = _rows_here(q_out, "q_out", rows, hq)
+    k, k_ld = (None, 0) if k_out is None else _rows_here(k_out, "k_out", rows, hk)
+    cache, scales, fmt = _q8_cache(kv, kv_scale, hk)
+    _check(load().omni_qwen3_rope_q8(src, ld, q_norm.data_ptr(), k_norm.data_ptr(), _i32_here(pos, "pos", 0),
+                                     _i32_here(slots, "slots", rows), q, q_ld, k, k_ld, cache, scales, fmt, rows, hq, hk,
+                                     float(eps), float(theta), _stream(stream)))
+
+
+def decode_plan_q8(rows: int, hq: int, hk: int, page: int, max_len: int, chunk: int = 0) -> DecodePlan:
+    """The plan for qwen3_attend_q8."""
+    plan = DecodePlan()
+    _check(load().omni_attn_decode_plan_init_q8(rows, hq, hk, page, max_len, chunk, ctypes.byref(plan)))
+    return plan
+
+
+def qwen3_attend_q8(q, kv, kv_scale, pos, seq, ragged, indptr, pages, page, out, hq, hk, scale, plan, workspace=None,
+                    stream=None):
+    """``qwen3_attend`` over the 8-bit cache: q rows [hq * 128], possibly strided;
+    rows with a negative position store zeros."""
+    rows = plan.rows
+    src, stride = _rows_here(q, "q", rows, hq)
+    cache, scales, fmt = _q8_cache(kv, kv_scale, hk)
+    _bf16_dev(out, "out"), _here(out, "out")
+    if out.numel() < rows * hq * HEAD_DIM:
+        raise OmniAttnError(EINVAL, f"out holds {out.numel()} elements, the plan's rows need {rows * hq * HEAD_DIM}")
+    if workspace is not None:
+        _here(workspace, "workspace")
+    _check(load().omni_qwen3_attend_q8(src, stride, cache, scales, fmt, _i32_here(pos, "pos", rows),
+                                       None if seq is None else _i32_here(seq, "seq", rows), int(ragged),
+                                       _i32_here(indptr, "indptr", 1 if ragged else rows + 1),
+                                       _i32_here(pages, "pages", 0), page, out.data_ptr(), hq, hk, float(scale),
+                                       ctypes.byref(plan), _ws(plan, workspace), _stream(stream)))
+    return out
+
+
+@dataclass
+class Prompt:
+    plan: PromptPlan
+    work: object  # device int32 tensor
+
+
+def prompt_plan(lens, hq, hk, device="cuda", exact_p=False) -> Prompt:
+    """Host plan of causal attention over packed prompts of these lengths;
+    uploads the work list. exact_p: as in prefill_plan."""
+    import numpy as np
+
+    lens_a = np.ascontiguousarray(lens, dtype=np.int32)
+    plan = PromptPlan()
+    L = load()
+    ptr = lens_a.ctypes.data_as(ctypes.c_void_p)
+    rc = L.omni_attn_prompt_plan_init(len(lens_a), ptr, hq, hk, None, 0, ctypes.byref(plan))
+    if rc not in (OK, EWORKSPACE):
+        _check(rc)
+    work_h = np.zeros(max(1, int(plan.work_bytes) // 4), dtype=np.int32)
+    _check(L.omni_attn_prompt_plan_init(len(lens_a), ptr, hq, hk, work_h.ctypes.data_as(ctypes.c_void_p), len(work_h),
+                                        ctypes.byref(plan)))
+    plan.exact_p = 1 if exact_p else 0
+    return Prompt(plan, _torch.from_numpy(work_h).to(device))
+
+
+def prompt_run(pp: Prompt, q, k, v, out, scale, stream=None):
+    """Causal attention of packed prompts: q rows [hq * 128], k and v rows
+    [hk * 128], possibly strided (parts of one qkv row); out contiguous rows."""
+    plan = pp.plan
+    rows, hq, hk = plan.rows, plan.hq, plan.hk
+    (qp, qs), (kp, ks), (vp, vs) = _rows_here(q, "q", rows, hq), _rows_here(k, "k", rows, hk), _rows_here(v, "v", rows, hk)
+    _bf16_dev(out, "out"), _here(out, "out"), _here(pp.work, "the plan's work list")
+    if out.numel() < rows * hq * HEAD_DIM:
+        raise OmniAttnError(EINVAL, f"out holds {out.numel()} elements, the plan's rows need {rows * hq * HEAD_DIM}")
+    _check(load().omni_attn_prompt_run(ctypes.byref(plan), qp, qs, kp, ks, vp, vs, out.data_ptr(), float(scale),
+                                       pp.work.data_ptr(), _stream(stream)))
     return out
 
 
