@@ -239,12 +239,56 @@ __device__ __forceinline__ int split_len_of(const DecodeQ8Args& a, int len) {
   return max(a.chunk, ((len + a.splits - 1) / a.splits + kTile - 1) / kTile * kTile);
 }
 
-// One workgroup per (split, K/V head, row): a tile of 64 keys at a time, scores
-// into LDS, the softmax's running maximum and sum per query head, and thread d
-// (of 128) adds up dim d.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Eight stored bytes as bf16, exactly (E4M3 has 4 significant bits, the integers 7).
 template <int FMT>
-__global__ __launch_bounds__(kThreads) void decode_q8(DecodeQ8Args a) {
-  const int split = blockIdx.x, kh = blockIdx.y, n = blockIdx.z, G = a.hq / a.hk, tid = threadIdx.x;
+__device__ __forceinline__ bf16x8 bf16_of(uint32_t w0, uint32_t w1) {
+  uint4 u;
+  if constexpr (FMT == kQ8E4m3) {
+    u.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w0, 1.f, false));
+    u.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w0, 1.f, true));
+    u.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w1, 1.f, false));
+    u.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w1, 1.f, true));
+  } else {
+    float v[8];
+    from_bytes<FMT>(w0, v), from_bytes<FMT>(w1, v + 4);
+    u = pack8(v);
+  }
+  return __builtin_bit_cast(bf16x8, u);
+}
+
+__device__ __forceinline__ int from_lane(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane << 2, v); }
+
+// The larger of v in the four lanes with the same lane % 16.
+__device__ __forceinline__ float max_of_groups(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+constexpr int kDecodeWaves = kThreads / 64;
+constexpr int kBlocksPerTile = kTile / kQ8Block;
+
+// One workgroup per (split, K/V head, row); its waves take the split's 64-key
+// tiles in turn, each with a running maximum, sum and O of its own, merged
+// through LDS at the end. Lane l is column n = l % 16 (query head) and group
+// g = l / 16 of the v_mfma_f32_16x16x32_bf16 operands:
+//   S^T (16 keys x 16 heads), four of them: row 4 b + r of product j is token
+//     4 j + r of the tile's block b, so a lane ends with all 16 tokens of block
+//     g for its head, in order, which is P^T's operand as it stands: no data
+//     crosses lanes between the two products but the maximum.
+//   O^T (16 dims x 16 heads) += V^T . P^T: V lies [dim][token] in the cache, so
+//     a lane's 16 bytes are block g's tokens of one dim, operand order again.
+// P is carried as two bf16 terms (hi + lo, 16 bits): the matrix cores are a
+// tenth of the time. Both scales act per block, that is per lane: on the scores
+// and, an exact power of two, on P.
+template <int FMT>
+__global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
+  const int kh = blockIdx.y, n = blockIdx.z, G = a.hq / a.hk, tid = threadIdx.x;
+  const int split = rotated_split(blockIdx.x, kh + a.hk * n, a.splits);
   const int p = a.pos[n];
   const int len = p < 0 ? 0 : p + 1;
   const int64_t h0 = (int64_t)n * a.hq + kh * G;
@@ -254,92 +298,161 @@ __global__ __launch_bounds__(kThreads) void decode_q8(DecodeQ8Args a) {
     return;
   }
   const int split_len = split_len_of(a, len);
+  if ((int64_t)split * split_len >= len) return;
   const int t0 = split * split_len, t1 = min(len, t0 + split_len);
-  if (t0 >= len) return;
   const int32_t* pg = a.pages + a.indptr[a.ragged ? a.seq[n] : n];
-  __shared__ float s_q[kMostGroup][kHead], s_p[kMostGroup][kTile], s_alpha[kMostGroup], s_m[kMostGroup], s_l[kMostGroup];
-  for (int i = tid; i < G * kHead; i += kThreads)
-    s_q[i / kHead][i % kHead] = lo_bf16(a.q[(int64_t)n * a.q_stride + (int64_t)kh * G * kHead + i]);
-  if (tid < G) s_m[tid] = -INFINITY, s_l[tid] = 0.f;
-  float acc[kMostGroup];
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int tiles = (t1 - t0 + kTile - 1) / kTile;
+  const int mine = (tiles - wave + kDecodeWaves - 1) / kDecodeWaves;  // tiles wave, wave + 4, ..
+  const int last_block = (t1 - 1) / kQ8Block;
+
+  // q: product step kk holds dims 64 (kk / 2) + 16 g + 8 (kk % 2) .. + 7.
+  bf16x8 q[4];
+  {
+    const bf16_t* qp = a.q + (int64_t)n * a.q_stride + (int64_t)(kh * G + min(col, G - 1)) * kHead;
 #pragma unroll
-  for (int g = 0; g < kMostGroup; ++g) acc[g] = 0.f;
-  __syncthreads();
-  const auto block_of = [&](int t) {
-    const int b = t / kQ8Block, j = page_index(a.pd, b);
-    return page_slot(a.pd, pg[j], b);
-  };
-  for (int t = t0; t < t1; t += kTile) {
-    {  // scores: thread (key, quarter of the query heads)
-      const int key = t + (tid & 63), part = tid >> 6;
-      float k[kHead];
-      if (key < t1) {
-        const int64_t at = block_of(key) * 2 * a.hk + kh;
-        const float sc = pow2_biased(a.kv_scale[at]) * a.scale_log2;
-        const uint4* src = reinterpret_cast<const uint4*>(a.kv + at * kQ8HeadBytes + (key & 15) * kHead);
-#pragma unroll
-        for (int i = 0; i < kHead / 16; ++i) {
-          const uint4 w = src[i];
-          from_bytes<FMT>(w.x, k + 16 * i), from_bytes<FMT>(w.y, k + 16 * i + 4);
-          from_bytes<FMT>(w.z, k + 16 * i + 8), from_bytes<FMT>(w.w, k + 16 * i + 12);
-        }
-        for (int g = part; g < G; g += 4) {
-          float s = 0.f;
-#pragma unroll
-          for (int d = 0; d < kHead; ++d) s = fmaf(k[d], s_q[g][d], s);
-          s_p[g][tid & 63] = s * sc;
-        }
-      } else {
-        for (int g = part; g < G; g += 4) s_p[g][tid & 63] = -INFINITY;
-      }
-    }
-    __syncthreads();
-    for (int g = tid >> 6; g < G; g += 4) {
-      const int lane = tid & 63;
-      float x = s_p[g][lane], mx = x;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-      const float was = s_m[g], top = fmaxf(was, mx), base = top == -INFINITY ? 0.f : top;
-      x = fast_exp2(x - base);
-      s_p[g][lane] = x;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-      const float alpha = fast_exp2(was - base);
-      if (lane == 0) s_alpha[g] = alpha, s_m[g] = top, s_l[g] = s_l[g] * alpha + x;
-    }
-    __syncthreads();
-    if (tid < kHead) {
-#pragma unroll
-      for (int g = 0; g < kMostGroup; ++g)
-        if (g < G) acc[g] *= s_alpha[g];
-      for (int b = 0; b < kTile / kQ8Block && t + kQ8Block * b < t1; ++b) {
-        const int64_t at = block_of(t + kQ8Block * b) * 2 * a.hk + a.hk + kh;
-        const float sc = pow2_biased(a.kv_scale[at]);
-        const uint4 w = *reinterpret_cast<const uint4*>(a.kv + at * kQ8HeadBytes + tid * kQ8Block);
-        float v[16];
-        from_bytes<FMT>(w.x, v), from_bytes<FMT>(w.y, v + 4), from_bytes<FMT>(w.z, v + 8), from_bytes<FMT>(w.w, v + 12);
-#pragma unroll
-        for (int i = 0; i < kQ8Block; ++i) {
-          const float x = t + kQ8Block * b + i < t1 ? v[i] * sc : 0.f;
-#pragma unroll
-          for (int g = 0; g < kMostGroup; ++g)
-            if (g < G) acc[g] = fmaf(s_p[g][kQ8Block * b + i], x, acc[g]);
-        }
-      }
-    }
-    __syncthreads();
+    for (int kk = 0; kk < 4; ++kk)
+      q[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + 64 * (kk >> 1) + 16 * grp + 8 * (kk & 1)));
   }
-  if (tid < kHead) {
+
+  // Blocks of 16 of the wave's tiles at a time: lane 4 k + b holds block b of
+  // tile k and its two exponents.
+  const int64_t row_blocks = 2LL * a.hk;
+  int ids = 0, exps = 0;
+  auto next_blocks = [&](int k0) __attribute__((always_inline)) {
+    const int tile = wave + kDecodeWaves * (k0 + (lane >> 2));
+    const int b = min(t0 / kQ8Block + tile * kBlocksPerTile + (lane & 3), last_block);
+    ids = (int)page_slot(a.pd, pg[page_index(a.pd, b)], b);
+    const uint8_t* e = a.kv_scale + ids * row_blocks + kh;
+    exps = e[0] | e[a.hk] << 16;
+  };
+
+  uint4 kr[4][2], vr[8];
+  auto load_k = [&](int k) __attribute__((always_inline)) {
+    const int64_t block = from_lane(ids, 4 * (k & 15) + (col >> 2));
+    const uint8_t* kb = a.kv + (block * row_blocks + kh) * kQ8HeadBytes + (col & 3) * kHead + 16 * grp;
 #pragma unroll
-    for (int g = 0; g < kMostGroup; ++g) {
-      if (g >= G) break;
-      const float o = acc[g] / s_l[g];
-      if (split_len >= len) {
-        a.out[(h0 + g) * kHead + tid] = (bf16_t)f2bf(o);
-      } else {
-        a.ws_o[((h0 + g) * a.splits + split) * kHead + tid] = o;
-        if (tid == 0) a.ws_lse[(h0 + g) * a.splits + split] = s_m[g] + __log2f(s_l[g]);
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) kr[j][c] = ldg16_stream(kb + 4 * j * kHead + 64 * c);
+  };
+  auto load_v = [&](int k) __attribute__((always_inline)) {
+    const int64_t block = from_lane(ids, 4 * (k & 15) + grp);
+    const uint8_t* vb = a.kv + (block * row_blocks + a.hk + kh) * kQ8HeadBytes + col * kQ8Block;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vr[i] = ldg16_stream(vb + i * 16 * kQ8Block);
+  };
+
+  f32x4 o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  if (mine > 0) {
+    next_blocks(0);
+    load_k(0);
+  }
+  for (int k = 0; k < mine; ++k) {
+    // V of this tile, then (when its scores are taken) K of the next: one of the two is always in flight.
+    load_v(k);
+    const int e2 = from_lane(exps, 4 * (k & 15) + grp);
+    const int seen = t1 - t0 - (wave + kDecodeWaves * k) * kTile - kQ8Block * grp;  // tokens of block g that count
+    float s[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of<FMT>(kr[j][c].x, kr[j][c].y), q[2 * c], d, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of<FMT>(kr[j][c].z, kr[j][c].w), q[2 * c + 1], d, 0, 0, 0);
       }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[4 * j + r] = d[r];
+    }
+    if (k + 1 < mine) {
+      if (((k + 1) & 15) == 0) next_blocks(k + 1);
+      load_k(k + 1);
+    }
+    const float ks = pow2_biased(e2 & 0xff) * a.scale_log2, vs = pow2_biased(e2 >> 16);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) s[t] *= ks;
+    if (__any(seen < kQ8Block)) {  // the row's last tile: nothing past its last token counts, whatever it holds
+#pragma unroll
+      for (int t = 0; t < 16; ++t)
+        if (t >= seen) s[t] = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int left = min(max(seen - 4 * w, 0), 4);
+        const uint32_t stay = left == 4 ? ~0u : (1u << (8 * left)) - 1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) (&vr[i].x)[w] &= stay;
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int t = 1; t < 16; ++t) mx = fmaxf(mx, s[t]);
+    mx = max_of_groups(mx);
+    // The base moves only when the maximum grows by more than 8 (log2): p <= 2^8.
+    const bool grow = mx > m + 8.f;
+    if (__any(grow)) {
+      const float alpha = grow ? fast_exp2(m - mx) : 1.f;
+      m = grow ? mx : m;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] *= alpha;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      s[t] = fast_exp2(s[t] - base);
+      l += s[t];
+      s[t] *= vs;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint4 hi = pack8(s + 8 * t);
+      float rest[8];
+      widen8(hi, rest);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) rest[e] = s[8 * t + e] - rest[e];
+      const bf16x8 ph = __builtin_bit_cast(bf16x8, hi), pl = __builtin_bit_cast(bf16x8, pack8(rest));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bf16x8 v = t == 0 ? bf16_of<FMT>(vr[i].x, vr[i].y) : bf16_of<FMT>(vr[i].z, vr[i].w);
+        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph, o[i], 0, 0, 0);
+        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl, o[i], 0, 0, 0);
+      }
+    }
+  }
+
+  // The waves' parts, merged: O rows [head][dim], then (m, l).
+  __shared__ float s_o[kDecodeWaves][kMostGroup][kHead + 4], s_m[kDecodeWaves][kMostGroup], s_l[kDecodeWaves][kMostGroup];
+  l += xor_lane(l, 16);
+  l += xor_lane(l, 32);
+  if (col < G) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<f32x4*>(&s_o[wave][col][16 * i + 4 * grp]) = o[i];
+    if (grp == 0) s_m[wave][col] = m, s_l[wave][col] = l;
+  }
+  __syncthreads();
+  const int waves = min(tiles, kDecodeWaves);
+  for (int i = tid; i < G * kHead; i += kThreads) {
+    const int g = i / kHead, d = i % kHead;
+    float top = s_m[0][g];
+    for (int w = 1; w < waves; ++w) top = fmaxf(top, s_m[w][g]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float num = 0.f, den = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      const float e = fast_exp2(s_m[w][g] - base);
+      num = fmaf(s_o[w][g][d], e, num);
+      den = fmaf(s_l[w][g], e, den);
+    }
+    if (split_len >= len) {
+      a.out[(h0 + g) * kHead + d] = (bf16_t)f2bf(num / den);
+    } else {
+      // den = 0: every score is -inf, and the split weighs nothing beside the others.
+      a.ws_o[((h0 + g) * a.splits + split) * kHead + d] = den == 0.f ? 0.f : num / den;
+      if (d == 0) a.ws_lse[(h0 + g) * a.splits + split] = base + __log2f(den);
     }
   }
 }
