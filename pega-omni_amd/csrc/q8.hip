@@ -239,6 +239,14 @@ __device__ __forceinline__ int split_len_of(const DecodeQ8Args& a, int len) {
   return max(a.chunk, ((len + a.splits - 1) / a.splits + kTile - 1) / kTile * kTile);
 }
 
+// rotated_split evens out the splits over the XCDs; but an XCD hands its
+// workgroups to its 32 CUs in turn, and where S divides 32 its CU would get the
+// same split index from every one of them (a row's last splits are the ones that
+// are short or empty). So the rotation moves on by one every 256 workgroups too.
+__device__ __forceinline__ int spread_split(int slot, int u, int S) {
+  return (int)((rotated_split(slot, u, S) + (((int64_t)S * u) >> 8)) % S);
+}
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -288,8 +296,9 @@ constexpr int kBlocksPerTile = kTile / kQ8Block;
 template <int FMT>
 __global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
   const int kh = blockIdx.y, n = blockIdx.z, G = a.hq / a.hk, tid = threadIdx.x;
-  const int split = rotated_split(blockIdx.x, kh + a.hk * n, a.splits);
+  const int split = spread_split(blockIdx.x, kh + a.hk * n, a.splits);
   const int p = a.pos[n];
+  const int32_t* pg = a.pages + a.indptr[a.ragged ? max(a.seq[n], 0) : n];
   const int len = p < 0 ? 0 : p + 1;
   const int64_t h0 = (int64_t)n * a.hq + kh * G;
   if (len == 0) {
@@ -300,7 +309,6 @@ __global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
   const int split_len = split_len_of(a, len);
   if ((int64_t)split * split_len >= len) return;
   const int t0 = split * split_len, t1 = min(len, t0 + split_len);
-  const int32_t* pg = a.pages + a.indptr[a.ragged ? a.seq[n] : n];
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int tiles = (t1 - t0 + kTile - 1) / kTile;
@@ -335,7 +343,7 @@ __global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) kr[j][c] = ldg16_stream(kb + 4 * j * kHead + 64 * c);
+      for (int c = 0; c < 2; ++c) kr[j][c] = ldg16(kb + 4 * j * kHead + 64 * c);
   };
   auto load_v = [&](int k) __attribute__((always_inline)) {
     const int64_t block = from_lane(ids, 4 * (k & 15) + grp);
@@ -458,24 +466,65 @@ __global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
 }
 
 // Merge the splits of a (row, head): sum of o_i 2^(lse_i - max) over the sum of
-// those weights.
-__global__ __launch_bounds__(kHead) void merge_q8(DecodeQ8Args a) {
+// those weights. 32 lanes of 4 dims, eight groups that take the splits in turn,
+// kMergeBatch at a time: the partials are asked for before their weights are
+// known, so a row of up to 32 splits costs one memory round trip behind pos.
+constexpr int kMergeGroups = kThreads / 32;
+constexpr int kMergeBatch = 4;
+
+__global__ __launch_bounds__(kThreads) void merge_q8(DecodeQ8Args a) {
   const int64_t h = blockIdx.x;
-  const int n = (int)(h / a.hq), d = threadIdx.x;
-  const int len = a.pos[n] < 0 ? 0 : a.pos[n] + 1;
+  const int tid = threadIdx.x, lane = tid & 31, grp = tid >> 5;
+  const float* lse = a.ws_lse + h * a.splits;
+  const float* part = a.ws_o + h * a.splits * kHead + 4 * lane;
+  const int p = a.pos[h / a.hq];
+  const int len = p < 0 ? 0 : p + 1;
   const int split_len = split_len_of(a, len);
   if (split_len >= len) return;
   const int used = (len + split_len - 1) / split_len;
-  const float* lse = a.ws_lse + h * a.splits;
-  float top = -INFINITY;
-  for (int i = 0; i < used; ++i) top = fmaxf(top, lse[i]);
-  float num = 0.f, den = 0.f;
-  for (int i = 0; i < used; ++i) {
-    const float w = fast_exp2(lse[i] - top);
-    num = fmaf(a.ws_o[(h * a.splits + i) * kHead + d], w, num);
-    den += w;
+  f32x4 num = {0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, den = 0.f;  // of this group's splits
+  for (int i0 = grp; i0 < used; i0 += kMergeGroups * kMergeBatch) {
+    f32x4 o[kMergeBatch];
+    float e[kMergeBatch];
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j) {
+      const int i = min(i0 + kMergeGroups * j, used - 1);
+      e[j] = lse[i];
+      o[j] = *reinterpret_cast<const f32x4*>(part + (int64_t)i * kHead);
+    }
+    float mx = top;
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j) mx = fmaxf(mx, e[j]);  // one seen twice changes no maximum
+    const float base = mx == -INFINITY ? 0.f : mx, alpha = fast_exp2(top - base);
+    top = mx;
+    num *= alpha, den *= alpha;
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j) {
+      if (i0 + kMergeGroups * j >= used) break;
+      const float w = fast_exp2(e[j] - base);
+      num += o[j] * w, den += w;
+    }
   }
-  a.out[h * kHead + d] = (bf16_t)f2bf(num / den);
+  __shared__ f32x4 s_num[kMergeGroups][32];
+  __shared__ float s_top[kMergeGroups], s_den[kMergeGroups];
+  s_num[grp][lane] = num;
+  if (lane == 0) s_top[grp] = top, s_den[grp] = den;
+  __syncthreads();
+  if (grp != 0) return;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < kMergeGroups; ++g) mx = fmaxf(mx, s_top[g]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  num = f32x4{0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+  for (int g = 0; g < kMergeGroups; ++g) {
+    const float w = fast_exp2(s_top[g] - base);
+    num += s_num[g][lane] * w;
+    den = fmaf(s_den[g], w, den);
+  }
+  *reinterpret_cast<uint2*>(a.out + h * kHead + 4 * lane) =
+      make_uint2(pack_bf16x2(num[0] / den, num[1] / den), pack_bf16x2(num[2] / den, num[3] / den));
 }
 
 }  // namespace
@@ -497,7 +546,7 @@ int launch_decode_q8(const DecodeQ8Args& a, int rows, hipStream_t stream) {
     decode_q8<kQ8Int8><<<grid, kThreads, 0, stream>>>(a);
   if (check_launch() != 0) return -3;
   if (a.splits > 1) {
-    merge_q8<<<dim3((unsigned)(rows * a.hq)), kHead, 0, stream>>>(a);
+    merge_q8<<<dim3((unsigned)(rows * a.hq)), kThreads, 0, stream>>>(a);
     return check_launch();
   }
   return 0;
