@@ -761,12 +761,31 @@ int omni_qwen3_attend_dense(const void* qkv, const void* kv, int per, int base, 
 
 namespace {
 
-// Split size of a decode bucket over the 8-bit cache.
+// Split size of a decode bucket over the 8-bit cache: the one with the least
+// estimated time. What a launch takes, us, from sweeps of 17 shapes over splits
+// of 64 keys to none (1 to 128 rows, 1 to 32 K/V heads, 300 to 130,000 keys):
+//   the keys' bytes at 6.2 TB/s, with rows 0.6 of max_len long; or, where few
+//   workgroups run, a wave's walk through its tiles, 1.05 for each 32 keys of its
+//   quarter of a split;
+//   2 for each round of 1024 resident workgroups (four a CU);
+//   with splits, 3 for the merge's launch and 1.3 for every 32 splits of a row.
+// Measured at the choice / at the best split of the sweep: 1 row of 2400 keys,
+// hk = 8, 128 keys 8.3 / 8.3; of 8000, 256 keys 11.0 / 11.0; 16 rows of 200-2400
+// 256 keys 15.5 / 15.5; 64 rows none 37.4 / 37.4; 21 rows of 512-5120 512 keys 29.6 /
+// 29.6; 4 rows of 100,000-130,000 2048 keys 170.5 / 169.2.
 int pick_chunk_q8(int rows, int hk, int max_len) {
-  const long long units = (long long)rows * hk;
-  int chunk = 1024;
-  while (chunk > 128 && units * (((long long)max_len + chunk - 1) / chunk) < 1024) chunk /= 2;
-  return chunk;
+  const double units = (double)rows * hk, read = units * max_len * 0.6 * 256 / 6.2e6;
+  int best = 0;
+  double least = 0;
+  for (int chunk : {128, 256, 384, 512, 768, 1024, 1536, 2048, 4096, 8192, 16384, 32768, 0}) {
+    if (chunk == 0 || chunk >= max_len) chunk = (int)std::min<int64_t>(((int64_t)max_len + 63) / 64 * 64, INT_MAX / 64 * 64);
+    const double splits = std::ceil((double)max_len / chunk);
+    const double t = std::max(read, 1.05 * chunk / 128) + 2 * std::ceil(0.6 * units * splits / 1024) +
+                     (splits > 1 ? 3 + 1.3 * std::ceil(splits / 32) : 0);
+    if (best == 0 || t < least) best = chunk, least = t;
+    if (chunk >= max_len) break;
+  }
+  return best;
 }
 
 int q8_format(int format, const char* who) {

@@ -231,12 +231,13 @@ __global__ __launch_bounds__(kThreads) void rope_q8(RopeQ8Args a) {
 // ------------------------------------------------------------------- decode
 
 constexpr int kMostGroup = 16;  // query heads per K/V head
-constexpr int kTile = 64;       // keys per step: four blocks
+constexpr int kTile = 32;       // keys per step: two blocks
+constexpr int kIds = 64 / (kTile / kQ8Block);  // tiles whose blocks a wave looks up at once
 
 // Keys per split of a row of len keys: the plan's, or more where a row is
-// longer than the plan's bound (whole tiles).
+// longer than the plan's bound (multiples of 64 keys, as the plan's).
 __device__ __forceinline__ int split_len_of(const DecodeQ8Args& a, int len) {
-  return max(a.chunk, ((len + a.splits - 1) / a.splits + kTile - 1) / kTile * kTile);
+  return max(a.chunk, ((len + a.splits - 1) / a.splits + 63) / 64 * 64);
 }
 
 // rotated_split evens out the splits over the XCDs; but an XCD hands its
@@ -280,21 +281,24 @@ __device__ __forceinline__ float max_of_groups(float v) {
 constexpr int kDecodeWaves = kThreads / 64;
 constexpr int kBlocksPerTile = kTile / kQ8Block;
 
-// One workgroup per (split, K/V head, row); its waves take the split's 64-key
+// One workgroup per (split, K/V head, row); its waves take the split's 32-key
 // tiles in turn, each with a running maximum, sum and O of its own, merged
 // through LDS at the end. Lane l is column n = l % 16 (query head) and group
 // g = l / 16 of the v_mfma_f32_16x16x32_bf16 operands:
-//   S^T (16 keys x 16 heads), four of them: row 4 b + r of product j is token
-//     4 j + r of the tile's block b, so a lane ends with all 16 tokens of block
-//     g for its head, in order, which is P^T's operand as it stands: no data
-//     crosses lanes between the two products but the maximum.
-//   O^T (16 dims x 16 heads) += V^T . P^T: V lies [dim][token] in the cache, so
-//     a lane's 16 bytes are block g's tokens of one dim, operand order again.
+//   S^T (16 keys x 16 heads), two of them: row 4 x + r of product j is token
+//     8 (x % 2) + 4 j + r of the tile's block x / 2, so a lane ends with tokens
+//     8 (g % 2) .. + 7 of block g / 2 for its head, in order, which is P^T's
+//     operand as it stands: no data crosses lanes between the two products but
+//     the maximum.
+//   O^T (16 dims x 16 heads) += V^T . P^T: V lies [dim][token] in the cache. A
+//     lane loads the 16 tokens of one dim (groups 2 b and 2 b + 1 two dims of
+//     block b) and the two groups trade halves, which gives each its tokens of
+//     both dims.
 // P is carried as two bf16 terms (hi + lo, 16 bits): the matrix cores are a
 // tenth of the time. Both scales act per block, that is per lane: on the scores
 // and, an exact power of two, on P.
 template <int FMT>
-__global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
+__global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
   const int kh = blockIdx.y, n = blockIdx.z, G = a.hq / a.hk, tid = threadIdx.x;
   const int split = spread_split(blockIdx.x, kh + a.hk * n, a.splits);
   const int p = a.pos[n];
@@ -324,32 +328,32 @@ __global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
       q[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + 64 * (kk >> 1) + 16 * grp + 8 * (kk & 1)));
   }
 
-  // Blocks of 16 of the wave's tiles at a time: lane 4 k + b holds block b of
+  // Blocks of kIds of the wave's tiles at a time: lane 2 k + b holds block b of
   // tile k and its two exponents.
   const int64_t row_blocks = 2LL * a.hk;
   int ids = 0, exps = 0;
   auto next_blocks = [&](int k0) __attribute__((always_inline)) {
-    const int tile = wave + kDecodeWaves * (k0 + (lane >> 2));
-    const int b = min(t0 / kQ8Block + tile * kBlocksPerTile + (lane & 3), last_block);
+    const int tile = wave + kDecodeWaves * (k0 + (lane >> 1));
+    const int b = min(t0 / kQ8Block + tile * kBlocksPerTile + (lane & 1), last_block);
     ids = (int)page_slot(a.pd, pg[page_index(a.pd, b)], b);
     const uint8_t* e = a.kv_scale + ids * row_blocks + kh;
     exps = e[0] | e[a.hk] << 16;
   };
 
-  uint4 kr[4][2], vr[8];
+  uint4 kr[2][2], vr[4];
   auto load_k = [&](int k) __attribute__((always_inline)) {
-    const int64_t block = from_lane(ids, 4 * (k & 15) + (col >> 2));
-    const uint8_t* kb = a.kv + (block * row_blocks + kh) * kQ8HeadBytes + (col & 3) * kHead + 16 * grp;
+    const int64_t block = from_lane(ids, 2 * (k & (kIds - 1)) + (col >> 3));
+    const uint8_t* kb = a.kv + (block * row_blocks + kh) * kQ8HeadBytes + (2 * (col & 4) + (col & 3)) * kHead + 16 * grp;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int c = 0; c < 2; ++c) kr[j][c] = ldg16(kb + 4 * j * kHead + 64 * c);
   };
   auto load_v = [&](int k) __attribute__((always_inline)) {
-    const int64_t block = from_lane(ids, 4 * (k & 15) + grp);
-    const uint8_t* vb = a.kv + (block * row_blocks + a.hk + kh) * kQ8HeadBytes + col * kQ8Block;
+    const int64_t block = from_lane(ids, 2 * (k & (kIds - 1)) + (grp >> 1));
+    const uint8_t* vb = a.kv + (block * row_blocks + a.hk + kh) * kQ8HeadBytes + (16 * (grp & 1) + col) * kQ8Block;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) vr[i] = ldg16_stream(vb + i * 16 * kQ8Block);
+    for (int i = 0; i < 4; ++i) vr[i] = ldg16_stream(vb + i * 32 * kQ8Block);
   };
 
   f32x4 o[8];
@@ -363,11 +367,11 @@ __global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
   for (int k = 0; k < mine; ++k) {
     // V of this tile, then (when its scores are taken) K of the next: one of the two is always in flight.
     load_v(k);
-    const int e2 = from_lane(exps, 4 * (k & 15) + grp);
-    const int seen = t1 - t0 - (wave + kDecodeWaves * k) * kTile - kQ8Block * grp;  // tokens of block g that count
-    float s[16];
+    const int e2 = from_lane(exps, 2 * (k & (kIds - 1)) + (grp >> 1));
+    const int left = t1 - t0 - (wave + kDecodeWaves * k) * kTile;  // keys from this tile on
+    float s[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -378,27 +382,28 @@ __global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
       for (int r = 0; r < 4; ++r) s[4 * j + r] = d[r];
     }
     if (k + 1 < mine) {
-      if (((k + 1) & 15) == 0) next_blocks(k + 1);
+      if (((k + 1) & (kIds - 1)) == 0) next_blocks(k + 1);
       load_k(k + 1);
     }
     const float ks = pow2_biased(e2 & 0xff) * a.scale_log2, vs = pow2_biased(e2 >> 16);
 #pragma unroll
-    for (int t = 0; t < 16; ++t) s[t] *= ks;
-    if (__any(seen < kQ8Block)) {  // the row's last tile: nothing past its last token counts, whatever it holds
+    for (int t = 0; t < 8; ++t) s[t] *= ks;
+    if (left < kTile) {  // the row's last tile: nothing past its last token counts, whatever it holds
 #pragma unroll
-      for (int t = 0; t < 16; ++t)
-        if (t >= seen) s[t] = -INFINITY;
+      for (int t = 0; t < 8; ++t)
+        if (8 * grp + t >= left) s[t] = -INFINITY;
+      const int tokens = left - kQ8Block * (grp >> 1);  // of this lane's block
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const int left = min(max(seen - 4 * w, 0), 4);
-        const uint32_t stay = left == 4 ? ~0u : (1u << (8 * left)) - 1;
+        const int n_ok = min(max(tokens - 4 * w, 0), 4);
+        const uint32_t stay = n_ok == 4 ? ~0u : (1u << (8 * n_ok)) - 1;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) (&vr[i].x)[w] &= stay;
+        for (int i = 0; i < 4; ++i) (&vr[i].x)[w] &= stay;
       }
     }
     float mx = s[0];
 #pragma unroll
-    for (int t = 1; t < 16; ++t) mx = fmaxf(mx, s[t]);
+    for (int t = 1; t < 8; ++t) mx = fmaxf(mx, s[t]);
     mx = max_of_groups(mx);
     // The base moves only when the maximum grows by more than 8 (log2): p <= 2^8.
     const bool grow = mx > m + 8.f;
@@ -411,25 +416,27 @@ __global__ __launch_bounds__(kThreads, 3) void decode_q8(DecodeQ8Args a) {
     }
     const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
+    for (int t = 0; t < 8; ++t) {
       s[t] = fast_exp2(s[t] - base);
       l += s[t];
       s[t] *= vs;
     }
+    const uint4 hi = pack8(s);
+    float rest[8];
+    widen8(hi, rest);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint4 hi = pack8(s + 8 * t);
-      float rest[8];
-      widen8(hi, rest);
+    for (int t = 0; t < 8; ++t) rest[t] = s[t] - rest[t];
+    const bf16x8 ph = __builtin_bit_cast(bf16x8, hi), pl = __builtin_bit_cast(bf16x8, pack8(rest));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) rest[e] = s[8 * t + e] - rest[e];
-      const bf16x8 ph = __builtin_bit_cast(bf16x8, hi), pl = __builtin_bit_cast(bf16x8, pack8(rest));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bf16x8 v = t == 0 ? bf16_of<FMT>(vr[i].x, vr[i].y) : bf16_of<FMT>(vr[i].z, vr[i].w);
-        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph, o[i], 0, 0, 0);
-        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl, o[i], 0, 0, 0);
-      }
+    for (int i = 0; i < 4; ++i) {
+      // Even groups keep tokens 0-7 of their dim and take those of the odd group's, and the other way round.
+      const auto a0 = __builtin_amdgcn_permlane16_swap(vr[i].x, vr[i].z, false, false);
+      const auto a1 = __builtin_amdgcn_permlane16_swap(vr[i].y, vr[i].w, false, false);
+      const bf16x8 v0 = bf16_of<FMT>(a0[0], a1[0]), v1 = bf16_of<FMT>(a0[1], a1[1]);
+      o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, ph, o[2 * i], 0, 0, 0);
+      o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, ph, o[2 * i + 1], 0, 0, 0);
+      o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pl, o[2 * i], 0, 0, 0);
+      o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pl, o[2 * i + 1], 0, 0, 0);
     }
   }
 
