@@ -805,7 +805,8 @@ int omni_attn_step_tables(const int32_t* first, const int32_t* count, const int3
                           const int32_t* free_state, int row_cap, int page_cap, int32_t* pos, int32_t* slots,
                           int32_t* seq, int32_t* row_indptr, int32_t* indptr, int32_t* pages, int32_t* status,
                           void* stream) {
-  if (nseq < 0 || page <= 0 || ring < 0 || table_ld < 0 || num_lines < 0 || row_cap < 0 || page_cap < 0)
+  if (nseq < 0 || page <= 0 || ring < 0 || table_ld < 0 || num_lines < 0 || row_cap < 0 || row_cap == INT_MAX ||
+      page_cap < 0 || page_cap == INT_MAX)
     return fail(OMNI_ATTN_EINVAL, "step_tables: nseq=%d page=%d ring=%d table_ld=%lld num_lines=%d row_cap=%d page_cap=%d",
                 nseq, page, ring, (long long)table_ld, num_lines, row_cap, page_cap);
   if (nseq > 0 && (!first || !count || !table)) return fail(OMNI_ATTN_EINVAL, "step_tables: null first, count or table");

@@ -59,140 +59,144 @@ __device__ __forceinline__ SeqShare seq_share(const TablesArgs& a, int s) {
   return r;
 }
 
+// Sums of counts in 0 .. 2^31 - 1 that stop at 2^31 - 1 (still associative), so a
+// total past int32 shows as one past every capacity.
+__device__ __forceinline__ int add_sat(int x, int y) { return (int)min((uint32_t)x + (uint32_t)y, 0x7fffffffu); }
+__device__ __forceinline__ int4 add_sat(int4 x, int4 y) {
+  return {add_sat(x.x, y.x), add_sat(x.y, y.y), add_sat(x.z, y.z), add_sat(x.w, y.w)};
+}
+
 // Inclusive sums over the workgroup's threads, in thread order.
 __device__ __forceinline__ int4 scan4(int4 v, int4* wave_sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int4 u = {__shfl_up(v.x, d), __shfl_up(v.y, d), __shfl_up(v.z, d), __shfl_up(v.w, d)};
-    if (lane >= d) v = {v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w};
+    if (lane >= d) v = add_sat(v, u);
   }
-  __syncthreads();
   if (lane == 63) wave_sums[wave] = v;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    const int4 u = wave_sums[w];
-    v = {v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w};
-  }
+  for (int w = 0; w < wave; ++w) v = add_sat(v, wave_sums[w]);
   return v;
 }
 
-// The first of n ends above x (n where none is).
-__device__ __forceinline__ int owner(const int* ends, int n, int x) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (ends[mid] > x)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  return lo;
-}
-
+// Every workgroup: the sums over all sequences (one scan of 256 sequences gives
+// totals and offsets; more sequences are added up first), then its share of each
+// output, a row or page finding its sequence by bisection of the sums in LDS.
+// Two memory round trips, the lengths and a page id, and the launch are what a
+// call takes.
 __global__ __launch_bounds__(kTabThreads) void step_tables(TablesArgs a) {
-  const int tid = threadIdx.x, wg = blockIdx.x;
-  const int64_t step = (int64_t)gridDim.x * kTabThreads;
+  const int tid = threadIdx.x, wg = blockIdx.x, first_x = wg * kTabThreads + tid, step = gridDim.x * kTabThreads;
   __shared__ int4 s_wave[kTabWaves];
-  __shared__ unsigned long long s_total[4];
-  __shared__ unsigned s_codes;  // bit c: code c
-  __shared__ int s_rows[kTabThreads], s_pages[kTabThreads], s_taken[kTabThreads], s_back[kTabThreads];
-  __shared__ int s_first[kTabThreads], s_held[kTabThreads], s_line[kTabThreads];
+  __shared__ int s_codes[kTabWaves];
+  __shared__ int4 s_end[kTabThreads];            // rows, pages, taken and given back up to a sequence
+  __shared__ int s_first[kTabThreads], s_held[kTabThreads];
+  __shared__ int64_t s_line[kTabThreads];        // the sequence's line in the table
 
-  // Totals, in 64 bits, and whether the step can be made at all.
-  if (tid < 4) s_total[tid] = 0;
-  if (tid == 0) s_codes = 0;
-  __syncthreads();
-  unsigned long long rows = 0, pages = 0, taken = 0, back = 0;
-  unsigned codes = 0;
-  for (int s = tid; s < a.nseq; s += kTabThreads) {
-    const SeqShare r = seq_share(a, s);
-    if (r.code) codes |= 1u << r.code;
-    rows += r.rows, pages += r.pages, taken += r.taken, back += r.back;
-  }
-  // Integer sums: the order of the additions does not change them.
-  atomicAdd(&s_total[0], rows);
-  atomicAdd(&s_total[1], pages);
-  atomicAdd(&s_total[2], taken);
-  atomicAdd(&s_total[3], back);
-  if (codes) atomicOr(&s_codes, codes);
-  __syncthreads();
-  rows = s_total[0], pages = s_total[1], taken = s_total[2], back = s_total[3];
-  codes = s_codes;
   const int head = a.free_pages ? a.free_state[0] : 0, avail = a.free_pages ? a.free_state[1] : 0;
-  if (a.free_pages) {
-    if (head < 0 || head >= a.num_pages || avail < 0 || avail > a.num_pages || avail + back > (unsigned)a.num_pages)
-      codes |= 1u << 1;
-    if (taken > (unsigned)max(avail, 0)) codes |= 1u << 5;
-  }
-  if (rows > (unsigned)a.row_cap) codes |= 1u << 2;
-  if (pages > (unsigned)a.page_cap) codes |= 1u << 3;
-  const int code = codes ? __ffs(codes) - 1 : 0;
-  if (code) rows = pages = taken = back = 0;  // nothing is built, and the table and the queue stay
+  int codes = 0;  // bit c: code c
+  if (a.free_pages && (head < 0 || head >= a.num_pages || avail < 0 || avail > a.num_pages)) codes |= 1 << 1;
 
-  if (wg == 0 && tid == 0) {
+  // Totals, and whether the step can be made at all.
+  const bool one_scan = a.nseq <= kTabThreads;
+  SeqShare r{};
+  int4 sum{};
+  for (int s = tid; s < a.nseq; s += kTabThreads) {
+    r = seq_share(a, s);
+    if (r.code) codes |= 1 << r.code;
+    sum = add_sat(sum, int4{r.rows, r.pages, r.taken, r.back});
+  }
+  int4 end = scan4(sum, s_wave);
+  s_end[tid] = end;
+  for (int c = 1; c <= 5; ++c)
+    if (__any(codes >> c & 1)) codes |= 1 << c;
+  if ((tid & 63) == 0) s_codes[tid >> 6] = codes;
+  __syncthreads();
+  int4 total = s_end[kTabThreads - 1];
+#pragma unroll
+  for (int w = 0; w < kTabWaves; ++w) codes |= s_codes[w];
+  if (a.free_pages) {
+    if (add_sat(max(avail, 0), total.w) > a.num_pages) codes |= 1 << 1;
+    if (total.z > avail) codes |= 1 << 5;
+  }
+  if (total.x > a.row_cap) codes |= 1 << 2;
+  if (total.y > a.page_cap) codes |= 1 << 3;
+  const int code = codes ? __ffs(codes) - 1 : 0;
+  if (code) total = int4{0, 0, 0, 0};  // nothing is built, and the table and the queue stay
+
+  // Entry `head + k` of the queue, 0 <= k <= num_pages.
+  const auto queue = [&](int k) {
+    const uint32_t i = (uint32_t)head + (uint32_t)k;
+    return i >= (uint32_t)a.num_pages ? i - (uint32_t)a.num_pages : i;
+  };
+  if (first_x == 0) {
     a.status[0] = code;
-    a.status[1] = (int)rows;
-    a.status[2] = (int)pages;
-    a.status[3] = a.free_pages ? code ? head : (int)(((int64_t)head + (int64_t)taken) % a.num_pages) : 0;
-    a.status[4] = a.free_pages ? (int)(avail - (int64_t)taken + (int64_t)back) : 0;
+    a.status[1] = total.x;
+    a.status[2] = total.y;
+    a.status[3] = !a.free_pages ? 0 : code ? head : (int)queue(total.z);
+    a.status[4] = !a.free_pages ? 0 : avail - total.z + total.w;
     a.row_indptr[0] = 0;
     a.indptr[0] = 0;
   }
-  for (int64_t r = (int64_t)rows + (int64_t)wg * kTabThreads + tid; r < a.row_cap; r += step)
-    a.pos[r] = a.slots[r] = a.seq[r] = -1;
+  for (int64_t x = (int64_t)total.x + first_x; x < a.row_cap; x += step) a.pos[x] = a.slots[x] = a.seq[x] = -1;
   if (code) {
-    for (int64_t s = (int64_t)wg * kTabThreads + tid; s < a.nseq; s += step) a.row_indptr[s + 1] = a.indptr[s + 1] = 0;
+    for (int64_t s = first_x; s < a.nseq; s += step) a.row_indptr[s + 1] = a.indptr[s + 1] = 0;
     return;
   }
 
-  const auto queue = [&](int64_t k) { return (int)((head + k) % a.num_pages); };
-  int4 base{};  // rows, pages, taken and given back before these sequences
+  int4 base{};  // the sums before the sequences at hand
   for (int s0 = 0; s0 < a.nseq; s0 += kTabThreads) {
     const int n = min(kTabThreads, a.nseq - s0);
-    SeqShare r{};
-    if (tid < n) r = seq_share(a, s0 + tid);
-    const int4 in = {r.rows, r.pages, r.taken, r.back};
-    int4 end = scan4(in, s_wave);
-    end = {base.x + end.x, base.y + end.y, base.z + end.z, base.w + end.w};
-    s_rows[tid] = end.x, s_pages[tid] = end.y, s_taken[tid] = end.z, s_back[tid] = end.w;
+    if (!one_scan) {
+      __syncthreads();  // the last sequences' sums have been read
+      r = SeqShare{};
+      if (tid < n) r = seq_share(a, s0 + tid);
+      end = add_sat(base, scan4(int4{r.rows, r.pages, r.taken, r.back}, s_wave));
+      s_end[tid] = end;
+    }
     if (tid < n) {
-      s_first[tid] = a.first[s0 + tid], s_held[tid] = r.held, s_line[tid] = r.line;
+      s_first[tid] = a.first[s0 + tid], s_held[tid] = r.held, s_line[tid] = r.line * a.table_ld;
       if (wg == 0) a.row_indptr[s0 + tid + 1] = end.x, a.indptr[s0 + tid + 1] = end.y;
     }
     __syncthreads();
-    const int4 top = {s_rows[n - 1], s_pages[n - 1], s_taken[n - 1], s_back[n - 1]};
-    const auto before = [&](const int* ends, int i, int b) { return i > 0 ? ends[i - 1] : b; };
+    const int4 top = s_end[n - 1];
+    const auto before = [&](int i) { return i > 0 ? s_end[i - 1] : base; };
+    // The sequence (of those at hand) whose range holds x; `of` picks the sum.
+    const auto owner = [&](int x, auto of) {
+      int lo = 0, hi = n;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (of(s_end[mid]) > x)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      return lo;
+    };
     const auto page_of = [&](int i, int j) {  // page j of sequence s0 + i
-      return j < s_held[i] ? a.table[(int64_t)s_line[i] * a.table_ld + j]
-                           : a.free_pages[queue((int64_t)before(s_taken, i, base.z) + j - s_held[i])];
+      return j < s_held[i] ? a.table[s_line[i] + j] : a.free_pages[queue(before(i).z + j - s_held[i])];
     };
-    // This workgroup's share of a range that goes on from `from`: every index x with x / 256 % gridDim.x == wg.
-    const auto first_at = [&](int from) {
-      const int64_t mine = (int64_t)wg * kTabThreads + tid;
-      return from <= mine ? mine : mine + (from - mine + step - 1) / step * step;
-    };
-    for (int64_t x = first_at(base.x); x < top.x; x += step) {
-      const int i = owner(s_rows, n, (int)x), p = s_first[i] + (int)x - before(s_rows, i, base.x);
+    for (int64_t x = (int64_t)base.x + first_x; x < top.x; x += step) {
+      const int i = owner((int)x, [](int4 v) { return v.x; }), p = s_first[i] + (int)x - before(i).x;
       const int q = a.ring > 0 ? p % a.ring : p, j = page_index(a.pd, q);
+      const int id = page_of(i, j);
       a.pos[x] = p;
-      a.slots[x] = (int)page_slot(a.pd, page_of(i, j), q);
       a.seq[x] = s0 + i;
+      a.slots[x] = (int)page_slot(a.pd, id, q);
     }
-    for (int64_t x = first_at(base.y); x < top.y; x += step) {
-      const int i = owner(s_pages, n, (int)x);
-      a.pages[x] = page_of(i, (int)x - before(s_pages, i, base.y));
+    for (int64_t x = (int64_t)base.y + first_x; x < top.y; x += step) {
+      const int i = owner((int)x, [](int4 v) { return v.y; });
+      a.pages[x] = page_of(i, (int)x - before(i).y);
     }
-    for (int64_t x = first_at(base.z); x < top.z; x += step) {
-      const int i = owner(s_taken, n, (int)x);
-      a.table[(int64_t)s_line[i] * a.table_ld + s_held[i] + (int)x - before(s_taken, i, base.z)] = a.free_pages[queue(x)];
+    for (int64_t x = (int64_t)base.z + first_x; x < top.z; x += step) {
+      const int i = owner((int)x, [](int4 v) { return v.z; });
+      a.table[s_line[i] + s_held[i] + (int)x - before(i).z] = a.free_pages[queue((int)x)];
     }
-    for (int64_t x = first_at(base.w); x < top.w; x += step) {
-      const int i = owner(s_back, n, (int)x);
-      a.free_pages[queue((int64_t)avail + x)] = a.table[(int64_t)s_line[i] * a.table_ld + (int)x - before(s_back, i, base.w)];
+    for (int64_t x = (int64_t)base.w + first_x; x < top.w; x += step) {
+      const int i = owner((int)x, [](int4 v) { return v.w; });
+      a.free_pages[queue(avail + (int)x)] = a.table[s_line[i] + (int)x - before(i).w];
     }
     base = top;
-    __syncthreads();
   }
 }
 
