@@ -555,39 +555,73 @@ _Q8_FORMATS = {_torch.float8_e4m3fn: 0, _torch.int8: 1}
 _Q8_SCALES = (_torch.uint8, _torch.float8_e8m0fnu)
 
 
-def _here(t, name):
-    """The device the call launches on holds t (the stream is the current device's)."""
-    if not t.is_cuda or t.get_device() != _torch.cuda.current_device():
+# A call launches on the current device, whose stream it takes: every tensor has
+# to lie there. The device is asked for once per call (`d` below; the raw call
+# where torch has it), each tensor's attributes once.
+_current_device = getattr(_torch._C, "_cuda_getDevice", None) or _torch.cuda.current_device
+_I32, _BF16 = _torch.int32, _torch.bfloat16
+
+
+def _device_of(t, name):
+    d = t.get_device()
+    if d < 0 or d != _current_device():
         raise OmniAttnError(EINVAL, f"{name} must lie on the current device")
+    return d
 
 
-def _i32_here(t, name, least):
-    if t.dtype != _torch.int32 or not t.is_contiguous() or t.numel() < least:
+def _off_device(name):
+    return OmniAttnError(EINVAL, f"{name} must lie on the current device, with the other tensors")
+
+
+def _i32_on(t, name, least, d):
+    if t.dtype is not _I32 or t.numel() < least or not t.is_contiguous():
         raise OmniAttnError(EINVAL, f"{name} must be a contiguous int32 tensor of at least {least}")
-    _here(t, name)
+    if t.get_device() != d:
+        raise _off_device(name)
     return t.data_ptr()
 
 
-def _rows_here(t, name, rows, heads):
+def _bf16_on(t, name, least, d):
+    if t.dtype is not _BF16 or t.numel() < least or not t.is_contiguous():
+        raise OmniAttnError(EINVAL, f"{name} must be a contiguous bf16 tensor of at least {least}")
+    if t.get_device() != d:
+        raise _off_device(name)
+    return t.data_ptr()
+
+
+def _rows_on(t, name, rows, heads, d):
     """Pointer and row stride of at least `rows` bf16 rows of heads x 128."""
-    if t.dtype != _torch.bfloat16 or t.dim() != 2 or t.shape[0] < rows or t.shape[1] != heads * HEAD_DIM:
-        raise OmniAttnError(EINVAL, f"{name} must be bf16 rows [{rows}][{heads * HEAD_DIM}]")
-    if t.stride(1) != 1:
+    width = heads * HEAD_DIM
+    shape = t.shape
+    if t.dtype is not _BF16 or len(shape) != 2 or shape[0] < rows or shape[1] != width:
+        raise OmniAttnError(EINVAL, f"{name} must be bf16 rows [{rows}][{width}]")
+    stride, one = t.stride()
+    if one != 1:
         raise OmniAttnError(EINVAL, f"{name}: the elements of a row must be adjacent")
-    _here(t, name)
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * HEAD_DIM
+    if t.get_device() != d:
+        raise _off_device(name)
+    return t.data_ptr(), stride if shape[0] > 1 else width
 
 
-def _q8_cache(kv, kv_scale, hk):
+def _q8_cache(kv, kv_scale, hk, d):
     """Pointers of a cache and its exponents, and its format."""
-    if kv.dtype not in _Q8_FORMATS or kv.dim() != 3 or kv.shape[1] != 2 * hk or kv.shape[2] != 16 * HEAD_DIM:
+    fmt = _Q8_FORMATS.get(kv.dtype)
+    shape = kv.shape
+    if fmt is None or len(shape) != 3 or shape[1] != 2 * hk or shape[2] != 16 * HEAD_DIM:
         raise OmniAttnError(EINVAL, f"kv must be float8_e4m3fn or int8 [blocks][{2 * hk}][2048]")
-    if kv_scale.dtype not in _Q8_SCALES or kv_scale.shape != kv.shape[:2]:
-        raise OmniAttnError(EINVAL, f"kv_scale must be uint8 or float8_e8m0fnu [{kv.shape[0]}][{2 * hk}]")
+    if kv_scale.dtype not in _Q8_SCALES or kv_scale.shape != shape[:2]:
+        raise OmniAttnError(EINVAL, f"kv_scale must be uint8 or float8_e8m0fnu [{shape[0]}][{2 * hk}]")
     if not kv.is_contiguous() or not kv_scale.is_contiguous():
         raise OmniAttnError(EINVAL, "kv and kv_scale must be contiguous")
-    _here(kv, "kv"), _here(kv_scale, "kv_scale")
-    return kv.data_ptr(), kv_scale.data_ptr(), _Q8_FORMATS[kv.dtype]
+    if kv.get_device() != d or kv_scale.get_device() != d:
+        raise _off_device("kv and kv_scale")
+    return kv.data_ptr(), kv_scale.data_ptr(), fmt
+
+
+def _stream_on(stream, d):
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(d)
+    return _stream(stream)
 
 
 def q8_cache(pages, page, hk, dtype=_torch.float8_e4m3fn, device="cuda"):
@@ -608,20 +642,24 @@ def step_tables(first, count, lines, table, free_pages, free_state, pos, slots, 
     requests (count < 0) given back. lines None: line s; free_pages None: the
     table holds every page. ``status`` = [code, rows, pages, head, free entries];
     ``status[3:5]`` is the next call's free_state, with another status."""
-    n = first.numel()
-    if table.dtype != _torch.int32 or table.dim() != 2 or not table.is_contiguous():
-        raise OmniAttnError(EINVAL, "table must be a contiguous int32 tensor [lines][pages]")
-    _here(table, "table")
-    rows = pos.numel()
+    d = _device_of(first, "first")
+    n, rows = first.numel(), pos.numel()
+    shape = table.shape
+    if len(shape) != 2:
+        raise OmniAttnError(EINVAL, "table must be an int32 tensor [lines][pages]")
+    if free_pages is None:
+        free_ptr = state_ptr = None
+        num_pages = 0
+    else:
+        num_pages = free_pages.numel()
+        free_ptr = _i32_on(free_pages, "free_pages", 1, d)
+        state_ptr = None if free_state is None else _i32_on(free_state, "free_state", 2, d)
     _check(load().omni_attn_step_tables(
-        _i32_here(first, "first", 0), _i32_here(count, "count", n),
-        None if lines is None else _i32_here(lines, "lines", n), n, page, ring, table.data_ptr(), table.shape[1],
-        table.shape[0], None if free_pages is None else _i32_here(free_pages, "free_pages", 1),
-        0 if free_pages is None else free_pages.numel(),
-        None if free_state is None else _i32_here(free_state, "free_state", 2), rows, pages.numel(),
-        _i32_here(pos, "pos", 0), _i32_here(slots, "slots", rows), _i32_here(seq, "seq", rows),
-        _i32_here(row_indptr, "row_indptr", n + 1), _i32_here(indptr, "indptr", n + 1), _i32_here(pages, "pages", 0),
-        _i32_here(status, "status", 5), _stream(stream)))
+        _i32_on(first, "first", 0, d), _i32_on(count, "count", n, d), None if lines is None else _i32_on(lines, "lines", n, d),
+        n, page, ring, _i32_on(table, "table", 0, d), shape[1], shape[0], free_ptr, num_pages, state_ptr, rows,
+        pages.numel(), _i32_on(pos, "pos", 0, d), _i32_on(slots, "slots", rows, d), _i32_on(seq, "seq", rows, d),
+        _i32_on(row_indptr, "row_indptr", n + 1, d), _i32_on(indptr, "indptr", n + 1, d), _i32_on(pages, "pages", 0, d),
+        _i32_on(status, "status", 5, d), _stream_on(stream, d)))
     return status
 
 
@@ -631,17 +669,14 @@ def qwen3_rope_q8(qkv, q_norm, k_norm, pos, slots, q_out, k_out, kv, kv_scale, h
     of the 8-bit cache. Rows may be strided; rows with a negative slot are
     skipped."""
     rows = pos.numel()
-    for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        _bf16_dev(t, n), _here(t, n)
-        if t.numel() != HEAD_DIM:
-            raise OmniAttnError(EINVAL, f"{n} must have {HEAD_DIM} elements")
-    src, ld = _rows_here(qkv, "qkv", rows, hq + 2 * hk)
-    q, q_ld = _rows_here(q_out, "q_out", rows, hq)
-    k, k_ld = (None, 0) if k_out is None else _rows_here(k_out, "k_out", rows, hk)
-    cache, scales, fmt = _q8_cache(kv, kv_scale, hk)
-    _check(load().omni_qwen3_rope_q8(src, ld, q_norm.data_ptr(), k_norm.data_ptr(), _i32_here(pos, "pos", 0),
-                                     _i32_here(slots, "slots", rows), q, q_ld, k, k_ld, cache, scales, fmt, rows, hq, hk,
-                                     float(eps), float(theta), _stream(stream)))
+    d = _device_of(qkv, "qkv")
+    src, ld = _rows_on(qkv, "qkv", rows, hq + 2 * hk, d)
+    q, q_ld = _rows_on(q_out, "q_out", rows, hq, d)
+    k, k_ld = (None, 0) if k_out is None else _rows_on(k_out, "k_out", rows, hk, d)
+    cache, scales, fmt = _q8_cache(kv, kv_scale, hk, d)
+    _check(load().omni_qwen3_rope_q8(src, ld, _bf16_on(q_norm, "q_norm", HEAD_DIM, d), _bf16_on(k_norm, "k_norm", HEAD_DIM, d),
+                                     _i32_on(pos, "pos", 0, d), _i32_on(slots, "slots", rows, d), q, q_ld, k, k_ld, cache,
+                                     scales, fmt, rows, hq, hk, eps, theta, _stream_on(stream, d)))
 
 
 def decode_plan_q8(rows: int, hq: int, hk: int, page: int, max_len: int, chunk: int = 0) -> DecodePlan:
@@ -656,18 +691,16 @@ def qwen3_attend_q8(q, kv, kv_scale, pos, seq, ragged, indptr, pages, page, out,
     """``qwen3_attend`` over the 8-bit cache: q rows [hq * 128], possibly strided;
     rows with a negative position store zeros."""
     rows = plan.rows
-    src, stride = _rows_here(q, "q", rows, hq)
-    cache, scales, fmt = _q8_cache(kv, kv_scale, hk)
-    _bf16_dev(out, "out"), _here(out, "out")
-    if out.numel() < rows * hq * HEAD_DIM:
-        raise OmniAttnError(EINVAL, f"out holds {out.numel()} elements, the plan's rows need {rows * hq * HEAD_DIM}")
-    if workspace is not None:
-        _here(workspace, "workspace")
-    _check(load().omni_qwen3_attend_q8(src, stride, cache, scales, fmt, _i32_here(pos, "pos", rows),
-                                       None if seq is None else _i32_here(seq, "seq", rows), int(ragged),
-                                       _i32_here(indptr, "indptr", 1 if ragged else rows + 1),
-                                       _i32_here(pages, "pages", 0), page, out.data_ptr(), hq, hk, float(scale),
-                                       ctypes.byref(plan), _ws(plan, workspace), _stream(stream)))
+    d = _device_of(q, "q")
+    src, stride = _rows_on(q, "q", rows, hq, d)
+    cache, scales, fmt = _q8_cache(kv, kv_scale, hk, d)
+    if workspace is not None and workspace.get_device() != d:
+        raise _off_device("workspace")
+    _check(load().omni_qwen3_attend_q8(src, stride, cache, scales, fmt, _i32_on(pos, "pos", rows, d),
+                                       None if seq is None else _i32_on(seq, "seq", rows, d), 1 if ragged else 0,
+                                       _i32_on(indptr, "indptr", 1 if ragged else rows + 1, d),
+                                       _i32_on(pages, "pages", 0, d), page, _bf16_on(out, "out", rows * hq * HEAD_DIM, d),
+                                       hq, hk, scale, ctypes.byref(plan), _ws(plan, workspace), _stream_on(stream, d)))
     return out
 
 
@@ -701,12 +734,11 @@ def prompt_run(pp: Prompt, q, k, v, out, scale, stream=None):
     [hk * 128], possibly strided (parts of one qkv row); out contiguous rows."""
     plan = pp.plan
     rows, hq, hk = plan.rows, plan.hq, plan.hk
-    (qp, qs), (kp, ks), (vp, vs) = _rows_here(q, "q", rows, hq), _rows_here(k, "k", rows, hk), _rows_here(v, "v", rows, hk)
-    _bf16_dev(out, "out"), _here(out, "out"), _here(pp.work, "the plan's work list")
-    if out.numel() < rows * hq * HEAD_DIM:
-        raise OmniAttnError(EINVAL, f"out holds {out.numel()} elements, the plan's rows need {rows * hq * HEAD_DIM}")
-    _check(load().omni_attn_prompt_run(ctypes.byref(plan), qp, qs, kp, ks, vp, vs, out.data_ptr(), float(scale),
-                                       pp.work.data_ptr(), _stream(stream)))
+    d = _device_of(q, "q")
+    (qp, qs), (kp, ks), (vp, vs) = _rows_on(q, "q", rows, hq, d), _rows_on(k, "k", rows, hk, d), _rows_on(v, "v", rows, hk, d)
+    _check(load().omni_attn_prompt_run(ctypes.byref(plan), qp, qs, kp, ks, vp, vs,
+                                       _bf16_on(out, "out", rows * hq * HEAD_DIM, d), scale,
+                                       _i32_on(pp.work, "the plan's work list", 0, d), _stream_on(stream, d)))
     return out
 
 
