@@ -19,36 +19,30 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float row16_max(float v) {
-  v = fmaxf(v, dpp<kQuadSwap1>(v));
-  v = fmaxf(v, dpp<kQuadSwap2>(v));
-  v = fmaxf(v, dpp<kRowHalfMirror>(v));
-  v = fmaxf(v, dpp<kRowMirror>(v));
-  return v;
-}
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 
-template <int CTRL>
-__device__ __forceinline__ int dpp_or(int v) {
-  return v | __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false);
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
 }
-__device__ __forceinline__ int row16_or(int v) {
-  return dpp_or<kRowMirror>(dpp_or<kRowHalfMirror>(dpp_or<kQuadSwap2>(dpp_or<kQuadSwap1>(v))));
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max_u16x2(uint32_t v) {
+  return max_u16x2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
+}
+// The larger of each half over the 16 lanes of a DPP row.
+__device__ __forceinline__ uint32_t row16_max_u16x2(uint32_t v) {
+  return dpp_max_u16x2<kRowMirror>(dpp_max_u16x2<kRowHalfMirror>(dpp_max_u16x2<kQuadSwap2>(dpp_max_u16x2<kQuadSwap1>(v))));
 }
 
 // 2^(biased - 127) for 1 <= biased <= 254.
 __device__ __forceinline__ float pow2_biased(int biased) { return __int_as_float(biased << 23); }
 
-// The exponent of a block whose largest finite magnitude is amax: from amax =
-// m 2^x with 1 <= m < 2, and top = 1.75 2^8 (448) or 1.984375 2^6 (127).
+// The exponent of a block whose largest finite magnitude has the bf16 bits `most`:
+// from most = m 2^x with 1 <= m < 2, and top = 1.75 2^8 (448) or 1.984375 2^6 (127).
 template <int FMT>
-__device__ __forceinline__ int block_exponent(float amax) {
-  const uint32_t bits = __float_as_uint(amax);
-  const uint32_t top = __float_as_uint(FMT == kQ8E4m3 ? 448.f : 127.f);
-  const int e = (int)(bits >> 23) - (int)(top >> 23) + 127 + ((bits & 0x7fffffu) > (top & 0x7fffffu) ? 1 : 0);
-  return max(e, 1);
+__device__ __forceinline__ int block_exponent(int most) {
+  constexpr int top = FMT == kQ8E4m3 ? 0x43e0 : 0x42fe;
+  return max((most >> 7) - (top >> 7) + 127 + ((most & 0x7f) > (top & 0x7f) ? 1 : 0), 1);
 }
-
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // Four values, already divided by the block's scale, to four bytes. E4M3 holds
 // no infinity: infinities become NaN. Integers hold neither: a NaN becomes 0, an
@@ -56,9 +50,7 @@ __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0
 template <int FMT>
 __device__ __forceinline__ uint32_t to_bytes(float a, float b, float c, float d) {
   if constexpr (FMT == kQ8E4m3) {
-    const float nan = __uint_as_float(0x7fc00000u);
-    a = finite(a) ? a : nan, b = finite(b) ? b : nan, c = finite(c) ? c : nan, d = finite(d) ? d : nan;
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
   } else {
     const auto one = [](float x) {
@@ -66,6 +58,24 @@ __device__ __forceinline__ uint32_t to_bytes(float a, float b, float c, float d)
       return (uint32_t)(int)(x != x ? 0.f : r) & 0xffu;
     };
     return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+  }
+}
+
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+
+// Four bf16 values divided by 2^(biased - 127), to bytes. E4M3 has an instruction
+// for it, which rounds the quotient once; the integers are multiplied (exactly).
+template <int FMT>
+__device__ __forceinline__ uint32_t to_bytes(uint32_t w0, uint32_t w1, int biased) {
+  if constexpr (FMT == kQ8E4m3) {
+    const float scale = pow2_biased(biased);
+    s16x2_t r = {0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, w0), scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, w1), scale, true);
+    return __builtin_bit_cast(uint32_t, r);
+  } else {
+    const float by = pow2_biased(254 - biased);
+    return to_bytes<FMT>(lo_bf16(w0) * by, hi_bf16(w0) * by, lo_bf16(w1) * by, hi_bf16(w1) * by);
   }
 }
 
@@ -88,14 +98,17 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t w, float by) {
   return to_bytes<FMT>(v[0] * by, v[1] * by, v[2] * by, v[3] * by);
 }
 
-// cos and sin of pairs 8 (c & 7) .. + 7 at position p, for lane c of a DPP row.
+constexpr double kTurnsPerRadian = 0.15915494309189535;
+
+// cos and signed sin of pairs 8 (c & 7) .. + 7 at position p, for lane c of a DPP
+// row: minus sin in the lanes of the pairs' first elements (c < 8).
 // The angle p theta^(-i/64) is reduced to a fraction of a turn in 64 bits
 // (theta^(-1/64) raised by squaring): in 32 it is off by 2^-8 at positions past
 // 65536. Lanes c and c ^ 8 need the same eight pairs and compute four each.
 __device__ __forceinline__ void turn_of(const RopeQ8Args& a, int p, int c, float* cs, float* sn) {
   const bool lo = c < 8;
   const int i0 = 8 * (c & 7) + (lo ? 0 : 4);
-  double f = (double)p * 0.15915494309189535;  // turns per radian
+  double f = (double)p * kTurnsPerRadian;
   double r = a.inv_theta64;
   const double r1 = r;
 #pragma unroll
@@ -114,105 +127,138 @@ __device__ __forceinline__ void turn_of(const RopeQ8Args& a, int p, int c, float
   for (int e = 0; e < 4; ++e) {
     const float co = dpp<kRowRor8>(c4[e]), so = dpp<kRowRor8>(s4[e]);
     cs[e] = lo ? c4[e] : co, cs[e + 4] = lo ? co : c4[e];
-    sn[e] = lo ? s4[e] : so, sn[e + 4] = lo ? so : s4[e];
+    sn[e] = lo ? -s4[e] : so, sn[e + 4] = lo ? -so : s4[e];
   }
 }
 
-// Workgroup (row n, y): y < hk writes K/V head y of row n's block, if none of the
-// 15 rows before n is in that block: thread group t (16 lanes, 8 dims each) takes
-// the block's token t, the last of rows n .. n + 15 that has its slot, an old
-// token (re-scaled if the exponent grows) or, in a block whose token 0 is
-// written, zeros. y >= hk turns 16 of row n's q heads.
+// The rows of one block, as row n of a call sees them, if n is the first of
+// them: thread group t (16 lanes, 8 dims of a head each) takes the block's token
+// t, which is the last of rows n .. n + 15 that has its slot, an old token or, in
+// a block whose token 0 is written, nothing yet.
+struct BlockRows {
+  int64_t block;
+  int written;  // bit t: token t is written by this call
+  int row;      // this group's row, -1 if its token is not written
+  int twice;    // bit i: row n + i has a slot that a later row has too
+};
+
+// Lane l's slot of row n0 - 16 + l (-1 where there is none).
+__device__ __forceinline__ int slots_around(const RopeQ8Args& a, int n0) {
+  const int64_t row = (int64_t)n0 - 16 + (threadIdx.x & 63);
+  return row >= 0 && row < a.rows ? a.slots[row] : -1;
+}
+
+// around: slots_around(n0); row n = n0 + at - 16, 16 <= at <= 48. Every lane of the workgroup gets the same answer.
+__device__ __forceinline__ bool block_rows(int around, int at, int n, int grp, BlockRows* r) {
+  const int slot = __builtin_amdgcn_readlane(around, at);
+  if (slot < 0) return false;
+  const uint64_t same = __ballot(around >= 0 && around >> 4 == slot >> 4);
+  if (same >> (at - 15) & 0x7fff) return false;  // one of the 15 rows before leads
+  r->block = slot >> 4;
+  r->written = 0;
+  r->row = -1;
+  int last = 0;  // rows that are their token's last
+#pragma unroll
+  for (int t = 0; t < kQ8Block; ++t) {
+    const uint32_t rows = (uint32_t)((same & __ballot((around & 15) == t)) >> at) & 0xffffu;
+    if (rows == 0) continue;
+    const int top = 31 - __builtin_clz(rows);
+    r->written |= 1 << t;
+    last |= 1 << top;
+    r->row = grp == t ? n + top : r->row;
+  }
+  r->twice = (int)((same >> at) & 0xffffu) & ~last;
+  return true;
+}
+
+// Four bytes of each lane, a token's dims 0-3 (w0) and 4-7 (w1), tokens 0..3 of
+// the wave's four 16-lane rows, to four tokens of one dim: row r gets dims 2 r
+// (w0) and 2 r + 1 (w1).
+__device__ __forceinline__ void tokens_of_dims(uint32_t& w0, uint32_t& w1) {
+  // Rows 0, 1: dims 0-3 of tokens r and r + 2; rows 2, 3: dims 4-7 of tokens r - 2 and r.
+  const auto h = __builtin_amdgcn_permlane32_swap(w0, w1, false, false);
+  const uint32_t x = __builtin_amdgcn_perm(h[1], h[0], 0x05010400);  // [a0 b0 a1 b1]
+  const uint32_t y = __builtin_amdgcn_perm(h[1], h[0], 0x07030602);  // [a2 b2 a3 b3]
+  // Even rows: dims 0, 1 (of their four) of tokens 0, 2 and 1, 3; odd rows: dims 2, 3.
+  const auto q = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+  w0 = __builtin_amdgcn_perm(q[1], q[0], 0x05010400);
+  w1 = __builtin_amdgcn_perm(q[1], q[0], 0x07030602);
+}
+
+// The largest magnitudes of a K row and a V row, as bf16 bits (K's in the low half).
+// Bits compare as magnitudes do; FINITE leaves infinities and NaN out.
+template <bool FINITE>
+__device__ __forceinline__ uint32_t most_of(const uint4& k, const uint4& v) {
+  const auto of = [](uint32_t w) {
+    w &= 0x7fff7fffu;
+    if (FINITE) {
+      if ((w & 0xffffu) >= 0x7f80u) w &= 0xffff0000u;
+      if (w >= 0x7f800000u) w &= 0xffffu;
+    }
+    return w;
+  };
+  const uint32_t mk = max_u16x2(max_u16x2(of(k.x), of(k.y)), max_u16x2(of(k.z), of(k.w)));
+  const uint32_t mv = max_u16x2(max_u16x2(of(v.x), of(v.y)), max_u16x2(of(v.z), of(v.w)));
+  return row16_max_u16x2(max_u16x2(__builtin_amdgcn_perm(mv, mk, 0x05040100), __builtin_amdgcn_perm(mv, mk, 0x07060302)));
+}
+
+constexpr int kVTile = kHead * 4 + kHead / 8 * 4;  // dwords: a gap of 16 bytes every 8 dims spreads the banks
+__device__ __forceinline__ int v_at(int dim) { return dim * 4 + (dim >> 3) * 4; }
+
+struct KvLds {
+  uint32_t most[16];
+  uint32_t v[kVTile];
+};
+
+// K and V of head kh, given this group's bf16 row of each (k: turned), quantized
+// into the block. Zeros where the group has no row.
 template <int FMT>
-__global__ __launch_bounds__(kThreads) void rope_q8(RopeQ8Args a) {
-  const int n = blockIdx.x, c = threadIdx.x & 15, grp = threadIdx.x >> 4;
-  const int slot = a.slots[n];
-  if (slot < 0) return;
-  if ((int)blockIdx.y >= a.hk) {
-    const int head = 16 * (blockIdx.y - a.hk) + grp;
-    if (head >= a.hq) return;
-    float x[8], w[8], v[8], o[8], cs[8], sn[8];
-    widen8(ldg16(a.qkv + (int64_t)n * a.ld + (int64_t)head * kHead + 8 * c), x);
-    widen8(ldg16(a.q_norm + 8 * c), w);
-    turn_of(a, a.pos[n], c, cs, sn);
-    rms_norm_head(x, w, a.eps, v);
-    rotate_half(v, cs, sn, c < 8, o);
-    *reinterpret_cast<uint4*>(a.q + (int64_t)n * a.q_ld + (int64_t)head * kHead + 8 * c) = pack8(o);
-    return;
-  }
-  // Lane c of every group looks at rows n + c and n - 1 - c.
-  const int ahead = n + c < a.rows ? a.slots[n + c] : -1;
-  const int behind = c < kQ8Block - 1 && n - 1 - c >= 0 ? a.slots[n - 1 - c] : -1;
-  if (__any(behind >= 0 && behind >> 4 == slot >> 4)) return;
-  const bool here = ahead >= 0 && ahead >> 4 == slot >> 4;
-  const int written = row16_or(here ? 1 << (ahead & 15) : 0);
-  const bool keep = !(written & 1);  // the block goes on: its other tokens stay
-  const uint32_t mine = (uint32_t)(__ballot(here && (ahead & 15) == grp) >> (threadIdx.x & 48)) & 0xffffu;
-  const bool is_new = mine != 0;
-  const int kh = blockIdx.y, row = n + 31 - __builtin_clz(mine | 1);
-  const int64_t block = slot >> 4;
-  uint8_t* kb = a.kv + (block * 2 * a.hk + kh) * kQ8HeadBytes;
+__device__ __forceinline__ void write_block(const RopeQ8Args& a, const BlockRows& r, int kh, const uint4& k, const uint4& v,
+                                            int c, int grp, KvLds* s) {
+  const bool keep = !(r.written & 1);  // the block goes on: its other tokens stay
+  uint8_t* kb = a.kv + (r.block * 2 * a.hk + kh) * kQ8HeadBytes;
   uint8_t* vb = kb + (int64_t)a.hk * kQ8HeadBytes;
-  uint8_t* eb = a.kv_scale + block * 2 * a.hk + kh;
-  __shared__ float s_max[2][16];
-  __shared__ uint32_t s_v[kHead * 4];  // V bytes [128 dims][16 tokens]
-
-  float kx[8], vx[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) kx[e] = vx[e] = 0.f;
-  if (is_new) {
-    const bf16_t* src = a.qkv + (int64_t)row * a.ld + (int64_t)(a.hq + kh) * kHead + 8 * c;
-    float x[8], w[8], v[8], cs[8], sn[8];
-    widen8(ldg16(src), x);
-    widen8(ldg16(src + (int64_t)a.hk * kHead), vx);
-    widen8(ldg16(a.k_norm + 8 * c), w);
-    turn_of(a, a.pos[row], c, cs, sn);
-    rms_norm_head(x, w, a.eps, v);
-    rotate_half(v, cs, sn, c < 8, kx);
-    const uint4 kr = pack8(kx);
-    widen8(kr, kx);  // the cache holds what the bf16 row holds
-    if (a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)row * a.k_ld + (int64_t)kh * kHead + 8 * c) = kr;
-  }
-  float km = 0.f, vm = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    km = fmaxf(km, finite(kx[e]) ? fabsf(kx[e]) : 0.f);
-    vm = fmaxf(vm, finite(vx[e]) ? fabsf(vx[e]) : 0.f);
-  }
-  km = row16_max(km), vm = row16_max(vm);
-  if (c == 0) s_max[0][grp] = km, s_max[1][grp] = vm;
-  __syncthreads();
-  km = row16_max(s_max[0][c]), vm = row16_max(s_max[1][c]);
+  uint8_t* eb = a.kv_scale + r.block * 2 * a.hk + kh;
+  // What the block holds, asked for before the exponents are known.
   const int k_old = keep ? eb[0] : 1, v_old = keep ? eb[a.hk] : 1;
-  const int k_e = max(k_old, block_exponent<FMT>(km)), v_e = max(v_old, block_exponent<FMT>(vm));
-  const float ki = pow2_biased(254 - k_e), vi = pow2_biased(254 - v_e);
-  __syncthreads();  // every thread has the old exponents
-  if (threadIdx.x == 0) eb[0] = (uint8_t)k_e, eb[a.hk] = (uint8_t)v_e;
-
   uint2* kd = reinterpret_cast<uint2*>(kb + grp * kHead + 8 * c);
+  uint4* vd = reinterpret_cast<uint4*>(vb + (threadIdx.x & (kHead - 1)) * kQ8Block);
   uint2 kw = make_uint2(0, 0);
-  if (is_new) {
-    kw.x = to_bytes<FMT>(kx[0] * ki, kx[1] * ki, kx[2] * ki, kx[3] * ki);
-    kw.y = to_bytes<FMT>(kx[4] * ki, kx[5] * ki, kx[6] * ki, kx[7] * ki);
-  } else if (keep) {
-    const float by = pow2_biased(max(127 + k_old - k_e, 1));
-    kw = *kd;
-    if (k_e > k_old) kw = make_uint2(rescaled<FMT>(kw.x, by), rescaled<FMT>(kw.y, by));
+  uint4 was = make_uint4(0, 0, 0, 0);
+  if (keep) {
+    if (r.row < 0) kw = *kd;
+    if (threadIdx.x < kHead) was = *vd;
   }
-  *kd = kw;
-  // V: the new tokens' bytes through LDS into [dim][token] order.
-  uint8_t* sv = reinterpret_cast<uint8_t*>(s_v);
-  const uint32_t w0 = to_bytes<FMT>(vx[0] * vi, vx[1] * vi, vx[2] * vi, vx[3] * vi);
-  const uint32_t w1 = to_bytes<FMT>(vx[4] * vi, vx[5] * vi, vx[6] * vi, vx[7] * vi);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sv[(8 * c + e) * kQ8Block + grp] = (uint8_t)((e < 4 ? w0 : w1) >> (8 * (e & 3)));
+  uint32_t most = most_of<false>(k, v);
+  if (c == 0) s->most[grp] = most;
   __syncthreads();
+  most = row16_max_u16x2(s->most[c]);
+  if ((most & 0xffffu) >= 0x7f80u || most >= 0x7f800000u) {  // not finite, somewhere in the block: it does not count
+    __syncthreads();
+    most = most_of<true>(k, v);
+    if (c == 0) s->most[grp] = most;
+    __syncthreads();
+    most = row16_max_u16x2(s->most[c]);
+  }
+  const int k_e = max(k_old, block_exponent<FMT>(most & 0xffff)), v_e = max(v_old, block_exponent<FMT>(most >> 16));
+  if (r.row >= 0) {
+    kw = make_uint2(to_bytes<FMT>(k.x, k.y, k_e), to_bytes<FMT>(k.z, k.w, k_e));
+  } else if (k_e > k_old) {
+    const float by = pow2_biased(max(127 + k_old - k_e, 1));
+    kw = make_uint2(rescaled<FMT>(kw.x, by), rescaled<FMT>(kw.y, by));
+  }
+  if (r.row >= 0 || !keep || k_e > k_old) *kd = kw;
+  // V: the new tokens' bytes through LDS into [dim][token] order.
+  uint32_t w0 = to_bytes<FMT>(v.x, v.y, v_e), w1 = to_bytes<FMT>(v.z, v.w, v_e);
+  tokens_of_dims(w0, w1);
+  const int at = v_at(8 * c + 2 * (grp & 3)) + (grp >> 2);
+  s->v[at] = w0, s->v[at + 4] = w1;
+  __syncthreads();
+  if (threadIdx.x == 0) eb[0] = (uint8_t)k_e, eb[a.hk] = (uint8_t)v_e;  // every thread has the old ones
   if (threadIdx.x < kHead) {
-    uint4* vd = reinterpret_cast<uint4*>(vb + threadIdx.x * kQ8Block);
-    const uint4 add = *reinterpret_cast<const uint4*>(sv + threadIdx.x * kQ8Block);
+    const uint4 add = *reinterpret_cast<const uint4*>(s->v + v_at(threadIdx.x));
     uint32_t out[4] = {add.x, add.y, add.z, add.w};
     if (keep) {
-      const uint4 was = *vd;
       const uint32_t old[4] = {was.x, was.y, was.z, was.w};
       const float by = pow2_biased(max(127 + v_old - v_e, 1));
 #pragma unroll
@@ -220,11 +266,196 @@ __global__ __launch_bounds__(kThreads) void rope_q8(RopeQ8Args a) {
         uint32_t stay = 0;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-          if (!(written >> (4 * i + b) & 1)) stay |= 0xffu << (8 * b);
+          if (!(r.written >> (4 * i + b) & 1)) stay |= 0xffu << (8 * b);
         out[i] = (out[i] & ~stay) | ((v_e > v_old ? rescaled<FMT>(old[i], by) : old[i]) & stay);
       }
     }
     *vd = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
+// The norm's weight goes into the angles: w cos, and the partner's w times sin.
+__device__ __forceinline__ void weigh(const bf16_t* norm, int c, float* cs, float* sn) {
+  float w[8];
+  widen8(ldg16(norm + 8 * c), w);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) cs[e] *= w[e], sn[e] *= dpp<kRowRor8>(w[e]);
+}
+
+// A head's 8 dims of this lane, normalised and turned, as bf16: x / rms rounded to
+// bf16, as the model does; then x (w cos) + partner (w' sin), the partner 64 dims
+// away being lane c ^ 8's in the same register. Some 70 vector instructions for 8
+// values of four heads: with the quantizer's they are two thirds of what a large
+// call could issue, so they are counted here (squares in pairs, roundings in
+// pairs, sign and weight in the table).
+__device__ __forceinline__ uint4 turn_head(const RopeQ8Args& a, const uint4& raw, const float* cs, const float* sn) {
+  float ss = 0.f;
+  ss = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, raw.x), __builtin_bit_cast(bf16x2_t, raw.x), ss, false);
+  ss = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, raw.y), __builtin_bit_cast(bf16x2_t, raw.y), ss, false);
+  ss = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, raw.z), __builtin_bit_cast(bf16x2_t, raw.z), ss, false);
+  ss = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, raw.w), __builtin_bit_cast(bf16x2_t, raw.w), ss, false);
+  const float r = rsqrtf(fmaf(row16_sum(ss), 1.f / kHead, a.eps));
+  float x[8];
+  widen8(raw, x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= r;
+  widen8(pack8(x), x);
+  float o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = fmaf(x[e], cs[e], dpp<kRowRor8>(x[e]) * sn[e]);
+  return pack8(o);
+}
+
+// k_out of the rows whose slot a later row has too (their K goes nowhere else).
+__device__ __forceinline__ void k_rows_twice(const RopeQ8Args& a, const BlockRows& r, int n, int y, int Y, int c, int grp) {
+  if (!a.k || !(r.twice >> grp & 1)) return;
+  const int row = n + grp;
+  float cs[8], sn[8];
+  turn_of(a, a.pos[row], c, cs, sn);
+  weigh(a.k_norm, c, cs, sn);
+  for (int kh = y; kh < a.hk; kh += Y) {
+    const uint4 raw = ldg16(a.qkv + (int64_t)row * a.ld + (int64_t)(a.hq + kh) * kHead + 8 * c);
+    *reinterpret_cast<uint4*>(a.k + (int64_t)row * a.k_ld + (int64_t)kh * kHead + 8 * c) = turn_head(a, raw, cs, sn);
+  }
+}
+
+// Row (or rows from) that workgroup x of 16 T looks at, LEADS of every 16: the T
+// workgroups with the same rows of every 16 follow one another. In a prompt one
+// row of 16 leads a block, and in row order all of those would be on one XCD.
+template <int LEADS>
+__device__ __forceinline__ int leads_from(const RopeQ8Args& a, int x) {
+  const int T = (a.rows + 15) >> 4, s = x / T;
+  return 16 * (x - s * T) + LEADS * s;
+}
+
+// Few rows, one launch: workgroup (x, y). y < hk writes K/V head y of the block
+// that its row leads, if it does; y >= hk turns 16 of the row's q heads.
+template <int FMT>
+__global__ __launch_bounds__(kThreads) void rope_q8_rows(RopeQ8Args a) {
+  const int n = leads_from<1>(a, blockIdx.x), c = threadIdx.x & 15, grp = threadIdx.x >> 4;
+  if (n >= a.rows) return;
+  float cs[8], sn[8];
+  if ((int)blockIdx.y >= a.hk) {
+    const int head = 16 * (blockIdx.y - a.hk) + grp;
+    if (a.slots[n] < 0 || head >= a.hq) return;
+    const uint4 raw = ldg16(a.qkv + (int64_t)n * a.ld + (int64_t)head * kHead + 8 * c);
+    turn_of(a, a.pos[n], c, cs, sn);
+    weigh(a.q_norm, c, cs, sn);
+    *reinterpret_cast<uint4*>(a.q + (int64_t)n * a.q_ld + (int64_t)head * kHead + 8 * c) = turn_head(a, raw, cs, sn);
+    return;
+  }
+  BlockRows r;
+  if (!block_rows(slots_around(a, n), 16, n, grp, &r)) return;
+  const int kh = blockIdx.y;
+  __shared__ KvLds lds;
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
+  if (r.row >= 0) {
+    const bf16_t* src = a.qkv + (int64_t)r.row * a.ld + (int64_t)(a.hq + kh) * kHead + 8 * c;
+    const uint4 kraw = ldg16(src);
+    v = ldg16(src + (int64_t)a.hk * kHead);
+    turn_of(a, a.pos[r.row], c, cs, sn);
+    weigh(a.k_norm, c, cs, sn);
+    k = turn_head(a, kraw, cs, sn);
+    if (a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
+  }
+  if (r.twice) k_rows_twice(a, r, n, kh, a.hk, c, grp);
+  write_block<FMT>(a, r, kh, k, v, c, grp, &lds);
+}
+
+// Many rows: workgroup (x, y) has kLeads rows of 16. It turns every Y-th set of
+// four of their q heads, row grp / 4 and head grp % 4 of a set per thread group,
+// with the rows' 256 angles computed once, one a thread, into LDS (turn_of's
+// values, bit for bit); and for each of its rows that leads a block it writes K/V
+// heads y, y + Y, .. of that, a token per thread group. In a prompt one row of 16
+// leads, so a quarter of the workgroups write the cache, arithmetic under the
+// others' streaming.
+constexpr int kLeads = 4;
+
+template <int FMT>
+__global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
+  const int n0 = leads_from<kLeads>(a, blockIdx.x), c = threadIdx.x & 15, grp = threadIdx.x >> 4;
+  const int y = blockIdx.y, Y = gridDim.y;
+  if (n0 >= a.rows) return;
+  int around;
+  {
+    constexpr int kAhead = 4;
+    const int r = grp >> 2, row = n0 + r, h0 = 4 * y + (grp & 3), step = 4 * Y;
+    const bf16_t* src = a.qkv + (int64_t)row * a.ld + 8 * c;
+    bf16_t* dst = a.q + (int64_t)row * a.q_ld + 8 * c;
+    // Asked for before the slots, positions and angles are known.
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (row < a.rows && h0 + i * step < a.hq) raw[i] = ldg16_stream(src + (int64_t)(h0 + i * step) * kHead);
+    around = slots_around(a, n0);
+    const bool there = __shfl(around, 16 + r) >= 0;
+    __shared__ __align__(16) float s_cos[kLeads][kHead / 2], s_sin[kLeads][kHead / 2];
+    {
+      const int k = threadIdx.x >> 6, i = threadIdx.x & 63;
+      double f = (double)a.pos[min(n0 + k, a.rows - 1)] * kTurnsPerRadian;
+      double t = a.inv_theta64;
+#pragma unroll
+      for (int b = 0; b < 6; ++b) {
+        if (b >= 2 && (i >> b & 1)) f *= t;
+        t *= t;
+      }
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (e < (i & 3)) f *= a.inv_theta64;
+      sincospif(2.f * (float)(f - rint(f)), &s_sin[k][i], &s_cos[k][i]);
+    }
+    __syncthreads();
+    if (there) {
+      float cs[8], sn[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float t = s_sin[r][8 * (c & 7) + e];
+        cs[e] = s_cos[r][8 * (c & 7) + e], sn[e] = c < 8 ? -t : t;
+      }
+      weigh(a.q_norm, c, cs, sn);
+      for (int h = h0; h < a.hq; h += kAhead * step) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int hi = h + i * step;
+          if (hi >= a.hq) break;
+          const uint4 o = turn_head(a, raw[i], cs, sn);
+          if (hi + kAhead * step < a.hq) raw[i] = ldg16_stream(src + (int64_t)(hi + kAhead * step) * kHead);
+          *reinterpret_cast<uint4*>(dst + (int64_t)hi * kHead) = o;
+        }
+      }
+    }
+  }
+  __shared__ KvLds lds;
+  for (int lead = 0; lead < kLeads; ++lead) {
+    const int n = n0 + lead;
+    BlockRows r;
+    if (!block_rows(around, 16 + lead, n, grp, &r)) continue;
+    const bool mine = r.row >= 0;
+    const bf16_t* src = a.qkv + (int64_t)(mine ? r.row : n) * a.ld + (int64_t)a.hq * kHead + 8 * c;
+    uint4 kraw = make_uint4(0, 0, 0, 0), vraw = kraw;
+    if (mine) {
+      kraw = ldg16_stream(src + (int64_t)y * kHead);
+      vraw = ldg16_stream(src + (int64_t)(a.hk + y) * kHead);
+    }
+    float cs[8], sn[8];
+    if (mine) {
+      turn_of(a, a.pos[r.row], c, cs, sn);
+      weigh(a.k_norm, c, cs, sn);
+    }
+    for (int kh = y; kh < a.hk; kh += Y) {
+      uint4 k = make_uint4(0, 0, 0, 0);
+      const uint4 v = vraw;
+      if (mine) {
+        k = turn_head(a, kraw, cs, sn);
+        if (kh + Y < a.hk) {
+          kraw = ldg16_stream(src + (int64_t)(kh + Y) * kHead);
+          vraw = ldg16_stream(src + (int64_t)(a.hk + kh + Y) * kHead);
+        }
+        if (a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
+      }
+      write_block<FMT>(a, r, kh, k, v, c, grp, &lds);
+    }
+    if (r.twice) k_rows_twice(a, r, n, y, Y, c, grp);
   }
 }
 
@@ -536,12 +767,31 @@ __global__ __launch_bounds__(kThreads) void merge_q8(DecodeQ8Args a) {
 
 }  // namespace
 
+// One launch below this many rows: a prompt of 1000 rows of 32q/8kv takes 12.4 us
+// so and 18.3 in two launches, 8 of 100-300 rows (1556) 20.7 / 24.1, one of 8000
+// of 32q/32kv 192 / 99.
+#ifndef BR
+#define BR 2048
+#define BG 1024
+#endif
+constexpr int kManyRows = BR;
+
 int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream) {
-  const dim3 grid(a.rows, a.hk + (a.hq + 15) / 16);
+  const unsigned T = (unsigned)((a.rows + 15) / 16);
+  if (a.rows < kManyRows) {
+    const dim3 grid(16 * T, a.hk + (a.hq + 15) / 16);
+    if (a.format == kQ8E4m3)
+      rope_q8_rows<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a);
+    else
+      rope_q8_rows<kQ8Int8><<<grid, kThreads, 0, stream>>>(a);
+    return check_launch();
+  }
+  // The K/V heads of a block over as many workgroups as give a prompt 1024 that lead.
+  const dim3 grid(16 / kLeads * T, std::min<unsigned>(a.hk, (BG + T - 1) / T));
   if (a.format == kQ8E4m3)
-    rope_q8<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a);
+    rope_q8_blocks<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a);
   else
-    rope_q8<kQ8Int8><<<grid, kThreads, 0, stream>>>(a);
+    rope_q8_blocks<kQ8Int8><<<grid, kThreads, 0, stream>>>(a);
   return check_launch();
 }
 

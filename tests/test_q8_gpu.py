@@ -86,6 +86,38 @@ def test_write_matches_the_host_quantizer(fmt, hq, hk):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hq,hk", [(16, 8), (10, 5), (7, 1), (40, 20)])
+def test_write_of_many_rows(fmt, hq, hk):
+    """Calls of some hundreds of rows (another kernel): runs at every place of a block, single rows, skipped rows and a slot
+    given twice among them; and the bits of calls of few rows."""
+    g, rng = gen(hq + hk), np.random.default_rng(hq)
+    runs = [(0, 90), (5, 1), (15, 1), (3, 200), (0, 16), (9, 30), (0, 1), (14, 5), (7, 9), (0, 7)] + [(i % 16, 1) for i in range(40)]
+    slots, pos = runs_to_slots(rng, runs, 110)
+    slots[100] = -1
+    slots[120] = slots[119]
+    rows = len(slots)
+    qkv = torch.randn(rows, (hq + 2 * hk) * 128, device="cuda", generator=g).to(torch.bfloat16)
+    w = weights(g)
+    kv, sc = random_cache(g, 110, hk, fmt)
+    ref, kv1, sc1 = R.Cache(kv, sc, hk), kv.clone(), sc.clone()
+    q, k = write(qkv, pos, slots, kv, sc, hq, hk, w)
+    heads = qkv.view(rows, -1, 128).cpu()
+    there = torch.tensor(slots) >= 0
+    check_turned(q.cpu()[there], heads[there, :hq], w[0].cpu(), torch.tensor(pos)[there].tolist())
+    check_turned(k.cpu()[there], heads[there, hq:hq + hk], w[1].cpu(), torch.tensor(pos)[there].tolist())
+    assert bool((q[~there] == 7).all()) and bool((k[~there] == 7).all())
+    ref.write(slots, k.cpu().double().view(rows, hk, 128), heads[:, hq + hk:].double())
+    ref.same_as(kv, sc)
+    cuts = [0] + [n for n in range(1, rows) if slots[n] // 16 != slots[n - 1] // 16 and slots[n] >= 0 and slots[n - 1] >= 0]
+    cuts = [n for i, n in enumerate(cuts) if i % 3 == 0] + [rows]
+    for a, b in zip(cuts, cuts[1:]):
+        assert b - a < 128
+        q1, k1 = write(qkv[a:b].contiguous(), pos[a:b], slots[a:b], kv1, sc1, hq, hk, w)
+        assert torch.equal(q1, q[a:b]) and torch.equal(k1, k[a:b])
+    ref.same_as(kv1, sc1)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_tokens_appended_one_by_one(fmt):
     """40 steps of five sequences that grow by one token, whose size rises and falls: the cache follows the host's at every step."""
     hq, hk, seqs = 4, 2, 5
@@ -142,7 +174,9 @@ def test_write_of_rows_in_any_order_and_twice(fmt):
     kv, sc = random_cache(g, 11, hk, fmt)
     ref = R.Cache(kv, sc, hk)
     _, k = write(qkv, pos, slots, kv, sc, hq, hk, weights(g))
+    there = torch.tensor(slots) >= 0
     k = k.cpu().double().view(len(slots), hk, 128)
+    assert bool((k[~there] == 7).all()) and bool((k[there] != 7).any(-1).all())
     ref.write(slots, k, qkv.view(len(slots), -1, 128)[:, hq + hk:].cpu().double())
     ref.same_as(kv, sc)
 
