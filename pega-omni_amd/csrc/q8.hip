@@ -362,69 +362,20 @@ __global__ __launch_bounds__(kThreads) void rope_q8_rows(RopeQ8Args a) {
   write_block<FMT>(a, r, kh, k, v, c, grp, &lds);
 }
 
-// Many rows: workgroup (x, y) has kLeads rows of 16. It turns every Y-th set of
-// four of their q heads, row grp / 4 and head grp % 4 of a set per thread group,
-// with the rows' 256 angles computed once, one a thread, into LDS (turn_of's
-// values, bit for bit); and for each of its rows that leads a block it writes K/V
-// heads y, y + Y, .. of that, a token per thread group. In a prompt one row of 16
-// leads, so a quarter of the workgroups write the cache, arithmetic under the
-// others' streaming.
+// Many rows, the cache: workgroup (x, y) looks at kLeads rows of 16, and for each
+// that leads a block writes K/V heads y, y + Y, .. of it, a token per thread
+// group, its angles computed once, two heads' loads ahead. In a prompt one row of
+// 16 leads; of single rows each does, so a workgroup looks at no more than four.
+// (With one row per workgroup, of 25,850 rows of 12 prompts the workgroups that
+// end at once took some 50 us.)
 constexpr int kLeads = 4;
 
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
+  constexpr int kAhead = 2;
   const int n0 = leads_from<kLeads>(a, blockIdx.x), c = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const int y = blockIdx.y, Y = gridDim.y;
-  if (n0 >= a.rows) return;
-  int around;
-  {
-    constexpr int kAhead = 4;
-    const int r = grp >> 2, row = n0 + r, h0 = 4 * y + (grp & 3), step = 4 * Y;
-    const bf16_t* src = a.qkv + (int64_t)row * a.ld + 8 * c;
-    bf16_t* dst = a.q + (int64_t)row * a.q_ld + 8 * c;
-    // Asked for before the slots, positions and angles are known.
-    uint4 raw[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (row < a.rows && h0 + i * step < a.hq) raw[i] = ldg16_stream(src + (int64_t)(h0 + i * step) * kHead);
-    around = slots_around(a, n0);
-    const bool there = __shfl(around, 16 + r) >= 0;
-    __shared__ __align__(16) float s_cos[kLeads][kHead / 2], s_sin[kLeads][kHead / 2];
-    {
-      const int k = threadIdx.x >> 6, i = threadIdx.x & 63;
-      double f = (double)a.pos[min(n0 + k, a.rows - 1)] * kTurnsPerRadian;
-      double t = a.inv_theta64;
-#pragma unroll
-      for (int b = 0; b < 6; ++b) {
-        if (b >= 2 && (i >> b & 1)) f *= t;
-        t *= t;
-      }
-#pragma unroll
-      for (int e = 0; e < 3; ++e)
-        if (e < (i & 3)) f *= a.inv_theta64;
-      sincospif(2.f * (float)(f - rint(f)), &s_sin[k][i], &s_cos[k][i]);
-    }
-    __syncthreads();
-    if (there) {
-      float cs[8], sn[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float t = s_sin[r][8 * (c & 7) + e];
-        cs[e] = s_cos[r][8 * (c & 7) + e], sn[e] = c < 8 ? -t : t;
-      }
-      weigh(a.q_norm, c, cs, sn);
-      for (int h = h0; h < a.hq; h += kAhead * step) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int hi = h + i * step;
-          if (hi >= a.hq) break;
-          const uint4 o = turn_head(a, raw[i], cs, sn);
-          if (hi + kAhead * step < a.hq) raw[i] = ldg16_stream(src + (int64_t)(hi + kAhead * step) * kHead);
-          *reinterpret_cast<uint4*>(dst + (int64_t)hi * kHead) = o;
-        }
-      }
-    }
-  }
+  const int around = slots_around(a, n0);
   __shared__ KvLds lds;
   for (int lead = 0; lead < kLeads; ++lead) {
     const int n = n0 + lead;
@@ -432,31 +383,81 @@ __global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
     if (!block_rows(around, 16 + lead, n, grp, &r)) continue;
     const bool mine = r.row >= 0;
     const bf16_t* src = a.qkv + (int64_t)(mine ? r.row : n) * a.ld + (int64_t)a.hq * kHead + 8 * c;
-    uint4 kraw = make_uint4(0, 0, 0, 0), vraw = kraw;
-    if (mine) {
-      kraw = ldg16_stream(src + (int64_t)y * kHead);
-      vraw = ldg16_stream(src + (int64_t)(a.hk + y) * kHead);
-    }
+    uint4 kraw[kAhead], vraw[kAhead];
+    const auto load = [&](int i, int kh) __attribute__((always_inline)) {
+      kraw[i] = vraw[i] = make_uint4(0, 0, 0, 0);
+      if (mine && kh < a.hk) {
+        kraw[i] = ldg16_stream(src + (int64_t)kh * kHead);
+        vraw[i] = ldg16_stream(src + (int64_t)(a.hk + kh) * kHead);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(i, y + i * Y);
     float cs[8], sn[8];
     if (mine) {
       turn_of(a, a.pos[r.row], c, cs, sn);
       weigh(a.k_norm, c, cs, sn);
     }
-    for (int kh = y; kh < a.hk; kh += Y) {
-      uint4 k = make_uint4(0, 0, 0, 0);
-      const uint4 v = vraw;
-      if (mine) {
-        k = turn_head(a, kraw, cs, sn);
-        if (kh + Y < a.hk) {
-          kraw = ldg16_stream(src + (int64_t)(kh + Y) * kHead);
-          vraw = ldg16_stream(src + (int64_t)(a.hk + kh + Y) * kHead);
-        }
-        if (a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
+    for (int k0 = y; k0 < a.hk; k0 += kAhead * Y) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int kh = k0 + i * Y;
+        if (kh >= a.hk) break;
+        uint4 k = make_uint4(0, 0, 0, 0);
+        const uint4 v = vraw[i];
+        if (mine) k = turn_head(a, kraw[i], cs, sn);
+        load(i, kh + kAhead * Y);
+        if (mine && a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
+        write_block<FMT>(a, r, kh, k, v, c, grp, &lds);
       }
-      write_block<FMT>(a, r, kh, k, v, c, grp, &lds);
     }
     if (r.twice) k_rows_twice(a, r, n, y, Y, c, grp);
   }
+}
+
+// Many rows, q: one workgroup per row (2, 4, 8 or 16 rows of at most 8, 4, 2 or 1
+// heads), a head per thread group. Up to kAhead heads of a group are asked for
+// before the rows' angles are computed, 64 of them a row, once, into LDS:
+// turn_of's values, bit for bit.
+__global__ __launch_bounds__(kThreads) void turn_q_rows(RopeQ8Args a, int rows_shift) {
+  constexpr int kAhead = 4;
+  const int c = threadIdx.x & 15, grp = threadIdx.x >> 4, per = 16 >> rows_shift;  // heads at a time
+  const int n0 = blockIdx.x << rows_shift, row = n0 + grp / per, h0 = grp & (per - 1);
+  const bf16_t* src = a.qkv + (int64_t)row * a.ld + 8 * c;
+  bf16_t* dst = a.q + (int64_t)row * a.q_ld + 8 * c;
+  uint4 raw[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (row < a.rows && h0 + i * per < a.hq) raw[i] = ldg16_stream(src + (int64_t)(h0 + i * per) * kHead);
+  __shared__ __align__(16) float s_cos[16][kHead / 2], s_sin[16][kHead / 2];
+  for (int t = threadIdx.x; t < (kHead / 2) << rows_shift; t += kThreads) {
+    const int i = t & (kHead / 2 - 1), k = t / (kHead / 2);
+    double f = (double)a.pos[min(n0 + k, a.rows - 1)] * kTurnsPerRadian;
+    double r = a.inv_theta64;
+#pragma unroll
+    for (int b = 0; b < 6; ++b) {
+      if (b >= 2 && (i >> b & 1)) f *= r;
+      r *= r;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < (i & 3)) f *= a.inv_theta64;
+    sincospif(2.f * (float)(f - rint(f)), &s_sin[k][i], &s_cos[k][i]);
+  }
+  __syncthreads();
+  if (row >= a.rows || a.slots[row] < 0) return;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = s_sin[grp / per][8 * (c & 7) + e];
+    cs[e] = s_cos[grp / per][8 * (c & 7) + e], sn[e] = c < 8 ? -t : t;
+  }
+  weigh(a.q_norm, c, cs, sn);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (h0 + i * per < a.hq) *reinterpret_cast<uint4*>(dst + (int64_t)(h0 + i * per) * kHead) = turn_head(a, raw[i], cs, sn);
+  for (int h = h0 + kAhead * per; h < a.hq; h += per)
+    *reinterpret_cast<uint4*>(dst + (int64_t)h * kHead) = turn_head(a, ldg16_stream(src + (int64_t)h * kHead), cs, sn);
 }
 
 // ------------------------------------------------------------------- decode
@@ -767,14 +768,10 @@ __global__ __launch_bounds__(kThreads) void merge_q8(DecodeQ8Args a) {
 
 }  // namespace
 
-// One launch below this many rows: a prompt of 1000 rows of 32q/8kv takes 12.4 us
-// so and 18.3 in two launches, 8 of 100-300 rows (1556) 20.7 / 24.1, one of 8000
-// of 32q/32kv 192 / 99.
-#ifndef BR
-#define BR 2048
-#define BG 1024
-#endif
-constexpr int kManyRows = BR;
+// One launch below this many rows, two from there: 1000 rows of a prompt of
+// 32q/8kv take 11.8 us in one and 17 in two, 8 of 100-300 rows (1556) 19.5 / 24,
+// 8000 rows of 32q/32kv 192 / 93.
+constexpr int kManyRows = 2048;
 
 int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream) {
   const unsigned T = (unsigned)((a.rows + 15) / 16);
@@ -787,11 +784,15 @@ int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream) {
     return check_launch();
   }
   // The K/V heads of a block over as many workgroups as give a prompt 1024 that lead.
-  const dim3 grid(16 / kLeads * T, std::min<unsigned>(a.hk, (BG + T - 1) / T));
+  const dim3 grid(16 / kLeads * T, std::min<unsigned>(a.hk, (1024 + T - 1) / T));
   if (a.format == kQ8E4m3)
     rope_q8_blocks<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a);
   else
     rope_q8_blocks<kQ8Int8><<<grid, kThreads, 0, stream>>>(a);
+  if (check_launch() != 0) return -3;
+  int shift = 0;
+  while (shift < 4 && (16 >> (shift + 1)) >= a.hq) ++shift;
+  turn_q_rows<<<dim3((unsigned)(((int64_t)a.rows + (1 << shift) - 1) >> shift)), kThreads, 0, stream>>>(a, shift);
   return check_launch();
 }
 
