@@ -100,6 +100,20 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t w, float by) {
 
 constexpr double kTurnsPerRadian = 0.15915494309189535;
 
+// sin and cos of f turns, |f| below 2^29. The nearest quarter turn goes in 64
+// bits, so that the rest keeps f32's relative precision (a fraction of a whole
+// turn rounded to f32 was off by 2e-7 radians, and a third of the bf16 values of
+// K and q that differ from a 64-bit computation's differed for it).
+__device__ __forceinline__ void sincos_turns(double f, float* sn, float* cs) {
+  const double k = rint(4. * f);
+  float s, c;
+  sincospif(2.f * (float)fma(-0.25, k, f), &s, &c);
+  const int q = (int)k;
+  const float s1 = q & 1 ? c : s, c1 = q & 1 ? s : c;
+  *sn = q & 2 ? -s1 : s1;
+  *cs = (q + 1) & 2 ? -c1 : c1;
+}
+
 // cos and signed sin of pairs 8 (c & 7) .. + 7 at position p, for lane c of a DPP
 // row: minus sin in the lanes of the pairs' first elements (c < 8).
 // The angle p theta^(-i/64) is reduced to a fraction of a turn in 64 bits
@@ -119,8 +133,7 @@ __device__ __forceinline__ void turn_of(const RopeQ8Args& a, int p, int c, float
   float c4[4], s4[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float t = (float)(f - rint(f));
-    sincospif(2.f * t, &s4[e], &c4[e]);
+    sincos_turns(f, &s4[e], &c4[e]);
     f *= r1;
   }
 #pragma unroll
@@ -274,32 +287,30 @@ __device__ __forceinline__ void write_block(const RopeQ8Args& a, const BlockRows
   }
 }
 
-// The norm's weight goes into the angles: w cos, and the partner's w times sin.
-__device__ __forceinline__ void weigh(const bf16_t* norm, int c, float* cs, float* sn) {
-  float w[8];
-  widen8(ldg16(norm + 8 * c), w);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) cs[e] *= w[e], sn[e] *= dpp<kRowRor8>(w[e]);
+// 1 / sqrt(v) to half a step: the instruction's value and a Newton step.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float r = rsqrtf(v);
+  return fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
+}
+
+__device__ __forceinline__ float dot2(uint32_t a, float sum) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, a), __builtin_bit_cast(bf16x2_t, a), sum, false);
 }
 
 // A head's 8 dims of this lane, normalised and turned, as bf16: x / rms rounded to
-// bf16, as the model does; then x (w cos) + partner (w' sin), the partner 64 dims
-// away being lane c ^ 8's in the same register. Some 70 vector instructions for 8
-// values of four heads: with the quantizer's they are two thirds of what a large
-// call could issue, so they are counted here (squares in pairs, roundings in
-// pairs, sign and weight in the table).
-__device__ __forceinline__ uint4 turn_head(const RopeQ8Args& a, const uint4& raw, const float* cs, const float* sn) {
-  float ss = 0.f;
-  ss = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, raw.x), __builtin_bit_cast(bf16x2_t, raw.x), ss, false);
-  ss = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, raw.y), __builtin_bit_cast(bf16x2_t, raw.y), ss, false);
-  ss = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, raw.z), __builtin_bit_cast(bf16x2_t, raw.z), ss, false);
-  ss = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, raw.w), __builtin_bit_cast(bf16x2_t, raw.w), ss, false);
-  const float r = rsqrtf(fmaf(row16_sum(ss), 1.f / kHead, a.eps));
+// bf16, as the model does, times the weight (exact in f32); then x cos + partner
+// sin, the partner 64 dims away being lane c ^ 8's in the same register.
+__device__ __forceinline__ uint4 turn_head(const RopeQ8Args& a, const uint4& raw, const float* w, const float* cs,
+                                           const float* sn) {
+  const float ss = dot2(raw.x, dot2(raw.y, dot2(raw.z, dot2(raw.w, 0.f))));
+  const float r = inv_sqrt(fmaf(row16_sum(ss), 1.f / kHead, a.eps));
   float x[8];
   widen8(raw, x);
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] *= r;
   widen8(pack8(x), x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= w[e];
   float o[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = fmaf(x[e], cs[e], dpp<kRowRor8>(x[e]) * sn[e]);
@@ -310,12 +321,12 @@ __device__ __forceinline__ uint4 turn_head(const RopeQ8Args& a, const uint4& raw
 __device__ __forceinline__ void k_rows_twice(const RopeQ8Args& a, const BlockRows& r, int n, int y, int Y, int c, int grp) {
   if (!a.k || !(r.twice >> grp & 1)) return;
   const int row = n + grp;
-  float cs[8], sn[8];
+  float cs[8], sn[8], w[8];
   turn_of(a, a.pos[row], c, cs, sn);
-  weigh(a.k_norm, c, cs, sn);
+  widen8(ldg16(a.k_norm + 8 * c), w);
   for (int kh = y; kh < a.hk; kh += Y) {
     const uint4 raw = ldg16(a.qkv + (int64_t)row * a.ld + (int64_t)(a.hq + kh) * kHead + 8 * c);
-    *reinterpret_cast<uint4*>(a.k + (int64_t)row * a.k_ld + (int64_t)kh * kHead + 8 * c) = turn_head(a, raw, cs, sn);
+    *reinterpret_cast<uint4*>(a.k + (int64_t)row * a.k_ld + (int64_t)kh * kHead + 8 * c) = turn_head(a, raw, w, cs, sn);
   }
 }
 
@@ -334,14 +345,14 @@ template <int FMT>
 __global__ __launch_bounds__(kThreads) void rope_q8_rows(RopeQ8Args a) {
   const int n = leads_from<1>(a, blockIdx.x), c = threadIdx.x & 15, grp = threadIdx.x >> 4;
   if (n >= a.rows) return;
-  float cs[8], sn[8];
+  float cs[8], sn[8], w[8];
   if ((int)blockIdx.y >= a.hk) {
     const int head = 16 * (blockIdx.y - a.hk) + grp;
     if (a.slots[n] < 0 || head >= a.hq) return;
     const uint4 raw = ldg16(a.qkv + (int64_t)n * a.ld + (int64_t)head * kHead + 8 * c);
     turn_of(a, a.pos[n], c, cs, sn);
-    weigh(a.q_norm, c, cs, sn);
-    *reinterpret_cast<uint4*>(a.q + (int64_t)n * a.q_ld + (int64_t)head * kHead + 8 * c) = turn_head(a, raw, cs, sn);
+    widen8(ldg16(a.q_norm + 8 * c), w);
+    *reinterpret_cast<uint4*>(a.q + (int64_t)n * a.q_ld + (int64_t)head * kHead + 8 * c) = turn_head(a, raw, w, cs, sn);
     return;
   }
   BlockRows r;
@@ -354,8 +365,8 @@ __global__ __launch_bounds__(kThreads) void rope_q8_rows(RopeQ8Args a) {
     const uint4 kraw = ldg16(src);
     v = ldg16(src + (int64_t)a.hk * kHead);
     turn_of(a, a.pos[r.row], c, cs, sn);
-    weigh(a.k_norm, c, cs, sn);
-    k = turn_head(a, kraw, cs, sn);
+    widen8(ldg16(a.k_norm + 8 * c), w);
+    k = turn_head(a, kraw, w, cs, sn);
     if (a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
   }
   if (r.twice) k_rows_twice(a, r, n, kh, a.hk, c, grp);
@@ -393,10 +404,10 @@ __global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
     };
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) load(i, y + i * Y);
-    float cs[8], sn[8];
+    float cs[8], sn[8], w[8];
     if (mine) {
       turn_of(a, a.pos[r.row], c, cs, sn);
-      weigh(a.k_norm, c, cs, sn);
+      widen8(ldg16(a.k_norm + 8 * c), w);
     }
     for (int k0 = y; k0 < a.hk; k0 += kAhead * Y) {
 #pragma unroll
@@ -405,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
         if (kh >= a.hk) break;
         uint4 k = make_uint4(0, 0, 0, 0);
         const uint4 v = vraw[i];
-        if (mine) k = turn_head(a, kraw[i], cs, sn);
+        if (mine) k = turn_head(a, kraw[i], w, cs, sn);
         load(i, kh + kAhead * Y);
         if (mine && a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
         write_block<FMT>(a, r, kh, k, v, c, grp, &lds);
@@ -442,22 +453,22 @@ __global__ __launch_bounds__(kThreads) void turn_q_rows(RopeQ8Args a, int rows_s
 #pragma unroll
     for (int e = 0; e < 3; ++e)
       if (e < (i & 3)) f *= a.inv_theta64;
-    sincospif(2.f * (float)(f - rint(f)), &s_sin[k][i], &s_cos[k][i]);
+    sincos_turns(f, &s_sin[k][i], &s_cos[k][i]);
   }
   __syncthreads();
   if (row >= a.rows || a.slots[row] < 0) return;
-  float cs[8], sn[8];
+  float cs[8], sn[8], w[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float t = s_sin[grp / per][8 * (c & 7) + e];
     cs[e] = s_cos[grp / per][8 * (c & 7) + e], sn[e] = c < 8 ? -t : t;
   }
-  weigh(a.q_norm, c, cs, sn);
+  widen8(ldg16(a.q_norm + 8 * c), w);
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
-    if (h0 + i * per < a.hq) *reinterpret_cast<uint4*>(dst + (int64_t)(h0 + i * per) * kHead) = turn_head(a, raw[i], cs, sn);
+    if (h0 + i * per < a.hq) *reinterpret_cast<uint4*>(dst + (int64_t)(h0 + i * per) * kHead) = turn_head(a, raw[i], w, cs, sn);
   for (int h = h0 + kAhead * per; h < a.hq; h += per)
-    *reinterpret_cast<uint4*>(dst + (int64_t)h * kHead) = turn_head(a, ldg16_stream(src + (int64_t)h * kHead), cs, sn);
+    *reinterpret_cast<uint4*>(dst + (int64_t)h * kHead) = turn_head(a, ldg16_stream(src + (int64_t)h * kHead), w, cs, sn);
 }
 
 // ------------------------------------------------------------------- decode
