@@ -25,12 +25,16 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
 }
 template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_max_u16x2(uint32_t v) {
-  return max_u16x2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
+__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
 }
-// The larger of each half over the 16 lanes of a DPP row.
-__device__ __forceinline__ uint32_t row16_max_u16x2(uint32_t v) {
-  return dpp_max_u16x2<kRowMirror>(dpp_max_u16x2<kRowHalfMirror>(dpp_max_u16x2<kQuadSwap2>(dpp_max_u16x2<kQuadSwap1>(v))));
+// The larger of each over the 16 lanes of a DPP row (side by side: a DPP read waits
+// for the write before it).
+__device__ __forceinline__ void row16_max2(uint32_t& a, uint32_t& b) {
+  a = dpp_max_u32<kQuadSwap1>(a), b = dpp_max_u32<kQuadSwap1>(b);
+  a = dpp_max_u32<kQuadSwap2>(a), b = dpp_max_u32<kQuadSwap2>(b);
+  a = dpp_max_u32<kRowHalfMirror>(a), b = dpp_max_u32<kRowHalfMirror>(b);
+  a = dpp_max_u32<kRowMirror>(a), b = dpp_max_u32<kRowMirror>(b);
 }
 
 // 2^(biased - 127) for 1 <= biased <= 254.
@@ -103,15 +107,18 @@ constexpr double kTurnsPerRadian = 0.15915494309189535;
 // sin and cos of f turns, |f| below 2^29. The nearest quarter turn goes in 64
 // bits, so that the rest keeps f32's relative precision (a fraction of a whole
 // turn rounded to f32 was off by 2e-7 radians, and a third of the bf16 values of
-// K and q that differ from a 64-bit computation's differed for it).
+// K and q that differ from a 64-bit computation's differed for it). The rest, x
+// of at most pi / 4, takes the Taylor series to x^9 and x^10, whose next terms
+// are below 2e-9: a third of the instructions of the library's call.
 __device__ __forceinline__ void sincos_turns(double f, float* sn, float* cs) {
   const double k = rint(4. * f);
-  float s, c;
-  sincospif(2.f * (float)fma(-0.25, k, f), &s, &c);
+  const float x = (float)(fma(-0.25, k, f) * 6.283185307179586), y = x * x;
+  const float s = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
+  const float c = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
   const int q = (int)k;
   const float s1 = q & 1 ? c : s, c1 = q & 1 ? s : c;
-  *sn = q & 2 ? -s1 : s1;
-  *cs = (q + 1) & 2 ? -c1 : c1;
+  *sn = __int_as_float(__float_as_int(s1) ^ (q & 2) << 30);
+  *cs = __int_as_float(__float_as_int(c1) ^ (q + 1 & 2) << 30);
 }
 
 // cos and signed sin of pairs 8 (c & 7) .. + 7 at position p, for lane c of a DPP
@@ -163,6 +170,7 @@ __device__ __forceinline__ int slots_around(const RopeQ8Args& a, int n0) {
 
 // around: slots_around(n0); row n = n0 + at - 16, 16 <= at <= 48. Every lane of the workgroup gets the same answer.
 __device__ __forceinline__ bool block_rows(int around, int at, int n, int grp, BlockRows* r) {
+  asm("" : "+v"(around));  // the 16 comparisons below are made here: kept over a loop of rows they spill
   const int slot = __builtin_amdgcn_readlane(around, at);
   if (slot < 0) return false;
   const uint64_t same = __ballot(around >= 0 && around >> 4 == slot >> 4);
@@ -198,10 +206,10 @@ __device__ __forceinline__ void tokens_of_dims(uint32_t& w0, uint32_t& w1) {
   w1 = __builtin_amdgcn_perm(q[1], q[0], 0x07030602);
 }
 
-// The largest magnitudes of a K row and a V row, as bf16 bits (K's in the low half).
-// Bits compare as magnitudes do; FINITE leaves infinities and NaN out.
+// The largest magnitude of eight bf16 values of a lane, as bf16 bits. Bits compare
+// as magnitudes do; FINITE leaves infinities and NaN out.
 template <bool FINITE>
-__device__ __forceinline__ uint32_t most_of(const uint4& k, const uint4& v) {
+__device__ __forceinline__ uint32_t most_of(const uint4& x) {
   const auto of = [](uint32_t w) {
     w &= 0x7fff7fffu;
     if (FINITE) {
@@ -210,80 +218,109 @@ __device__ __forceinline__ uint32_t most_of(const uint4& k, const uint4& v) {
     }
     return w;
   };
-  const uint32_t mk = max_u16x2(max_u16x2(of(k.x), of(k.y)), max_u16x2(of(k.z), of(k.w)));
-  const uint32_t mv = max_u16x2(max_u16x2(of(v.x), of(v.y)), max_u16x2(of(v.z), of(v.w)));
-  return row16_max_u16x2(max_u16x2(__builtin_amdgcn_perm(mv, mk, 0x05040100), __builtin_amdgcn_perm(mv, mk, 0x07060302)));
+  const uint32_t m = max_u16x2(max_u16x2(of(x.x), of(x.y)), max_u16x2(of(x.z), of(x.w)));
+  return max(m & 0xffffu, m >> 16);
 }
 
 constexpr int kVTile = kHead * 4 + kHead / 8 * 4;  // dwords: a gap of 16 bytes every 8 dims spreads the banks
 __device__ __forceinline__ int v_at(int dim) { return dim * 4 + (dim >> 3) * 4; }
 
 struct KvLds {
-  uint32_t most[16];
+  uint2 most[16];
   uint32_t v[kVTile];
 };
 
-// K and V of head kh, given this group's bf16 row of each (k: turned), quantized
-// into the block. Zeros where the group has no row.
-template <int FMT>
-__device__ __forceinline__ void write_block(const RopeQ8Args& a, const BlockRows& r, int kh, const uint4& k, const uint4& v,
-                                            int c, int grp, KvLds* s) {
+// K and V of H heads at once (kh, kh + step, ..; those below hk), given this
+// group's bf16 row of each (k: turned), quantized into the block. Zeros where the
+// group has no row. Two barriers for all of them, which is what a head waits for:
+// of 12 prompts of 25,850 rows the cache's part takes 58 us with one head at a
+// time, 51 with two, 63 with four (registers).
+template <int FMT, int H>
+__device__ __forceinline__ void write_block(const RopeQ8Args& a, const BlockRows& r, int kh, int step, const uint4* k,
+                                            const uint4* v, int c, int grp, KvLds* s) {
   const bool keep = !(r.written & 1);  // the block goes on: its other tokens stay
   uint8_t* kb = a.kv + (r.block * 2 * a.hk + kh) * kQ8HeadBytes;
-  uint8_t* vb = kb + (int64_t)a.hk * kQ8HeadBytes;
   uint8_t* eb = a.kv_scale + r.block * 2 * a.hk + kh;
+  const int64_t to_v = (int64_t)a.hk * kQ8HeadBytes, next = (int64_t)step * kQ8HeadBytes;
+  const int k_at = grp * kHead + 8 * c, v_at_byte = (threadIdx.x & (kHead - 1)) * kQ8Block;
   // What the block holds, asked for before the exponents are known.
-  const int k_old = keep ? eb[0] : 1, v_old = keep ? eb[a.hk] : 1;
-  uint2* kd = reinterpret_cast<uint2*>(kb + grp * kHead + 8 * c);
-  uint4* vd = reinterpret_cast<uint4*>(vb + (threadIdx.x & (kHead - 1)) * kQ8Block);
-  uint2 kw = make_uint2(0, 0);
-  uint4 was = make_uint4(0, 0, 0, 0);
-  if (keep) {
-    if (r.row < 0) kw = *kd;
-    if (threadIdx.x < kHead) was = *vd;
-  }
-  uint32_t most = most_of<false>(k, v);
-  if (c == 0) s->most[grp] = most;
-  __syncthreads();
-  most = row16_max_u16x2(s->most[c]);
-  if ((most & 0xffffu) >= 0x7f80u || most >= 0x7f800000u) {  // not finite, somewhere in the block: it does not count
-    __syncthreads();
-    most = most_of<true>(k, v);
-    if (c == 0) s->most[grp] = most;
-    __syncthreads();
-    most = row16_max_u16x2(s->most[c]);
-  }
-  const int k_e = max(k_old, block_exponent<FMT>(most & 0xffff)), v_e = max(v_old, block_exponent<FMT>(most >> 16));
-  if (r.row >= 0) {
-    kw = make_uint2(to_bytes<FMT>(k.x, k.y, k_e), to_bytes<FMT>(k.z, k.w, k_e));
-  } else if (k_e > k_old) {
-    const float by = pow2_biased(max(127 + k_old - k_e, 1));
-    kw = make_uint2(rescaled<FMT>(kw.x, by), rescaled<FMT>(kw.y, by));
-  }
-  if (r.row >= 0 || !keep || k_e > k_old) *kd = kw;
-  // V: the new tokens' bytes through LDS into [dim][token] order.
-  uint32_t w0 = to_bytes<FMT>(v.x, v.y, v_e), w1 = to_bytes<FMT>(v.z, v.w, v_e);
-  tokens_of_dims(w0, w1);
-  const int at = v_at(8 * c + 2 * (grp & 3)) + (grp >> 2);
-  s->v[at] = w0, s->v[at + 4] = w1;
-  __syncthreads();
-  if (threadIdx.x == 0) eb[0] = (uint8_t)k_e, eb[a.hk] = (uint8_t)v_e;  // every thread has the old ones
-  if (threadIdx.x < kHead) {
-    const uint4 add = *reinterpret_cast<const uint4*>(s->v + v_at(threadIdx.x));
-    uint32_t out[4] = {add.x, add.y, add.z, add.w};
-    if (keep) {
-      const uint32_t old[4] = {was.x, was.y, was.z, was.w};
-      const float by = pow2_biased(max(127 + v_old - v_e, 1));
+  int k_old[H], v_old[H];
+  uint2 kw[H];
+  uint4 was[H];
+  uint32_t km[H], vm[H];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t stay = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          if (!(r.written >> (4 * i + b) & 1)) stay |= 0xffu << (8 * b);
-        out[i] = (out[i] & ~stay) | ((v_e > v_old ? rescaled<FMT>(old[i], by) : old[i]) & stay);
-      }
+  for (int h = 0; h < H; ++h) {
+    k_old[h] = v_old[h] = 1;
+    kw[h] = make_uint2(0, 0), was[h] = make_uint4(0, 0, 0, 0);
+    if (keep && kh + h * step < a.hk) {
+      k_old[h] = eb[h * step], v_old[h] = eb[h * step + a.hk];
+      if (r.row < 0) kw[h] = *reinterpret_cast<const uint2*>(kb + h * next + k_at);
+      if (threadIdx.x < kHead) was[h] = *reinterpret_cast<const uint4*>(kb + h * next + to_v + v_at_byte);
     }
-    *vd = make_uint4(out[0], out[1], out[2], out[3]);
+    km[h] = most_of<false>(k[h]), vm[h] = most_of<false>(v[h]);
+  }
+  const auto of_block = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      row16_max2(km[h], vm[h]);
+      if (c == 0) s[h].most[grp] = make_uint2(km[h], vm[h]);
+    }
+    __syncthreads();
+    uint32_t top = 0;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      km[h] = s[h].most[c].x, vm[h] = s[h].most[c].y;
+      row16_max2(km[h], vm[h]);
+      top = max(top, max(km[h], vm[h]));
+    }
+    return top;
+  };
+  if (of_block() >= 0x7f80u) {  // not finite, somewhere in the blocks: it does not count
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < H; ++h) km[h] = most_of<true>(k[h]), vm[h] = most_of<true>(v[h]);
+    of_block();
+  }
+  int k_e[H], v_e[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    k_e[h] = max(k_old[h], block_exponent<FMT>(km[h])), v_e[h] = max(v_old[h], block_exponent<FMT>(vm[h]));
+    // V: the new tokens' bytes through LDS into [dim][token] order.
+    uint32_t w0 = to_bytes<FMT>(v[h].x, v[h].y, v_e[h]), w1 = to_bytes<FMT>(v[h].z, v[h].w, v_e[h]);
+    tokens_of_dims(w0, w1);
+    const int at = v_at(8 * c + 2 * (grp & 3)) + (grp >> 2);
+    s[h].v[at] = w0, s[h].v[at + 4] = w1;
+    if (r.row >= 0) {
+      kw[h] = make_uint2(to_bytes<FMT>(k[h].x, k[h].y, k_e[h]), to_bytes<FMT>(k[h].z, k[h].w, k_e[h]));
+    } else if (k_e[h] > k_old[h]) {
+      const float by = pow2_biased(max(127 + k_old[h] - k_e[h], 1));
+      kw[h] = make_uint2(rescaled<FMT>(kw[h].x, by), rescaled<FMT>(kw[h].y, by));
+    }
+    if (kh + h * step < a.hk && (r.row >= 0 || !keep || k_e[h] > k_old[h]))
+      *reinterpret_cast<uint2*>(kb + h * next + k_at) = kw[h];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    if (kh + h * step >= a.hk) break;
+    if (threadIdx.x == 0) eb[h * step] = (uint8_t)k_e[h], eb[h * step + a.hk] = (uint8_t)v_e[h];  // every thread has the old ones
+    if (threadIdx.x < kHead) {
+      const uint4 add = *reinterpret_cast<const uint4*>(s[h].v + v_at(threadIdx.x));
+      uint32_t out[4] = {add.x, add.y, add.z, add.w};
+      if (keep) {
+        const uint32_t old[4] = {was[h].x, was[h].y, was[h].z, was[h].w};
+        const float by = pow2_biased(max(127 + v_old[h] - v_e[h], 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t stay = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (!(r.written >> (4 * i + b) & 1)) stay |= 0xffu << (8 * b);
+          out[i] = (out[i] & ~stay) | ((v_e[h] > v_old[h] ? rescaled<FMT>(old[i], by) : old[i]) & stay);
+        }
+      }
+      *reinterpret_cast<uint4*>(kb + h * next + to_v + v_at_byte) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
   }
 }
 
@@ -370,31 +407,30 @@ __global__ __launch_bounds__(kThreads) void rope_q8_rows(RopeQ8Args a) {
     if (a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
   }
   if (r.twice) k_rows_twice(a, r, n, kh, a.hk, c, grp);
-  write_block<FMT>(a, r, kh, k, v, c, grp, &lds);
+  write_block<FMT, 1>(a, r, kh, a.hk, &k, &v, c, grp, &lds);
 }
 
 // Many rows, the cache: workgroup (x, y) looks at kLeads rows of 16, and for each
 // that leads a block writes K/V heads y, y + Y, .. of it, a token per thread
-// group, its angles computed once, two heads' loads ahead. In a prompt one row of
+// group, its angles computed once, kAtOnce heads at a time. In a prompt one row of
 // 16 leads; of single rows each does, so a workgroup looks at no more than four.
 // (With one row per workgroup, of 25,850 rows of 12 prompts the workgroups that
 // end at once took some 50 us.)
-constexpr int kLeads = 4;
+constexpr int kLeads = 4, kAtOnce = 2;
 
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
-  constexpr int kAhead = 2;
   const int n0 = leads_from<kLeads>(a, blockIdx.x), c = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const int y = blockIdx.y, Y = gridDim.y;
   const int around = slots_around(a, n0);
-  __shared__ KvLds lds;
+  __shared__ KvLds lds[kAtOnce];
   for (int lead = 0; lead < kLeads; ++lead) {
     const int n = n0 + lead;
     BlockRows r;
     if (!block_rows(around, 16 + lead, n, grp, &r)) continue;
     const bool mine = r.row >= 0;
     const bf16_t* src = a.qkv + (int64_t)(mine ? r.row : n) * a.ld + (int64_t)a.hq * kHead + 8 * c;
-    uint4 kraw[kAhead], vraw[kAhead];
+    uint4 kraw[kAtOnce], vraw[kAtOnce];
     const auto load = [&](int i, int kh) __attribute__((always_inline)) {
       kraw[i] = vraw[i] = make_uint4(0, 0, 0, 0);
       if (mine && kh < a.hk) {
@@ -403,24 +439,25 @@ __global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
       }
     };
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(i, y + i * Y);
+    for (int i = 0; i < kAtOnce; ++i) load(i, y + i * Y);
     float cs[8], sn[8], w[8];
     if (mine) {
       turn_of(a, a.pos[r.row], c, cs, sn);
       widen8(ldg16(a.k_norm + 8 * c), w);
     }
-    for (int k0 = y; k0 < a.hk; k0 += kAhead * Y) {
+    for (int kh = y; kh < a.hk; kh += kAtOnce * Y) {
+      uint4 k[kAtOnce], v[kAtOnce];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int kh = k0 + i * Y;
-        if (kh >= a.hk) break;
-        uint4 k = make_uint4(0, 0, 0, 0);
-        const uint4 v = vraw[i];
-        if (mine) k = turn_head(a, kraw[i], w, cs, sn);
-        load(i, kh + kAhead * Y);
-        if (mine && a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
-        write_block<FMT>(a, r, kh, k, v, c, grp, &lds);
+      for (int i = 0; i < kAtOnce; ++i) {
+        k[i] = make_uint4(0, 0, 0, 0), v[i] = vraw[i];
+        if (mine) k[i] = turn_head(a, kraw[i], w, cs, sn);
+        load(i, kh + (kAtOnce + i) * Y);
       }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i)
+        if (mine && a.k && kh + i * Y < a.hk)
+          *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)(kh + i * Y) * kHead + 8 * c) = k[i];
+      write_block<FMT, kAtOnce>(a, r, kh, Y, k, v, c, grp, lds);
     }
     if (r.twice) k_rows_twice(a, r, n, y, Y, c, grp);
   }
