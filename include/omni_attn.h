@@ -396,7 +396,8 @@ int64_t omni_hidream_workspace_bytes(void);
 #define OMNI_ATTN_TABLES_EXHAUSTED 5 /* fewer free pages than the step needs */
 /* The lowest that applies. Sequences of a call have different lines (a done
  * request's line is free from the next call on), and the table's and the
- * queue's page ids are the caller's to keep in the pool. */
+ * queue's page ids are the caller's to keep in the pool. Calls that share a
+ * table or a queue follow one another on a stream. */
 int omni_attn_step_tables(const int32_t* first, const int32_t* count, const int32_t* lines, int nseq, int page, int ring,
                           int32_t* table, int64_t table_ld, int num_lines, int32_t* free_pages, int num_pages,
                           const int32_t* free_state, int row_cap, int page_cap, int32_t* pos, int32_t* slots,
@@ -432,7 +433,9 @@ int omni_attn_decode_plan_init_q8(int rows, int hq, int hk, int page, int max_le
 /* omni_qwen3_attend over the 8-bit cache: row n of sequence s = ragged ? seq[n] :
  * n sees keys 0..pos[n]; a row with pos[n] < 0 stores zeros (seq[n] is not
  * read). q rows [hq][128] of stride q_stride (a multiple of 8). P is carried in
- * 16 bits or more. Tokens past pos[n] may hold anything. */
+ * 16 bits. Tokens past pos[n] may hold anything, and pages past its last are not
+ * looked at. A workspace serves one call at a time: two captured graphs that may
+ * run at once need one each. */
 int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const void* kv_scale, int format,
                          const int32_t* pos, const int32_t* seq, int ragged, const int32_t* indptr, const int32_t* pages,
                          int page, void* out, int hq, int hk, float scale, const omni_attn_decode_plan* plan,
@@ -460,7 +463,10 @@ int omni_attn_prompt_plan_init(int nseq, const int32_t* lens_h, int hq, int hk, 
  * [hq][128], k and v rows [hk][128], at strides that are multiples of 8 elements
  * (k and v at most 2^22): parts of one qkv row, or buffers of their own. out
  * rows [hq][128]; rows past the plan's are left as they were. A row's bits
- * depend on its own prompt alone. */
+ * depend on its own prompt alone, and what another prompt holds never reaches
+ * it; of its own prompt, an infinity or NaN in a later V row does where the two
+ * share a tile of 128 keys (a masked key weighs 0, and 0 times those is NaN).
+ * `work` is the device copy of this plan's work list. */
 int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64_t q_stride, const void* k,
                          int64_t k_stride, const void* v, int64_t v_stride, void* out, float scale, const int32_t* work,
                          void* stream);

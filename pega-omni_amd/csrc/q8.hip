@@ -104,7 +104,7 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t w, float by) {
 
 constexpr double kTurnsPerRadian = 0.15915494309189535;
 
-// sin and cos of f turns, |f| below 2^29. The nearest quarter turn goes in 64
+// sin and cos of f turns. The nearest quarter turn goes in 64
 // bits, so that the rest keeps f32's relative precision (a fraction of a whole
 // turn rounded to f32 was off by 2e-7 radians, and a third of the bf16 values of
 // K and q that differ from a 64-bit computation's differed for it). The rest, x
@@ -115,7 +115,7 @@ __device__ __forceinline__ void sincos_turns(double f, float* sn, float* cs) {
   const float x = (float)(fma(-0.25, k, f) * 6.283185307179586), y = x * x;
   const float s = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
   const float c = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
-  const int q = (int)k;
+  const int q = (int)(4. * __builtin_amdgcn_fract(0.25 * k));  // k modulo 4
   const float s1 = q & 1 ? c : s, c1 = q & 1 ? s : c;
   *sn = __int_as_float(__float_as_int(s1) ^ (q & 2) << 30);
   *cs = __int_as_float(__float_as_int(c1) ^ (q + 1 & 2) << 30);
@@ -324,10 +324,11 @@ __device__ __forceinline__ void write_block(const RopeQ8Args& a, const BlockRows
   }
 }
 
-// 1 / sqrt(v) to half a step: the instruction's value and a Newton step.
+// 1 / sqrt(v) to half a step: the instruction's value and a Newton step (which
+// would make NaN of 1 / sqrt(infinity)).
 __device__ __forceinline__ float inv_sqrt(float v) {
   const float r = rsqrtf(v);
-  return fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
+  return v < INFINITY ? fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r) : r;
 }
 
 __device__ __forceinline__ float dot2(uint32_t a, float sum) {
@@ -517,7 +518,7 @@ constexpr int kIds = 64 / (kTile / kQ8Block);  // tiles whose blocks a wave look
 // Keys per split of a row of len keys: the plan's, or more where a row is
 // longer than the plan's bound (multiples of 64 keys, as the plan's).
 __device__ __forceinline__ int split_len_of(const DecodeQ8Args& a, int len) {
-  return max(a.chunk, ((len + a.splits - 1) / a.splits + 63) / 64 * 64);
+  return max(a.chunk, ((len - 1) / a.splits + 64) / 64 * 64);
 }
 
 // rotated_split evens out the splits over the XCDs; but an XCD hands its

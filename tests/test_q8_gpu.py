@@ -209,8 +209,9 @@ def test_write_in_place_strided_and_without_k():
         assert torch.equal(rows_in[:, :64], wide[:, :64]) and torch.equal(rows_in[:, -8:], wide[:, -8:])
 
 
-@pytest.mark.parametrize("theta", [1e4, 1e6, 5e6])
+@pytest.mark.parametrize("theta", [0.5, 1.0, 1e4, 1e6, 5e6])
 def test_far_positions(theta):
+    """2^31 positions of a turn that theta below 1 speeds up leave 2^-20 of the f64 angle."""
     hq, hk = 4, 1
     pos = [0, 1, 40959, 65537, 1 << 20, (1 << 24) + 1, (1 << 30) + 12345, (1 << 31) - 2]
     g = gen(6)
@@ -221,6 +222,18 @@ def test_far_positions(theta):
     heads = qkv.view(8, -1, 128).cpu()
     check_turned(q, heads[:, :hq], w[0].cpu(), pos, theta)
     check_turned(k, heads[:, hq:hq + 1], w[1].cpu(), pos, theta)
+
+
+def test_heads_of_zeros_and_of_overflowing_squares():
+    """A head of zeros stays zero (eps keeps 1 / rms finite); where the f32 sum of squares overflows, 1 / rms is 0 and so is the head."""
+    hq, hk = 2, 1
+    qkv = torch.randn(3, 4 * 128, device="cuda", generator=gen(2)).to(torch.bfloat16)
+    qkv[0, :128], qkv[1, 128:256], qkv[2, 256:384] = 0, 1e30, 3e38
+    kv, sc = random_cache(gen(2), 3, hk, torch.float8_e4m3fn)
+    q, k = write(qkv, [5, 6, 7], [0, 16, 32], kv, sc, hq, hk, weights(gen(2)))
+    assert bool((q[0, :128] == 0).all()) and bool((q[1, 128:] == 0).all()) and bool((k[2] == 0).all())
+    assert bool(q.isfinite().all()) and bool(k.isfinite().all())
+    assert bool((kv.float()[2, 0] == 0).all()) and int(sc.view(torch.uint8)[2, 0]) == 1
 
 
 # ------------------------------------------------------------------- decode
