@@ -551,6 +551,17 @@ __device__ __forceinline__ bf16x8 bf16_of(uint32_t w0, uint32_t w1) {
 
 __device__ __forceinline__ int from_lane(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane << 2, v); }
 
+// Lanes col < 8 of 16 keep x and take their y from lane col + 8's x; lanes
+// col >= 8 keep y and take their x from lane col - 8's y.
+__device__ __forceinline__ void trade_halves(uint4& x, uint4& y) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int x0 = (int)(&x.x)[w], y0 = (int)(&y.x)[w];
+    (&x.x)[w] = (uint32_t)__builtin_amdgcn_update_dpp(x0, y0, 0x128, 0xf, 0xc, false);
+    (&y.x)[w] = (uint32_t)__builtin_amdgcn_update_dpp(y0, x0, 0x128, 0xf, 0x3, false);
+  }
+}
+
 // The larger of v in the four lanes with the same lane % 16.
 __device__ __forceinline__ float max_of_groups(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -570,7 +581,8 @@ constexpr int kBlocksPerTile = kTile / kQ8Block;
 //     8 (x % 2) + 4 j + r of the tile's block x / 2, so a lane ends with tokens
 //     8 (g % 2) .. + 7 of block g / 2 for its head, in order, which is P^T's
 //     operand as it stands: no data crosses lanes between the two products but
-//     the maximum.
+//     the maximum. K is loaded in whole lines of 128 bytes, eight lanes a key,
+//     and columns n and n + 8 trade halves.
 //   O^T (16 dims x 16 heads) += V^T . P^T: V lies [dim][token] in the cache. A
 //     lane loads the 16 tokens of one dim (groups 2 b and 2 b + 1 two dims of
 //     block b) and the two groups trade halves, which gives each its tokens of
@@ -578,6 +590,15 @@ constexpr int kBlocksPerTile = kTile / kQ8Block;
 // P is carried as two bf16 terms (hi + lo, 16 bits): the matrix cores are a
 // tenth of the time. Both scales act per block, that is per lane: on the scores
 // and, an exact power of two, on P.
+// The cache's bytes bound it, each read once and kept in no cache (loads of K as
+// 64-byte halves of its lines: 269 / 170 us for the first and last of these, with
+// cached loads 266 / 168): 128 rows of 1600 keys of 32 heads (1.68 GB) take 264 us,
+// 6.4 TB/s; 4 of 100,000-130,000 keys of 32q/8kv in 4096-key splits (0.94 GB) 162 with
+// the merge, 5.8; 64 of 200-2400 of 16q/8kv (0.17 GB) 36.8, 4.6, where the longest
+// rows' walks show. Loads alone, nothing computed, took 265 of 272 us when the
+// first stood at that; 64-key tiles, two or three tiles asked for ahead, and
+// two or three workgroups a CU in place of four were no faster. A lone row is
+// bound by latency: 1 row of 8000 keys in 256-key splits takes 10.8 with the merge.
 template <int FMT>
 __global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
   const int kh = blockIdx.y, n = blockIdx.z, G = a.hq / a.hk, tid = threadIdx.x;
@@ -623,12 +644,13 @@ __global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
 
   uint4 kr[2][2], vr[4];
   auto load_k = [&](int k) __attribute__((always_inline)) {
-    const int64_t block = from_lane(ids, 2 * (k & (kIds - 1)) + (col >> 3));
-    const uint8_t* kb = a.kv + (block * row_blocks + kh) * kQ8HeadBytes + (2 * (col & 4) + (col & 3)) * kHead + 16 * grp;
+    const uint8_t* kb = a.kv + kh * kQ8HeadBytes + (2 * (col & 4) + (col & 3)) * kHead + 16 * grp + 8 * (col & 8);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int b = 0; b < 2; ++b) {
+      const int64_t block = __builtin_amdgcn_readlane(ids, 2 * (k & (kIds - 1)) + b);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) kr[j][c] = ldg16(kb + 4 * j * kHead + 64 * c);
+      for (int j = 0; j < 2; ++j) kr[j][b] = ldg16_stream(kb + block * row_blocks * kQ8HeadBytes + 4 * j * kHead);
+    }
   };
   auto load_v = [&](int k) __attribute__((always_inline)) {
     const int64_t block = from_lane(ids, 2 * (k & (kIds - 1)) + (grp >> 1));
@@ -654,6 +676,7 @@ __global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       f32x4 d = {0.f, 0.f, 0.f, 0.f};
+      trade_halves(kr[j][0], kr[j][1]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of<FMT>(kr[j][c].x, kr[j][c].y), q[2 * c], d, 0, 0, 0);
