@@ -37,6 +37,8 @@ __device__ __forceinline__ void row16_max2(uint32_t& a, uint32_t& b) {
   a = dpp_max_u32<kRowMirror>(a), b = dpp_max_u32<kRowMirror>(b);
 }
 
+__device__ __forceinline__ int from_lane(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane << 2, v); }
+
 // 2^(biased - 127) for 1 <= biased <= 254.
 __device__ __forceinline__ float pow2_biased(int biased) { return __int_as_float(biased << 23); }
 
@@ -151,6 +153,33 @@ __device__ __forceinline__ void turn_of(const RopeQ8Args& a, int p, int c, float
   }
 }
 
+// turn_of's values, bit for bit, through LDS: each pair's once for all heads of a row.
+struct TurnLds {
+  float cs[kHead / 2], sn[kHead / 2];
+};
+
+__device__ __forceinline__ void put_turn(const RopeQ8Args& a, int p, int i, TurnLds* s) {
+  double f = (double)p * kTurnsPerRadian;
+  double r = a.inv_theta64;
+#pragma unroll
+  for (int b = 0; b < 6; ++b) {
+    if (b >= 2 && (i >> b & 1)) f *= r;
+    r *= r;
+  }
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < (i & 3)) f *= a.inv_theta64;
+  sincos_turns(f, &s->sn[i], &s->cs[i]);
+}
+
+__device__ __forceinline__ void get_turn(const TurnLds& s, int c, float* cs, float* sn) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = s.sn[8 * (c & 7) + e];
+    cs[e] = s.cs[8 * (c & 7) + e], sn[e] = c < 8 ? -t : t;
+  }
+}
+
 // The rows of one block, as row n of a call sees them, if n is the first of
 // them: thread group t (16 lanes, 8 dims of a head each) takes the block's token
 // t, which is the last of rows n .. n + 15 that has its slot, an old token or, in
@@ -168,6 +197,13 @@ __device__ __forceinline__ int slots_around(const RopeQ8Args& a, int n0) {
   return row >= 0 && row < a.rows ? a.slots[row] : -1;
 }
 
+// Whether row n0 + at - 16 (not skipped) is the only row of its block.
+__device__ __forceinline__ bool is_alone(int around, int at) {
+  const int slot = __builtin_amdgcn_readlane(around, at);
+  const uint64_t same = __ballot(around >= 0 && around >> 4 == slot >> 4);
+  return slot >= 0 && (same >> (at - 15) & 0x7fffffff) == 1 << 15;
+}
+
 // around: slots_around(n0); row n = n0 + at - 16, 16 <= at <= 48. Every lane of the workgroup gets the same answer.
 __device__ __forceinline__ bool block_rows(int around, int at, int n, int grp, BlockRows* r) {
   asm("" : "+v"(around));  // the 16 comparisons below are made here: kept over a loop of rows they spill
@@ -175,6 +211,7 @@ __device__ __forceinline__ bool block_rows(int around, int at, int n, int grp, B
   if (slot < 0) return false;
   const uint64_t same = __ballot(around >= 0 && around >> 4 == slot >> 4);
   if (same >> (at - 15) & 0x7fff) return false;  // one of the 15 rows before leads
+  if ((same >> at & 0xffff) == 1) return false;   // alone
   r->block = slot >> 4;
   r->written = 0;
   r->row = -1;
@@ -368,6 +405,99 @@ __device__ __forceinline__ void k_rows_twice(const RopeQ8Args& a, const BlockRow
   }
 }
 
+// K and V of the only row of its block, by one wave: heads kh0 and kh0 + 1 (the
+// second if there is one), each K in one 16-lane group and V in the next, 8 dims a
+// lane; then all 64 lanes each head's bytes: V whole, as the token is a byte of
+// every dim's 16 (lane l dims l and l + 64), K's other tokens if there is
+// something to change in them. No barrier, and what a workgroup did for a head of
+// one row it does for two heads of four: 64 rows of 16q/8kv 5.0 -> 4.3 us, 512 13.2 ->
+// 7.9 (1.2 -> 2.1 TB/s), 512 of 32q/32kv 46 -> 26, 2200 of 32q/8kv 96 -> 35.
+template <int FMT>
+__device__ __forceinline__ void write_alone(const RopeQ8Args& a, int row, int slot, int kh0, const TurnLds& turn) {
+  const int lane = threadIdx.x & 63, c = lane & 15, head = lane >> 5, token = slot & (kQ8Block - 1);
+  const bool is_v = lane & 16, two = kh0 + 1 < a.hk, mine = head == 0 || two, keep = token != 0;
+  const int64_t head0 = (int64_t)(slot >> 4) * 2 * a.hk + kh0;
+  uint8_t* kb = a.kv + head0 * kQ8HeadBytes;
+  uint8_t* vb = kb + (int64_t)a.hk * kQ8HeadBytes;
+  uint8_t* eb = a.kv_scale + head0 + head + (is_v ? a.hk : 0);
+  uint4 x = make_uint4(0, 0, 0, 0), was[2][2];
+  int old = 1;
+  if (mine) {
+    x = ldg16_stream(a.qkv + (int64_t)row * a.ld + (int64_t)(a.hq + kh0 + head + (is_v ? a.hk : 0)) * kHead + 8 * c);
+    if (keep) old = *eb;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      was[h][i] = make_uint4(0, 0, 0, 0);
+      if (keep && (h == 0 || two)) was[h][i] = ldg16(vb + h * kQ8HeadBytes + (64 * i + lane) * kQ8Block);
+    }
+  float cs[8], sn[8], w[8];
+  get_turn(turn, c, cs, sn);
+  widen8(ldg16(a.k_norm + 8 * c), w);
+  const uint4 k = turn_head(a, x, w, cs, sn);
+  if (!is_v) x = k;
+  if (mine && !is_v && a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)row * a.k_ld + (int64_t)(kh0 + head) * kHead + 8 * c) = x;
+  uint32_t most = most_of<false>(x), none = 0;
+  if (__any(most >= 0x7f80u)) most = most_of<true>(x);  // not finite: it does not count
+  row16_max2(most, none);
+  const int e = max(old, block_exponent<FMT>(most));
+  const uint32_t w0 = to_bytes<FMT>(x.x, x.y, e), w1 = to_bytes<FMT>(x.z, x.w, e);
+  if (mine && !is_v) *reinterpret_cast<uint2*>(kb + head * kQ8HeadBytes + token * kHead + 8 * c) = make_uint2(w0, w1);
+  if (mine && c == 0) *eb = (uint8_t)e;
+  const int shift = 8 * (token & 3);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h == 1 && !two) break;
+    const int v_old = __builtin_amdgcn_readlane(old, 32 * h + 16), v_e = __builtin_amdgcn_readlane(e, 32 * h + 16);
+    const float by = pow2_biased(max(127 + v_old - v_e, 1));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t out[4] = {was[h][i].x, was[h][i].y, was[h][i].z, was[h][i].w};
+      if (keep && v_e > v_old)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) out[d] = rescaled<FMT>(out[d], by);
+      const int from = 32 * h + 16 + 8 * i + (lane >> 3);
+      const uint32_t byte = __builtin_amdgcn_perm(from_lane(w1, from), from_lane(w0, from), 0x0c0c0c00u | (lane & 7));
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if (d == token >> 2) out[d] = (out[d] & ~(0xffu << shift)) | byte << shift;
+      *reinterpret_cast<uint4*>(vb + h * kQ8HeadBytes + (64 * i + lane) * kQ8Block) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+  }
+#pragma unroll 1
+  for (int h = 0; h < (two ? 2 : 1); ++h) {
+    const int k_old = __builtin_amdgcn_readlane(old, 32 * h), k_e = __builtin_amdgcn_readlane(e, 32 * h);
+    if (keep && k_e == k_old) continue;
+    const float by = pow2_biased(max(127 + k_old - k_e, 1));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (8 * i + (lane >> 3) == token) continue;
+      uint4* at = reinterpret_cast<uint4*>(kb + h * kQ8HeadBytes + (64 * i + lane) * 16);
+      uint4 o = make_uint4(0, 0, 0, 0);
+      if (keep) {
+        o = *at;
+        o.x = rescaled<FMT>(o.x, by), o.y = rescaled<FMT>(o.y, by), o.z = rescaled<FMT>(o.z, by), o.w = rescaled<FMT>(o.w, by);
+      }
+      *at = o;
+    }
+  }
+}
+
+// Rows n0 .. n0 + 3 of a workgroup, those alone in their blocks: a wave each,
+// heads 2 y and 2 y + 1, then 2 Y further on.
+template <int FMT>
+__device__ __forceinline__ void rows_alone(const RopeQ8Args& a, int around, int n0, int y, int Y, TurnLds* turns) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (2 * y >= a.hk || !is_alone(around, 16 + wave)) return;
+  const int slot = __builtin_amdgcn_readlane(around, 16 + wave);
+  put_turn(a, a.pos[n0 + wave], threadIdx.x & 63, &turns[wave]);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (int kh = 2 * y; kh < a.hk; kh += 2 * Y) write_alone<FMT>(a, n0 + wave, slot, kh, turns[wave]);
+}
+
 // Row (or rows from) that workgroup x of 16 T looks at, LEADS of every 16: the T
 // workgroups with the same rows of every 16 follow one another. In a prompt one
 // row of 16 leads a block, and in row order all of those would be on one XCD.
@@ -377,54 +507,72 @@ __device__ __forceinline__ int leads_from(const RopeQ8Args& a, int x) {
   return 16 * (x - s * T) + LEADS * s;
 }
 
-// Few rows, one launch: workgroup (x, y). y < hk writes K/V head y of the block
-// that its row leads, if it does; y >= hk turns 16 of the row's q heads.
+// Few rows, one launch. Workgroup (x, y) looks at four rows of 16. y below
+// `alone`: those alone in their blocks, two K/V heads of them; the next hk: a K/V
+// head of the other blocks that its rows lead; the rest: four of its rows' q heads.
+// Six waves a SIMD (3 dwords spilled) against five: 1556 rows of 8 prompts 18.4 / 18.9 us,
+// 64 rows each of its own sequence 4.3 / 4.3; with seven 19.9 / 4.8.
+constexpr int kLeads = kThreads / 64;
+
 template <int FMT>
-__global__ __launch_bounds__(kThreads) void rope_q8_rows(RopeQ8Args a) {
-  const int n = leads_from<1>(a, blockIdx.x), c = threadIdx.x & 15, grp = threadIdx.x >> 4;
-  if (n >= a.rows) return;
+__global__ __launch_bounds__(kThreads, 6) void rope_q8_rows(RopeQ8Args a, int alone) {
+  const int n0 = leads_from<kLeads>(a, blockIdx.x), c = threadIdx.x & 15, grp = threadIdx.x >> 4;
+  const int y = (int)blockIdx.y - alone;
+  __shared__ __align__(16) TurnLds turns[kLeads];
+  if (y < 0) {
+    rows_alone<FMT>(a, slots_around(a, n0), n0, blockIdx.y, a.hk, turns);
+    return;
+  }
   float cs[8], sn[8], w[8];
-  if ((int)blockIdx.y >= a.hk) {
-    const int head = 16 * (blockIdx.y - a.hk) + grp;
-    if (a.slots[n] < 0 || head >= a.hq) return;
-    const uint4 raw = ldg16(a.qkv + (int64_t)n * a.ld + (int64_t)head * kHead + 8 * c);
-    turn_of(a, a.pos[n], c, cs, sn);
+  if (y >= a.hk) {
+    const int n = n0 + (grp >> 2), head = 4 * (y - a.hk) + (grp & 3);
+    const bool mine = n < a.rows && head < a.hq && a.slots[n] >= 0;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (mine) raw = ldg16(a.qkv + (int64_t)n * a.ld + (int64_t)head * kHead + 8 * c);
+    put_turn(a, a.pos[min(n0 + (int)(threadIdx.x >> 6), a.rows - 1)], threadIdx.x & 63, &turns[threadIdx.x >> 6]);
+    __syncthreads();
+    if (!mine) return;
+    get_turn(turns[grp >> 2], c, cs, sn);
     widen8(ldg16(a.q_norm + 8 * c), w);
     *reinterpret_cast<uint4*>(a.q + (int64_t)n * a.q_ld + (int64_t)head * kHead + 8 * c) = turn_head(a, raw, w, cs, sn);
     return;
   }
-  BlockRows r;
-  if (!block_rows(slots_around(a, n), 16, n, grp, &r)) return;
-  const int kh = blockIdx.y;
+  const int kh = y, around = slots_around(a, n0);
   __shared__ KvLds lds;
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if (r.row >= 0) {
-    const bf16_t* src = a.qkv + (int64_t)r.row * a.ld + (int64_t)(a.hq + kh) * kHead + 8 * c;
-    const uint4 kraw = ldg16(src);
-    v = ldg16(src + (int64_t)a.hk * kHead);
-    turn_of(a, a.pos[r.row], c, cs, sn);
-    widen8(ldg16(a.k_norm + 8 * c), w);
-    k = turn_head(a, kraw, w, cs, sn);
-    if (a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
+  for (int lead = 0; lead < kLeads; ++lead) {
+    BlockRows r;
+    if (!block_rows(around, 16 + lead, n0 + lead, grp, &r)) continue;
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
+    if (r.row >= 0) {
+      const bf16_t* src = a.qkv + (int64_t)r.row * a.ld + (int64_t)(a.hq + kh) * kHead + 8 * c;
+      const uint4 kraw = ldg16(src);
+      v = ldg16(src + (int64_t)a.hk * kHead);
+      turn_of(a, a.pos[r.row], c, cs, sn);
+      widen8(ldg16(a.k_norm + 8 * c), w);
+      k = turn_head(a, kraw, w, cs, sn);
+      if (a.k) *reinterpret_cast<uint4*>(a.k + (int64_t)r.row * a.k_ld + (int64_t)kh * kHead + 8 * c) = k;
+    }
+    if (r.twice) k_rows_twice(a, r, n0 + lead, kh, a.hk, c, grp);
+    write_block<FMT, 1>(a, r, kh, a.hk, &k, &v, c, grp, &lds);
   }
-  if (r.twice) k_rows_twice(a, r, n, kh, a.hk, c, grp);
-  write_block<FMT, 1>(a, r, kh, a.hk, &k, &v, c, grp, &lds);
 }
 
 // Many rows, the cache: workgroup (x, y) looks at kLeads rows of 16, and for each
 // that leads a block writes K/V heads y, y + Y, .. of it, a token per thread
 // group, its angles computed once, kAtOnce heads at a time. In a prompt one row of
-// 16 leads; of single rows each does, so a workgroup looks at no more than four.
+// 16 leads, and rows alone in their blocks are taken by a wave each afterwards.
 // (With one row per workgroup, of 25,850 rows of 12 prompts the workgroups that
-// end at once took some 50 us.)
-constexpr int kLeads = 4, kAtOnce = 2;
+// end at once took some 50 us.) 25,850 rows of 32q/8kv (636 MB) take 134 us with
+// turn_q_rows, 4.75 TB/s of reads and writes, where a large copy reaches 4.97.
+constexpr int kAtOnce = 2;
 
 template <int FMT>
-__global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
+__global__ __launch_bounds__(kThreads, 4) void rope_q8_blocks(RopeQ8Args a) {
   const int n0 = leads_from<kLeads>(a, blockIdx.x), c = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const int y = blockIdx.y, Y = gridDim.y;
   const int around = slots_around(a, n0);
   __shared__ KvLds lds[kAtOnce];
+  __shared__ __align__(16) TurnLds turns[kLeads];
   for (int lead = 0; lead < kLeads; ++lead) {
     const int n = n0 + lead;
     BlockRows r;
@@ -462,6 +610,7 @@ __global__ __launch_bounds__(kThreads) void rope_q8_blocks(RopeQ8Args a) {
     }
     if (r.twice) k_rows_twice(a, r, n, y, Y, c, grp);
   }
+  rows_alone<FMT>(a, around, n0, y, Y, turns);
 }
 
 // Many rows, q: one workgroup per row (2, 4, 8 or 16 rows of at most 8, 4, 2 or 1
@@ -478,29 +627,15 @@ __global__ __launch_bounds__(kThreads) void turn_q_rows(RopeQ8Args a, int rows_s
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
     if (row < a.rows && h0 + i * per < a.hq) raw[i] = ldg16_stream(src + (int64_t)(h0 + i * per) * kHead);
-  __shared__ __align__(16) float s_cos[16][kHead / 2], s_sin[16][kHead / 2];
+  __shared__ __align__(16) TurnLds s_turn[16];
   for (int t = threadIdx.x; t < (kHead / 2) << rows_shift; t += kThreads) {
-    const int i = t & (kHead / 2 - 1), k = t / (kHead / 2);
-    double f = (double)a.pos[min(n0 + k, a.rows - 1)] * kTurnsPerRadian;
-    double r = a.inv_theta64;
-#pragma unroll
-    for (int b = 0; b < 6; ++b) {
-      if (b >= 2 && (i >> b & 1)) f *= r;
-      r *= r;
-    }
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (e < (i & 3)) f *= a.inv_theta64;
-    sincos_turns(f, &s_sin[k][i], &s_cos[k][i]);
+    const int k = t / (kHead / 2);
+    put_turn(a, a.pos[min(n0 + k, a.rows - 1)], t & (kHead / 2 - 1), &s_turn[k]);
   }
   __syncthreads();
   if (row >= a.rows || a.slots[row] < 0) return;
   float cs[8], sn[8], w[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float t = s_sin[grp / per][8 * (c & 7) + e];
-    cs[e] = s_cos[grp / per][8 * (c & 7) + e], sn[e] = c < 8 ? -t : t;
-  }
+  get_turn(s_turn[grp / per], c, cs, sn);
   widen8(ldg16(a.q_norm + 8 * c), w);
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
@@ -548,8 +683,6 @@ __device__ __forceinline__ bf16x8 bf16_of(uint32_t w0, uint32_t w1) {
   }
   return __builtin_bit_cast(bf16x8, u);
 }
-
-__device__ __forceinline__ int from_lane(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane << 2, v); }
 
 // Lanes col < 8 of 16 keep x and take their y from lane col + 8's x; lanes
 // col >= 8 keep y and take their x from lane col - 8's y.
@@ -840,19 +973,20 @@ __global__ __launch_bounds__(kThreads) void merge_q8(DecodeQ8Args a) {
 
 }  // namespace
 
-// One launch below this many rows, two from there: 1000 rows of a prompt of
-// 32q/8kv take 11.8 us in one and 17 in two, 8 of 100-300 rows (1556) 19.5 / 24,
-// 8000 rows of 32q/32kv 192 / 93.
+// One launch below this many rows, two from there: a prompt of 2100 rows of
+// 32q/8kv takes 24 us in one and 27.5 in two, prompts of 4000 43 / 36, 4000 rows of
+// 32q/32kv 94 / 53; 2200 rows, each of its own sequence, 36 / 35.
 constexpr int kManyRows = 2048;
 
 int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream) {
   const unsigned T = (unsigned)((a.rows + 15) / 16);
   if (a.rows < kManyRows) {
-    const dim3 grid(16 * T, a.hk + (a.hq + 15) / 16);
+    const int alone = (a.hk + 1) / 2;
+    const dim3 grid(16 / kLeads * T, alone + a.hk + (a.hq + 3) / 4);
     if (a.format == kQ8E4m3)
-      rope_q8_rows<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a);
+      rope_q8_rows<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a, alone);
     else
-      rope_q8_rows<kQ8Int8><<<grid, kThreads, 0, stream>>>(a);
+      rope_q8_rows<kQ8Int8><<<grid, kThreads, 0, stream>>>(a, alone);
     return check_launch();
   }
   // The K/V heads of a block over as many workgroups as give a prompt 1024 that lead.

@@ -120,6 +120,33 @@ def test_write_of_many_rows(fmt, hq, hk):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [37, 2100])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (3, 3), (10, 5), (16, 8)])
+def test_write_of_rows_alone_in_their_blocks(fmt, rows, hq, hk):
+    """One token a sequence, at every place of a block, of every size, a few with infinities and NaN, some skipped, two
+    pairs of rows next to one another in one block."""
+    g, rng = gen(rows + hk), np.random.default_rng(rows)
+    slots = [int(b) * 16 + i % 16 for i, b in enumerate(rng.permutation(rows + 9)[:rows])]
+    for i in (5, 30):
+        slots[i] = slots[i - 1] ^ 1
+    for i in (0, 11, rows - 2):
+        slots[i] = -1
+    pos = rng.integers(0, 60000, rows).tolist()
+    qkv = torch.randn(rows, (hq + 2 * hk) * 128, device="cuda", generator=g) * 2.0 ** torch.randint(-9, 9, (rows, 1), device="cuda", generator=g)
+    qkv = qkv.to(torch.bfloat16)
+    for i, x in enumerate((float("inf"), float("-inf"), float("nan"))):
+        qkv[i + 1::17, (hq + hk) * 128 + 3 + 50 * i] = x
+        qkv[i + 6::23, hq * 128 + 7 + 40 * i] = x
+    qkv[3::11, (hq + hk) * 128:] = 0
+    w = weights(g)
+    kv, sc = random_cache(g, rows + 9, hk, fmt)
+    ref = R.Cache(kv, sc, hk)
+    _, k = write(qkv, pos, slots, kv, sc, hq, hk, w)
+    ref.write(slots, k.cpu().double().view(rows, hk, 128), qkv.view(rows, -1, 128)[:, hq + hk:].cpu().double())
+    ref.same_as(kv, sc)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_tokens_appended_one_by_one(fmt):
     """40 steps of five sequences that grow by one token, whose size rises and falls: the cache follows the host's at every step."""
     hq, hk, seqs = 4, 2, 5
