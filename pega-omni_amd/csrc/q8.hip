@@ -973,14 +973,16 @@ __global__ __launch_bounds__(kThreads) void merge_q8(DecodeQ8Args a) {
 
 }  // namespace
 
-// One launch below this many rows, two from there: a prompt of 2100 rows of
-// 32q/8kv takes 24 us in one and 27.5 in two, prompts of 4000 43 / 36, 4000 rows of
-// 32q/32kv 94 / 53; 2200 rows, each of its own sequence, 36 / 35.
-constexpr int kManyRows = 2048;
+// One launch below this many heads over all rows, two from there (us in one / in two):
+// prompts of 2700 rows of 32q/8kv (130,000 heads) 28.5 / 30.3, of 3300 34.0 / 30.9; 4000 of
+// 16q/8kv (128,000) 29.3 / 30.4; 1000 of 32q/32kv (96,000) 25.7 / 25.3, 1300 31.7 / 28.1;
+// 20,000 of 8q/1kv (200,000) 39.1 / 39.4; rows of as many sequences, 1900 of 32q/8kv
+// (91,000) 30.8 / 32.6, 3000 47.6 / 44.2.
+constexpr int64_t kManyHeads = 1 << 17;
 
 int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream) {
   const unsigned T = (unsigned)((a.rows + 15) / 16);
-  if (a.rows < kManyRows) {
+  if ((int64_t)a.rows * (a.hq + 2 * (int64_t)a.hk) < kManyHeads) {
     const int alone = (a.hk + 1) / 2;
     const dim3 grid(16 / kLeads * T, alone + a.hk + (a.hq + 3) / 4);
     if (a.format == kQ8E4m3)

@@ -86,20 +86,22 @@ def test_write_matches_the_host_quantizer(fmt, hq, hk):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("hq,hk", [(16, 8), (10, 5), (7, 1), (40, 20)])
+@pytest.mark.parametrize("hq,hk", [(16, 8), (10, 5), (7, 1), (1, 1), (3, 3), (40, 20), (33, 33)])
 def test_write_of_many_rows(fmt, hq, hk):
-    """Calls of 2048 rows and more (other kernels): runs at every place of a block, single rows, skipped rows and a slot
-    given twice among them; and the bits of calls of few rows."""
+    """Calls of 131,072 heads and more over their rows (other kernels): runs at every place of a block, single rows,
+    skipped rows and a slot given twice among them; and the bits of calls of few rows."""
     g, rng = gen(hq + hk), np.random.default_rng(hq)
     runs = [(0, 90), (5, 1), (15, 1), (3, 200), (0, 16), (9, 30), (0, 1), (14, 5), (7, 9), (0, 7)] + [(i % 16, 1) for i in range(40)]
     runs += [(0, 900), (11, 800), (2, 3)]
-    slots, pos = runs_to_slots(rng, runs, 220)
+    runs += [(0, max(0, 131072 // (hq + 2 * hk) - 2000))]
+    blocks = 220 + runs[-1][1] // 16
+    slots, pos = runs_to_slots(rng, runs, blocks)
     slots[100] = -1
     slots[120] = slots[119]
     rows = len(slots)
     qkv = torch.randn(rows, (hq + 2 * hk) * 128, device="cuda", generator=g).to(torch.bfloat16)
     w = weights(g)
-    kv, sc = random_cache(g, 220, hk, fmt)
+    kv, sc = random_cache(g, blocks, hk, fmt)
     ref, kv1, sc1 = R.Cache(kv, sc, hk), kv.clone(), sc.clone()
     q, k = write(qkv, pos, slots, kv, sc, hq, hk, w)
     heads = qkv.view(rows, -1, 128).cpu()
@@ -110,10 +112,9 @@ def test_write_of_many_rows(fmt, hq, hk):
     ref.write(slots, k.cpu().double().view(rows, hk, 128), heads[:, hq + hk:].double())
     ref.same_as(kv, sc)
     cuts = [0] + [n for n in range(1, rows) if slots[n] // 16 != slots[n - 1] // 16 and slots[n] >= 0 and slots[n - 1] >= 0]
-    assert rows >= 2048
+    assert rows * (hq + 2 * hk) >= 131072
     cuts = [n for i, n in enumerate(cuts) if i % 3 == 0] + [rows]
     for a, b in zip(cuts, cuts[1:]):
-        assert b - a < 2048
         q1, k1 = write(qkv[a:b].contiguous(), pos[a:b], slots[a:b], kv1, sc1, hq, hk, w)
         assert torch.equal(q1, q[a:b]) and torch.equal(k1, k[a:b])
     ref.same_as(kv1, sc1)
