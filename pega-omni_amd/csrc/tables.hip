@@ -22,9 +22,6 @@ namespace omni {
 
 namespace {
 
-constexpr int kTabThreads = 256;
-constexpr int kTabWaves = kTabThreads / 64;
-
 // What a sequence adds to the step: rows, pages listed, pages taken, pages given back.
 struct SeqShare {
   int rows, pages, taken, back, held, line, code;
@@ -80,28 +77,33 @@ __device__ __forceinline__ int4 scan4(int4 v, int4* wave_sums) {
   return v;
 }
 
-// Every workgroup: the sums over all sequences (one scan of 256 sequences gives
-// totals and offsets; more sequences are added up first), then its share of each
-// output, a row or page finding its sequence by bisection of the sums in LDS.
-// Two memory round trips, the lengths and a page id, and the launch are what a
-// call takes.
-__global__ __launch_bounds__(kTabThreads) void step_tables(TablesArgs a) {
-  const int tid = threadIdx.x, wg = blockIdx.x, first_x = wg * kTabThreads + tid, step = gridDim.x * kTabThreads;
-  __shared__ int4 s_wave[kTabWaves];
-  __shared__ int s_codes[kTabWaves];
-  __shared__ int4 s_end[kTabThreads];            // rows, pages, taken and given back up to a sequence
-  __shared__ int s_first[kTabThreads], s_held[kTabThreads];
-  __shared__ int64_t s_line[kTabThreads];        // the sequence's line in the table
+// Every workgroup: the sums over all sequences (one scan of as many sequences as
+// threads gives totals and offsets; more sequences are added up first), then its
+// share of each output, a row or page finding its sequence by bisection of the sums
+// in LDS. Bytes bound nothing here (40 KB for 64 sequences of some 1500 tokens, a
+// microsecond's worth for the largest steps): two memory round trips, the lengths
+// and a page id, and the launch are what a call takes, 5.3 us for 64 sequences of
+// one new token and 6.9 for 128, 24 of them prompts of 30-4096 (with 64-bit sums and a
+// second pass over the sequences 14.6).
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void step_tables(TablesArgs a) {
+  constexpr int kWaves = THREADS / 64;
+  const int tid = threadIdx.x, wg = blockIdx.x, first_x = wg * THREADS + tid, step = gridDim.x * THREADS;
+  __shared__ int4 s_wave[kWaves];
+  __shared__ int s_codes[kWaves];
+  __shared__ int4 s_end[THREADS];            // rows, pages, taken and given back up to a sequence
+  __shared__ int s_first[THREADS], s_held[THREADS];
+  __shared__ int64_t s_line[THREADS];        // the sequence's line in the table
 
   const int head = a.free_pages ? a.free_state[0] : 0, avail = a.free_pages ? a.free_state[1] : 0;
   int codes = 0;  // bit c: code c
   if (a.free_pages && (head < 0 || head >= a.num_pages || avail < 0 || avail > a.num_pages)) codes |= 1 << 1;
 
   // Totals, and whether the step can be made at all.
-  const bool one_scan = a.nseq <= kTabThreads;
+  const bool one_scan = a.nseq <= THREADS;
   SeqShare r{};
   int4 sum{};
-  for (int s = tid; s < a.nseq; s += kTabThreads) {
+  for (int s = tid; s < a.nseq; s += THREADS) {
     r = seq_share(a, s);
     if (r.code) codes |= 1 << r.code;
     sum = add_sat(sum, int4{r.rows, r.pages, r.taken, r.back});
@@ -112,9 +114,9 @@ __global__ __launch_bounds__(kTabThreads) void step_tables(TablesArgs a) {
     if (__any(codes >> c & 1)) codes |= 1 << c;
   if ((tid & 63) == 0) s_codes[tid >> 6] = codes;
   __syncthreads();
-  int4 total = s_end[kTabThreads - 1];
+  int4 total = s_end[THREADS - 1];
 #pragma unroll
-  for (int w = 0; w < kTabWaves; ++w) codes |= s_codes[w];
+  for (int w = 0; w < kWaves; ++w) codes |= s_codes[w];
   if (a.free_pages) {
     if (add_sat(max(avail, 0), total.w) > a.num_pages) codes |= 1 << 1;
     if (total.z > avail) codes |= 1 << 5;
@@ -145,8 +147,8 @@ __global__ __launch_bounds__(kTabThreads) void step_tables(TablesArgs a) {
   }
 
   int4 base{};  // the sums before the sequences at hand
-  for (int s0 = 0; s0 < a.nseq; s0 += kTabThreads) {
-    const int n = min(kTabThreads, a.nseq - s0);
+  for (int s0 = 0; s0 < a.nseq; s0 += THREADS) {
+    const int n = min(THREADS, a.nseq - s0);
     if (!one_scan) {
       __syncthreads();  // the last sequences' sums have been read
       r = SeqShare{};
@@ -202,10 +204,18 @@ __global__ __launch_bounds__(kTabThreads) void step_tables(TablesArgs a) {
 
 }  // namespace
 
+// As many threads as sequences, to 1024: one scan gives every offset. us in 256 / 512 /
+// 1024 threads: 286 sequences 11.6 / 7.7 / 8.6, 512 12.6 / 8.2 / 9.0, 1024 21.5 / 14.7 /
+// 10.0, 4090 74 / 46 / 32.
 int launch_tables(const TablesArgs& a, hipStream_t stream) {
   const int most = std::max(std::max(a.row_cap, a.page_cap), a.nseq);
-  const int grid = std::max(1, std::min(1024, (int)(((int64_t)most + kTabThreads - 1) / kTabThreads)));
-  step_tables<<<grid, kTabThreads, 0, stream>>>(a);
+  const auto grid = [&](int threads) { return (int)std::max<int64_t>(1, std::min<int64_t>(1 << 18, (int64_t)most + threads - 1) / threads); };
+  if (a.nseq <= 256)
+    step_tables<256><<<grid(256), 256, 0, stream>>>(a);
+  else if (a.nseq <= 512)
+    step_tables<512><<<grid(512), 512, 0, stream>>>(a);
+  else
+    step_tables<1024><<<grid(1024), 1024, 0, stream>>>(a);
   return check_launch();
 }
 

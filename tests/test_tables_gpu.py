@@ -82,7 +82,8 @@ def lengths(rng, nseq, ctx, new, done):
 @pytest.mark.parametrize("nseq,ctx,new,page,ring,leased", [
     (0, 0, 0, 16, 0, False), (1, 0, 1, 16, 0, False), (1, 100, 1, 16, 0, False), (5, 40, 33, 16, 0, False),
     (64, 2400, 1, 16, 0, False), (64, 300, 200, 16, 0, True), (255, 50, 20, 16, 0, False), (256, 50, 20, 16, 0, False),
-    (257, 50, 20, 16, 0, False), (700, 90, 9, 16, 0, False), (30, 400, 90, 10, 0, False), (30, 400, 90, 1, 0, False),
+    (257, 50, 20, 16, 0, False), (512, 70, 30, 16, 0, False), (513, 90, 9, 16, 0, True), (700, 90, 9, 16, 0, False),
+    (1024, 60, 9, 16, 0, False), (1025, 60, 9, 16, 0, False), (2600, 40, 5, 16, 48, False), (30, 400, 90, 10, 0, False), (30, 400, 90, 1, 0, False),
     (40, 900, 60, 16, 300, False), (40, 900, 60, 16, 301, True), (9, 700, 2000, 64, 0, False),
 ])
 def test_matches_host_loops(nseq, ctx, new, page, ring, leased):
