@@ -770,9 +770,10 @@ namespace {
 //   2 for each round of 1024 resident workgroups (four a CU);
 //   with splits, 3 for the merge's launch and 1.3 for every 32 splits of a row.
 // Measured at the choice / at the best split of the sweep: 1 row of 2400 keys,
-// hk = 8, 128 keys 8.3 / 8.3; of 8000, 256 keys 11.0 / 11.0; 16 rows of 200-2400
-// 256 keys 15.5 / 15.5; 64 rows none 37.4 / 37.4; 21 rows of 512-5120 512 keys 29.6 /
-// 29.6; 4 rows of 100,000-130,000 2048 keys 170.5 / 169.2.
+// hk = 8, 128 keys 8.1 / 8.1; of 8000, 256 keys 10.7 / 10.7; 16 rows of 200-2400
+// 256 keys 15.5 / 15.1; 64 rows none 32.4 / 32.4; 21 rows of 512-5120 512 keys 29.4 /
+// 29.3; 4 rows of 100,000-130,000 4096 keys 162 / 153 (8192); 2 of 60,000, hk = 2, 768
+// keys 25.0 / 22.8 (1024).
 int pick_chunk_q8(int rows, int hk, int max_len) {
   const double units = (double)rows * hk, read = units * max_len * 0.6 * 256 / 6.2e6;
   int best = 0;

@@ -236,8 +236,10 @@ struct DecodeQ8Args {
   int ragged;
   PageDiv pd;  // blocks per page
   int chunk, splits;
+  int per_round;   // rows whose workgroups fill the GPU once; 0: rows in their order
+  int len_shift;   // row lengths >> len_shift fit 6 bits (longer ones count as 63)
   float scale_log2;
 };
-int launch_decode_q8(const DecodeQ8Args& a, int rows, hipStream_t stream);
+int launch_decode_q8(DecodeQ8Args a, int rows, hipStream_t stream);
 
 }  // namespace omni

@@ -648,6 +648,7 @@ __global__ __launch_bounds__(kThreads) void turn_q_rows(RopeQ8Args a, int rows_s
 
 constexpr int kMostGroup = 16;  // query heads per K/V head
 constexpr int kTile = 32;       // keys per step: two blocks
+constexpr int kCus = 256;       // workgroups go to the CUs in turn
 constexpr int kIds = 64 / (kTile / kQ8Block);  // tiles whose blocks a wave looks up at once
 
 // Keys per split of a row of len keys: the plan's, or more where a row is
@@ -706,6 +707,58 @@ __device__ __forceinline__ float max_of_groups(float v) {
 constexpr int kDecodeWaves = kThreads / 64;
 constexpr int kBlocksPerTile = kTile / kQ8Block;
 
+// The row of workgroup index n, and its position. Where the workgroups are more than
+// the GPU takes at once, long rows come first and every other round of rows (what
+// fills the GPU once) runs backwards, so that a CU's rows add up to much the same:
+// index n takes the t-th longest of its 256 rows, by lengths of 6 bits, ties in their
+// order. Every wave finds it from the positions it would wait for anyway, by bits
+// of the length that have more than t rows at or above them. us in the rows' order /
+// so ordered: 64 rows of 200-2400 keys of 16q/8kv 37.1 / 32.4, of 500-5000 of 32q/8kv
+// 76 / 66, 256 of 100-3000 145 / 130, 128 of 100-3000 of 32q/32kv 271 / 256; rows of one
+// length pay for it, 128 of 1600 of 32q/32kv 265.1 / 266.1.
+__device__ __forceinline__ int row_of(const DecodeQ8Args& a, int n, int rows, int* p) {
+  if (a.per_round == 0) {
+    *p = a.pos[n];
+    return n;
+  }
+  const int first = n & ~255, R = min(256, rows - first), lane = threadIdx.x & 63;
+  const int from = (n - first) / a.per_round * a.per_round, at = n - first - from;
+  int t = from / a.per_round & 1 ? min(R, from + a.per_round) - 1 - at : n - first;
+  int pos[4], key[4];  // of rows first + 64 c + lane
+#pragma unroll
+  for (int c = 0; c < 4; ++c) pos[c] = 64 * c + lane < R ? a.pos[first + 64 * c + lane] : -1;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) key[c] = 64 * c + lane < R ? min(max(pos[c], 0) >> a.len_shift, 63) : -1;
+  int k = 0, above = 0;
+#pragma unroll
+  for (int b = 5; b >= 0; --b) {
+    const int tried = k | 1 << b;
+    int count = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) count += __popcll(__ballot(key[c] >= tried));
+    if (count > t)
+      k = tried;
+    else
+      above = count;
+  }
+  t -= above;
+  int row = n;
+  *p = -1;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint64_t same = __ballot(key[c] == k);
+    const int count = __popcll(same);
+    if (t >= 0 && t < count) {
+      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+      const int l = __builtin_ctzll(__ballot(key[c] == k && before == t));
+      row = first + 64 * c + l;
+      *p = __builtin_amdgcn_readlane(pos[c], l);
+    }
+    t -= count;
+  }
+  return row;
+}
+
 // One workgroup per (split, K/V head, row); its waves take the split's 32-key
 // tiles in turn, each with a running maximum, sum and O of its own, merged
 // through LDS at the end. Lane l is column n = l % 16 (query head) and group
@@ -727,16 +780,17 @@ constexpr int kBlocksPerTile = kTile / kQ8Block;
 // 64-byte halves of its lines: 269 / 170 us for the first and last of these, with
 // cached loads 266 / 168): 128 rows of 1600 keys of 32 heads (1.68 GB) take 264 us,
 // 6.4 TB/s; 4 of 100,000-130,000 keys of 32q/8kv in 4096-key splits (0.94 GB) 162 with
-// the merge, 5.8; 64 of 200-2400 of 16q/8kv (0.17 GB) 36.8, 4.6, where the longest
+// the merge, 5.8; 64 of 200-2400 of 16q/8kv (0.17 GB) 32.4, 5.2, where the longest
 // rows' walks show. Loads alone, nothing computed, took 265 of 272 us when the
 // first stood at that; 64-key tiles, two or three tiles asked for ahead, and
 // two or three workgroups a CU in place of four were no faster. A lone row is
 // bound by latency: 1 row of 8000 keys in 256-key splits takes 10.8 with the merge.
 template <int FMT>
 __global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
-  const int kh = blockIdx.y, n = blockIdx.z, G = a.hq / a.hk, tid = threadIdx.x;
-  const int split = spread_split(blockIdx.x, kh + a.hk * n, a.splits);
-  const int p = a.pos[n];
+  const int kh = blockIdx.y, G = a.hq / a.hk, tid = threadIdx.x;
+  const int split = spread_split(blockIdx.x, kh + a.hk * blockIdx.z, a.splits);
+  int p;
+  const int n = row_of(a, blockIdx.z, gridDim.z, &p);
   const int32_t* pg = a.pages + a.indptr[a.ragged ? max(a.seq[n], 0) : n];
   const int len = p < 0 ? 0 : p + 1;
   const int64_t h0 = (int64_t)n * a.hq + kh * G;
@@ -1004,7 +1058,11 @@ int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream) {
   return check_launch();
 }
 
-int launch_decode_q8(const DecodeQ8Args& a, int rows, hipStream_t stream) {
+int launch_decode_q8(DecodeQ8Args a, int rows, hipStream_t stream) {
+  // Splits even the rows out themselves (21 rows of 512-5120 keys of 32q/8kv in 512-key
+  // splits 28.5 us, 31 so ordered).
+  a.per_round = a.splits == 1 && (int64_t)rows * a.hk > kCus ? std::max(kCus / a.hk, 1) : 0;
+  while (a.chunk >> a.len_shift >= 64) ++a.len_shift;
   const dim3 grid(a.splits, a.hk, rows);
   if (a.format == kQ8E4m3)
     decode_q8<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a);

@@ -440,3 +440,36 @@ def test_decode_replays_with_new_lengths():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(d.out, want)
+
+
+@pytest.mark.parametrize("hk", [1, 3, 8, 300])
+@pytest.mark.parametrize("rows", [2, 33, 65, 257, 600])
+def test_decode_of_many_rows_in_any_order_of_lengths(rows, hk):
+    """Rows of lengths in falling, rising and random order, equal, far longer than the plan and without keys, in one split
+    each: every row keeps the bits that it has alone."""
+    if rows * hk > 20000:
+        rows = 20000 // hk
+    g, rng = gen(rows + hk), np.random.default_rng(rows)
+    kv, sc = random_cache(g, 40, hk, torch.int8)
+    q = torch.randn(rows, hk * 128, device="cuda", generator=g).to(torch.bfloat16)
+    lens = np.minimum(rng.integers(-1, 600, rows), 500)
+    lens[rows // 2:] = np.sort(lens[rows // 2:])
+    if rows > 40:
+        lens[30:60] = 77
+    pages = i32([rng.permutation(40)[:38] for _ in range(rows)])
+    indptr = i32(np.arange(rows + 1) * 38)
+    out = torch.zeros(rows, hk * 128, dtype=torch.bfloat16, device="cuda")
+
+    def run(lo, hi):
+        plan = oa.decode_plan_q8(hi - lo, hk, hk, 16, 128, 128)
+        assert plan.splits == 1
+        o = torch.full((hi - lo, hk * 128), 3.0, dtype=torch.bfloat16, device="cuda")
+        oa.qwen3_attend_q8(q[lo:hi], kv, sc, i32(lens[lo:hi] - 1), None, 0, indptr[lo:], pages.view(-1), 16, o, hk, hk, 0.09,
+                           plan, oa.workspace_for(plan))
+        return o
+
+    out = run(0, rows)
+    few = max(1, 256 // hk)
+    alone = torch.cat([run(lo, min(lo + few, rows)) for lo in range(0, rows, few)])
+    assert torch.equal(out, alone)
+    assert bool((out[torch.from_numpy(lens <= 0).cuda()] == 0).all())
