@@ -3,19 +3,22 @@
 Usage: python pega-omni_amd/build.py   (or __graft_entry__.build()).
 Every source under csrc/ is compiled to an object in _build/ and linked into
 pega-omni_amd/libomni_attn.so, the library the C ABI in include/omni_attn.h
-names.
+names. mirror/tensors.cpp (host code, against torch's headers) becomes
+pega-omni_amd/omni_tensors.so, the Python mirror's checks of a call's tensors.
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libomni_attn.so")
 BUILD = os.path.join(HERE, "_build")
+TENSORS = os.path.join(HERE, "omni_tensors.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [
@@ -48,10 +51,28 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _build_tensors() -> None:
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    inc, lib = os.path.join(root, "include"), os.path.join(root, "lib")
+    tmp = TENSORS + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], os.path.join(HERE, "mirror", "tensors.cpp"), "-o", tmp,
+           "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on tensors.cpp:\n{r.stderr}")
+    os.replace(tmp, TENSORS)
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     with ThreadPoolExecutor(max_workers=4) as ex:
+        tensors = ex.submit(_build_tensors)
         objs = list(ex.map(_compile, sources()))
+        tensors.result()
     tmp = OUT + ".tmp"
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)

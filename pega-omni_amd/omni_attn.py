@@ -551,15 +551,34 @@ def hidream_attend_ws(q, k, v, out, q_len, kv_len_at, q_stride, causal, scale_lo
 
 # ------------------------------------------ serving over an 8-bit block cache
 TABLES_OK, TABLES_BAD, TABLES_ROWS, TABLES_PAGES, TABLES_LINE, TABLES_EXHAUSTED = range(6)
-_Q8_FORMATS = {_torch.float8_e4m3fn: 0, _torch.int8: 1}
-_Q8_SCALES = (_torch.uint8, _torch.float8_e8m0fnu)
+_Q8_DTYPES = (_torch.float8_e4m3fn, _torch.int8)
 
 
 # A call launches on the current device, whose stream it takes: every tensor has
-# to lie there. The device is asked for once per call (`d` below; the raw call
-# where torch has it), each tensor's attributes once.
+# to lie there. omni_tensors checks them all in one call (its source lists the
+# kinds); the device is asked for once (the raw call where torch has it).
 _current_device = getattr(_torch._C, "_cuda_getDevice", None) or _torch.cuda.current_device
-_I32, _BF16 = _torch.int32, _torch.bfloat16
+
+
+def _load_tensors():
+    import importlib.machinery
+    import importlib.util
+
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "omni_tensors.so")
+    if not os.path.exists(path):
+        raise OmniAttnError(ELAUNCH, f"{path} is missing: build it with pega-omni_amd/build.py")
+    loader = importlib.machinery.ExtensionFileLoader("omni_tensors", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("omni_tensors", loader))
+    loader.exec_module(module)
+    module.set_error(OmniAttnError, EINVAL)
+    return module
+
+
+def _take(*args):
+    """omni_tensors.take, in whose place it stands until the first call."""
+    global _take
+    _take = _load_tensors().take
+    return _take(*args)
 
 
 def _device_of(t, name):
@@ -567,55 +586,6 @@ def _device_of(t, name):
     if d < 0 or d != _current_device():
         raise OmniAttnError(EINVAL, f"{name} must lie on the current device")
     return d
-
-
-def _off_device(name):
-    return OmniAttnError(EINVAL, f"{name} must lie on the current device, with the other tensors")
-
-
-def _i32_on(t, name, least, d):
-    if t.dtype is not _I32 or t.numel() < least or not t.is_contiguous():
-        raise OmniAttnError(EINVAL, f"{name} must be a contiguous int32 tensor of at least {least}")
-    if t.get_device() != d:
-        raise _off_device(name)
-    return t.data_ptr()
-
-
-def _bf16_on(t, name, least, d):
-    if t.dtype is not _BF16 or t.numel() < least or not t.is_contiguous():
-        raise OmniAttnError(EINVAL, f"{name} must be a contiguous bf16 tensor of at least {least}")
-    if t.get_device() != d:
-        raise _off_device(name)
-    return t.data_ptr()
-
-
-def _rows_on(t, name, rows, heads, d):
-    """Pointer and row stride of at least `rows` bf16 rows of heads x 128."""
-    width = heads * HEAD_DIM
-    shape = t.shape
-    if t.dtype is not _BF16 or len(shape) != 2 or shape[0] < rows or shape[1] != width:
-        raise OmniAttnError(EINVAL, f"{name} must be bf16 rows [{rows}][{width}]")
-    stride, one = t.stride()
-    if one != 1:
-        raise OmniAttnError(EINVAL, f"{name}: the elements of a row must be adjacent")
-    if t.get_device() != d:
-        raise _off_device(name)
-    return t.data_ptr(), stride if shape[0] > 1 else width
-
-
-def _q8_cache(kv, kv_scale, hk, d):
-    """Pointers of a cache and its exponents, and its format."""
-    fmt = _Q8_FORMATS.get(kv.dtype)
-    shape = kv.shape
-    if fmt is None or len(shape) != 3 or shape[1] != 2 * hk or shape[2] != 16 * HEAD_DIM:
-        raise OmniAttnError(EINVAL, f"kv must be float8_e4m3fn or int8 [blocks][{2 * hk}][2048]")
-    if kv_scale.dtype not in _Q8_SCALES or kv_scale.shape != shape[:2]:
-        raise OmniAttnError(EINVAL, f"kv_scale must be uint8 or float8_e8m0fnu [{shape[0]}][{2 * hk}]")
-    if not kv.is_contiguous() or not kv_scale.is_contiguous():
-        raise OmniAttnError(EINVAL, "kv and kv_scale must be contiguous")
-    if kv.get_device() != d or kv_scale.get_device() != d:
-        raise _off_device("kv and kv_scale")
-    return kv.data_ptr(), kv_scale.data_ptr(), fmt
 
 
 def _stream_on(stream, d):
@@ -626,7 +596,7 @@ def _stream_on(stream, d):
 
 def q8_cache(pages, page, hk, dtype=_torch.float8_e4m3fn, device="cuda"):
     """A zeroed 8-bit cache of `pages` pages: (kv [blocks][2 hk][2048], kv_scale [blocks][2 hk] exponents)."""
-    if page <= 0 or page % 16 or dtype not in _Q8_FORMATS or pages < 0 or hk <= 0:
+    if page <= 0 or page % 16 or dtype not in _Q8_DTYPES or pages < 0 or hk <= 0:
         raise OmniAttnError(EINVAL, f"q8_cache: pages={pages} page={page} hk={hk} dtype={dtype}")
     blocks = pages * (page // 16)
     kv = _torch.zeros(blocks, 2 * hk, 16 * HEAD_DIM, dtype=_torch.uint8, device=device).view(dtype)
@@ -647,19 +617,14 @@ def step_tables(first, count, lines, table, free_pages, free_state, pos, slots, 
     shape = table.shape
     if len(shape) != 2:
         raise OmniAttnError(EINVAL, "table must be an int32 tensor [lines][pages]")
-    if free_pages is None:
-        free_ptr = state_ptr = None
-        num_pages = 0
-    else:
-        num_pages = free_pages.numel()
-        free_ptr = _i32_on(free_pages, "free_pages", 1, d)
-        state_ptr = None if free_state is None else _i32_on(free_state, "free_state", 2, d)
-    _check(load().omni_attn_step_tables(
-        _i32_on(first, "first", 0, d), _i32_on(count, "count", n, d), None if lines is None else _i32_on(lines, "lines", n, d),
-        n, page, ring, _i32_on(table, "table", 0, d), shape[1], shape[0], free_ptr, num_pages, state_ptr, rows,
-        pages.numel(), _i32_on(pos, "pos", 0, d), _i32_on(slots, "slots", rows, d), _i32_on(seq, "seq", rows, d),
-        _i32_on(row_indptr, "row_indptr", n + 1, d), _i32_on(indptr, "indptr", n + 1, d), _i32_on(pages, "pages", 0, d),
-        _i32_on(status, "status", 5, d), _stream_on(stream, d)))
+    num_pages = 0 if free_pages is None else free_pages.numel()
+    (p_first, p_count, p_lines, p_table, p_free, p_state, p_pos, p_slots, p_seq, p_rows, p_indptr, p_pages, p_status) = _take(
+        "iiIiIIiiiiiii", "first count lines table free_pages free_state pos slots seq row_indptr indptr pages status", d,
+        first, 0, count, n, lines, n, table, 0, free_pages, 1, None if free_pages is None else free_state, 2, pos, 0,
+        slots, rows, seq, rows, row_indptr, n + 1, indptr, n + 1, pages, 0, status, 5)
+    _check(load().omni_attn_step_tables(p_first, p_count, p_lines, n, page, ring, p_table, shape[1], shape[0], p_free,
+                                        num_pages, p_state, rows, pages.numel(), p_pos, p_slots, p_seq, p_rows, p_indptr,
+                                        p_pages, p_status, _stream_on(stream, d)))
     return status
 
 
@@ -670,13 +635,11 @@ def qwen3_rope_q8(qkv, q_norm, k_norm, pos, slots, q_out, k_out, kv, kv_scale, h
     skipped."""
     rows = pos.numel()
     d = _device_of(qkv, "qkv")
-    src, ld = _rows_on(qkv, "qkv", rows, hq + 2 * hk, d)
-    q, q_ld = _rows_on(q_out, "q_out", rows, hq, d)
-    k, k_ld = (None, 0) if k_out is None else _rows_on(k_out, "k_out", rows, hk, d)
-    cache, scales, fmt = _q8_cache(kv, kv_scale, hk, d)
-    _check(load().omni_qwen3_rope_q8(src, ld, _bf16_on(q_norm, "q_norm", HEAD_DIM, d), _bf16_on(k_norm, "k_norm", HEAD_DIM, d),
-                                     _i32_on(pos, "pos", 0, d), _i32_on(slots, "slots", rows, d), q, q_ld, k, k_ld, cache,
-                                     scales, fmt, rows, hq, hk, eps, theta, _stream_on(stream, d)))
+    src, ld, p_qn, p_kn, p_pos, p_slots, q, q_ld, k, k_ld, cache, scales, fmt = _take(
+        "rbbiirRc", "qkv q_norm k_norm pos slots q_out k_out kv", d, qkv, rows, (hq + 2 * hk) * HEAD_DIM, q_norm, HEAD_DIM,
+        k_norm, HEAD_DIM, pos, 0, slots, rows, q_out, rows, hq * HEAD_DIM, k_out, rows, hk * HEAD_DIM, kv, kv_scale, 2 * hk)
+    _check(load().omni_qwen3_rope_q8(src, ld, p_qn, p_kn, p_pos, p_slots, q, q_ld, k, k_ld, cache, scales, fmt, rows, hq,
+                                     hk, eps, theta, _stream_on(stream, d)))
 
 
 def decode_plan_q8(rows: int, hq: int, hk: int, page: int, max_len: int, chunk: int = 0) -> DecodePlan:
@@ -692,15 +655,14 @@ def qwen3_attend_q8(q, kv, kv_scale, pos, seq, ragged, indptr, pages, page, out,
     rows with a negative position store zeros."""
     rows = plan.rows
     d = _device_of(q, "q")
-    src, stride = _rows_on(q, "q", rows, hq, d)
-    cache, scales, fmt = _q8_cache(kv, kv_scale, hk, d)
+    src, stride, cache, scales, fmt, p_pos, p_seq, p_indptr, p_pages, p_out = _take(
+        "rciIiib", "q kv pos seq indptr pages out", d, q, rows, hq * HEAD_DIM, kv, kv_scale, 2 * hk, pos, rows, seq, rows,
+        indptr, 1 if ragged else rows + 1, pages, 0, out, rows * hq * HEAD_DIM)
     if workspace is not None and workspace.get_device() != d:
-        raise _off_device("workspace")
-    _check(load().omni_qwen3_attend_q8(src, stride, cache, scales, fmt, _i32_on(pos, "pos", rows, d),
-                                       None if seq is None else _i32_on(seq, "seq", rows, d), 1 if ragged else 0,
-                                       _i32_on(indptr, "indptr", 1 if ragged else rows + 1, d),
-                                       _i32_on(pages, "pages", 0, d), page, _bf16_on(out, "out", rows * hq * HEAD_DIM, d),
-                                       hq, hk, scale, ctypes.byref(plan), _ws(plan, workspace), _stream_on(stream, d)))
+        raise OmniAttnError(EINVAL, "workspace must lie on the current device, with the other tensors")
+    _check(load().omni_qwen3_attend_q8(src, stride, cache, scales, fmt, p_pos, p_seq, 1 if ragged else 0, p_indptr, p_pages,
+                                       page, p_out, hq, hk, scale, ctypes.byref(plan), _ws(plan, workspace),
+                                       _stream_on(stream, d)))
     return out
 
 
@@ -735,10 +697,11 @@ def prompt_run(pp: Prompt, q, k, v, out, scale, stream=None):
     plan = pp.plan
     rows, hq, hk = plan.rows, plan.hq, plan.hk
     d = _device_of(q, "q")
-    (qp, qs), (kp, ks), (vp, vs) = _rows_on(q, "q", rows, hq, d), _rows_on(k, "k", rows, hk, d), _rows_on(v, "v", rows, hk, d)
-    _check(load().omni_attn_prompt_run(ctypes.byref(plan), qp, qs, kp, ks, vp, vs,
-                                       _bf16_on(out, "out", rows * hq * HEAD_DIM, d), scale,
-                                       _i32_on(pp.work, "the plan's work list", 0, d), _stream_on(stream, d)))
+    p_q, q_ld, p_k, k_ld, p_v, v_ld, p_out, p_work = _take(
+        "rrrbi", "q k v out work", d, q, rows, hq * HEAD_DIM, k, rows, hk * HEAD_DIM, v, rows, hk * HEAD_DIM, out,
+        rows * hq * HEAD_DIM, pp.work, 0)
+    _check(load().omni_attn_prompt_run(ctypes.byref(plan), p_q, q_ld, p_k, k_ld, p_v, v_ld, p_out, scale, p_work,
+                                       _stream_on(stream, d)))
     return out
 
 

@@ -241,3 +241,29 @@ def test_the_tables_reference_agrees_with_the_row_builder():
         rows.push(table[s, :(first[s] + count[s] + 15) // 16], first[s], count[s], s)
     for mine, theirs in (("pos", rows.pos), ("slots", rows.slot), ("seq", rows.seq), ("indptr", rows.indptr), ("pages", rows.pages)):
         assert np.array_equal(want[mine], theirs), mine
+
+
+def test_the_checks_of_tensors_name_the_one_at_fault():
+    i, b = torch.zeros(6, dtype=torch.int32), torch.zeros(3, 8, dtype=torch.bfloat16)
+    kv, sc = torch.zeros(2, 4, 2048, dtype=torch.int8), torch.zeros(2, 4, dtype=torch.uint8)
+
+    def said(*a):
+        with pytest.raises(oa.OmniAttnError) as e:
+            oa._take(*a)
+        assert e.value.args
+        return str(e.value)
+
+    assert "x must lie on the current device" in said("i", "x", 0, i, 6)
+    assert "y must be a contiguous int32 tensor of at least 7" in said("Ii", "x y", 0, None, 0, i, 7)
+    assert "y must be a contiguous bf16" in said("Ib", "x y", 0, None, 0, i, 1)
+    assert "contiguous" in said("i", "x", 0, i[::2], 1)
+    assert "rows must be bf16 rows [4][8]" in said("r", "rows", 0, b, 4, 8)
+    assert "rows must be bf16 rows [3][9]" in said("r", "rows", 0, b, 3, 9)
+    assert "adjacent" in said("r", "rows", 0, b.t(), 8, 3)
+    assert "kv must be float8_e4m3fn or int8 [blocks][6][2048]" in said("c", "kv", 0, kv, sc, 6)
+    assert "kv_scale" in said("c", "kv", 0, kv, sc[:1], 4)
+    assert "x must be a tensor" in said("i", "x", 0, 5, 0)
+    assert "x must be a tensor" in said("i", "x", 0, None, 0)
+    assert "too few" in said("i", "x", 0, i) and "too many" in said("I", "x", 0, None, 0, 0)
+    assert "integer" in said("i", "x", 0, i, "6") and "no such kind" in said("z", "x", 0, i, 0, 0)
+    assert oa._take("IRI", "x y z", 0, None, 0, None, 1, 1, None, 0) == (None, None, 0, None)
