@@ -791,7 +791,7 @@ __global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
   const int split = spread_split(blockIdx.x, kh + a.hk * blockIdx.z, a.splits);
   int p;
   const int n = row_of(a, blockIdx.z, gridDim.z, &p);
-  const int32_t* pg = a.pages + a.indptr[a.ragged ? max(a.seq[n], 0) : n];
+  const int32_t* pg = a.pages + a.indptr[!a.ragged ? n : p < 0 ? 0 : max(a.seq[n], 0)];  // no keys: any sequence may stand there
   const int len = p < 0 ? 0 : p + 1;
   const int64_t h0 = (int64_t)n * a.hq + kh * G;
   if (len == 0) {

@@ -34,7 +34,7 @@ int64_t int_of(PyObject* o) {
   const long long v = PyLong_AsLongLong(o);
   if (v == -1 && PyErr_Occurred()) {
     PyErr_Clear();
-    throw Bad{"a count is not an integer"};
+    throw Bad{": a count is not an integer"};
   }
   return v;
 }

@@ -473,3 +473,14 @@ def test_decode_of_many_rows_in_any_order_of_lengths(rows, hk):
     alone = torch.cat([run(lo, min(lo + few, rows)) for lo in range(0, rows, few)])
     assert torch.equal(out, alone)
     assert bool((out[torch.from_numpy(lens <= 0).cuda()] == 0).all())
+
+
+def test_decode_rows_without_keys_may_name_any_sequence():
+    d = Decode([40, 20], 4, 2, 16, torch.int8, rows_of=[(0, 39), (2 ** 31 - 1, -1), (1, 19), (-7, -5)])
+    d.run(max_len=64)
+    assert bool((d.out[[1, 3]] == 0).all())
+    d.rows = [(0, 39), (0, -1), (1, 19), (1, -1)]
+    want = d.out.clone()
+    d.out.fill_(7)
+    d.run(max_len=64)
+    assert torch.equal(d.out, want)
