@@ -556,7 +556,8 @@ _Q8_DTYPES = (_torch.float8_e4m3fn, _torch.int8)
 
 # A call launches on the current device, whose stream it takes: every tensor has
 # to lie there. omni_tensors checks them all in one call (its source lists the
-# kinds); the device is asked for once (the raw call where torch has it).
+# kinds); the device is asked for once (the raw call where torch has it; -1, where
+# nothing lies, if the first tensor is the host's).
 _current_device = getattr(_torch._C, "_cuda_getDevice", None) or _torch.cuda.current_device
 
 
@@ -579,13 +580,6 @@ def _take(*args):
     global _take
     _take = _load_tensors().take
     return _take(*args)
-
-
-def _device_of(t, name):
-    d = t.get_device()
-    if d < 0 or d != _current_device():
-        raise OmniAttnError(EINVAL, f"{name} must lie on the current device")
-    return d
 
 
 def _stream_on(stream, d):
@@ -612,7 +606,7 @@ def step_tables(first, count, lines, table, free_pages, free_state, pos, slots, 
     requests (count < 0) given back. lines None: line s; free_pages None: the
     table holds every page. ``status`` = [code, rows, pages, head, free entries];
     ``status[3:5]`` is the next call's free_state, with another status."""
-    d = _device_of(first, "first")
+    d = _current_device() if first.is_cuda else -1
     n, rows = first.numel(), pos.numel()
     shape = table.shape
     if len(shape) != 2:
@@ -634,7 +628,7 @@ def qwen3_rope_q8(qkv, q_norm, k_norm, pos, slots, q_out, k_out, kv, kv_scale, h
     of the 8-bit cache. Rows may be strided; rows with a negative slot are
     skipped."""
     rows = pos.numel()
-    d = _device_of(qkv, "qkv")
+    d = _current_device() if qkv.is_cuda else -1
     src, ld, p_qn, p_kn, p_pos, p_slots, q, q_ld, k, k_ld, cache, scales, fmt = _take(
         "rbbiirRc", "qkv q_norm k_norm pos slots q_out k_out kv", d, qkv, rows, (hq + 2 * hk) * HEAD_DIM, q_norm, HEAD_DIM,
         k_norm, HEAD_DIM, pos, 0, slots, rows, q_out, rows, hq * HEAD_DIM, k_out, rows, hk * HEAD_DIM, kv, kv_scale, 2 * hk)
@@ -654,7 +648,7 @@ def qwen3_attend_q8(q, kv, kv_scale, pos, seq, ragged, indptr, pages, page, out,
     """``qwen3_attend`` over the 8-bit cache: q rows [hq * 128], possibly strided;
     rows with a negative position store zeros."""
     rows = plan.rows
-    d = _device_of(q, "q")
+    d = _current_device() if q.is_cuda else -1
     src, stride, cache, scales, fmt, p_pos, p_seq, p_indptr, p_pages, p_out = _take(
         "rciIiib", "q kv pos seq indptr pages out", d, q, rows, hq * HEAD_DIM, kv, kv_scale, 2 * hk, pos, rows, seq, rows,
         indptr, 1 if ragged else rows + 1, pages, 0, out, rows * hq * HEAD_DIM)
@@ -696,7 +690,7 @@ def prompt_run(pp: Prompt, q, k, v, out, scale, stream=None):
     [hk * 128], possibly strided (parts of one qkv row); out contiguous rows."""
     plan = pp.plan
     rows, hq, hk = plan.rows, plan.hq, plan.hk
-    d = _device_of(q, "q")
+    d = _current_device() if q.is_cuda else -1
     p_q, q_ld, p_k, k_ld, p_v, v_ld, p_out, p_work = _take(
         "rrrbi", "q k v out work", d, q, rows, hq * HEAD_DIM, k, rows, hk * HEAD_DIM, v, rows, hk * HEAD_DIM, out,
         rows * hq * HEAD_DIM, pp.work, 0)
