@@ -762,27 +762,29 @@ int omni_qwen3_attend_dense(const void* qkv, const void* kv, int per, int base, 
 namespace {
 
 // Split size of a decode bucket over the 8-bit cache: the one with the least
-// estimated time. What a launch takes, us, from sweeps of 17 shapes over splits
+// estimated time. What a launch takes, us, from sweeps of 45 shapes over splits
 // of 64 keys to none (1 to 128 rows, 1 to 32 K/V heads, 300 to 130,000 keys):
 //   the keys' bytes at 6.2 TB/s, with rows 0.6 of max_len long; or, where few
 //   workgroups run, a wave's walk through its tiles, 1.05 for each 32 keys of its
 //   quarter of a split;
-//   2 for each round of 1024 resident workgroups (four a CU);
-//   with splits, 3 for the merge's launch and 1.3 for every 32 splits of a row.
+//   0.19 of a walk for the CUs that end first, 0.1 where unsplit rows start longest first;
+//   0.5 for each 1024 workgroups;
+//   with splits, 3 for the merge's launch and 3 for every 32 splits of a row.
 // Measured at the choice / at the best split of the sweep: 1 row of 2400 keys,
 // hk = 8, 128 keys 8.1 / 8.1; of 8000, 256 keys 10.7 / 10.7; 16 rows of 200-2400
 // 256 keys 15.5 / 15.1; 64 rows none 32.4 / 32.4; 21 rows of 512-5120 512 keys 29.4 /
-// 29.3; 4 rows of 100,000-130,000 4096 keys 162 / 153 (8192); 2 of 60,000, hk = 2, 768
-// keys 25.0 / 22.8 (1024).
+// 29.3; 5 of 20,000-90,000 1536 keys 111 / 108 (2048); 4 of 100,000-130,000 4096 keys
+// 162 / 153 (8192, which rows of unlike lengths cannot fill); 2 of 60,000, hk = 2,
+// 1024 keys 22.4 / 22.4; 1 of 40,000, hk = 1, 768 keys 15.7 / 14.8 (512).
 int pick_chunk_q8(int rows, int hk, int max_len) {
   const double units = (double)rows * hk, read = units * max_len * 0.6 * 256 / 6.2e6;
   int best = 0;
   double least = 0;
   for (int chunk : {128, 256, 384, 512, 768, 1024, 1536, 2048, 4096, 8192, 16384, 32768, 0}) {
     if (chunk == 0 || chunk >= max_len) chunk = (int)std::min<int64_t>(((int64_t)max_len + 63) / 64 * 64, INT_MAX / 64 * 64);
-    const double splits = std::ceil((double)max_len / chunk);
-    const double t = std::max(read, 1.05 * chunk / 128) + 2 * std::ceil(0.6 * units * splits / 1024) +
-                     (splits > 1 ? 3 + 1.3 * std::ceil(splits / 32) : 0);
+    const double splits = std::ceil((double)max_len / chunk), walk = 1.05 * chunk / 128;
+    const double t = std::max(read, walk) + (splits == 1 && units > 256 ? 0.1 : 0.19) * walk + 0.5 * units * splits / 1024 +
+                     (splits > 1 ? 3 + 3 * std::ceil(splits / 32) : 0);
     if (best == 0 || t < least) best = chunk, least = t;
     if (chunk >= max_len) break;
   }

@@ -15,7 +15,7 @@ P = 0x10000  # a made-up, aligned address
 
 # ------------------------------------------------------------------ plans
 @pytest.mark.parametrize("rows,hk,max_len,chunk,splits", [
-    (1, 8, 1, 64, 1), (1, 8, 300, 320, 1), (1, 8, 2400, 128, 19), (1, 8, 8000, 256, 32), (1, 1, 40000, 512, 79),
+    (1, 8, 1, 64, 1), (1, 8, 300, 320, 1), (1, 8, 2400, 128, 19), (1, 8, 8000, 256, 32), (1, 1, 40000, 768, 53),
     (4, 8, 512, 512, 1), (16, 8, 2400, 256, 10), (32, 8, 1000, 1024, 1), (64, 8, 2400, 2432, 1), (21, 8, 5120, 512, 10),
     (128, 32, 3000, 3008, 1), (4, 8, 130000, 4096, 32),
 ])
