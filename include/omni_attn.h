@@ -369,14 +369,20 @@ int64_t omni_hidream_workspace_bytes(void);
  * gets count[s] new rows; count[s] < 0 says that the request is done. Its pages
  * are the entries of line lines[s] (s where lines is NULL) of the block table
  * [num_lines][table_ld], first ones first. With ring > 0 position p lives at
- * index p % ring.
+ * index p % ring, and a step has at most ring rows of a sequence.
  *
  * Written: pos, slots and seq of every new row, sequences in order (slot =
  * page id * page + index % page); row_indptr [nseq + 1], the rows of each
- * sequence; indptr [nseq + 1] and pages, its page ids up to its last new token,
- * as omni_qwen3_attend and omni_qwen3_attend_q8 read them. Rows past the last
+ * sequence; indptr [nseq + 1] and pages, its page ids up to its last new token
+ * (or the ring's last), as the paged attentions read them. Rows past the last
  * get pos, slots and seq -1 (up to row_cap); pages past the last stay as they
  * were.
+ * A ring's tables are for the calls that cap a row's keys with context = ring:
+ * omni_lm_attend, omni_lm_attend_fp8 and omni_lm_rope_attend_fp8, after one new
+ * token a sequence. omni_qwen3_attend, the prefill and the calls over the 8-bit
+ * cache (omni_qwen3_rope_q8, omni_qwen3_attend_q8) know no ring: they see keys
+ * 0..pos, and past the ring would look up pages that the sequence does not
+ * list. They take tables made with ring = 0 only.
  *
  * Pages come from the free queue: entries head, head + 1, .. (modulo num_pages)
  * of free_pages [num_pages], num_pages being the pool's pages, with free_state =
@@ -389,7 +395,7 @@ int64_t omni_hidream_workspace_bytes(void);
  * next call's free_state (so two status buffers take turns: free_state must not
  * lie in status). code 0: done. Otherwise nothing is taken, all rows are -1,
  * row_indptr and indptr are zeros, and code says why: */
-#define OMNI_ATTN_TABLES_BAD 1       /* negative first, position past int32, line or free_state out of range */
+#define OMNI_ATTN_TABLES_BAD 1       /* negative first, position past int32, count > ring, line or free_state out of range */
 #define OMNI_ATTN_TABLES_ROWS 2      /* more rows than row_cap */
 #define OMNI_ATTN_TABLES_PAGES 3     /* more pages than page_cap */
 #define OMNI_ATTN_TABLES_LINE 4      /* a sequence needs more than table_ld pages */
@@ -415,8 +421,9 @@ int omni_attn_step_tables(const int32_t* first, const int32_t* count, const int3
  * rows (rows of a sequence do), in any order; of rows with one slot the last
  * counts; a block whose rows stand further apart is left unspecified. The
  * block's other tokens stay, re-rounded if the exponent grows; but rows that
- * hold its first slot start it anew (the other tokens become zeros). So a ring
- * that wraps inside a block is not served.
+ * hold its first slot start it anew (the other tokens become zeros). So rings are
+ * not served, whatever their size: a row that comes back to a block's first slot
+ * clears 15 tokens that are still in the window.
  *
  * NaN and infinities do not count for the exponent. E4M3 stores both as NaN;
  * integers store NaN as 0 and infinities as +-127. Row strides are multiples of

@@ -36,7 +36,9 @@ __device__ __forceinline__ SeqShare seq_share(const TablesArgs& a, int s) {
   SeqShare r{};
   const int first = a.first[s], count = a.count[s];
   r.line = a.lines ? a.lines[s] : s;
-  if (first < 0 || (count > 0 && first > 0x7fffffff - count) || r.line < 0 || r.line >= a.num_lines) {
+  // More rows than a ring holds would give several of them one slot.
+  if (first < 0 || (count > 0 && first > 0x7fffffff - count) || (a.ring > 0 && count > a.ring) || r.line < 0 ||
+      r.line >= a.num_lines) {
     r.code = 1;
     return r;
   }

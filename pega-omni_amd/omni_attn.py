@@ -605,7 +605,9 @@ def step_tables(first, count, lines, table, free_pages, free_state, pos, slots, 
     [head, free entries]) into ``table`` [lines][pages per line], pages of done
     requests (count < 0) given back. lines None: line s; free_pages None: the
     table holds every page. ``status`` = [code, rows, pages, head, free entries];
-    ``status[3:5]`` is the next call's free_state, with another status."""
+    ``status[3:5]`` is the next call's free_state, with another status. ring > 0:
+    tables for the calls with a context cap (``lm_attend`` with context = ring),
+    not for the 8-bit cache's."""
     d = _current_device() if first.is_cuda else -1
     n, rows = first.numel(), pos.numel()
     shape = table.shape
