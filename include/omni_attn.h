@@ -233,7 +233,8 @@ int omni_attn_prefill_plan_init(int rows, int hq, int hk, int page, const int32_
 /* Ragged causal prefill with the semantics of qwen3_attend(ragged = 1): row n
  * sees keys 0..pos[n] of sequence seq[n] through the page table. `work` is
  * the device copy of the plan's work list. A row's bits depend on its own
- * keys and position alone, not on the other rows or tiles of the call. */
+ * keys and position alone, not on the other rows or tiles of the call. Any
+ * finite scale, zero and negative ones too (and so the DiT calls below). */
 int omni_attn_prefill_run(const omni_attn_prefill_plan* plan, const void* qkv, const void* kv, const int32_t* pos,
                           const int32_t* seq, const int32_t* indptr, const int32_t* pages, void* out, float scale,
                           const int32_t* work, void* stream);

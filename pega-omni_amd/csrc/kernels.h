@@ -91,7 +91,8 @@ struct TiledArgs {
   int64_t q_bstride, kv_bstride, out_bstride;
   bf16_t* out;
   int hq, hk;
-  float scale_log2;
+  float scale_log2;  // any finite value
+  uint32_t q_sign;   // set by the launch: flips the signs of two bf16 of Q where the scale is negative
   // Tail split (dense, uniform key ranges): items >= split_from run as
   // split_k key chunks each, writing f32 partials to ws (one segment per
   // chunk: O[128 rows][128] then (m, l)[128 rows]); 0 chunks = no split.

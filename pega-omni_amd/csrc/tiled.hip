@@ -477,6 +477,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   for (int kk = 0; kk < 8; ++kk) {
     uint4 u = *reinterpret_cast<const uint4*>(q_lds + (k_lane ^ (16 * kk)));
     if (!row_ok) u = make_uint4(0, 0, 0, 0);
+    u.x ^= a.q_sign, u.y ^= a.q_sign, u.z ^= a.q_sign, u.w ^= a.q_sign;
     qf[kk] = as_bf16x8(u);
   }
   __syncthreads();
@@ -919,9 +920,16 @@ void launch_g(const TiledArgs& a, int grid, int items, int ntiles, hipStream_t s
 }
 
 template <int SRC>  // kDense, kPacked, or kPagedWave for any page size
-int launch_tiled(const TiledArgs& a, int items, int ntiles, hipStream_t stream) {
+int launch_tiled(TiledArgs a, int items, int ntiles, hipStream_t stream) {
   constexpr bool LISTED = SRC != kDense;
   if (items <= 0) return 0;
+  // The kernel takes masks and maxima of the raw scores, so the factor behind them
+  // is positive: a negative scale's sign goes to Q. And a masked key's -inf times 0
+  // would be NaN: the least positive factor leaves it -inf and weighs every key
+  // that a row sees alike.
+  a.q_sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  a.scale_log2 = fabsf(a.scale_log2);
+  if (a.scale_log2 == 0.f) a.scale_log2 = 0x1p-149f;
   // Pages that are no multiple of a wave's rows keep whole tiles.
   const bool lane_pages = SRC == kPagedWave && a.pd.page % kRowsPerWave != 0;
   const bool parts = !lane_pages && (LISTED || a.split_k == 0);
