@@ -791,6 +791,8 @@ int pick_chunk_q8(int rows, int hk, int max_len) {
   return best;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;  // the kernels take exponentials to base 2
+
 int q8_format(int format, const char* who) {
   if (format != OMNI_ATTN_Q8_E4M3 && format != OMNI_ATTN_Q8_INT8)
     return fail(OMNI_ATTN_EINVAL, "%s: format=%d", who, format);
@@ -946,7 +948,7 @@ int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const 
     return fail(OMNI_ATTN_EINVAL, "%s: q, kv and out must be 16-byte aligned", who);
   if (!row_stride_ok(q_stride, hq))
     return fail(OMNI_ATTN_EINVAL, "%s: q_stride=%lld: a multiple of 8 that holds a row", who, (long long)q_stride);
-  if (!std::isfinite(scale)) return fail(OMNI_ATTN_EINVAL, "%s: non-finite scale", who);
+  if (!std::isfinite(scale * kLog2e)) return fail(OMNI_ATTN_EINVAL, "%s: scale * log2(e) is not finite", who);
   if (plan->splits > 1 && !workspace)
     return fail(OMNI_ATTN_EWORKSPACE, "%s: plan needs %lld workspace bytes", who, (long long)plan->workspace_bytes);
   if (!aligned16(workspace)) return fail(OMNI_ATTN_EINVAL, "%s: workspace must be 16-byte aligned", who);
@@ -969,7 +971,7 @@ int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const 
   a.pd = omni::make_page_div(page / 16);
   a.chunk = plan->chunk;
   a.splits = plan->splits;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2e;
   if (omni::launch_decode_q8(a, plan->rows, as_stream(stream)) != 0)
     return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));
   return ok();
@@ -1040,7 +1042,7 @@ int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64
       k_stride > omni::kMostPromptStride || v_stride > omni::kMostPromptStride)
     return fail(OMNI_ATTN_EINVAL, "prompt_run: row strides %lld / %lld / %lld: multiples of 8 that hold a row, k and v at most %lld",
                 (long long)q_stride, (long long)k_stride, (long long)v_stride, (long long)omni::kMostPromptStride);
-  if (!std::isfinite(scale)) return fail(OMNI_ATTN_EINVAL, "prompt_run: non-finite scale");
+  if (!std::isfinite(scale * kLog2e)) return fail(OMNI_ATTN_EINVAL, "prompt_run: scale * log2(e) is not finite");
   omni::TiledArgs a{};
   a.q = static_cast<const omni::bf16_t*>(q);
   a.q_stride = q_stride;
@@ -1053,7 +1055,7 @@ int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64
   a.out = static_cast<omni::bf16_t*>(out);
   a.hq = plan->hq;
   a.hk = plan->hk;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2e;
   a.exact_p = plan->exact_p;
   const int resident = resident_tiled_groups();
   a.quarters = omni::tiled_quarters(items, resident);
