@@ -5,6 +5,8 @@ Every source under csrc/ is compiled to an object in _build/ and linked into
 pega-omni_amd/libomni_attn.so, the library the C ABI in include/omni_attn.h
 names. mirror/tensors.cpp (host code, against torch's headers) becomes
 pega-omni_amd/omni_tensors.so, the Python mirror's checks of a call's tensors.
+The library needs neither torch nor g++: it is linked whatever becomes of that
+helper, which is left out where torch cannot be imported.
 """
 from __future__ import annotations
 
@@ -52,8 +54,12 @@ def _compile(src: str) -> str:
 
 
 def _build_tensors() -> None:
-    import torch
-
+    try:
+        import torch
+    except (ImportError, OSError) as e:
+        print(f"{TENSORS} not built, torch cannot be imported ({e}): the C library does not need it, the Python "
+              "mirror's 8-bit calls do", file=sys.stderr)
+        return
     root = os.path.dirname(torch.__file__)
     inc, lib = os.path.join(root, "include"), os.path.join(root, "lib")
     tmp = TENSORS + ".tmp"
@@ -72,15 +78,15 @@ def build(verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=4) as ex:
         tensors = ex.submit(_build_tensors)
         objs = list(ex.map(_compile, sources()))
+        tmp = OUT + ".tmp"
+        cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"link failed:\n{r.stderr}")
+        os.replace(tmp, OUT)
+        if verbose:
+            print(f"built {OUT}")
         tensors.result()
-    tmp = OUT + ".tmp"
-    cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stderr}")
-    os.replace(tmp, OUT)
-    if verbose:
-        print(f"built {OUT}")
     return OUT
 
 
