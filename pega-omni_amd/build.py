@@ -63,7 +63,9 @@ def _build_tensors() -> None:
     root = os.path.dirname(torch.__file__)
     inc, lib = os.path.join(root, "include"), os.path.join(root, "lib")
     tmp = TENSORS + ".tmp"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+    built_for = "torch %s, Python %d.%d" % (torch.__version__, *sys.version_info[:2])
+    cmd = ["g++", f'-DOMNI_BUILT_FOR="{built_for}"', "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
            "-I" + sysconfig.get_paths()["include"], os.path.join(HERE, "mirror", "tensors.cpp"), "-o", tmp,
            "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10"]

@@ -162,4 +162,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "omni_tensors", "The Python mirror'
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_omni_tensors() { return PyModule_Create(&module); }
+// The torch and Python whose headers it was compiled with: it reads their objects, so the mirror loads it beside no other.
+#ifndef OMNI_BUILT_FOR
+#error "build.py names the versions"
+#endif
+
+PyMODINIT_FUNC PyInit_omni_tensors() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", OMNI_BUILT_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 from dataclasses import dataclass
 
 # torch brings its own HIP runtime; it is loaded before the library so that the
@@ -571,6 +572,9 @@ def _load_tensors():
     loader = importlib.machinery.ExtensionFileLoader("omni_tensors", path)
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("omni_tensors", loader))
     loader.exec_module(module)
+    here = "torch %s, Python %d.%d" % (_torch.__version__, *sys.version_info[:2])
+    if module.built_for != here:
+        raise OmniAttnError(ELAUNCH, f"{path} was built for {module.built_for}, this is {here}: build it again")
     module.set_error(OmniAttnError, EINVAL)
     return module
 

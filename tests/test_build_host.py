@@ -48,3 +48,10 @@ def test_a_helper_that_does_not_compile_leaves_the_library(build):
     with pytest.raises(RuntimeError, match="tensors.cpp"):
         build.build()
     assert os.path.exists(build.OUT)
+
+
+def test_a_helper_of_another_torch_is_not_used(monkeypatch):
+    """It reads torch's objects by the layout of the headers that it was compiled with."""
+    monkeypatch.setattr(oa._torch, "__version__", "1.0.0")
+    with pytest.raises(oa.OmniAttnError, match="built for torch .*, this is torch 1.0.0"):
+        oa._load_tensors()
