@@ -428,13 +428,15 @@ int omni_attn_step_tables(const int32_t* first, const int32_t* count, const int3
  *
  * NaN and infinities do not count for the exponent. E4M3 stores both as NaN;
  * integers store NaN as 0 and infinities as +-127. Row strides are multiples of
- * 8 elements. */
+ * 8 elements. A call that no grid holds (2^24 rows; some 40,000 K/V heads) is
+ * OMNI_ATTN_EUNSUPPORTED, with nothing launched. */
 int omni_qwen3_rope_q8(const void* qkv, int64_t ld, const void* q_norm, const void* k_norm, const int32_t* pos,
                        const int32_t* slots, void* q_out, int64_t q_ld, void* k_out, int64_t k_ld, void* kv,
                        void* kv_scale, int format, int rows, int hq, int hk, float eps, float theta, void* stream);
 
 /* The plan for omni_qwen3_attend_q8: hq / hk from 1 to 16, page a multiple of
- * 16, chunk_hint a multiple of 64 (<= 0 picks from the shape). */
+ * 16, chunk_hint a multiple of 64 (<= 0 picks from the shape). Below 2^24 splits,
+ * and where there is more than one, rows * hq below 2^24. */
 int omni_attn_decode_plan_init_q8(int rows, int hq, int hk, int page, int max_len, int chunk_hint,
                                   omni_attn_decode_plan* plan);
 

@@ -859,7 +859,7 @@ int omni_qwen3_rope_q8(const void* qkv, int64_t ld, const void* q_norm, const vo
   if (rows < 0) return fail(OMNI_ATTN_EINVAL, "%s: rows=%d", who, rows);
   if (hq <= 0 || hk <= 0) return fail(OMNI_ATTN_EINVAL, "%s: hq=%d hk=%d", who, hq, hk);
   if (int rc = q8_format(format, who)) return rc;
-  if ((int64_t)hk + (hq + 15) / 16 > 65535) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many heads", who);
+  if (hk > 65535) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: hk=%d", who, hk);
   if (rows == 0) return ok();
   if (int rc = norm_rope_checks(q_norm, k_norm, eps, theta, who)) return rc;
   if (!qkv || !pos || !slots || !q_out || !kv || !kv_scale) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
@@ -887,7 +887,9 @@ int omni_qwen3_rope_q8(const void* qkv, int64_t ld, const void* q_norm, const vo
   a.hk = hk;
   a.eps = eps;
   a.inv_theta64 = std::pow((double)theta, -1.0 / 64.0);
-  if (omni::launch_rope_q8(a, as_stream(stream)) != 0)
+  const int rc = omni::launch_rope_q8(a, as_stream(stream));
+  if (rc == -2) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: rows=%d hq=%d hk=%d in one call", who, rows, hq, hk);
+  if (rc != 0)
     return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));
   return ok();
 }
@@ -918,6 +920,8 @@ int omni_attn_decode_plan_init_q8(int rows, int hq, int hk, int page, int max_le
   plan->max_len = max_len;
   plan->chunk = chunk;
   plan->splits = (int32_t)(((int64_t)max_len + chunk - 1) / chunk);
+  if (!omni::decode_q8_fits(rows, hq, plan->splits))
+    return fail(OMNI_ATTN_EUNSUPPORTED, "decode_plan_q8: rows=%d hq=%d in %d splits", rows, hq, plan->splits);
   plan->workspace_bytes =
       plan->splits > 1 ? (int64_t)rows * hq * plan->splits * (OMNI_ATTN_HEAD_DIM + 1) * (int64_t)sizeof(float) : 0;
   return ok();
@@ -941,6 +945,8 @@ int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const 
        plan->workspace_bytes < (int64_t)plan->rows * hq * plan->splits * (OMNI_ATTN_HEAD_DIM + 1) * (int64_t)sizeof(float)))
     return fail(OMNI_ATTN_EINVAL, "%s: plan is not self-consistent (rows=%d max_len=%d chunk=%d splits=%d group_heads=%d)",
                 who, plan->rows, plan->max_len, plan->chunk, plan->splits, plan->group_heads);
+  if (!omni::decode_q8_fits(plan->rows, hq, plan->splits))
+    return fail(OMNI_ATTN_EUNSUPPORTED, "%s: rows=%d hq=%d in %d splits", who, plan->rows, hq, plan->splits);
   if (plan->rows == 0) return ok();
   if (!q || !kv || !kv_scale || !pos || !indptr || !pages || !out || (ragged && !seq))
     return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
@@ -995,7 +1001,7 @@ int omni_attn_prompt_plan_init(int nseq, const int32_t* lens_h, int hq, int hk, 
     tiles += ((int64_t)lens_h[s] + per_tile - 1) / per_tile;
   }
   const int64_t items = tiles * hk;
-  if (rows > INT_MAX || items > (INT_MAX - omni::kPrefillWorkHeader) / 4)
+  if (rows > INT_MAX || !omni::grid_holds(items + omni::kXcds - 1, omni::kTiledThreads))
     return fail(OMNI_ATTN_EUNSUPPORTED, "prompt_plan: too many rows or tiles");
   plan->nseq = nseq;
   plan->rows = (int32_t)rows;
@@ -1033,6 +1039,8 @@ int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64
                 "prompt_run: plan is not one prompt_plan_init made (rows=%d tiles=%d hq=%d hk=%d tile_rows=%d workgroups=%d "
                 "exact_p=%d)",
                 plan->rows, plan->tiles, plan->hq, plan->hk, plan->tile_rows, plan->workgroups, plan->exact_p);
+  if (!omni::grid_holds(plan->workgroups, omni::kTiledThreads))
+    return fail(OMNI_ATTN_EUNSUPPORTED, "prompt_run: %d workgroups", plan->workgroups);
   if (plan->tiles == 0) return ok();
   if (!q || !k || !v || !out || !work) return fail(OMNI_ATTN_EINVAL, "prompt_run: null device pointer");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))

@@ -16,6 +16,13 @@ inline int check_launch() {
   return g_launch_status == hipSuccess ? 0 : -3;
 }
 
+// What a launch holds: fewer than 2^32 threads in x, at most 65,535 workgroups in y and z.
+constexpr int64_t kMostGridThreads = (1LL << 32) - 1;
+constexpr int kMostGridYZ = 65535;
+inline bool grid_holds(int64_t x, int threads, int64_t y = 1) {
+  return x * threads <= kMostGridThreads && y <= kMostGridYZ;
+}
+
 // Everything a decode launch reads; passed by value as the kernel argument.
 struct DecodeArgs {
   const bf16_t* qkv;
@@ -112,6 +119,7 @@ struct TiledArgs {
 // Packed (position, head) query rows per MFMA tile: one 8-wave workgroup, one per CU.
 constexpr int kTiledRows = 256;
 // Bytes of one partial segment of the tail split: O (f32) and (m, l) per packed row.
+constexpr int kTiledThreads = kTiledRows * 2;  // a wave for each 32 rows
 constexpr int64_t kSegmentBytes = (int64_t)kTiledRows * (128 + 2) * 4;
 
 // Prefill work list: a header of kPrefillWorkHeader int32 (entries 0..8: the
@@ -218,7 +226,7 @@ struct RopeQ8Args {
   float eps;
   double inv_theta64;  // theta^(-1/64): pair i turns by pos * inv_theta64^i
 };
-int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream);
+int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream);  // -2: more rows or heads than a grid holds, nothing launched
 
 struct DecodeQ8Args {
   const bf16_t* q;
@@ -241,6 +249,11 @@ struct DecodeQ8Args {
   int len_shift;   // row lengths >> len_shift fit 6 bits (longer ones count as 63)
   float scale_log2;
 };
+constexpr int kQ8Threads = 256;  // of every workgroup of the 8-bit cache's kernels
+// Whether decode's grid and (of splits) the merge's hold a call.
+inline bool decode_q8_fits(int rows, int hq, int splits) {
+  return grid_holds(splits, kQ8Threads) && (splits == 1 || grid_holds((int64_t)rows * hq, kQ8Threads));
+}
 int launch_decode_q8(DecodeQ8Args a, int rows, hipStream_t stream);
 
 }  // namespace omni

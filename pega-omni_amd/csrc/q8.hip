@@ -17,7 +17,7 @@ namespace omni {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kQ8Threads;
 
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 
@@ -1035,10 +1035,11 @@ __global__ __launch_bounds__(kThreads) void merge_q8(DecodeQ8Args a) {
 constexpr int64_t kManyHeads = 1 << 17;
 
 int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream) {
-  const unsigned T = (unsigned)((a.rows + 15) / 16);
+  const unsigned T = (unsigned)(((int64_t)a.rows + 15) / 16);
   if ((int64_t)a.rows * (a.hq + 2 * (int64_t)a.hk) < kManyHeads) {
     const int alone = (a.hk + 1) / 2;
     const dim3 grid(16 / kLeads * T, alone + a.hk + (a.hq + 3) / 4);
+    if (!grid_holds(grid.x, kThreads, grid.y)) return -2;
     if (a.format == kQ8E4m3)
       rope_q8_rows<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a, alone);
     else
@@ -1047,14 +1048,16 @@ int launch_rope_q8(const RopeQ8Args& a, hipStream_t stream) {
   }
   // The K/V heads of a block over as many workgroups as give a prompt 1024 that lead.
   const dim3 grid(16 / kLeads * T, std::min<unsigned>(a.hk, (1024 + T - 1) / T));
+  int shift = 0;
+  while (shift < 4 && (16 >> (shift + 1)) >= a.hq) ++shift;
+  const int64_t q_groups = ((int64_t)a.rows + (1 << shift) - 1) >> shift;
+  if (!grid_holds(grid.x, kThreads) || !grid_holds(q_groups, kThreads)) return -2;
   if (a.format == kQ8E4m3)
     rope_q8_blocks<kQ8E4m3><<<grid, kThreads, 0, stream>>>(a);
   else
     rope_q8_blocks<kQ8Int8><<<grid, kThreads, 0, stream>>>(a);
   if (check_launch() != 0) return -3;
-  int shift = 0;
-  while (shift < 4 && (16 >> (shift + 1)) >= a.hq) ++shift;
-  turn_q_rows<<<dim3((unsigned)(((int64_t)a.rows + (1 << shift) - 1) >> shift)), kThreads, 0, stream>>>(a, shift);
+  turn_q_rows<<<dim3((unsigned)q_groups), kThreads, 0, stream>>>(a, shift);
   return check_launch();
 }
 

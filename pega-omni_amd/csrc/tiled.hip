@@ -38,6 +38,7 @@ constexpr int kBN = 128;         // keys per tile
 constexpr int kMB = kBN / 32;    // 32-key blocks per tile
 constexpr int kWaves = kTiledRows / 32;  // one 32-row query block per wave
 constexpr int kThreads = 64 * kWaves;
+static_assert(kThreads == kTiledThreads);
 constexpr int kRowsPerWave = kBN / kWaves;  // K/V tile rows each wave loads
 constexpr int kDmas = 2 * kRowsPerWave / 4;  // LDS DMAs a wave issues per tile: K rows, then V rows
 // LDS per buffer: the K tile then the V tile, each [128 keys][128] bf16 in
