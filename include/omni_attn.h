@@ -443,7 +443,8 @@ int omni_attn_decode_plan_init_q8(int rows, int hq, int hk, int page, int max_le
 /* omni_qwen3_attend over the 8-bit cache: row n of sequence s = ragged ? seq[n] :
  * n sees keys 0..pos[n]; a row with pos[n] < 0 stores zeros (seq[n] is not
  * read). q rows [hq][128] of stride q_stride (a multiple of 8). P is carried in
- * 16 bits. Tokens past pos[n] may hold anything, and pages past its last are not
+ * 16 bits. Sums are of p V with p <= 1 and divided at the end: |V| summed over a
+ * row's keys so weighted has to stay below 2^128. Tokens past pos[n] may hold anything, and pages past its last are not
  * looked at. A workspace serves one call at a time: two captured graphs that may
  * run at once need one each. */
 int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const void* kv_scale, int format,

@@ -896,11 +896,12 @@ __global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
 #pragma unroll
     for (int t = 1; t < 8; ++t) mx = fmaxf(mx, s[t]);
     mx = max_of_groups(mx);
-    // The base moves only when the maximum grows by more than 8 (log2): p <= 2^8.
-    const bool grow = mx > m + 8.f;
+    // The base is set 8 (log2) above the maximum and moves when one passes it: it
+    // seldom moves, and p <= 1, so p V is no larger than V.
+    const bool grow = mx > m;
     if (__any(grow)) {
-      const float alpha = grow ? fast_exp2(m - mx) : 1.f;
-      m = grow ? mx : m;
+      const float to = mx + 8.f, alpha = grow ? fast_exp2(m - to) : 1.f;
+      m = grow ? to : m;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] *= alpha;
