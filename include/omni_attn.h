@@ -38,7 +38,7 @@ extern "C" {
 
 #define OMNI_ATTN_OK 0
 #define OMNI_ATTN_EINVAL (-1)       /* bad argument (null pointer, negative size) */
-#define OMNI_ATTN_EUNSUPPORTED (-2) /* shape the kernels do not implement */
+#define OMNI_ATTN_EUNSUPPORTED (-2) /* shape the kernels do not implement, or a plan past the host's memory */
 #define OMNI_ATTN_ELAUNCH (-3)      /* the HIP launch failed */
 #define OMNI_ATTN_EWORKSPACE (-4)   /* workspace missing or too small */
 #define OMNI_ATTN_ETABLE (-5)       /* page table / indptr failed host validation */

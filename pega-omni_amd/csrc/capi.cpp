@@ -360,7 +360,7 @@ int omni_attn_gather_kv(const void* kv, int hk, const int32_t* indptr, const int
 
 
 int omni_attn_prefill_plan_init(int rows, int hq, int hk, int page, const int32_t* seq_h, const int32_t* pos_h,
-                                int32_t* work_h, int64_t work_cap, omni_attn_prefill_plan* plan) {
+                                int32_t* work_h, int64_t work_cap, omni_attn_prefill_plan* plan) try {
   if (!plan) return fail(OMNI_ATTN_EINVAL, "prefill_plan: null plan");
   std::memset(plan, 0, sizeof *plan);
   if (rows < 0) return fail(OMNI_ATTN_EINVAL, "prefill_plan: rows=%d", rows);
@@ -405,6 +405,8 @@ int omni_attn_prefill_plan_init(int rows, int hq, int hk, int page, const int32_
     return fail(OMNI_ATTN_EWORKSPACE, "prefill_plan: work list needs %lld int32", (long long)need);
   plan->workgroups = write_work_list(tl, hk, work_h);
   return ok();
+} catch (const std::bad_alloc&) {
+  return fail(OMNI_ATTN_EUNSUPPORTED, "prefill_plan: no host memory for the tiles of %d rows", rows);
 }
 
 int omni_attn_prefill_run(const omni_attn_prefill_plan* plan, const void* qkv, const void* kv, const int32_t* pos,
@@ -984,7 +986,7 @@ int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const 
 }
 
 int omni_attn_prompt_plan_init(int nseq, const int32_t* lens_h, int hq, int hk, int32_t* work_h, int64_t work_cap,
-                               omni_attn_prompt_plan* plan) {
+                               omni_attn_prompt_plan* plan) try {
   if (!plan) return fail(OMNI_ATTN_EINVAL, "prompt_plan: null plan");
   std::memset(plan, 0, sizeof *plan);
   if (nseq < 0 || (nseq > 0 && !lens_h)) return fail(OMNI_ATTN_EINVAL, "prompt_plan: nseq=%d, null lengths", nseq);
@@ -1023,6 +1025,8 @@ int omni_attn_prompt_plan_init(int nseq, const int32_t* lens_h, int hq, int hk, 
     }
   plan->workgroups = write_work_list(tl, hk, work_h);
   return ok();
+} catch (const std::bad_alloc&) {
+  return fail(OMNI_ATTN_EUNSUPPORTED, "prompt_plan: no host memory for the tiles of %d prompts", nseq);
 }
 
 int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64_t q_stride, const void* k,

@@ -1,5 +1,9 @@
 """What the 8-bit serving calls refuse at the ends of their arguments' ranges,
 without a GPU: nothing here is launched (pointers are made up)."""
+import os
+import subprocess
+import sys
+
 import pytest
 
 import omni_attn as oa
@@ -48,3 +52,31 @@ def test_prompts_that_no_grid_holds():
     with pytest.raises(oa.OmniAttnError) as e:
         oa.prompt_plan(lens, 4, 2, device="cpu")
     assert e.value.code == oa.EUNSUPPORTED
+
+
+NO_MEMORY = """
+import ctypes, resource, sys
+import numpy as np
+import omni_attn as oa
+L = oa.load()
+p = lambda a: a.ctypes.data_as(ctypes.c_void_p)
+if sys.argv[1] == "prompt":
+    lens, work, plan = np.array([1 << 27], np.int32), np.zeros(16 + 4 * (1 << 22), np.int32), oa.PromptPlan()
+    call = lambda: L.omni_attn_prompt_plan_init(1, p(lens), 8, 1, p(work), len(work), ctypes.byref(plan))
+else:  # a tile for every row
+    pos, work, plan = np.zeros(1 << 21, np.int32), np.zeros(16 + 4 * (1 << 21), np.int32), oa.PrefillPlan()
+    call = lambda: L.omni_attn_prefill_plan_init(1 << 21, 8, 1, 16, p(pos), p(pos), p(work), len(work), ctypes.byref(plan))
+size = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize() + (4 << 20)
+resource.setrlimit(resource.RLIMIT_AS, (size, size))
+rc = call()
+assert rc == oa.EUNSUPPORTED and b"memory" in L.omni_attn_last_error(), rc
+print("refused")
+"""
+
+
+@pytest.mark.parametrize("which", ["prompt", "prefill"])
+def test_plans_without_host_memory_return_an_error(which):
+    """A plan's tiles (64 and 32 MiB here) are host memory; where there is none the C call says so, and throws nothing."""
+    here = os.path.dirname(oa.__file__)
+    r = subprocess.run([sys.executable, "-c", NO_MEMORY, which], capture_output=True, text=True, env={**os.environ, "PYTHONPATH": here})
+    assert r.returncode == 0 and "refused" in r.stdout, (r.returncode, r.stderr[-500:])
