@@ -699,7 +699,7 @@ def prompt_run(pp: Prompt, q, k, v, out, scale, stream=None):
     d = _current_device() if q.is_cuda else -1
     p_q, q_ld, p_k, k_ld, p_v, v_ld, p_out, p_work = _take(
         "rrrbi", "q k v out work", d, q, rows, hq * HEAD_DIM, k, rows, hk * HEAD_DIM, v, rows, hk * HEAD_DIM, out,
-        rows * hq * HEAD_DIM, pp.work, 0)
+        rows * hq * HEAD_DIM, pp.work, plan.work_bytes >> 2)
     _check(load().omni_attn_prompt_run(ctypes.byref(plan), p_q, q_ld, p_k, k_ld, p_v, v_ld, p_out, scale, p_work,
                                        _stream_on(stream, d)))
     return out
