@@ -35,3 +35,32 @@ def test_values_of_v_up_to_2_to_121(fmt, rise):
         d.run(chunk=chunk, scale=scale)
         assert bool(d.out.isfinite().all())
         d.check(scale)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("chunk", [0, 64])
+def test_pages_and_blocks_past_a_row_are_not_followed(page, chunk):
+    """Page ids past a row's last key name a page of NaN bytes with exponents of 255 (infinity): whatever weighs one of
+    its blocks, even by 0, is NaN. The blocks past the row in its last page hold the same."""
+    lens, at = [17, 16, 100, 300, 200], [3, 15, 63, 100, 199]
+    d = Decode(lens, 8, 2, page, torch.float8_e4m3fn, seed=page, rows_of=list(enumerate(at)))
+    per = page // 16
+    spare = next(p for p in range(d.kv.shape[0] // per) if p not in d.pages)
+
+    def poison(block):
+        d.kv.view(torch.uint8)[block] = 0x7F
+        d.sc.view(torch.uint8)[block] = 255
+
+    for b in range(per):
+        poison(spare * per + b)
+    for s, p in d.rows:
+        lo, hi = int(d.indptr[s]), int(d.indptr[s + 1])
+        last = lo + p // page
+        for b in range(p % page // 16 + 1, per):
+            poison(int(d.pages[last]) * per + b)
+        d.pages[last + 1:hi] = spare
+    assert (d.pages == spare).sum() > 0
+    d.run(chunk=chunk)
+    d.check()
+    d.run(chunk=chunk, ragged=False, max_len=400)
+    d.check()
