@@ -402,8 +402,9 @@ int64_t omni_hidream_workspace_bytes(void);
 #define OMNI_ATTN_TABLES_LINE 4      /* a sequence needs more than table_ld pages */
 #define OMNI_ATTN_TABLES_EXHAUSTED 5 /* fewer free pages than the step needs */
 /* The lowest that applies. Sequences of a call have different lines (a done
- * request's line is free from the next call on), and the table's and the
- * queue's page ids are the caller's to keep in the pool. Calls that share a
+ * request's line is free from the next call on), but for those that hold and get
+ * nothing (first = count = 0, the padding of a captured call). The table's and
+ * the queue's page ids are the caller's to keep in the pool. Calls that share a
  * table or a queue follow one another on a stream. */
 int omni_attn_step_tables(const int32_t* first, const int32_t* count, const int32_t* lines, int nseq, int page, int ring,
                           int32_t* table, int64_t table_ld, int num_lines, int32_t* free_pages, int num_pages,
@@ -442,11 +443,14 @@ int omni_attn_decode_plan_init_q8(int rows, int hq, int hk, int page, int max_le
 
 /* omni_qwen3_attend over the 8-bit cache: row n of sequence s = ragged ? seq[n] :
  * n sees keys 0..pos[n]; a row with pos[n] < 0 stores zeros (seq[n] is not
- * read). q rows [hq][128] of stride q_stride (a multiple of 8). P is carried in
- * 16 bits. Sums are of p V with p <= 1 and divided at the end: |V| summed over a
- * row's keys so weighted has to stay below 2^128. Tokens past pos[n] may hold anything, and pages past its last are not
- * looked at. A workspace serves one call at a time: two captured graphs that may
- * run at once need one each. */
+ * read; without ragged indptr has rows + 1 entries, and those of such rows may
+ * hold anything). q rows [hq][128] of stride q_stride (a multiple of 8). P is
+ * carried in 16 bits. Sums are of p V with p <= 1 and divided at the end: |V|
+ * summed over a row's keys so weighted has to stay below 2^128. Tokens past
+ * pos[n] may hold anything, and pages past its last are not looked at. Every row
+ * reads its keys for itself, the rows of one sequence (ragged) too. A workspace
+ * serves one call at a time: two captured graphs that may run at once need one
+ * each. */
 int omni_qwen3_attend_q8(const void* q, int64_t q_stride, const void* kv, const void* kv_scale, int format,
                          const int32_t* pos, const int32_t* seq, int ragged, const int32_t* indptr, const int32_t* pages,
                          int page, void* out, int hq, int hk, float scale, const omni_attn_decode_plan* plan,

@@ -102,7 +102,7 @@ struct TiledArgs {
   uint32_t q_sign;   // set by the launch: flips the signs of two bf16 of Q where the scale is negative
   // Tail split (dense, uniform key ranges): items >= split_from run as
   // split_k key chunks each, writing f32 partials to ws (one segment per
-  // chunk: O[128 rows][128] then (m, l)[128 rows]); 0 chunks = no split.
+  // chunk: O[kTiledRows][128] then (m, l)[kTiledRows]); 0 chunks = no split.
   int split_from, split_k;
   float* ws;
   // Row halves (no split): the last `halved` items (prefill: all or none) run

@@ -562,8 +562,9 @@ __global__ __launch_bounds__(kThreads, 6) void rope_q8_rows(RopeQ8Args a, int al
 // group, its angles computed once, kAtOnce heads at a time. In a prompt one row of
 // 16 leads, and rows alone in their blocks are taken by a wave each afterwards.
 // (With one row per workgroup, of 25,850 rows of 12 prompts the workgroups that
-// end at once took some 50 us.) 25,850 rows of 32q/8kv (636 MB) take 134 us with
-// turn_q_rows, 4.75 TB/s of reads and writes, where a large copy reaches 4.97.
+// end at once took some 50 us.) 25,850 rows of 32q/8kv (636 MB) take 122-128 us with
+// turn_q_rows, 5.0-5.2 TB/s of reads and writes, where a large copy reaches 4.8-5.0;
+// as integers 134.
 constexpr int kAtOnce = 2;
 
 template <int FMT>
@@ -776,15 +777,17 @@ __device__ __forceinline__ int row_of(const DecodeQ8Args& a, int n, int rows, in
 // P is carried as two bf16 terms (hi + lo, 16 bits): the matrix cores are a
 // tenth of the time. Both scales act per block, that is per lane: on the scores
 // and, an exact power of two, on P.
-// The cache's bytes bound it, each read once and kept in no cache (loads of K as
-// 64-byte halves of its lines: 269 / 170 us for the first and last of these, with
-// cached loads 266 / 168): 128 rows of 1600 keys of 32 heads (1.68 GB) take 264 us,
-// 6.4 TB/s; 4 of 100,000-130,000 keys of 32q/8kv in 4096-key splits (0.94 GB) 162 with
-// the merge, 5.8; 64 of 200-2400 of 16q/8kv (0.17 GB) 32.4, 5.2, where the longest
-// rows' walks show. Loads alone, nothing computed, took 265 of 272 us when the
-// first stood at that; 64-key tiles, two or three tiles asked for ahead, and
-// two or three workgroups a CU in place of four were no faster. A lone row is
-// bound by latency: 1 row of 8000 keys in 256-key splits takes 10.8 with the merge.
+// The cache's bytes bound it, each read once and kept in no cache (whole lines of K
+// past the caches / as 64-byte halves / cached: 128 rows of 1600 keys of 32 heads 264 /
+// 269 / 266 us, 4 of 100,000-130,000 of 32q/8kv 162 / 170 / 168). 128 rows of 100-3000
+// keys of 32 heads (1.63 GB) take 247 us, 6.6 TB/s (255 on another card); the 4 long
+// rows in 4096-key splits (0.94 GB) 153 with the merge, 6.1; 64 of 200-2400 of 16q/8kv
+// (0.17 GB) 30.5, 5.6, where the longest rows' walks show. Loads alone, nothing
+// computed, took 265 of 272 us on the 128 rows of 1600; 64-key tiles, two or three
+// tiles asked for ahead, and two or three workgroups a CU in place of four were no
+// faster. A lone row is bound by latency: 1 row of 8000 keys in 256-key splits takes
+// 10.8 with the merge. Under a plan far longer than its rows the splits are the
+// plan's: the 64 rows take 52 under one for 40,960 keys.
 template <int FMT>
 __global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
   const int kh = blockIdx.y, G = a.hq / a.hk, tid = threadIdx.x;

@@ -156,9 +156,9 @@ static_assert(kDmas == 8, "one DMA per K-step of the S stage");
 // And packed: K and V rows of prompts that lie one behind the other, each row
 // of a prompt seeing its own prompt's rows up to itself: dense loads from any
 // row stride, without page ids, in the paged prefill's work list. 12 prompts of
-// 300-4000 rows (some 24,000) of 32q/8kv take 0.50-0.51 ms (1.0 PFLOP/s; some 4 us of first loads and
-// last stores a tile of 128 packed rows, beside 3.5 us for each 128 keys), one of
-// 16,384 rows 1.78-1.84 ms (1.2), one of 187 rows of 16q/8kv 8.0 us. P is rounded to
+// 300-4000 rows (some 24,000) of 32q/8kv take 0.50-0.53 ms (1.0 PFLOP/s; some 4 us of first loads and
+// last stores a tile of 256 packed rows, beside 3.5 us for each 128 keys), one of
+// 16,384 rows 1.78-1.95 ms (1.1-1.2), one of 187 rows of 16q/8kv 7.7-8.2 us. P is rounded to
 // bf16 as in the other sources (error 0.0020 against 64 bits, 0.0016 of it the bf16
 // output's); EXACT carries it in two terms.
 constexpr int kDense = 0, kPagedWave = 1, kPagedLane = 2, kPacked = 3;
