@@ -478,10 +478,12 @@ int omni_attn_prompt_plan_init(int nseq, const int32_t* lens_h, int hq, int hk, 
  * [hq][128], k and v rows [hk][128], at strides that are multiples of 8 elements
  * (k and v at most 2^22): parts of one qkv row, or buffers of their own. out
  * rows [hq][128]; rows past the plan's are left as they were. scale: any value
- * that times log2(e) is finite, as for omni_qwen3_attend_q8. A row's bits
- * depend on its own prompt alone, and what another prompt holds never reaches
- * it; of its own prompt, an infinity or NaN in a later V row does where the two
- * share a tile of 128 keys (a masked key weighs 0, and 0 times those is NaN).
+ * that times log2(e) is finite, as for omni_qwen3_attend_q8. Weights reach 2^8 on
+ * the way: |V| summed over a row's keys so weighted has to stay below 2^128. A
+ * row's bits depend on its own prompt alone, and what another prompt holds never
+ * reaches it; of its own prompt, an infinity or NaN in a later V row does where
+ * the two share a tile of 128 keys (a masked key weighs 0, and 0 times those is
+ * NaN).
  * `work` is the device copy of this plan's work list. */
 int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64_t q_stride, const void* k,
                          int64_t k_stride, const void* v, int64_t v_stride, void* out, float scale, const int32_t* work,
