@@ -489,6 +489,84 @@ int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64
                          int64_t k_stride, const void* v, int64_t v_stride, void* out, float scale, const int32_t* work,
                          void* stream);
 
+/* ---------------------------------------------- pages that requests share */
+
+/* Candidates forked from one request share the whole pages of its prompt, in the
+ * tables and queues of omni_attn_step_tables, over a cache of any format. No
+ * counterpart in the reference, whose prefix reuse copies slots (omni_lm_copy_kv).
+ *
+ * shares [num_pages] counts the lines that hold a page beside the first: zeros at
+ * the start, and for every free page. omni_attn_step_tables knows nothing of it: a
+ * request that shares pages ends with omni_attn_pages_free, not with count < 0
+ * (one that shares none may end either way). New rows are written behind a line's
+ * last token, so never to a shared page.
+ *
+ * Lists of n entries are looked over before anything is written; an entry with
+ * tokens < 0 is none (the padding of a captured call). status int32[5] = {code,
+ * .., .., head, free entries} as in omni_attn_step_tables, &status[3] being the
+ * next call's free_state; free_state must not lie in status. Where code is not 0
+ * nothing is done; the lowest that applies:
+ *   OMNI_ATTN_TABLES_BAD        a line or free_state out of range, a line written twice
+ *   OMNI_ATTN_TABLES_PAGES      more moves than src and dst hold
+ *   OMNI_ATTN_TABLES_LINE       an entry has more than table_ld pages
+ *   OMNI_ATTN_TABLES_EXHAUSTED  fewer free pages than are needed
+ *   OMNI_ATTN_PAGES_UNHELD      (pages_free) more pages came back than were in use:
+ *                               shares, table and queue do not agree. The holders
+ *                               are counted down, and the queue stays
+ * Tables have at most 2^18 lines, pools that are compacted at most 2^20 pages. Page
+ * ids of a line that are outside the pool are passed over. Calls that share a
+ * table, a queue or shares follow one another on a stream. */
+#define OMNI_ATTN_PAGES_UNHELD 6
+
+/* Fork i: line children[i] begins with the first tokens[i] tokens of line
+ * parents[i]. It takes over the pages that these fill whole, whose shares go up by
+ * one; of the page that they fill in part, if there is one, it gets a copy: the
+ * queue's next page (in the order of the forks) stands in its line, and src[i] and
+ * dst[i] are the two, for omni_attn_pages_copy (-1 and -1 where there is none).
+ * Pages that the child's line held before are not given back. One parent may have
+ * many children; a child is no parent, and no child twice, of the same call.
+ * status[1] pages were taken, status[2] are shared. */
+int omni_attn_pages_fork(const int32_t* parents, const int32_t* children, const int32_t* tokens, int n, int page,
+                         int32_t* table, int64_t table_ld, int num_lines, const int32_t* free_pages, int num_pages,
+                         const int32_t* free_state, int32_t* shares, int32_t* src, int32_t* dst, int32_t* status,
+                         void* stream);
+
+/* Line lines[i], of tokens[i] tokens, ends: each of its pages loses a holder, and
+ * the pages that have none left go to the queue's end, in ascending order.
+ * status[1] pages came free, of status[2] that the lines held. The lines stay as
+ * they are. */
+int omni_attn_pages_free(const int32_t* lines, const int32_t* tokens, int n, int page, const int32_t* table,
+                         int64_t table_ld, int num_lines, int32_t* free_pages, int num_pages, const int32_t* free_state,
+                         int32_t* shares, int32_t* status, void* stream);
+
+/* The pages in use (those not in the queue) with ids from `limit` on move to free
+ * ones below it: the k-th such page, in ascending order, to the k-th free one.
+ * Written: src and dst [move_cap], the moves for omni_attn_pages_copy, -1 past the
+ * last; new_ids [num_pages], where each page is now (a free one: itself);
+ * table_out, every entry of the table mapped (ids outside the pool stay);
+ * shares_out; free_out [num_pages], the free pages in ascending order (so those
+ * below the limit first), -1 past the last. status = {code, moves, free pages below
+ * the limit, 0, free pages}: to shrink the pool, go on with num_pages = limit and
+ * status[2] free entries from head 0; to keep it, with &status[3].
+ * table_out may be the table; the other outputs are buffers of their own. Page
+ * lists that omni_attn_step_tables made before are out of date. */
+int omni_attn_pages_compact(const int32_t* table, int64_t table_ld, int num_lines, const int32_t* free_pages,
+                            int num_pages, const int32_t* free_state, const int32_t* shares, int limit,
+                            int32_t* table_out, int32_t* free_out, int32_t* shares_out, int32_t* new_ids, int32_t* src,
+                            int32_t* dst, int move_cap, int32_t* status, void* stream);
+
+/* Page dst[k] takes the bytes of page src[k], k < n (k < *count, if that is less;
+ * count may be NULL), in each of `layers` caches that lie layer_stride bytes apart:
+ * page_bytes of kv (a multiple of 16, as the stride is, kv 16-byte aligned), and
+ * scale_page_bytes of kv_scale (NULL: none). Pairs with an id outside the pool are
+ * none. A page that is both a source and a destination of one call gives an
+ * unspecified result, as does one that is a destination twice. The 8-bit cache:
+ * page_bytes = page / 16 * 2 * hk * 2048, scale_page_bytes = page / 16 * 2 * hk;
+ * bf16 slots: page_bytes = page * 2 * hk * 256. */
+int omni_attn_pages_copy(void* kv, int64_t page_bytes, int64_t layer_stride, void* kv_scale, int64_t scale_page_bytes,
+                         int64_t scale_layer_stride, int layers, int num_pages, const int32_t* src, const int32_t* dst,
+                         int n, const int32_t* count, void* stream);
+
 /* ------------------------------------------------------- host row builder */
 
 /* The engines' `Rows` (crates/omni-qwen3-tts/src/model.rs:266-303,

@@ -1078,6 +1078,152 @@ int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64
   return ok();
 }
 
+// ------------------------------------------------ pages that requests share
+
+namespace {
+
+// What fork and free have in common.
+int pages_common(omni::PagesArgs& a, int page, const char* who) {
+  if (a.n < 0 || page <= 0 || a.table_ld < 0 || a.num_lines < 0 || a.num_pages <= 0)
+    return fail(OMNI_ATTN_EINVAL, "%s: n=%d page=%d table_ld=%lld num_lines=%d num_pages=%d", who, a.n, page,
+                (long long)a.table_ld, a.num_lines, a.num_pages);
+  if (a.num_lines > omni::kMostLines) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d lines", who, a.num_lines);
+  if (!omni::grid_holds(a.n, 256)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d entries", who, a.n);
+  if (!a.free_pages || !a.free_state || !a.shares || !a.status) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (a.n > 0 && (!a.lines || !a.tokens || !a.table)) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (a.free_state + 2 > a.status && a.free_state < a.status + 5)
+    return fail(OMNI_ATTN_EINVAL, "%s: free_state lies in status (two status buffers take turns)", who);
+  a.pd = omni::make_page_div(page);
+  return 0;
+}
+
+}  // namespace
+
+int omni_attn_pages_fork(const int32_t* parents, const int32_t* children, const int32_t* tokens, int n, int page,
+                         int32_t* table, int64_t table_ld, int num_lines, const int32_t* free_pages, int num_pages,
+                         const int32_t* free_state, int32_t* shares, int32_t* src, int32_t* dst, int32_t* status,
+                         void* stream) {
+  omni::PagesArgs a{};
+  a.parents = parents;
+  a.lines = children;
+  a.tokens = tokens;
+  a.n = n;
+  a.table = table;
+  a.table_out = table;
+  a.table_ld = table_ld;
+  a.num_lines = num_lines;
+  a.free_pages = const_cast<int32_t*>(free_pages);  // read alone
+  a.num_pages = num_pages;
+  a.free_state = free_state;
+  a.shares = shares;
+  a.src = src;
+  a.dst = dst;
+  a.status = status;
+  if (int rc = pages_common(a, page, "pages_fork")) return rc;
+  if (n > 0 && (!parents || !src || !dst)) return fail(OMNI_ATTN_EINVAL, "pages_fork: null device pointer");
+  if (omni::launch_pages_fork(a, as_stream(stream)) != 0)
+    return fail(OMNI_ATTN_ELAUNCH, "pages_fork: launch failed: %s", hipGetErrorString(omni::g_launch_status));
+  return ok();
+}
+
+int omni_attn_pages_free(const int32_t* lines, const int32_t* tokens, int n, int page, const int32_t* table,
+                         int64_t table_ld, int num_lines, int32_t* free_pages, int num_pages, const int32_t* free_state,
+                         int32_t* shares, int32_t* status, void* stream) {
+  omni::PagesArgs a{};
+  a.lines = lines;
+  a.tokens = tokens;
+  a.n = n;
+  a.table = table;
+  a.table_ld = table_ld;
+  a.num_lines = num_lines;
+  a.free_pages = free_pages;
+  a.num_pages = num_pages;
+  a.free_state = free_state;
+  a.shares = shares;
+  a.status = status;
+  if (int rc = pages_common(a, page, "pages_free")) return rc;
+  if (omni::launch_pages_free(a, as_stream(stream)) != 0)
+    return fail(OMNI_ATTN_ELAUNCH, "pages_free: launch failed: %s", hipGetErrorString(omni::g_launch_status));
+  return ok();
+}
+
+int omni_attn_pages_compact(const int32_t* table, int64_t table_ld, int num_lines, const int32_t* free_pages,
+                            int num_pages, const int32_t* free_state, const int32_t* shares, int limit,
+                            int32_t* table_out, int32_t* free_out, int32_t* shares_out, int32_t* new_ids, int32_t* src,
+                            int32_t* dst, int move_cap, int32_t* status, void* stream) {
+  const char* who = "pages_compact";
+  if (table_ld < 0 || num_lines < 0 || num_pages <= 0 || limit < 0 || limit > num_pages || move_cap < 0)
+    return fail(OMNI_ATTN_EINVAL, "%s: table_ld=%lld num_lines=%d num_pages=%d limit=%d move_cap=%d", who,
+                (long long)table_ld, num_lines, num_pages, limit, move_cap);
+  if (num_pages > omni::kMostPool) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d pages", who, num_pages);
+  if (table_ld > INT_MAX) return fail(OMNI_ATTN_EINVAL, "%s: table_ld=%lld", who, (long long)table_ld);
+  const int64_t cells = table_ld * num_lines;
+  if (!free_pages || !free_state || !shares || !free_out || !shares_out || !new_ids || !status ||
+      (cells > 0 && (!table || !table_out)) || (move_cap > 0 && (!src || !dst)))
+    return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (free_state + 2 > status && free_state < status + 5)
+    return fail(OMNI_ATTN_EINVAL, "%s: free_state lies in status (two status buffers take turns)", who);
+  // Workgroups read all of the queue and any page's holders while others write.
+  if ((free_out + num_pages > free_pages && free_out < free_pages + num_pages) ||
+      (shares_out + num_pages > shares && shares_out < shares + num_pages))
+    return fail(OMNI_ATTN_EINVAL, "%s: free_out and shares_out are buffers of their own", who);
+  omni::CompactArgs a{};
+  a.table = table;
+  a.table_out = table_out;
+  a.cells = cells;
+  a.free_pages = free_pages;
+  a.free_out = free_out;
+  a.num_pages = num_pages;
+  a.limit = limit;
+  a.free_state = free_state;
+  a.shares = shares;
+  a.shares_out = shares_out;
+  a.new_ids = new_ids;
+  a.src = src;
+  a.dst = dst;
+  a.cap = move_cap;
+  a.status = status;
+  if (omni::launch_pages_compact(a, as_stream(stream)) != 0)
+    return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));
+  return ok();
+}
+
+int omni_attn_pages_copy(void* kv, int64_t page_bytes, int64_t layer_stride, void* kv_scale, int64_t scale_page_bytes,
+                         int64_t scale_layer_stride, int layers, int num_pages, const int32_t* src, const int32_t* dst,
+                         int n, const int32_t* count, void* stream) {
+  const char* who = "pages_copy";
+  if (n < 0 || layers < 0 || num_pages < 0 || page_bytes <= 0 || page_bytes % 16 != 0 || page_bytes > (1LL << 40) ||
+      layer_stride < 0 || layer_stride % 16 != 0)
+    return fail(OMNI_ATTN_EINVAL, "%s: n=%d layers=%d num_pages=%d page_bytes=%lld layer_stride=%lld", who, n, layers, num_pages,
+                (long long)page_bytes, (long long)layer_stride);
+  if (kv_scale && (scale_page_bytes < 0 || scale_page_bytes > (1LL << 40) || scale_layer_stride < 0))
+    return fail(OMNI_ATTN_EINVAL, "%s: scale_page_bytes=%lld scale_layer_stride=%lld", who, (long long)scale_page_bytes,
+                (long long)scale_layer_stride);
+  // Layers that overlap would write one another's pages.
+  if (layers > 1 && (layer_stride / page_bytes < num_pages ||
+                     (kv_scale && scale_page_bytes > 0 && scale_layer_stride / scale_page_bytes < num_pages)))
+    return fail(OMNI_ATTN_EINVAL, "%s: a layer's stride holds its %d pages", who, num_pages);
+  if (n == 0 || layers == 0 || num_pages == 0) return ok();
+  if (!kv || !src || !dst) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (!aligned16(kv)) return fail(OMNI_ATTN_EINVAL, "%s: kv must be 16-byte aligned", who);
+  omni::CopyArgs a{};
+  a.kv = static_cast<uint8_t*>(kv);
+  a.page_bytes = page_bytes;
+  a.layer_stride = layer_stride;
+  a.kv_scale = static_cast<uint8_t*>(kv_scale);
+  a.scale_page_bytes = scale_page_bytes;
+  a.scale_layer_stride = scale_layer_stride;
+  a.layers = layers;
+  a.num_pages = num_pages;
+  a.src = src;
+  a.dst = dst;
+  a.n = n;
+  a.count = count;
+  if (omni::launch_pages_copy(a, as_stream(stream)) != 0)
+    return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));
+  return ok();
+}
+
 // ------------------------------------------------------ head-64 ring attentions
 
 namespace {

@@ -201,6 +201,59 @@ struct TablesArgs {
 };
 int launch_tables(const TablesArgs& a, hipStream_t stream);
 
+// Pages of a cache (pages.hip): forked, given back, compacted, copied.
+constexpr int kMostLines = 1 << 18;  // of a table: a bit each in LDS
+constexpr int kMostPool = 1 << 20;   // pages of a pool that is compacted: likewise
+
+struct PagesArgs {
+  const int32_t* parents;  // fork: [n] table lines
+  const int32_t* lines;    // [n] the children, or the lines that end
+  const int32_t* tokens;   // [n]; negative: nothing to do
+  int n;
+  PageDiv pd;
+  const int32_t* table;  // [num_lines][table_ld]
+  int32_t* table_out;    // the same
+  int64_t table_ld;
+  int num_lines;
+  int32_t* free_pages;
+  int num_pages;
+  const int32_t* free_state;
+  int32_t* shares;       // [num_pages] lines that hold a page beside the first
+  int32_t *src, *dst;    // fork: [n] pages to copy
+  int32_t* status;       // {code, pages taken or given back, pages shared or dropped, first free entry, free entries}
+};
+int launch_pages_fork(const PagesArgs& a, hipStream_t stream);
+int launch_pages_free(const PagesArgs& a, hipStream_t stream);
+
+struct CompactArgs {
+  const int32_t* table;
+  int32_t* table_out;  // may be the table
+  int64_t cells;       // of the table
+  const int32_t* free_pages;
+  int32_t* free_out;
+  int num_pages, limit;
+  const int32_t* free_state;
+  const int32_t* shares;
+  int32_t* shares_out;
+  int32_t* new_ids;  // [num_pages]
+  int32_t *src, *dst;
+  int cap;  // entries of src and dst
+  int32_t* status;
+};
+int launch_pages_compact(const CompactArgs& a, hipStream_t stream);
+
+struct CopyArgs {
+  uint8_t* kv;
+  int64_t page_bytes, layer_stride;  // multiples of 16
+  uint8_t* kv_scale;                 // may be null
+  int64_t scale_page_bytes, scale_layer_stride;
+  int layers, num_pages;
+  const int32_t *src, *dst;  // pairs with a page outside the pool are none
+  int n;
+  const int32_t* count;  // pairs that count, or null: n
+};
+int launch_pages_copy(const CopyArgs& a, hipStream_t stream);
+
 // The 8-bit block cache (q8.hip): blocks of 16 tokens, [2 hk heads][2048]
 // bytes (K heads [16 tokens][128 dims], V heads [128 dims][16 tokens]) and one
 // biased power-of-two exponent per (block, head).

@@ -1,0 +1,422 @@
+// Pages of a paged cache (gfx950, wave64): forked requests share them, ended ones
+// give them back, a pool moves below a limit, and what has to move is copied.
+//
+// shares[p] counts the lines that hold page p beside the first: 0 for a page that one
+// line holds, and for a free one. So the row tables' takes and returns (tables.hip)
+// need not know of it as long as a request shares nothing.
+//
+// Every workgroup works out by itself what the whole call amounts to (whether it can
+// be made at all, which pages it takes), from the few numbers that say so, and then
+// does its share: no order between workgroups. Counts go up and down by integer
+// atomics, and what is put in an order (the queue, the moves) is put there by page
+// id or by the call's own order, so that the results have the same bits every time.
+#include "common.h"
+#include "kernels.h"
+
+#include <algorithm>
+
+namespace omni {
+
+namespace {
+
+constexpr int kBad = 1, kPages = 3, kLine = 4, kExhausted = 5, kUnheld = 6;
+
+__device__ __forceinline__ bool bad_state(int head, int avail, int num_pages) {
+  return head < 0 || head >= num_pages || avail < 0 || avail > num_pages;
+}
+
+// Entry head + k of the free queue, 0 <= k <= num_pages.
+__device__ __forceinline__ uint32_t queue_at(int head, int k, int num_pages) {
+  const uint32_t i = (uint32_t)head + (uint32_t)k;
+  return i >= (uint32_t)num_pages ? i - (uint32_t)num_pages : i;
+}
+
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// ------------------------------------------------------------------ fork, free
+
+// A call's lines, looked over by one workgroup: which lines it writes (`marked`), the
+// code, and sums over the entries, all of them and those before entry `me`.
+template <int THREADS>
+struct Looked {
+  uint32_t marked[kMostLines / 32];
+  int codes[THREADS / 64], part[THREADS / 64], before[THREADS / 64];
+  int pages[THREADS / 64];
+};
+
+// One workgroup per fork: the whole pages of the parent's line into the child's, a
+// holder more for each, and the queue's next page for the part-filled one, in the
+// order of the forks. Latency bounds it: the call's numbers, a page list, the stores,
+// one after the other (224 forks of up to 250 pages move 0.5 MB).
+constexpr int kForkThreads = 256;
+
+__global__ __launch_bounds__(kForkThreads) void pages_fork(PagesArgs a) {
+  const int tid = threadIdx.x, me = blockIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ Looked<kForkThreads> s;
+  for (int i = tid; i < (a.num_lines + 31) / 32; i += kForkThreads) s.marked[i] = 0;
+  const int head = a.free_state[0], avail = a.free_state[1];
+  __syncthreads();
+  int codes = bad_state(head, avail, a.num_pages) ? 1 << kBad : 0;
+  int part = 0, before = 0, pages = 0;
+  for (int i = tid; i < a.n; i += kForkThreads) {
+    const int tokens = a.tokens[i], p = a.parents[i], c = a.lines[i];
+    if (tokens < 0) continue;
+    if (p < 0 || p >= a.num_lines || c < 0 || c >= a.num_lines) {
+      codes |= 1 << kBad;
+      continue;
+    }
+    const int held = tokens > 0 ? page_index(a.pd, tokens - 1) + 1 : 0, full = page_index(a.pd, tokens);
+    if (held > a.table_ld) codes |= 1 << kLine;
+    if (atomicOr(&s.marked[c >> 5], 1u << (c & 31)) >> (c & 31) & 1) codes |= 1 << kBad;  // a child twice
+    part += held - full;
+    before += i < me ? held - full : 0;
+    pages = (int)min((uint32_t)pages + (uint32_t)full, 0x7fffffffu);
+  }
+  __syncthreads();
+  for (int i = tid; i < a.n; i += kForkThreads) {  // a child that is a parent too
+    const int p = a.parents[i];
+    if (a.tokens[i] >= 0 && p >= 0 && p < a.num_lines && (s.marked[p >> 5] >> (p & 31) & 1)) codes |= 1 << kBad;
+  }
+#pragma unroll
+  for (int c = kBad; c <= kExhausted; ++c)
+    if (__any(codes >> c & 1)) codes |= 1 << c;
+  part = wave_sum(part), before = wave_sum(before);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) pages = (int)min((uint32_t)pages + (uint32_t)__shfl_xor(pages, d), 0x7fffffffu);
+  if (lane == 0) s.codes[wave] = codes, s.part[wave] = part, s.before[wave] = before, s.pages[wave] = pages;
+  __syncthreads();
+  codes = part = before = pages = 0;
+#pragma unroll
+  for (int w = 0; w < kForkThreads / 64; ++w) {
+    codes |= s.codes[w], part += s.part[w], before += s.before[w];
+    pages = (int)min((uint32_t)pages + (uint32_t)s.pages[w], 0x7fffffffu);
+  }
+  if (part > avail) codes |= 1 << kExhausted;
+  const int code = codes ? __ffs(codes) - 1 : 0;
+  if (me == 0 && tid == 0) {
+    a.status[0] = code;
+    a.status[1] = code ? 0 : part;
+    a.status[2] = code ? 0 : pages;
+    a.status[3] = code ? head : (int)queue_at(head, part, a.num_pages);
+    a.status[4] = code ? avail : avail - part;
+  }
+  if (me >= a.n) return;
+  const int tokens = a.tokens[me];
+  if (code || tokens < 0) {
+    if (tid == 0) a.src[me] = a.dst[me] = -1;
+    return;
+  }
+  const int32_t* from = a.table + (int64_t)a.parents[me] * a.table_ld;
+  int32_t* to = a.table_out + (int64_t)a.lines[me] * a.table_ld;
+  const int full = page_index(a.pd, tokens);
+  for (int j = tid; j < full; j += kForkThreads) {
+    const int id = from[j];
+    to[j] = id;
+    if (id >= 0 && id < a.num_pages) atomicAdd(a.shares + id, 1);
+  }
+  if (tid == 0) {
+    const bool has_part = tokens > full * a.pd.page;
+    const int id = has_part ? a.free_pages[queue_at(head, before, a.num_pages)] : -1;
+    if (has_part) to[full] = id;
+    a.src[me] = has_part ? from[full] : -1;
+    a.dst[me] = id;
+  }
+}
+
+// Ended lines, a workgroup each: every page of theirs loses a holder. A page that had
+// none beside this one is at -1 afterwards, which pages_gather looks for.
+__global__ __launch_bounds__(kForkThreads) void pages_drop(PagesArgs a) {
+  const int tid = threadIdx.x, me = blockIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ Looked<kForkThreads> s;
+  for (int i = tid; i < (a.num_lines + 31) / 32; i += kForkThreads) s.marked[i] = 0;
+  const int head = a.free_state[0], avail = a.free_state[1];
+  __syncthreads();
+  int codes = bad_state(head, avail, a.num_pages) ? 1 << kBad : 0, pages = 0;
+  for (int i = tid; i < a.n; i += kForkThreads) {
+    const int tokens = a.tokens[i], c = a.lines[i];
+    if (tokens < 0) continue;
+    if (c < 0 || c >= a.num_lines) {
+      codes |= 1 << kBad;
+      continue;
+    }
+    const int held = tokens > 0 ? page_index(a.pd, tokens - 1) + 1 : 0;
+    if (held > a.table_ld) codes |= 1 << kLine;
+    if (atomicOr(&s.marked[c >> 5], 1u << (c & 31)) >> (c & 31) & 1) codes |= 1 << kBad;  // a line twice
+    pages = (int)min((uint32_t)pages + (uint32_t)held, 0x7fffffffu);
+  }
+#pragma unroll
+  for (int c = kBad; c <= kLine; ++c)
+    if (__any(codes >> c & 1)) codes |= 1 << c;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) pages = (int)min((uint32_t)pages + (uint32_t)__shfl_xor(pages, d), 0x7fffffffu);
+  if (lane == 0) s.codes[wave] = codes, s.pages[wave] = pages;
+  __syncthreads();
+  codes = pages = 0;
+#pragma unroll
+  for (int w = 0; w < kForkThreads / 64; ++w) {
+    codes |= s.codes[w];
+    pages = (int)min((uint32_t)pages + (uint32_t)s.pages[w], 0x7fffffffu);
+  }
+  const int code = codes ? __ffs(codes) - 1 : 0;
+  if (me == 0 && tid == 0) a.status[0] = code, a.status[2] = code ? 0 : pages;
+  if (code || me >= a.n || a.tokens[me] <= 0) return;
+  const int32_t* line = a.table + (int64_t)a.lines[me] * a.table_ld;
+  const int held = page_index(a.pd, a.tokens[me] - 1) + 1;
+  for (int j = tid; j < held; j += kForkThreads) {
+    const int id = line[j];
+    if (id >= 0 && id < a.num_pages) atomicSub(a.shares + id, 1);
+  }
+}
+
+// The pages without a holder, in ascending order, to the queue's end. One workgroup,
+// a wave for each sixteenth of the pool: counted, then written.
+constexpr int kGatherThreads = 1024;
+
+__global__ __launch_bounds__(kGatherThreads) void pages_gather(PagesArgs a) {
+  constexpr int kWaves = kGatherThreads / 64, kAhead = 8;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int head = a.free_state[0], avail = a.free_state[1];
+  if (a.status[0]) {
+    if (tid == 0) a.status[1] = 0, a.status[3] = head, a.status[4] = avail;
+    return;
+  }
+  __shared__ int s_count[kWaves];
+  // Rounds of 64 pages; the first `rounds % kWaves` waves have one more.
+  const int rounds = (a.num_pages + 63) / 64;
+  const int r0 = wave * (rounds / kWaves) + min(wave, rounds % kWaves), r1 = r0 + rounds / kWaves + (wave < rounds % kWaves ? 1 : 0);
+  // f(round, this lane's page, those of the round without a holder)
+  const auto each = [&](auto f) {
+    for (int r = r0; r < r1; r += kAhead) {
+      int v[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) v[i] = r + i < r1 && 64 * (r + i) + lane < a.num_pages ? a.shares[64 * (r + i) + lane] : 0;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) f(64 * (r + i) + lane, __ballot(v[i] < 0));
+    }
+  };
+  int count = 0;
+  each([&](int, uint64_t free) { count += __popcll(free); });
+  if (lane == 0) s_count[wave] = count;
+  __syncthreads();
+  int at = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) at += s_count[w];
+    total += s_count[w];
+  }
+  const bool fits = total <= a.num_pages - avail;  // else pages were given back that nobody held
+  if (tid == 0) {
+    if (!fits) a.status[0] = kUnheld;
+    a.status[1] = fits ? total : 0;
+    a.status[3] = head;
+    a.status[4] = fits ? avail + total : avail;
+  }
+  if (count == 0) return;
+  each([&](int p, uint64_t free) {
+    if (free >> lane & 1) {
+      a.shares[p] = 0;
+      if (fits) a.free_pages[queue_at(head, avail + at + __popcll(free & ((1ull << lane) - 1)), a.num_pages)] = p;
+    }
+    at += __popcll(free);
+  });
+}
+
+// ------------------------------------------------------------------ compact
+
+// The free pages as bits, and how many are free below each run of kRun.
+constexpr int kRun = 256;
+
+struct FreeBits {
+  uint32_t bits[kMostPool / 32];
+  int below[kMostPool / kRun + 1];
+  int sums[16];
+  int code;
+};
+
+// Free pages with an id below p.
+__device__ __forceinline__ int free_below(const FreeBits& s, int p) {
+  int c = s.below[p / kRun];
+  for (int w = p / kRun * (kRun / 32); w < p / 32; ++w) c += __popc(s.bits[w]);
+  return (p & 31) ? c + __popc(s.bits[p >> 5] & ((1u << (p & 31)) - 1)) : c;
+}
+
+// The k-th free page (k from 0; there is one).
+__device__ __forceinline__ int nth_free(const FreeBits& s, int k, int runs) {
+  int lo = 0, hi = runs - 1;
+  while (lo < hi) {  // the last run with at most k free pages before it
+    const int mid = (lo + hi + 1) >> 1;
+    if (s.below[mid] <= k)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  k -= s.below[lo];
+  int w = lo * (kRun / 32);
+  for (int c = __popc(s.bits[w]); k >= c; c = __popc(s.bits[w])) k -= c, ++w;
+  uint32_t b = s.bits[w];
+  for (; k > 0; --k) b &= b - 1;
+  return 32 * w + __ffs(b) - 1;
+}
+
+// The k-th page in use from `limit` on moves to the k-th free page below it. Every
+// workgroup reads the free queue into bits of its own, and then maps its share of the
+// table, the holders and the queue: one launch.
+constexpr int kCompactThreads = 1024;
+
+__global__ __launch_bounds__(kCompactThreads) void pages_compact(CompactArgs a) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t first = (int64_t)blockIdx.x * kCompactThreads + tid, step = (int64_t)gridDim.x * kCompactThreads;
+  __shared__ FreeBits s;
+  const int runs = (a.num_pages + kRun - 1) / kRun, words = runs * (kRun / 32);
+  const int head = a.free_state[0], avail = a.free_state[1];
+  for (int i = tid; i < words; i += kCompactThreads) s.bits[i] = 0;
+  if (tid == 0) s.code = 0;
+  __syncthreads();
+  bool bad = bad_state(head, avail, a.num_pages);
+  if (!bad)
+    for (int k = tid; k < avail; k += kCompactThreads) {
+      const int id = a.free_pages[queue_at(head, k, a.num_pages)];
+      if (id < 0 || id >= a.num_pages || (atomicOr(&s.bits[id >> 5], 1u << (id & 31)) >> (id & 31) & 1)) bad = true;
+    }
+  if (bad) s.code = kBad;
+  __syncthreads();
+  // Free pages before each run: four runs a thread, 4096 in all.
+  int c[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * tid + i;
+    c[i] = 0;
+    if (r < runs)
+      for (int w = 0; w < kRun / 32; ++w) c[i] += __popc(s.bits[r * (kRun / 32) + w]);
+    sum += c[i];
+  }
+  int at = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(at, d);
+    if (lane >= d) at += u;
+  }
+  if (lane == 63) s.sums[wave] = at;
+  __syncthreads();
+  at -= sum;
+  for (int w = 0; w < wave; ++w) at += s.sums[w];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (4 * tid + i <= runs) s.below[4 * tid + i] = at;
+    at += c[i];
+  }
+  if (tid == kCompactThreads - 1 && runs == 4 * kCompactThreads) s.below[runs] = at;
+  __syncthreads();
+
+  const int holes = free_below(s, a.limit);
+  const int moves = a.num_pages - a.limit - (avail - holes);  // pages in use from the limit on
+  int code = s.code;
+  if (!code && moves > a.cap) code = kPages;
+  if (!code && moves > holes) code = kExhausted;
+  if (first == 0) {
+    a.status[0] = code;
+    a.status[1] = code ? 0 : moves;
+    a.status[2] = code ? 0 : holes - moves;
+    a.status[3] = code ? head : 0;
+    a.status[4] = avail;
+  }
+  const auto is_free = [&](int p) { return s.bits[p >> 5] >> (p & 31) & 1; };
+  // Where page p, in use, is afterwards.
+  const auto moved = [&](int p) { return p < a.limit ? p : nth_free(s, p - a.limit - (free_below(s, p) - holes), runs); };
+  for (int64_t i = (code ? 0 : moves) + first; i < a.cap; i += step) a.src[i] = a.dst[i] = -1;
+  if (code) return;
+  for (int64_t i = first; i < a.num_pages; i += step) {
+    const int p = (int)i;
+    if (is_free(p)) {
+      const int k = free_below(s, p);
+      a.new_ids[p] = p;
+      if (p >= a.limit) {
+        a.free_out[holes - moves + (p - a.limit)] = p, a.shares_out[p] = 0;
+      } else if (k < moves) {
+        a.dst[k] = p;  // its holders come with the page that moves here
+      } else {
+        a.free_out[k - moves] = p, a.shares_out[p] = 0;
+      }
+    } else {
+      const int to = moved(p);
+      a.new_ids[p] = to;
+      a.shares_out[to] = a.shares[p];
+      if (p >= a.limit) {
+        a.src[p - a.limit - (free_below(s, p) - holes)] = p;
+        a.free_out[holes - moves + (p - a.limit)] = p, a.shares_out[p] = 0;
+      }
+    }
+  }
+  for (int64_t i = avail + first; i < a.num_pages; i += step) a.free_out[i] = -1;
+  for (int64_t i = first; i < a.cells; i += step) {
+    const int id = a.table[i];
+    a.table_out[i] = id >= a.limit && id < a.num_pages && !is_free(id) ? moved(id) : id;
+  }
+}
+
+// ------------------------------------------------------------------ copy
+
+// Pages src[k] to dst[k], k below the count, in every layer, and the bytes of their
+// scales. A workgroup takes 32 KiB at a time: eight 16-byte loads in flight a thread.
+constexpr int kCopyThreads = 256, kCopyAhead = 8, kCopyPart = kCopyThreads * kCopyAhead * 16;
+
+__global__ __launch_bounds__(kCopyThreads) void pages_copy(CopyArgs a) {
+  const int n = a.count ? min(max(*a.count, 0), a.n) : a.n;
+  const int parts = (int)((a.page_bytes + kCopyPart - 1) / kCopyPart);
+  const int64_t items = (int64_t)n * a.layers * parts;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int part = (int)(it % parts);
+    const int64_t at = it / parts;
+    const int layer = (int)(at % a.layers), k = (int)(at / a.layers);
+    const int src = a.src[k], dst = a.dst[k];
+    if (src < 0 || src >= a.num_pages || dst < 0 || dst >= a.num_pages) continue;
+    const uint8_t* from = a.kv + layer * a.layer_stride + src * a.page_bytes;
+    uint8_t* to = a.kv + layer * a.layer_stride + dst * a.page_bytes;
+    const int64_t b0 = (int64_t)part * kCopyPart + threadIdx.x * 16;
+    uint4 v[kCopyAhead];
+#pragma unroll
+    for (int i = 0; i < kCopyAhead; ++i)
+      if (b0 + i * (kCopyThreads * 16) < a.page_bytes) v[i] = ldg16_stream(from + b0 + i * (kCopyThreads * 16));
+#pragma unroll
+    for (int i = 0; i < kCopyAhead; ++i)
+      if (b0 + i * (kCopyThreads * 16) < a.page_bytes) *reinterpret_cast<uint4*>(to + b0 + i * (kCopyThreads * 16)) = v[i];
+    if (part == 0 && a.kv_scale) {
+      uint8_t* s = a.kv_scale + layer * a.scale_layer_stride;
+      for (int64_t b = threadIdx.x; b < a.scale_page_bytes; b += kCopyThreads)
+        s[dst * a.scale_page_bytes + b] = s[src * a.scale_page_bytes + b];
+    }
+  }
+}
+
+}  // namespace
+
+int launch_pages_fork(const PagesArgs& a, hipStream_t stream) {
+  pages_fork<<<dim3((unsigned)std::max(a.n, 1)), kForkThreads, 0, stream>>>(a);
+  return check_launch();
+}
+
+int launch_pages_free(const PagesArgs& a, hipStream_t stream) {
+  pages_drop<<<dim3((unsigned)std::max(a.n, 1)), kForkThreads, 0, stream>>>(a);
+  if (check_launch() != 0) return -3;
+  pages_gather<<<1, kGatherThreads, 0, stream>>>(a);
+  return check_launch();
+}
+
+int launch_pages_compact(const CompactArgs& a, hipStream_t stream) {
+  const int64_t most = std::max<int64_t>(std::max<int64_t>(a.num_pages, a.cap), a.cells);
+  const int64_t grid = std::min<int64_t>(256, (most + kCompactThreads - 1) / kCompactThreads);
+  pages_compact<<<dim3((unsigned)std::max<int64_t>(grid, 1)), kCompactThreads, 0, stream>>>(a);
+  return check_launch();
+}
+
+int launch_pages_copy(const CopyArgs& a, hipStream_t stream) {
+  const int64_t items = (int64_t)a.n * a.layers * ((a.page_bytes + kCopyPart - 1) / kCopyPart);
+  pages_copy<<<dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(items, 4096))), kCopyThreads, 0, stream>>>(a);
+  return check_launch();
+}
+
+}  // namespace omni

@@ -11,6 +11,8 @@
 //   b tensor, least           the same of bf16                       -> pointer
 //   r tensor, rows, width     bf16 [>= rows][width], elements of a row adjacent -> pointer, row stride
 //   c kv, kv_scale, 2 hk      the 8-bit cache and its exponents      -> pointer, pointer, format
+//   p kv, kv_scale, page      a cache of one layer or several, 8-bit or (kv_scale None) bf16 slots
+//                             -> pointer, pointer, layers, blocks (slots), bytes and exponents of one, and how many a page has
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -95,6 +97,35 @@ int take_one(char kind, PyObject* const* a, Py_ssize_t left, int64_t device, Ans
     out.put_ptr(t);
     out.put_ptr(s);
     out.put(PyLong_FromLong(format));
+  } else if (k == 'p') {
+    const int64_t page = int_of(a[2]);
+    const bool slots = a[1] == Py_None;
+    const auto type = t.scalar_type();
+    const int64_t lead = t.dim() - 3;  // layers before the blocks
+    const bool shaped = (lead == 0 || lead == 1) && t.size(lead + 1) > 0 && t.size(lead + 1) % 2 == 0;
+    if (slots ? type != at::kBFloat16 || !shaped || t.size(lead + 2) != 128
+              : (type != at::kFloat8_e4m3fn && type != at::kChar) || !shaped || t.size(lead + 2) != 2048)
+      throw Bad{slots ? " must be bf16 slots [slots][2 hk][128], or layers of them"
+                      : " must be float8_e4m3fn or int8 [blocks][2 hk][2048], or layers of it"};
+    const int64_t units = t.size(lead), heads = t.size(lead + 1), layers = lead ? t.size(0) : 1;
+    if (page <= 0 || (!slots && page % 16 != 0)) throw Bad{": page=" + std::to_string(page)};
+    const int64_t per = slots ? page : page / 16;
+    if (units % per != 0) throw Bad{" must hold whole pages"};
+    if (!t.is_contiguous()) throw Bad{" must be contiguous"};
+    check_device(t, device);
+    out.put_ptr(t);
+    if (slots) {
+      out.put(Py_NewRef(Py_None));
+    } else {
+      const at::Tensor& s = tensor_of(a[1], "");
+      const auto exps = s.scalar_type();
+      if ((exps != at::kByte && exps != at::kFloat8_e8m0fnu) || s.dim() != t.dim() - 1 || s.size(lead) != units ||
+          s.size(lead + 1) != heads || (lead && s.size(0) != layers) || !s.is_contiguous())
+        throw Bad{"'s kv_scale must be contiguous uint8 or float8_e8m0fnu of its shape without the last dimension"};
+      check_device(s, device);
+      out.put_ptr(s);
+    }
+    for (const int64_t v : {layers, units, heads * (slots ? 256 : 2048), slots ? 0 : heads, per}) out.put(PyLong_FromLongLong(v));
   } else {
     throw Bad{": no such kind"};
   }
@@ -119,7 +150,7 @@ PyObject* take(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return nullptr;
   }
   Py_ssize_t values = 0;
-  for (Py_ssize_t i = 0; i < letters; ++i) values += (kinds[i] | 0x20) == 'c' ? 3 : (kinds[i] | 0x20) == 'r' ? 2 : 1;
+  for (Py_ssize_t i = 0; i < letters; ++i) values += (kinds[i] | 0x20) == 'p' ? 7 : (kinds[i] | 0x20) == 'c' ? 3 : (kinds[i] | 0x20) == 'r' ? 2 : 1;
   PyObject* tuple = PyTuple_New(values);
   if (!tuple) return nullptr;
   Answer out{tuple};

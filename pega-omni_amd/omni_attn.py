@@ -65,6 +65,10 @@ EXPORTS = (
     "omni_qwen3_attend_q8",
     "omni_attn_prompt_plan_init",
     "omni_attn_prompt_run",
+    "omni_attn_pages_fork",
+    "omni_attn_pages_free",
+    "omni_attn_pages_compact",
+    "omni_attn_pages_copy",
     "omni_attn_rows_new",
     "omni_attn_rows_free",
     "omni_attn_rows_clear",
@@ -180,6 +184,10 @@ def load(path: str | None = None):
         "omni_qwen3_attend_q8": [P, i64, P, P, i32, P, P, i32, P, P, i32, P, i32, i32, f32, dplan, P, P],
         "omni_attn_prompt_plan_init": [i32, P, i32, i32, P, i64, qplan],
         "omni_attn_prompt_run": [qplan, P, i64, P, i64, P, i64, P, f32, P, P],
+        "omni_attn_pages_fork": [P, P, P, i32, i32, P, i64, i32, P, i32, P, P, P, P, P, P],
+        "omni_attn_pages_free": [P, P, i32, i32, P, i64, i32, P, i32, P, P, P, P],
+        "omni_attn_pages_compact": [P, i64, i32, P, i32, P, P, i32, P, P, P, P, P, P, i32, P, P],
+        "omni_attn_pages_copy": [P, i64, i64, P, i64, i64, i32, i32, P, P, i32, P, P],
         "omni_attn_rows_new": [i32, i32],
         "omni_attn_rows_free": [P],
         "omni_attn_rows_clear": [P],
@@ -703,6 +711,80 @@ def prompt_run(pp: Prompt, q, k, v, out, scale, stream=None):
     _check(load().omni_attn_prompt_run(ctypes.byref(plan), p_q, q_ld, p_k, k_ld, p_v, v_ld, p_out, scale, p_work,
                                        _stream_on(stream, d)))
     return out
+
+
+# ------------------------------------------------- pages that requests share
+PAGES_UNHELD = 6
+
+
+def _table_shape(table):
+    shape = table.shape
+    if len(shape) != 2:
+        raise OmniAttnError(EINVAL, "table must be an int32 tensor [lines][pages]")
+    return shape
+
+
+def pages_fork(parents, children, tokens, table, free_pages, free_state, shares, src, dst, status, page=16, stream=None):
+    """Line ``children[i]`` of ``table`` begins with the first ``tokens[i]`` tokens
+    of line ``parents[i]``: whole pages shared (``shares`` counts a page's holders
+    beside the first), the part-filled one a page of its own from the free queue,
+    to be copied by ``pages_copy(.., src, dst)``. ``status`` = [code, pages taken,
+    pages shared, head, free entries]; ``status[3:5]`` is the next call's free_state.
+    tokens < 0: no fork."""
+    d = _current_device() if parents.is_cuda else -1
+    n, (lines, ld), pool = parents.numel(), _table_shape(table), free_pages.numel()
+    (p_par, p_chi, p_tok, p_table, p_free, p_state, p_shares, p_src, p_dst, p_status) = _take(
+        "iiiiiiiiii", "parents children tokens table free_pages free_state shares src dst status", d, parents, 0, children, n,
+        tokens, n, table, 0, free_pages, 1, free_state, 2, shares, pool, src, n, dst, n, status, 5)
+    _check(load().omni_attn_pages_fork(p_par, p_chi, p_tok, n, page, p_table, ld, lines, p_free, pool, p_state, p_shares, p_src,
+                                       p_dst, p_status, _stream_on(stream, d)))
+    return status
+
+
+def pages_free(lines, tokens, table, free_pages, free_state, shares, status, page=16, stream=None):
+    """Lines ``lines[i]`` of ``tokens[i]`` tokens end: pages that nobody else holds
+    go to the free queue's end, in ascending order. ``status`` = [code, pages that
+    came free, pages that the lines held, head, free entries]."""
+    d = _current_device() if lines.is_cuda else -1
+    n, (num_lines, ld), pool = lines.numel(), _table_shape(table), free_pages.numel()
+    p_lines, p_tok, p_table, p_free, p_state, p_shares, p_status = _take(
+        "iiiiiii", "lines tokens table free_pages free_state shares status", d, lines, 0, tokens, n, table, 0, free_pages, 1,
+        free_state, 2, shares, pool, status, 5)
+    _check(load().omni_attn_pages_free(p_lines, p_tok, n, page, p_table, ld, num_lines, p_free, pool, p_state, p_shares, p_status,
+                                       _stream_on(stream, d)))
+    return status
+
+
+def pages_compact(table, free_pages, free_state, shares, limit, table_out, free_out, shares_out, new_ids, src, dst, status,
+                  stream=None):
+    """Pages in use from id ``limit`` on move to free ones below it: ``src`` and
+    ``dst`` (-1 past the last) for ``pages_copy(.., count=status[1:2])``, the table
+    (in place if table_out is it), the free queue in ascending order, the holders
+    and every page's new id. ``status`` = [code, moves, free pages below the limit,
+    0, free pages]."""
+    d = _current_device() if table.is_cuda else -1
+    (lines, ld), pool, cap = _table_shape(table), free_pages.numel(), src.numel()
+    (p_table, p_free, p_state, p_shares, p_tout, p_fout, p_sout, p_ids, p_src, p_dst, p_status) = _take(
+        "iiiiiiiiiii", "table free_pages free_state shares table_out free_out shares_out new_ids src dst status", d, table, 0,
+        free_pages, 1, free_state, 2, shares, pool, table_out, lines * ld, free_out, pool, shares_out, pool, new_ids, pool, src, 0,
+        dst, cap, status, 5)
+    _check(load().omni_attn_pages_compact(p_table, ld, lines, p_free, pool, p_state, p_shares, limit, p_tout, p_fout, p_sout, p_ids,
+                                          p_src, p_dst, cap, p_status, _stream_on(stream, d)))
+    return status
+
+
+def pages_copy(kv, kv_scale, src, dst, page=16, count=None, stream=None):
+    """Page ``dst[k]`` takes the bytes of page ``src[k]`` in every layer (ids outside
+    the pool: no copy; ``count``: a device int32, how many pairs count). kv and
+    kv_scale: the 8-bit cache, [blocks][2 hk][2048] and [blocks][2 hk]; kv_scale None:
+    bf16 slots [slots][2 hk][128]; either may have a dimension of layers before."""
+    d = _current_device() if kv.is_cuda else -1
+    n = src.numel()
+    p_kv, p_scale, layers, units, width, scales, per, p_src, p_dst, p_count = _take(
+        "piiI", "kv src dst count", d, kv, kv_scale, page, src, 0, dst, n, count, 1)
+    _check(load().omni_attn_pages_copy(p_kv, width * per, width * units, p_scale, scales * per, scales * units, layers, units // per,
+                                       p_src, p_dst, n, p_count, _stream_on(stream, d)))
+    return kv
 
 
 # ------------------------------------------------------------ host row builder
