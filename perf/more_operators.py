@@ -234,7 +234,8 @@ def prepare(case, seed):
     st["out"] = torch.zeros(sum(rows), hq * HEAD, dtype=torch.bfloat16, device="cuda")
     if own:
         oa = _oa()
-        st["plan"] = (oa.extend_plan if kind == "extend" else oa.cross_plan)(rows, hq, hk, st["most"])
+        keys = [f + c for f, c in seqs] if kind == "extend" else lens
+        st["plan"] = (oa.extend_plan if kind == "extend" else oa.cross_plan)(rows, hq, hk, st["most"], keys)
         st["ws"] = oa.workspace_for(st["plan"].plan)
     return st
 
