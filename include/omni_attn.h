@@ -489,6 +489,67 @@ int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64
                          int64_t k_stride, const void* v, int64_t v_stride, void* out, float scale, const int32_t* work,
                          void* stream);
 
+/* -------------------------- several rows per sequence, encoder states */
+
+/* Work list for calls in which several rows see the same keys: new rows of
+ * sequences over the 8-bit cache (omni_qwen3_extend_q8), or rows over encoder
+ * states (omni_attn_cross_run). The rows of a call lie packed, sequence behind
+ * sequence, counts[s] of them each. */
+typedef struct omni_attn_multi_plan {
+  int32_t cross;      /* 0: made by extend_plan_init, 1: by cross_plan_init */
+  int32_t nseq, rows, hq, hk; /* rows: the sum of the counts */
+  int32_t max_len;    /* bound on the keys that a row sees; longer ones still run, slower */
+  int32_t groups[2];  /* groups of at most 16 and of at most 32 packed (row, head) pairs of a kv head */
+  int32_t group_rows; /* rows in them */
+  int32_t chunk, splits; /* keys per split of a group's rows (a multiple of 64), ceil(max_len / chunk) */
+  int32_t tiles;      /* tiles of 256 packed rows (each runs once per kv head) */
+  int32_t tile_chunk, tile_splits; /* keys per split of a tile (a multiple of 128), ceil(max_len / tile_chunk) */
+  int64_t work_bytes; /* bytes of the int32 work list that the caller uploads */
+  int64_t workspace_bytes; /* device scratch of a run (split partials), 16-byte aligned */
+} omni_attn_multi_plan;
+
+/* Host: counts (zero allowed) to a work list. hq / hk from 1 to 16. keys_h (NULL:
+ * not known): how many keys each sequence's last row sees when the plan is made,
+ * for the order of the work and the size of the splits alone; the lengths of a run
+ * are read on the device. chunk_hint, a multiple of 64 (<= 0 picks from the
+ * shape), is the split of the groups. OMNI_ATTN_EWORKSPACE with plan->work_bytes
+ * set when work_h is too small. */
+int omni_attn_extend_plan_init(int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
+                               int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan);
+int omni_attn_cross_plan_init(int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
+                              int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan);
+
+/* omni_qwen3_attend_q8 for several rows a sequence, whose keys are read once for a
+ * group of rows: a prompt behind a shared prefix, a chunk of a long one, a few
+ * proposed tokens. Row n of the plan's sequence s sees keys 0..pos[n] of the cache,
+ * in which the call's own rows lie already (omni_qwen3_rope_q8); a row with pos[n]
+ * < 0 stores zeros. The rows of a sequence may have any positions. indptr has nseq +
+ * 1 entries. q rows [hq][128] of stride q_stride (a multiple of 8), out rows
+ * [hq][128]; rows past the plan's are left as they were.
+ * P is carried in 16 bits in groups and rounded to bf16 in tiles, which also take K
+ * and V as bf16 (exact, but for values that bf16 does not hold: 2^128, which
+ * rounding to 8 bits can make, and what lies below 2^-126). P is at most 1 on the
+ * way, as in omni_qwen3_attend_q8. Tokens past the last key that a row of the group
+ * or tile sees may hold anything; among their own keys, an infinity or NaN in V
+ * reaches the rows of its group or tile that see earlier keys only.
+ * A workspace serves one call at a time: two captured graphs that may run at once
+ * need one each. `work` is the device copy of this plan's work list. */
+int omni_qwen3_extend_q8(const omni_attn_multi_plan* plan, const void* q, int64_t q_stride, const void* kv,
+                         const void* kv_scale, int format, const int32_t* pos, const int32_t* indptr,
+                         const int32_t* pages, int page, void* out, float scale, const int32_t* work, void* workspace,
+                         void* stream);
+
+/* Cross attention: the plan's rows of sequence s see all keys of source e = of[s]
+ * (of NULL: e = s), that is rows first[e] .. first[e] + len[e] - 1 of k and v; where
+ * len[e] <= 0 they store zeros. Sequences may share a source, and rows over one
+ * source belong in one sequence of the plan (five candidates' new tokens: a count
+ * of 5). first and len are read on the device, so that a captured call serves other
+ * sources later. k and v rows [hk][128], q rows [hq][128], at strides that are
+ * multiples of 8 elements (k and v at most 2^22); the rest as above. */
+int omni_attn_cross_run(const omni_attn_multi_plan* plan, const void* q, int64_t q_stride, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, const int32_t* of, const int32_t* first,
+                        const int32_t* len, void* out, float scale, const int32_t* work, void* workspace, void* stream);
+
 /* ---------------------------------------------- pages that requests share */
 
 /* Candidates forked from one request share the whole pages of its prompt, in the

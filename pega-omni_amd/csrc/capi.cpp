@@ -778,8 +778,8 @@ namespace {
 // 29.3; 5 of 20,000-90,000 1536 keys 111 / 108 (2048); 4 of 100,000-130,000 4096 keys
 // 162 / 153 (8192, which rows of unlike lengths cannot fill); 2 of 60,000, hk = 2,
 // 1024 keys 22.4 / 22.4; 1 of 40,000, hk = 1, 768 keys 15.7 / 14.8 (512).
-int pick_chunk_q8(int rows, int hk, int max_len) {
-  const double units = (double)rows * hk, read = units * max_len * 0.6 * 256 / 6.2e6;
+int pick_chunk_keys(double units, int max_len, double mean_len, int key_bytes) {
+  const double read = units * mean_len * key_bytes / 6.2e6;
   int best = 0;
   double least = 0;
   for (int chunk : {128, 256, 384, 512, 768, 1024, 1536, 2048, 4096, 8192, 16384, 32768, 0}) {
@@ -791,6 +791,10 @@ int pick_chunk_q8(int rows, int hk, int max_len) {
     if (chunk >= max_len) break;
   }
   return best;
+}
+
+int pick_chunk_q8(int rows, int hk, int max_len) {
+  return pick_chunk_keys((double)rows * hk, max_len, max_len * 0.6, 256);
 }
 
 constexpr float kLog2e = 1.4426950408889634f;  // the kernels take exponentials to base 2
@@ -1076,6 +1080,202 @@ int omni_attn_prompt_run(const omni_attn_prompt_plan* plan, const void* q, int64
   if (rc == -2) return fail(OMNI_ATTN_EUNSUPPORTED, "prompt_run: shape not implemented");
   if (rc != 0) return fail(OMNI_ATTN_ELAUNCH, "prompt_run: launch failed: %s", hipGetErrorString(omni::g_launch_status));
   return ok();
+}
+
+// ------------------------------------ several rows per sequence, encoder states
+
+namespace {
+
+constexpr int64_t kPartialBytes = (OMNI_ATTN_HEAD_DIM + 1) * (int64_t)sizeof(float);
+
+// Rows of one sequence that a group of `cols` packed columns takes.
+int rows_of_group(int cols, int G) { return cols / G; }
+
+int64_t multi_workspace(const omni_attn_multi_plan& p) {
+  if (p.splits <= 1) return 0;
+  return (int64_t)p.group_rows * p.hq * p.splits * kPartialBytes + 4 * ((int64_t)p.groups[0] + p.groups[1]);
+}
+
+int64_t multi_work_ints(const omni_attn_multi_plan& p) { return 4 * ((int64_t)p.groups[0] + p.groups[1]); }
+
+// What a launch of the plan's groups holds.
+bool groups_fit(const omni_attn_multi_plan& p) {
+  for (int c = 0; c < 2; ++c) {
+    const int64_t rows = std::max(rows_of_group(16 * (c + 1), p.hq / p.hk), 1);
+    if (!omni::grid_holds((int64_t)p.groups[c] * p.hk * p.splits, omni::kRowsThreads) ||
+        (int64_t)p.groups[c] * p.hk * p.splits > INT_MAX ||
+        (p.splits > 1 && !omni::grid_holds((int64_t)p.groups[c] * ((rows * p.hq + 7) / 8), omni::kRowsThreads)))
+      return false;
+  }
+  return true;
+}
+
+int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
+                    int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan, const char* who) try {
+  if (!plan) return fail(OMNI_ATTN_EINVAL, "%s: null plan", who);
+  std::memset(plan, 0, sizeof *plan);
+  if (nseq < 0 || (nseq > 0 && !counts_h)) return fail(OMNI_ATTN_EINVAL, "%s: nseq=%d, null counts", who, nseq);
+  if (hk <= 0 || hq <= 0 || hq % hk != 0) return fail(OMNI_ATTN_EINVAL, "%s: hq=%d is not a multiple of hk=%d", who, hq, hk);
+  const int G = hq / hk;
+  if (G > 16) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: hq/hk=%d above 16", who, G);
+  if (max_len <= 0) return fail(OMNI_ATTN_EINVAL, "%s: max_len=%d", who, max_len);
+  if (chunk_hint > 0 && chunk_hint % 64 != 0) return fail(OMNI_ATTN_EINVAL, "%s: chunk=%d is not a multiple of 64", who, chunk_hint);
+  int64_t rows = 0;
+  for (int s = 0; s < nseq; ++s) {
+    if (counts_h[s] < 0) return fail(OMNI_ATTN_EINVAL, "%s: %d rows of sequence %d", who, counts_h[s], s);
+    if (keys_h && keys_h[s] < 0) return fail(OMNI_ATTN_EINVAL, "%s: %d keys of sequence %d", who, keys_h[s], s);
+    rows += counts_h[s];
+  }
+  if (rows > INT_MAX || rows * hq > (int64_t)INT_MAX * 8) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many rows", who);
+  plan->cross = cross;
+  plan->nseq = nseq;
+  plan->rows = (int32_t)rows;
+  plan->hq = hq;
+  plan->hk = hk;
+  plan->max_len = max_len;
+
+  // Groups: (sequence, first row, rows, keys), of at most 16 packed rows where the rest of a sequence fits, else 32.
+  std::vector<std::array<int32_t, 4>> groups[2];
+  const int small = rows_of_group(16, G), large = rows_of_group(32, G);
+  double keys = 0;
+  for (int32_t s = 0, at = 0; s < nseq; at += counts_h[s++])
+    for (int32_t f = 0; f < counts_h[s];) {
+      const int32_t left = counts_h[s] - f, n = std::min(left, left <= small ? small : large);
+      groups[n > small].push_back({s, at + f, n, keys_h ? keys_h[s] : 0});
+      keys += keys_h ? std::min(keys_h[s], max_len) : 0.6 * max_len;
+      f += n;
+      plan->group_rows += n;
+    }
+  for (int c = 0; c < 2; ++c) {
+    if (groups[c].size() > (size_t)INT_MAX) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many groups", who);
+    plan->groups[c] = (int32_t)groups[c].size();
+    std::stable_sort(groups[c].begin(), groups[c].end(), [](const auto& x, const auto& y) { return x[3] > y[3]; });
+  }
+  const double n = (double)groups[0].size() + (double)groups[1].size();
+  plan->chunk = chunk_hint > 0 ? chunk_hint : pick_chunk_keys(n * hk, max_len, n > 0 ? keys / n : 1, cross ? 512 : 256);
+  plan->splits = (int32_t)(((int64_t)max_len + plan->chunk - 1) / plan->chunk);
+  plan->tile_chunk = (int32_t)std::min<int64_t>(((int64_t)max_len + 127) / 128 * 128, INT_MAX / 128 * 128);
+  plan->tile_splits = (int32_t)(((int64_t)max_len + plan->tile_chunk - 1) / plan->tile_chunk);
+  if (!groups_fit(*plan)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, plan->rows, hq, plan->splits);
+  plan->workspace_bytes = multi_workspace(*plan);
+  const int64_t need = multi_work_ints(*plan);
+  plan->work_bytes = need * (int64_t)sizeof(int32_t);
+  if (need > 0 && (!work_h || need > work_cap))
+    return fail(OMNI_ATTN_EWORKSPACE, "%s: work list needs %lld int32", who, (long long)need);
+  int32_t at = 0;
+  for (auto& list : groups)
+    for (const auto& g : list) {
+      *work_h++ = g[0], *work_h++ = g[1], *work_h++ = g[2], *work_h++ = at;
+      at += g[2];
+    }
+  return ok();
+} catch (const std::bad_alloc&) {
+  return fail(OMNI_ATTN_EUNSUPPORTED, "%s: no host memory for the groups of %d sequences", who, nseq);
+}
+
+// The plan's own fields, and what both runs take.
+int multi_checks(const omni_attn_multi_plan* plan, int cross, const void* q, int64_t q_stride, const void* out, float scale,
+                 const int32_t* work, const void* workspace, const char* who) {
+  const omni_attn_multi_plan& p = *plan;
+  if (p.cross != cross) return fail(OMNI_ATTN_EINVAL, "%s: the plan was made for %s", who, p.cross ? "cross attention" : "the 8-bit cache");
+  if (p.rows < 0 || p.hk <= 0 || p.hq <= 0 || p.hq % p.hk != 0 || p.hq / p.hk > 16 || p.max_len <= 0 || p.groups[0] < 0 ||
+      p.groups[1] < 0 || p.group_rows < 0 || p.group_rows > p.rows || p.chunk <= 0 || p.chunk % 64 != 0 ||
+      p.splits != ((int64_t)p.max_len + p.chunk - 1) / p.chunk || p.tiles < 0 || p.tile_chunk <= 0 || p.tile_chunk % 128 != 0 ||
+      p.tile_splits != ((int64_t)p.max_len + p.tile_chunk - 1) / p.tile_chunk ||
+      p.work_bytes != multi_work_ints(p) * (int64_t)sizeof(int32_t) || p.workspace_bytes != multi_workspace(p))
+    return fail(OMNI_ATTN_EINVAL, "%s: plan is not one its plan_init made (rows=%d hq=%d hk=%d max_len=%d groups=%d,%d chunk=%d splits=%d)",
+                who, p.rows, p.hq, p.hk, p.max_len, p.groups[0], p.groups[1], p.chunk, p.splits);
+  if (!groups_fit(p)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, p.rows, p.hq, p.splits);
+  if (!std::isfinite(scale * kLog2e)) return fail(OMNI_ATTN_EINVAL, "%s: scale * log2(e) is not finite", who);
+  if (p.rows == 0) return 0;
+  if (!q || !out || !work) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (!aligned16(q) || !aligned16(out) || !aligned16(work))
+    return fail(OMNI_ATTN_EINVAL, "%s: q, out and work must be 16-byte aligned", who);
+  if (!row_stride_ok(q_stride, p.hq))
+    return fail(OMNI_ATTN_EINVAL, "%s: q_stride=%lld: a multiple of 8 that holds a row", who, (long long)q_stride);
+  if (p.workspace_bytes > 0 && !workspace)
+    return fail(OMNI_ATTN_EWORKSPACE, "%s: plan needs %lld workspace bytes", who, (long long)p.workspace_bytes);
+  if (!aligned16(workspace)) return fail(OMNI_ATTN_EINVAL, "%s: workspace must be 16-byte aligned", who);
+  return 0;
+}
+
+int multi_launch(omni::RowsArgs& a, const omni_attn_multi_plan& p, int source, const void* q, int64_t q_stride, void* out,
+                 float scale, const int32_t* work, void* workspace, void* stream, const char* who) {
+  a.q = static_cast<const omni::bf16_t*>(q);
+  a.q_stride = q_stride;
+  a.out = static_cast<omni::bf16_t*>(out);
+  a.items = work;
+  a.ws_o = static_cast<float*>(workspace);
+  const int64_t partials = (int64_t)p.group_rows * p.hq * p.splits;
+  a.ws_lse = a.ws_o ? a.ws_o + partials * OMNI_ATTN_HEAD_DIM : nullptr;
+  a.ws_used = a.ws_o ? reinterpret_cast<int32_t*>(a.ws_lse + partials) : nullptr;
+  a.hq = p.hq;
+  a.hk = p.hk;
+  a.chunk = p.chunk;
+  a.splits = p.splits;
+  a.scale_log2 = scale * kLog2e;
+  if (omni::launch_rows(a, source, p.groups, as_stream(stream)) != 0)
+    return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));
+  return ok();
+}
+
+}  // namespace
+
+int omni_attn_extend_plan_init(int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
+                               int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan) {
+  return multi_plan_init(0, nseq, counts_h, keys_h, hq, hk, max_len, chunk_hint, work_h, work_cap, plan, "extend_plan");
+}
+
+int omni_attn_cross_plan_init(int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
+                              int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan) {
+  return multi_plan_init(1, nseq, counts_h, keys_h, hq, hk, max_len, chunk_hint, work_h, work_cap, plan, "cross_plan");
+}
+
+int omni_qwen3_extend_q8(const omni_attn_multi_plan* plan, const void* q, int64_t q_stride, const void* kv,
+                         const void* kv_scale, int format, const int32_t* pos, const int32_t* indptr,
+                         const int32_t* pages, int page, void* out, float scale, const int32_t* work, void* workspace,
+                         void* stream) {
+  const char* who = "qwen3_extend_q8";
+  if (!plan) return fail(OMNI_ATTN_EINVAL, "%s: null plan", who);
+  if (int rc = q8_format(format, who)) return rc;
+  if (int rc = multi_checks(plan, 0, q, q_stride, out, scale, work, workspace, who)) return rc;
+  if (int rc = q8_shape(plan->hq, plan->hk, page, who)) return rc;
+  if (plan->rows == 0) return ok();
+  if (!kv || !kv_scale || !pos || !indptr || !pages) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (!aligned16(kv)) return fail(OMNI_ATTN_EINVAL, "%s: kv must be 16-byte aligned", who);
+  omni::RowsArgs a{};
+  a.kv = static_cast<const uint8_t*>(kv);
+  a.kv_scale = static_cast<const uint8_t*>(kv_scale);
+  a.pos = pos;
+  a.indptr = indptr;
+  a.pages = pages;
+  a.pd = omni::make_page_div(page / 16);
+  return multi_launch(a, *plan, format, q, q_stride, out, scale, work, workspace, stream, who);
+}
+
+int omni_attn_cross_run(const omni_attn_multi_plan* plan, const void* q, int64_t q_stride, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, const int32_t* of, const int32_t* first,
+                        const int32_t* len, void* out, float scale, const int32_t* work, void* workspace, void* stream) {
+  const char* who = "cross_run";
+  if (!plan) return fail(OMNI_ATTN_EINVAL, "%s: null plan", who);
+  if (int rc = multi_checks(plan, 1, q, q_stride, out, scale, work, workspace, who)) return rc;
+  if (plan->rows == 0) return ok();
+  if (!k || !v || !first || !len) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
+  if (!aligned16(k) || !aligned16(v)) return fail(OMNI_ATTN_EINVAL, "%s: k and v must be 16-byte aligned", who);
+  // A key tile is addressed with 32-bit byte offsets from its first row.
+  if (!row_stride_ok(k_stride, plan->hk) || !row_stride_ok(v_stride, plan->hk) || k_stride > omni::kMostPromptStride ||
+      v_stride > omni::kMostPromptStride)
+    return fail(OMNI_ATTN_EINVAL, "%s: row strides %lld / %lld: multiples of 8 that hold a row, at most %lld", who, (long long)k_stride,
+                (long long)v_stride, (long long)omni::kMostPromptStride);
+  omni::RowsArgs a{};
+  a.k = static_cast<const omni::bf16_t*>(k);
+  a.v = static_cast<const omni::bf16_t*>(v);
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.of = of;
+  a.first = first;
+  a.len = len;
+  return multi_launch(a, *plan, omni::kRowsBf16, q, q_stride, out, scale, work, workspace, stream, who);
 }
 
 // ------------------------------------------------ pages that requests share

@@ -309,4 +309,38 @@ inline bool decode_q8_fits(int rows, int hq, int splits) {
 }
 int launch_decode_q8(DecodeQ8Args a, int rows, hipStream_t stream);
 
+// Groups of rows that see the same keys (rows.hip): an item is (sequence, first row,
+// rows, its first row in the workspace).
+constexpr int kRowsThreads = 256;
+constexpr int kRowsBf16 = 2;  // source: bf16 rows, beside kQ8E4m3 and kQ8Int8
+
+struct RowsArgs {
+  const bf16_t* q;
+  int64_t q_stride;
+  // the 8-bit cache
+  const uint8_t* kv;
+  const uint8_t* kv_scale;
+  const int32_t* pos;  // negative: the row stores zeros
+  const int32_t* indptr;
+  const int32_t* pages;
+  PageDiv pd;  // blocks per page
+  // bf16 sources: rows first[e] .. + len[e] - 1 of k and v, e = of[sequence] (null: the sequence)
+  const bf16_t* k;
+  const bf16_t* v;
+  int64_t k_stride, v_stride;
+  const int32_t* of;
+  const int32_t* first;
+  const int32_t* len;
+  bf16_t* out;
+  const int32_t* items;
+  float* ws_o;       // [workspace rows][hq][splits][128]
+  float* ws_lse;     // [workspace rows][hq][splits]
+  int32_t* ws_used;  // splits that each group takes
+  int hq, hk;
+  int chunk, splits;
+  float scale_log2;
+};
+// groups: of at most 16, and of at most 32 packed rows; their items one list behind the other.
+int launch_rows(const RowsArgs& a, int source, const int* groups, hipStream_t stream);
+
 }  // namespace omni

@@ -9,6 +9,7 @@
 // K heads lie [16 tokens][128 dims]; V heads [128 dims][16 tokens].
 #include "common.h"
 #include "kernels.h"
+#include "q8_bytes.h"
 #include "rotary.h"
 
 #include <algorithm>
@@ -36,11 +37,6 @@ __device__ __forceinline__ void row16_max2(uint32_t& a, uint32_t& b) {
   a = dpp_max_u32<kRowHalfMirror>(a), b = dpp_max_u32<kRowHalfMirror>(b);
   a = dpp_max_u32<kRowMirror>(a), b = dpp_max_u32<kRowMirror>(b);
 }
-
-__device__ __forceinline__ int from_lane(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane << 2, v); }
-
-// 2^(biased - 127) for 1 <= biased <= 254.
-__device__ __forceinline__ float pow2_biased(int biased) { return __int_as_float(biased << 23); }
 
 // The exponent of a block whose largest finite magnitude has the bf16 bits `most`:
 // from most = m 2^x with 1 <= m < 2, and top = 1.75 2^8 (448) or 1.984375 2^6 (127).
@@ -82,18 +78,6 @@ __device__ __forceinline__ uint32_t to_bytes(uint32_t w0, uint32_t w1, int biase
   } else {
     const float by = pow2_biased(254 - biased);
     return to_bytes<FMT>(lo_bf16(w0) * by, hi_bf16(w0) * by, lo_bf16(w1) * by, hi_bf16(w1) * by);
-  }
-}
-
-// The four values of a word of bytes.
-template <int FMT>
-__device__ __forceinline__ void from_bytes(uint32_t w, float* v) {
-  if constexpr (FMT == kQ8E4m3) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-    v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(w >> (8 * i));
   }
 }
 
@@ -652,59 +636,6 @@ constexpr int kTile = 32;       // keys per step: two blocks
 constexpr int kCus = 256;       // workgroups go to the CUs in turn
 constexpr int kIds = 64 / (kTile / kQ8Block);  // tiles whose blocks a wave looks up at once
 
-// Keys per split of a row of len keys: the plan's, or more where a row is
-// longer than the plan's bound (multiples of 64 keys, as the plan's).
-__device__ __forceinline__ int split_len_of(const DecodeQ8Args& a, int len) {
-  return max(a.chunk, ((len - 1) / a.splits + 64) / 64 * 64);
-}
-
-// rotated_split evens out the splits over the XCDs; but an XCD hands its
-// workgroups to its 32 CUs in turn, and where S divides 32 its CU would get the
-// same split index from every one of them (a row's last splits are the ones that
-// are short or empty). So the rotation moves on by one every 256 workgroups too.
-__device__ __forceinline__ int spread_split(int slot, int u, int S) {
-  return (int)((rotated_split(slot, u, S) + (((int64_t)S * u) >> 8)) % S);
-}
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-// Eight stored bytes as bf16, exactly (E4M3 has 4 significant bits, the integers 7).
-template <int FMT>
-__device__ __forceinline__ bf16x8 bf16_of(uint32_t w0, uint32_t w1) {
-  uint4 u;
-  if constexpr (FMT == kQ8E4m3) {
-    u.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w0, 1.f, false));
-    u.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w0, 1.f, true));
-    u.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w1, 1.f, false));
-    u.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w1, 1.f, true));
-  } else {
-    float v[8];
-    from_bytes<FMT>(w0, v), from_bytes<FMT>(w1, v + 4);
-    u = pack8(v);
-  }
-  return __builtin_bit_cast(bf16x8, u);
-}
-
-// Lanes col < 8 of 16 keep x and take their y from lane col + 8's x; lanes
-// col >= 8 keep y and take their x from lane col - 8's y.
-__device__ __forceinline__ void trade_halves(uint4& x, uint4& y) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const int x0 = (int)(&x.x)[w], y0 = (int)(&y.x)[w];
-    (&x.x)[w] = (uint32_t)__builtin_amdgcn_update_dpp(x0, y0, 0x128, 0xf, 0xc, false);
-    (&y.x)[w] = (uint32_t)__builtin_amdgcn_update_dpp(y0, x0, 0x128, 0xf, 0x3, false);
-  }
-}
-
-// The larger of v in the four lanes with the same lane % 16.
-__device__ __forceinline__ float max_of_groups(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 constexpr int kDecodeWaves = kThreads / 64;
 constexpr int kBlocksPerTile = kTile / kQ8Block;
 
@@ -802,7 +733,7 @@ __global__ __launch_bounds__(kThreads, 4) void decode_q8(DecodeQ8Args a) {
       for (int i = tid; i < G * kHead; i += kThreads) a.out[h0 * kHead + i] = 0;
     return;
   }
-  const int split_len = split_len_of(a, len);
+  const int split_len = split_len_of(a.chunk, a.splits, len);
   if ((int64_t)split * split_len >= len) return;
   const int t0 = split * split_len, t1 = min(len, t0 + split_len);
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -981,7 +912,7 @@ __global__ __launch_bounds__(kThreads) void merge_q8(DecodeQ8Args a) {
   const float* part = a.ws_o + h * a.splits * kHead + 4 * lane;
   const int p = a.pos[h / a.hq];
   const int len = p < 0 ? 0 : p + 1;
-  const int split_len = split_len_of(a, len);
+  const int split_len = split_len_of(a.chunk, a.splits, len);
   if (split_len >= len) return;
   const int used = (len + split_len - 1) / split_len;
   f32x4 num = {0.f, 0.f, 0.f, 0.f};

@@ -1,0 +1,431 @@
+// Attention of a few rows that see the same keys (gfx950, wave64): several new rows
+// of a sequence over the 8-bit block cache, or rows over an encoder's bf16 states.
+// What a row sees is its own affair (keys 0..pos, or all of a source), but the keys
+// are read once for all rows of a group.
+//
+// A group is at most 16 NC packed (row, head) columns of one K/V head: R = 16 NC / G
+// rows. One workgroup per (group, K/V head, split of the keys); its waves take the
+// split's 32-key tiles in turn, each with running maxima, sums and O of its own, and
+// the four are merged through LDS at the end. Lane l is column n = l % 16 of a block
+// of 16 columns, and group g = l / 16 of v_mfma_f32_16x16x32_bf16's operands:
+//   S^T (16 keys x 16 columns), two of them: row 4 x + r of product j is key
+//     8 x + 4 j + r of the tile, so that a lane ends with keys 8 g .. 8 g + 7 for its
+//     column, in order, which is P^T's operand as it stands.
+//   O^T (16 dims x 16 columns) += V^T . P^T. The cache holds V as [dim][token]; bf16
+//     rows of V pass through the wave's own 8 KiB of LDS, from which transposing
+//     reads take eight keys of a dim.
+// K and V operands are made once a tile and serve NC columns blocks. P is carried as
+// two bf16 terms (hi + lo, 16 bits) and is at most 1 on the way: the running base
+// stands 8 (log2) above the maximum that moved it. The keys' bytes bound it.
+#include "common.h"
+#include "kernels.h"
+#include "q8_bytes.h"
+#include "rotary.h"
+
+#include <algorithm>
+
+namespace omni {
+
+namespace {
+
+constexpr int kThreads = kRowsThreads;
+constexpr int kWaves = kThreads / 64;
+constexpr int kTile = 32;  // keys per step: two blocks of the cache
+constexpr int kBlocksPerTile = kTile / kQ8Block;
+constexpr int kIds = 64 / kBlocksPerTile;  // tiles whose blocks a wave looks up at once
+constexpr int kBf16 = 2;                   // beside kQ8E4m3 and kQ8Int8
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+// ds_read_b64_tr_b16: within each 16 lanes, lane i receives element i % 4 of the
+// 8-byte chunks that lanes 4 e + i / 4 address, e = 0..3.
+__device__ __forceinline__ bf16x4 lds_read_tr(const bf16_t* p) {
+  typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p));
+}
+
+// Orders a wave's LDS accesses with its own of other lanes' data (LDS keeps a wave's
+// order; this keeps the compiler's).
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The larger of v over the 16 lanes of a DPP row, and the smaller.
+__device__ __forceinline__ int row16_max(int v) {
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) v = max(v, __shfl_xor(v, d));
+  return v;
+}
+__device__ __forceinline__ int row16_min(int v) {
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) v = min(v, __shfl_xor(v, d));
+  return v;
+}
+
+template <int SRC, int NC>
+__global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) void rows_attn(RowsArgs a) {
+  constexpr bool Q8 = SRC != kBf16;
+  constexpr int FMT = Q8 ? SRC : kQ8E4m3;
+  const int slot = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
+  const int kh = unit % a.hk, group = unit / a.hk, split = spread_split(slot, unit, a.splits);
+  const int4 item = reinterpret_cast<const int4*>(a.items)[group];  // sequence, first row, rows, row of the workspace
+  const int G = a.hq / a.hk, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
+  const int nrows = item.z;
+
+  // Columns: row c / G of the group, head c % G. Keys that each sees; a column that is none sees what the last does.
+  int64_t src0 = 0;  // bf16: the source's first row
+  int src_len = 0;
+  const int32_t* pg = nullptr;
+  if constexpr (Q8) {
+    pg = a.pages + a.indptr[item.x];
+  } else {
+    const int e = a.of ? a.of[item.x] : item.x;
+    src0 = a.first[e], src_len = max(a.len[e], 0);
+  }
+  int lim[NC], most = 0, least = INT_MAX;
+  bf16x8 q[NC][4];  // product step kk holds dims 64 (kk / 2) + 16 g + 8 (kk % 2) .. + 7
+#pragma unroll
+  for (int b = 0; b < NC; ++b) {
+    const int c = 16 * b + col, i = c / G;
+    const bool mine = i < nrows;
+    lim[b] = -1;
+    if (mine) {
+      lim[b] = Q8 ? max(a.pos[item.y + i], -1) + 1 : src_len;
+      most = max(most, lim[b]), least = min(least, lim[b]);
+    }
+    const bf16_t* qp = a.q + (int64_t)(item.y + (mine ? i : 0)) * a.q_stride + (int64_t)(kh * G + c % G) * kHead;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      q[b][kk] = __builtin_bit_cast(bf16x8, ldg16(qp + 64 * (kk >> 1) + 16 * grp + 8 * (kk & 1)));
+  }
+  most = __builtin_amdgcn_readfirstlane(row16_max(most));
+  least = __builtin_amdgcn_readfirstlane(row16_min(least));
+
+  const int split_len = most > 0 ? split_len_of(a.chunk, a.splits, most) : 0;
+  const int used = most > 0 ? (most - 1) / split_len + 1 : 0;
+  if (a.splits > 1 && split == 0 && kh == 0 && tid == 0) a.ws_used[group] = used;
+  const int packed = nrows * G;
+  if (used == 0) {
+    if (split == 0)
+      for (int i = tid; i < packed * kHead; i += kThreads)
+        a.out[((int64_t)(item.y + i / kHead / G) * a.hq + kh * G + i / kHead % G) * kHead + i % kHead] = 0;
+    return;
+  }
+  if (split >= used) return;
+  const int t0 = split * split_len, t1 = (int)min((int64_t)most, (int64_t)t0 + split_len);
+#pragma unroll
+  for (int b = 0; b < NC; ++b) lim[b] = lim[b] < 0 ? t1 : lim[b];
+  const int tiles = (t1 - t0 + kTile - 1) / kTile;
+  const int mine = (tiles - wave + kWaves - 1) / kWaves;  // tiles wave, wave + 4, ..
+
+  // 8-bit: blocks of kIds of the wave's tiles at a time: lane 2 k + b holds block b of tile k and its two exponents.
+  const int64_t row_blocks = 2LL * a.hk;
+  int ids = 0, exps = 0;
+  auto next_blocks = [&](int k0) __attribute__((always_inline)) {
+    const int tile = wave + kWaves * (k0 + (lane >> 1));
+    const int b = (int)min((int64_t)(t0 / kQ8Block) + (int64_t)tile * kBlocksPerTile + (lane & 1), (int64_t)((t1 - 1) / kQ8Block));
+    ids = (int)page_slot(a.pd, pg[page_index(a.pd, b)], b);
+    const uint8_t* e = a.kv_scale + ids * row_blocks + kh;
+    exps = e[0] | e[a.hk] << 16;
+  };
+  uint4 kr[Q8 ? 2 : 4][2], vr[Q8 ? 4 : 8];
+  auto load_k = [&](int k) __attribute__((always_inline)) {
+    if constexpr (Q8) {
+      const uint8_t* kb = a.kv + kh * kQ8HeadBytes + (2 * (col & 4) + (col & 3)) * kHead + 16 * grp + 8 * (col & 8);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int64_t block = __builtin_amdgcn_readlane(ids, 2 * (k & (kIds - 1)) + b);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) kr[j][b] = ldg16_stream(kb + block * row_blocks * kQ8HeadBytes + 4 * j * kHead);
+      }
+    } else {
+      const int n0 = t0 + (wave + kWaves * k) * kTile;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int key = min(n0 + 8 * (col >> 2) + 4 * j + (col & 3), t1 - 1);
+        const bf16_t* kp = a.k + (src0 + key) * a.k_stride + (int64_t)kh * kHead + 16 * grp;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) kr[2 * j + (kk >> 1)][kk & 1] = ldg16_stream(kp + 64 * (kk >> 1) + 8 * (kk & 1));
+      }
+    }
+  };
+  auto load_v = [&](int k) __attribute__((always_inline)) {
+    if constexpr (Q8) {
+      const int64_t block = from_lane(ids, 2 * (k & (kIds - 1)) + (grp >> 1));
+      const uint8_t* vb = a.kv + (block * row_blocks + a.hk + kh) * kQ8HeadBytes + (16 * (grp & 1) + col) * kQ8Block;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vr[i] = ldg16_stream(vb + i * 32 * kQ8Block);
+    } else {  // rows 4 i + g of the tile, 16-byte chunk col
+      const int n0 = t0 + (wave + kWaves * k) * kTile;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = min(n0 + 4 * i + grp, t1 - 1);
+        vr[i] = ldg16_stream(a.v + (src0 + key) * a.v_stride + (int64_t)kh * kHead + 8 * col);
+      }
+    }
+  };
+
+  f32x4 o[NC][8];
+  float m[NC], l[NC];
+#pragma unroll
+  for (int b = 0; b < NC; ++b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[b] = -INFINITY, l[b] = 0.f;
+  }
+  // One buffer for the waves' tiles of V (bf16) and, in the end, their parts of a block of columns.
+  constexpr int kPart = 16 * (kHead + 4);
+  constexpr int kLdsFloats = kWaves * kPart;  // 33 KiB, a wave's tile of V being 8
+  __shared__ __align__(16) float s_buf[kLdsFloats];
+  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+  bf16_t* v_lds = reinterpret_cast<bf16_t*>(s_buf) + wave * (kTile * kHead);
+
+  if (mine > 0) {
+    if constexpr (Q8) next_blocks(0);
+    load_k(0);
+  }
+  for (int k = 0; k < mine; ++k) {
+    // V of this tile, then (when its scores are taken) K of the next: one of the two is always in flight.
+    load_v(k);
+    int e2 = 0;
+    if constexpr (Q8) e2 = from_lane(exps, 2 * (k & (kIds - 1)) + (grp >> 1));
+    const int n0 = t0 + (wave + kWaves * k) * kTile, left = t1 - n0;  // keys from this tile on
+    float s[NC][8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      f32x4 d[NC];
+#pragma unroll
+      for (int b = 0; b < NC; ++b) d[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (Q8) trade_halves(kr[j][0], kr[j][1]);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        bf16x8 ka;
+        if constexpr (Q8) {
+          const uint4& w = kr[j][kk >> 1];
+          ka = kk & 1 ? bf16_of<FMT>(w.z, w.w) : bf16_of<FMT>(w.x, w.y);
+        } else {
+          ka = __builtin_bit_cast(bf16x8, kr[2 * j + (kk >> 1)][kk & 1]);
+        }
+#pragma unroll
+        for (int b = 0; b < NC; ++b) d[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, q[b][kk], d[b], 0, 0, 0);
+      }
+#pragma unroll
+      for (int b = 0; b < NC; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[b][4 * j + r] = d[b][r];
+    }
+    if (k + 1 < mine) {
+      if (Q8 && ((k + 1) & (kIds - 1)) == 0) next_blocks(k + 1);
+      load_k(k + 1);
+    }
+    const float ks = Q8 ? pow2_biased(e2 & 0xff) * a.scale_log2 : a.scale_log2, vs = Q8 ? pow2_biased(e2 >> 16) : 1.f;
+#pragma unroll
+    for (int b = 0; b < NC; ++b)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) s[b][t] *= ks;
+    if (n0 + kTile > least) {  // keys that some row does not see
+#pragma unroll
+      for (int b = 0; b < NC; ++b)
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          if (n0 + 8 * grp + t >= lim[b]) s[b][t] = -INFINITY;
+    }
+    if (left < kTile) {  // nothing past the last key that any row sees counts, whatever it holds
+      if constexpr (Q8) {
+        const int tokens = left - kQ8Block * (grp >> 1);  // of this lane's block
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int n_ok = min(max(tokens - 4 * w, 0), 4);
+          const uint32_t stay = n_ok == 4 ? ~0u : (1u << (8 * n_ok)) - 1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) (&vr[i].x)[w] &= stay;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (4 * i + grp >= left) vr[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    bf16x8 ph[NC], pl[NC];
+#pragma unroll
+    for (int b = 0; b < NC; ++b) {
+      float mx = s[b][0];
+#pragma unroll
+      for (int t = 1; t < 8; ++t) mx = fmaxf(mx, s[b][t]);
+      mx = max_of_groups(mx);
+      const bool grow = mx > m[b];
+      if (__any(grow)) {
+        const float to = mx + 8.f, alpha = grow ? fast_exp2(m[b] - to) : 1.f;
+        m[b] = grow ? to : m[b];
+        l[b] *= alpha;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[b][i] *= alpha;
+      }
+      const float base = m[b] == -INFINITY ? 0.f : m[b];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        s[b][t] = fast_exp2(s[b][t] - base);
+        l[b] += s[b][t];
+        s[b][t] *= vs;
+      }
+      const uint4 hi = pack8(s[b]);
+      float rest[8];
+      widen8(hi, rest);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) rest[t] = s[b][t] - rest[t];
+      ph[b] = __builtin_bit_cast(bf16x8, hi), pl[b] = __builtin_bit_cast(bf16x8, pack8(rest));
+    }
+    const auto weigh = [&](int i, const bf16x8& v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < NC; ++b) {
+        o[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph[b], o[b][i], 0, 0, 0);
+        o[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl[b], o[b][i], 0, 0, 0);
+      }
+    };
+    if constexpr (Q8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // Even groups keep tokens 0-7 of their dim and take those of the odd group's, and the other way round.
+        const auto a0 = __builtin_amdgcn_permlane16_swap(vr[i].x, vr[i].z, false, false);
+        const auto a1 = __builtin_amdgcn_permlane16_swap(vr[i].y, vr[i].w, false, false);
+        weigh(2 * i, bf16_of<FMT>(a0[0], a1[0]));
+        weigh(2 * i + 1, bf16_of<FMT>(a0[1], a1[1]));
+      }
+    } else {
+      // 32-byte unit u of row r lies in unit u ^ (r % 4 + 4 (r / 8 % 2)): the 8 rows x
+      // 32 bytes that 32 lanes of a transposing read take are disjoint banks.
+      wave_lds_fence();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + grp, f = (r & 3) | (r >> 3 & 1) << 2;
+        *reinterpret_cast<uint4*>(v_lds + r * kHead + 16 * ((col >> 1) ^ f) + 8 * (col & 1)) = vr[i];
+      }
+      wave_lds_fence();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        bf16x4 part[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 8 * grp + 4 * h + (col >> 2), f = (r & 3) | (r >> 3 & 1) << 2;
+          part[h] = lds_read_tr(v_lds + r * kHead + 16 * (i ^ f) + 4 * (col & 3));
+        }
+        weigh(i, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    }
+  }
+
+  // The waves' parts, merged, a block of columns at a time: O rows [column][dim], then (m, l).
+  const int waves = min(tiles, kWaves);
+#pragma unroll
+  for (int b = 0; b < NC; ++b) {
+    if (16 * b >= packed) break;
+    l[b] += xor_lane(l[b], 16);
+    l[b] += xor_lane(l[b], 32);
+    __syncthreads();  // V's tiles and the block before have been read
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<f32x4*>(s_buf + wave * kPart + col * (kHead + 4) + 16 * i + 4 * grp) = o[b][i];
+    if (grp == 0) s_m[wave][col] = m[b], s_l[wave][col] = l[b];
+    __syncthreads();
+    for (int i = tid; i < min(packed - 16 * b, 16) * kHead; i += kThreads) {
+      const int g = i / kHead, d = i % kHead, c = 16 * b + g, row = c / G, head = kh * G + c % G;
+      float top = s_m[0][g];
+      for (int w = 1; w < waves; ++w) top = fmaxf(top, s_m[w][g]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float num = 0.f, den = 0.f;
+      for (int w = 0; w < waves; ++w) {
+        const float e = fast_exp2(s_m[w][g] - base);
+        num = fmaf(s_buf[w * kPart + g * (kHead + 4) + d], e, num);
+        den = fmaf(s_l[w][g], e, den);
+      }
+      if (used == 1) {
+        const bool none = Q8 && a.pos[item.y + row] < 0;  // among rows that see keys
+        a.out[((int64_t)(item.y + row) * a.hq + head) * kHead + d] = none ? 0 : (bf16_t)f2bf(num / den);
+      } else {
+        // den = 0: the row sees nothing of this split (or every score is -inf): it weighs nothing beside the others.
+        const int64_t at = ((int64_t)(item.w + row) * a.hq + head) * a.splits + split;
+        a.ws_o[at * kHead + d] = den == 0.f ? 0.f : num / den;
+        if (d == 0) a.ws_lse[at] = base + __log2f(den);
+      }
+    }
+  }
+}
+
+// The splits of a group's rows, merged: sum of o_i 2^(lse_i - max) over the sum of
+// those weights. 32 lanes of 4 dims a (row, head), kMergeBatch splits at a time, asked
+// for before their weights are known.
+constexpr int kMergeRows = kThreads / 32;
+constexpr int kMergeBatch = 16;
+
+template <bool Q8>
+__global__ __launch_bounds__(kThreads) void rows_merge(RowsArgs a, int parts) {
+  const int group = blockIdx.x / parts;
+  const int used = a.ws_used[group];
+  if (used <= 1) return;
+  const int4 item = reinterpret_cast<const int4*>(a.items)[group];
+  const int x = (blockIdx.x % parts) * kMergeRows + (threadIdx.x >> 5), row = x / a.hq, head = x % a.hq;
+  if (row >= item.z) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t h = (int64_t)(item.w + row) * a.hq + head;
+  const float* lse = a.ws_lse + h * a.splits;
+  const float* part = a.ws_o + h * a.splits * kHead + 4 * lane;
+  f32x4 num = {0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, den = 0.f;
+  for (int i0 = 0; i0 < used; i0 += kMergeBatch) {
+    f32x4 o[kMergeBatch];
+    float e[kMergeBatch];
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j) {
+      const int i = min(i0 + j, used - 1);
+      e[j] = lse[i];
+      o[j] = *reinterpret_cast<const f32x4*>(part + (int64_t)i * kHead);
+    }
+    float mx = top;
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j) mx = fmaxf(mx, e[j]);  // one seen twice changes no maximum
+    const float base = mx == -INFINITY ? 0.f : mx, alpha = fast_exp2(top - base);
+    top = mx;
+    num *= alpha, den *= alpha;
+#pragma unroll
+    for (int j = 0; j < kMergeBatch; ++j) {
+      const float w = i0 + j < used ? fast_exp2(e[j] - base) : 0.f;
+      num += o[j] * w, den += w;
+    }
+  }
+  uint2 w = make_uint2(pack_bf16x2(num[0] / den, num[1] / den), pack_bf16x2(num[2] / den, num[3] / den));
+  if (Q8 && a.pos[item.y + row] < 0) w = make_uint2(0, 0);
+  *reinterpret_cast<uint2*>(a.out + ((int64_t)(item.y + row) * a.hq + head) * kHead + 4 * lane) = w;
+}
+
+template <int SRC>
+int launch(RowsArgs a, const int* groups, hipStream_t stream) {
+  RowsArgs x = a;
+  for (int c = 0; c < 2; ++c) {
+    if (groups[c] == 0) continue;
+    const unsigned grid = (unsigned)((int64_t)groups[c] * a.hk * a.splits);
+    if (c == 0)
+      rows_attn<SRC, 1><<<grid, kThreads, 0, stream>>>(x);
+    else
+      rows_attn<SRC, 2><<<grid, kThreads, 0, stream>>>(x);
+    if (check_launch() != 0) return -3;
+    if (a.splits > 1) {
+      const int rows = std::max((c + 1) * 16 / (a.hq / a.hk), 1), parts = (rows * a.hq + kMergeRows - 1) / kMergeRows;
+      rows_merge<SRC != kBf16><<<(unsigned)((int64_t)groups[c] * parts), kThreads, 0, stream>>>(x, parts);
+      if (check_launch() != 0) return -3;
+    }
+    x.items += 4 * (int64_t)groups[c], x.ws_used += groups[c];
+  }
+  return 0;
+}
+
+}  // namespace
+
+int launch_rows(const RowsArgs& a, int source, const int* groups, hipStream_t stream) {
+  return source == kRowsBf16 ? launch<kBf16>(a, groups, stream)
+         : source == kQ8E4m3 ? launch<kQ8E4m3>(a, groups, stream)
+                             : launch<kQ8Int8>(a, groups, stream);
+}
+
+}  // namespace omni

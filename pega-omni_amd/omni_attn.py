@@ -65,6 +65,10 @@ EXPORTS = (
     "omni_qwen3_attend_q8",
     "omni_attn_prompt_plan_init",
     "omni_attn_prompt_run",
+    "omni_attn_extend_plan_init",
+    "omni_attn_cross_plan_init",
+    "omni_qwen3_extend_q8",
+    "omni_attn_cross_run",
     "omni_attn_pages_fork",
     "omni_attn_pages_free",
     "omni_attn_pages_compact",
@@ -128,6 +132,26 @@ class PromptPlan(ctypes.Structure):
     ]
 
 
+class MultiPlan(ctypes.Structure):
+    _fields_ = [
+        ("cross", ctypes.c_int32),
+        ("nseq", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("hq", ctypes.c_int32),
+        ("hk", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("groups", ctypes.c_int32 * 2),
+        ("group_rows", ctypes.c_int32),
+        ("chunk", ctypes.c_int32),
+        ("splits", ctypes.c_int32),
+        ("tiles", ctypes.c_int32),
+        ("tile_chunk", ctypes.c_int32),
+        ("tile_splits", ctypes.c_int32),
+        ("work_bytes", ctypes.c_int64),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -145,6 +169,7 @@ def load(path: str | None = None):
     dplan = ctypes.POINTER(DecodePlan)
     pplan = ctypes.POINTER(PrefillPlan)
     qplan = ctypes.POINTER(PromptPlan)
+    mplan = ctypes.POINTER(MultiPlan)
     sig = {
         "omni_attn_decode_plan_init": [i32, i32, i32, i32, i32, i32, dplan],
         "omni_attn_decode_plan_init_fp8": [i32, i32, i32, i32, i32, dplan],
@@ -184,6 +209,10 @@ def load(path: str | None = None):
         "omni_qwen3_attend_q8": [P, i64, P, P, i32, P, P, i32, P, P, i32, P, i32, i32, f32, dplan, P, P],
         "omni_attn_prompt_plan_init": [i32, P, i32, i32, P, i64, qplan],
         "omni_attn_prompt_run": [qplan, P, i64, P, i64, P, i64, P, f32, P, P],
+        "omni_attn_extend_plan_init": [i32, P, P, i32, i32, i32, i32, P, i64, mplan],
+        "omni_attn_cross_plan_init": [i32, P, P, i32, i32, i32, i32, P, i64, mplan],
+        "omni_qwen3_extend_q8": [mplan, P, i64, P, P, i32, P, P, P, i32, P, f32, P, P, P],
+        "omni_attn_cross_run": [mplan, P, i64, P, i64, P, i64, P, P, P, P, f32, P, P, P],
         "omni_attn_pages_fork": [P, P, P, i32, i32, P, i64, i32, P, i32, P, P, P, P, P, P],
         "omni_attn_pages_free": [P, P, i32, i32, P, i64, i32, P, i32, P, P, P, P],
         "omni_attn_pages_compact": [P, i64, i32, P, i32, P, P, i32, P, P, P, P, P, P, i32, P, P],
@@ -710,6 +739,81 @@ def prompt_run(pp: Prompt, q, k, v, out, scale, stream=None):
         rows * hq * HEAD_DIM, pp.work, plan.work_bytes >> 2)
     _check(load().omni_attn_prompt_run(ctypes.byref(plan), p_q, q_ld, p_k, k_ld, p_v, v_ld, p_out, scale, p_work,
                                        _stream_on(stream, d)))
+    return out
+
+
+# ------------------------------------- several rows per sequence, encoder states
+@dataclass
+class Multi:
+    plan: MultiPlan
+    work: object  # device int32 tensor
+
+
+def _multi_plan(init, counts, keys, hq, hk, max_len, chunk, device) -> Multi:
+    import numpy as np
+
+    counts_a = np.ascontiguousarray(counts, dtype=np.int32)
+    keys_a = None if keys is None else np.ascontiguousarray(keys, dtype=np.int32)
+    if keys_a is not None and len(keys_a) != len(counts_a):
+        raise OmniAttnError(EINVAL, f"{len(keys_a)} lengths for {len(counts_a)} sequences")
+    ptr = lambda a: None if a is None else a.ctypes.data_as(ctypes.c_void_p)
+    plan = MultiPlan()
+    rc = init(len(counts_a), ptr(counts_a), ptr(keys_a), hq, hk, max_len, chunk, None, 0, ctypes.byref(plan))
+    if rc not in (OK, EWORKSPACE):
+        _check(rc)
+    work_h = np.zeros(max(4, int(plan.work_bytes) // 4), dtype=np.int32)
+    _check(init(len(counts_a), ptr(counts_a), ptr(keys_a), hq, hk, max_len, chunk, ptr(work_h), len(work_h), ctypes.byref(plan)))
+    return Multi(plan, _torch.from_numpy(work_h).to(device))
+
+
+def extend_plan(counts, hq, hk, max_len, keys=None, chunk=0, device="cuda") -> Multi:
+    """Host plan of qwen3_extend_q8 for ``counts[s]`` rows of each sequence;
+    uploads the work list. ``keys``: how many keys each sequence's last row sees
+    now, if known (order and split sizes alone); the workspace is
+    ``workspace_for(plan.plan)``."""
+    return _multi_plan(load().omni_attn_extend_plan_init, counts, keys, hq, hk, max_len, chunk, device)
+
+
+def cross_plan(counts, hq, hk, max_len, keys=None, chunk=0, device="cuda") -> Multi:
+    """Host plan of cross_run for ``counts[s]`` rows over each source, as extend_plan."""
+    return _multi_plan(load().omni_attn_cross_plan_init, counts, keys, hq, hk, max_len, chunk, device)
+
+
+def _multi_ws(plan, workspace, d):
+    if workspace is not None and workspace.get_device() != d:
+        raise OmniAttnError(EINVAL, "workspace must lie on the current device, with the other tensors")
+    return _ws(plan, workspace)
+
+
+def qwen3_extend_q8(mp: Multi, q, kv, kv_scale, pos, indptr, pages, page, out, scale, workspace=None, stream=None):
+    """Attention of several new rows per sequence over the 8-bit cache: row n of
+    the plan's sequence s sees keys 0..pos[n] (the call's rows among them); rows
+    with a negative position store zeros. q rows [hq * 128], possibly strided."""
+    plan = mp.plan
+    rows, hq = plan.rows, plan.hq
+    d = _current_device() if q.is_cuda else -1
+    src, stride, cache, scales, fmt, p_pos, p_indptr, p_pages, p_out, p_work = _take(
+        "rciiibi", "q kv pos indptr pages out work", d, q, rows, hq * HEAD_DIM, kv, kv_scale, 2 * plan.hk, pos, rows, indptr,
+        plan.nseq + 1, pages, 0, out, rows * hq * HEAD_DIM, mp.work, plan.work_bytes >> 2)
+    _check(load().omni_qwen3_extend_q8(ctypes.byref(plan), src, stride, cache, scales, fmt, p_pos, p_indptr, p_pages, page, p_out,
+                                       scale, p_work, _multi_ws(plan, workspace, d), _stream_on(stream, d)))
+    return out
+
+
+def cross_run(mp: Multi, q, k, v, of, first, length, out, scale, workspace=None, stream=None):
+    """Cross attention: the plan's rows of sequence s see rows first[e] ..
+    first[e] + length[e] - 1 of k and v, e = of[s] (of None: s); zeros where there
+    are none. q rows [hq * 128], k and v rows [hk * 128], possibly strided (k and v
+    parts of one row)."""
+    plan = mp.plan
+    rows, hq, hk = plan.rows, plan.hq, plan.hk
+    d = _current_device() if q.is_cuda else -1
+    p_q, q_ld, p_k, k_ld, p_v, v_ld, p_of, p_first, p_len, p_out, p_work = _take(
+        "rrrIiibi", "q k v of first length out work", d, q, rows, hq * HEAD_DIM, k, 0, hk * HEAD_DIM, v, 0, hk * HEAD_DIM, of,
+        plan.nseq, first, 0 if of is not None else plan.nseq, length, first.numel(), out, rows * hq * HEAD_DIM, mp.work,
+        plan.work_bytes >> 2)
+    _check(load().omni_attn_cross_run(ctypes.byref(plan), p_q, q_ld, p_k, k_ld, p_v, v_ld, p_of, p_first, p_len, p_out, scale, p_work,
+                                      _multi_ws(plan, workspace, d), _stream_on(stream, d)))
     return out
 
 

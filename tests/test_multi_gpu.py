@@ -1,0 +1,302 @@
+"""Several rows per sequence over the 8-bit cache, and rows over encoder states, on the
+GPU: against 64 bits, at the counts, lengths and head layouts where groups, tiles and
+splits begin and end; with rubbish in every place that no row sees; in graphs."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import multi_refs as M
+import omni_attn as oa
+import serve_refs as R
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = [torch.float8_e4m3fn, torch.int8]
+SCALE = 128 ** -0.5
+
+
+def i32(a):
+    return torch.from_numpy(np.array(a, dtype=np.int32).copy()).cuda()
+
+
+def bf16(g, *shape):
+    return torch.randn(*shape, device="cuda", generator=g).to(torch.bfloat16)
+
+
+class Cache:
+    """Sequences of the given lengths in an 8-bit cache; every token that is none of theirs is NaN (E4M3) or the largest integer
+    under the largest exponent."""
+
+    def __init__(self, seed, lens, hk, page, fmt, spare=3):
+        rng = np.random.default_rng(seed)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        need = [-(-n // page) for n in lens]
+        pool, per = sum(need) + spare, page // 16
+        self.kv, self.sc = oa.q8_cache(pool, page, hk, fmt)
+        x = torch.randn(self.kv.shape, device="cuda", generator=g)
+        self.kv.copy_((x * 90).clamp(-448, 448).to(fmt) if fmt == torch.float8_e4m3fn else (x * 40).round().clamp(-127, 127).to(fmt))
+        self.sc.view(torch.uint8).copy_(torch.randint(116, 123, self.sc.shape, device="cuda", generator=g).to(torch.uint8))
+        ids = rng.permutation(pool)
+        self.hk, self.page, self.lens = hk, page, lens
+        indptr, pages = [0], []
+        live = torch.zeros(pool * page, dtype=torch.bool)
+        self.slots = []
+        for n, c in zip(lens, need):
+            mine = [int(x) for x in ids[len(pages):len(pages) + c]]
+            pages += mine
+            indptr.append(len(pages))
+            at = [mine[t // page] * page + t % page for t in range(n)]
+            self.slots.append(at)
+            live[at] = True
+        self.indptr, self.pages = i32(indptr), i32(pages if pages else [0])
+        raw = self.kv.view(torch.uint8)
+        bad = 0x7f
+        dead = (~live).view(-1, 16).cuda()
+        k = raw[:, :hk].view(-1, hk, 16, 128)
+        k[dead[:, None].expand(-1, hk, -1)] = bad
+        v = raw[:, hk:].view(-1, hk, 128, 16).transpose(2, 3)
+        v[dead[:, None].expand(-1, hk, -1)] = bad
+        self.sc.view(torch.uint8)[dead.all(1)] = 254
+        assert per >= 1
+
+    def tokens(self, s):
+        if not hasattr(self, "_t"):
+            self._t = R.Cache(self.kv, self.sc, self.hk).tokens()
+        return self._t[0][self.slots[s]], self._t[1][self.slots[s]]
+
+
+def extend(c, counts, hq, pos=None, chunk=0, keys=True, extra=2, seed=1, max_len=None, stream=None, stride=0, scale=SCALE):
+    """Runs the call on the last counts[s] tokens of each sequence (or at `pos`), checks it against 64 bits; the plan and the output."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rows = sum(counts)
+    if pos is None:
+        pos = [n - k + i for n, k in zip(c.lens, counts) for i in range(k)]
+    q = bf16(g, rows + extra, hq * 128 + stride)[:, :hq * 128]
+    out = torch.full((rows + extra, hq * 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    mp = oa.extend_plan(counts, hq, c.hk, max_len or max(c.lens + [1]), c.lens if keys else None, chunk)
+    ws = oa.workspace_for(mp.plan)
+    if ws is not None:
+        ws.fill_(0xff)
+    torch.cuda.synchronize()
+    oa.qwen3_extend_q8(mp, q, c.kv, c.sc, i32(pos if rows else [0]), c.indptr, c.pages, c.page, out, scale, ws, stream)
+    torch.cuda.synchronize()
+    assert bool((out[rows:] == 7).all())
+    at = 0
+    for s, k in enumerate(counts):
+        if k:
+            kk, vv = c.tokens(s)
+            lim = [p + 1 for p in pos[at:at + k]]
+            want, size = M.rows_of(q[at:at + k].cpu().view(k, hq, 128), kk, vv, lim, scale)
+            got = out[at:at + k].cpu().double().view(k, hq, 128)
+            err = (got - want).abs() - M.bound(want, size, mp.plan.tiles > 0)
+            assert bool((err <= 0).all()), f"sequence {s}: {float(err.max()):.3g} at {int(err.argmax())}, {err.isnan().any()}"
+            for i, n in enumerate(lim):
+                if n <= 0:
+                    assert bool((out[at + i] == 0).all())
+        at += k
+    return mp, out
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (3, 1), (8, 2), (5, 1), (16, 2), (14, 1), (16, 1)])
+def test_extend_of_few_rows(hq, hk, fmt):
+    """Groups of one row to a little more than two groups', lengths about a tile and a block, a sequence without rows."""
+    g = hq // hk
+    counts = [1, 16 // g, 0, 16 // g + 1, 32 // g, 32 // g + 1, 2, 3]
+    lens = [1, 16 // g + 31, 9, 32 + 16 // g, 32 // g, 130, 33, 64]
+    c = Cache(hq * 7 + hk, lens, hk, 16, fmt)
+    mp, _ = extend(c, counts, hq)
+    assert mp.plan.rows == sum(counts)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("page", [16, 48, 256])
+@pytest.mark.parametrize("chunk", [64, 128, 0])
+def test_extend_in_splits(page, chunk, fmt):
+    """Rows that end in different splits, rows in the first split alone, one to thirty splits."""
+    lens = [1900, 700, 129, 128, 64, 65, 5]
+    counts = [4, 70, 3, 1, 2, 5, 5]
+    c = Cache(page + chunk, lens, 2, page, fmt)
+    extend(c, counts, 8, chunk=chunk, keys=chunk != 128)
+    extend(c, counts, 2, chunk=chunk, seed=2)
+
+
+def test_extend_past_the_plans_bound():
+    """Rows longer than max_len run in splits that grow."""
+    c = Cache(5, [900, 40], 2, 16, torch.float8_e4m3fn)
+    mp, _ = extend(c, [3, 2], 4, chunk=64, max_len=128)
+    assert mp.plan.splits == 2
+
+
+def test_extend_at_any_positions():
+    """Positions in no order, twice the same, far behind, and rows that are none."""
+    c = Cache(6, [300, 75], 2, 16, torch.int8)
+    pos = [299, 0, -1, 150, 150, 31, 32, -7, 74, -1, 3]
+    for chunk in (0, 64):
+        extend(c, [8, 3], 4, pos=pos, chunk=chunk)
+    extend(c, [8, 3], 4, pos=[-1] * 11, chunk=64)
+
+
+def test_extend_equals_decode_on_single_rows():
+    """One row a sequence: the row of omni_qwen3_attend_q8, to the rounding of the output."""
+    lens = [1, 17, 500, 1234]
+    c = Cache(9, lens, 2, 16, torch.float8_e4m3fn)
+    mp, out = extend(c, [1] * 4, 8, extra=0)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = bf16(g, 4, 8 * 128)
+    plan = oa.decode_plan_q8(4, 8, 2, 16, max(lens))
+    other = torch.zeros_like(out)
+    oa.qwen3_attend_q8(q, c.kv, c.sc, i32([n - 1 for n in lens]), None, 0, c.indptr, c.pages, 16, other, 8, 2, SCALE, plan, oa.workspace_for(plan))
+    torch.cuda.synchronize()
+    assert bool(((out.float() - other.float()).abs() <= 2.0 ** -7 * other.float().abs() + 2.0 ** -12).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, -SCALE, 3.0, -40.0])
+def test_extend_scales(scale):
+    c = Cache(12, [80, 41], 1, 16, torch.int8)
+    if abs(scale) < 1:
+        extend(c, [5, 20], 2, scale=scale)
+        return
+    # One key takes nearly all the weight: which one is a matter of the scores' own rounding; finite, and within the values.
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = bf16(g, 25, 256)
+    out = torch.zeros_like(q)
+    mp = oa.extend_plan([5, 20], 2, 1, 80)
+    oa.qwen3_extend_q8(mp, q, c.kv, c.sc, i32(list(range(75, 80)) + list(range(21, 41))), c.indptr, c.pages, 16, out, scale, oa.workspace_for(mp.plan))
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(out).all()) and float(out.abs().max()) <= 127 * 2.0 ** (122 - 127) * 1.01
+
+
+@pytest.mark.parametrize("stride", [8, 128])
+def test_extend_of_strided_rows_on_another_stream(stride):
+    c = Cache(13, [90, 33], 2, 32, torch.int8)
+    extend(c, [20, 1], 4, stride=stride, stream=torch.cuda.Stream())
+
+
+# ------------------------------------------------------------------ cross
+def cross(seed, counts, lens, hq, hk, chunk=0, keys=True, of=None, max_len=None, extra=2, layout="one", stream=None, scale=SCALE):
+    """Sources of the given lengths in any order, NaN between them; the call against 64 bits."""
+    rng = np.random.default_rng(seed)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    order = rng.permutation(len(lens))
+    first, at = [0] * len(lens), 1
+    for e in order:
+        first[e] = at
+        at += max(0, lens[e]) + int(rng.integers(0, 3))
+    total = at + 1
+    k, v = bf16(g, total, hk * 128), bf16(g, total, hk * 128)
+    live = torch.zeros(total, dtype=torch.bool)
+    for e, n in enumerate(lens):
+        live[first[e]:first[e] + max(0, n)] = True
+    k[~live.cuda()], v[~live.cuda()] = math.nan, math.nan
+    if layout == "one":  # parts of one row
+        kv = torch.cat([k, v], 1)
+        k, v = kv[:, :hk * 128], kv[:, hk * 128:]
+    elif layout == "apart":
+        pad = torch.zeros(total, hk * 128 + 8, dtype=torch.bfloat16, device="cuda")
+        pad[:, 8:] = v
+        v = pad[:, 8:]
+    rows = sum(counts)
+    q = bf16(g, rows + extra, hq * 128)
+    out = torch.full((rows + extra, hq * 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    named = list(range(len(counts))) if of is None else of
+    mp = oa.cross_plan(counts, hq, hk, max_len or max(lens + [1]), [max(0, lens[e]) for e in named] if keys else None, chunk)
+    ws = oa.workspace_for(mp.plan)
+    if ws is not None:
+        ws.fill_(0xff)
+    torch.cuda.synchronize()
+    oa.cross_run(mp, q, k, v, None if of is None else i32(of), i32(first), i32(lens), out, scale, ws, stream)
+    torch.cuda.synchronize()
+    assert bool((out[rows:] == 7).all())
+    at = 0
+    for s, c in enumerate(counts):
+        e = named[s]
+        n = max(0, lens[e])
+        part = slice(first[e], first[e] + n)
+        want, size = M.rows_of(q[at:at + c].cpu().view(c, hq, 128), k[part].cpu().view(n, hk, 128), v[part].cpu().view(n, hk, 128), [n] * c, scale)
+        got = out[at:at + c].cpu().double().view(c, hq, 128)
+        err = (got - want).abs() - M.bound(want, size, mp.plan.tiles > 0)
+        assert c == 0 or bool((err <= 0).all()), f"sequence {s}: {float(err.max()):.3g}, {err.isnan().any()}"
+        at += c
+    return mp, out
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (3, 1), (8, 2), (5, 1), (16, 2), (14, 1), (16, 1), (4, 4)])
+@pytest.mark.parametrize("layout", ["own", "one", "apart"])
+def test_cross_of_few_rows(hq, hk, layout):
+    g = hq // hk
+    counts = [1, 16 // g, 0, 16 // g + 1, 32 // g, 32 // g + 1, 2, 3, 5]
+    lens = [1, 31, 9, 32, 33, 130, 0, 64, -3]
+    cross(hq * 5 + hk, counts, lens, hq, hk, layout=layout)
+
+
+@pytest.mark.parametrize("chunk", [64, 128, 0])
+def test_cross_in_splits(chunk):
+    cross(chunk, [4, 70, 3, 1, 2, 5, 5], [1900, 700, 129, 128, 0, 65, 5], 8, 2, chunk=chunk, keys=chunk != 128)
+
+
+def test_cross_over_shared_sources():
+    cross(3, [5, 5, 1, 40, 2], [300, 77, 12], 4, 2, of=[1, 0, 1, 1, 2])
+
+
+def test_cross_past_the_plans_bound():
+    mp, _ = cross(4, [3, 2], [900, 40], 4, 2, chunk=64, max_len=128)
+    assert mp.plan.splits == 2
+
+
+@pytest.mark.parametrize("scale", [0.0, -SCALE])
+def test_cross_scales_on_another_stream(scale):
+    cross(5, [3, 20], [200, 40], 2, 1, scale=scale, stream=torch.cuda.Stream())
+
+
+def test_no_rows_and_no_sequences():
+    for counts in ([], [0, 0]):
+        mp = oa.cross_plan(counts, 4, 2, 10)
+        out = torch.full((2, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+        q, k = torch.zeros(1, 512, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 256, dtype=torch.bfloat16, device="cuda")
+        oa.cross_run(mp, q, k, k, None, i32([0, 0]), i32([0, 0]), out, SCALE)
+        torch.cuda.synchronize()
+        assert bool((out == 7).all())
+
+
+# ------------------------------------------------------------------ graphs
+def test_two_graphs_with_workspaces_of_their_own():
+    """Extend and cross captured together, twice; lengths and positions move on between replays, eager work in between."""
+    hq, hk, lens, counts = 8, 2, [400, 90, 33], [4, 20, 2]
+    c = Cache(21, lens, hk, 16, torch.float8_e4m3fn)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rows = sum(counts)
+    q = bf16(g, rows, hq * 128)
+    kv = bf16(g, 500, 2 * hk * 128)
+    k, v = kv[:, :hk * 128], kv[:, hk * 128:]
+    start = [n - m + i - 30 for n, m in zip(lens, counts) for i in range(m)]
+    pos, first, length = i32(start), i32([0, 200, 333]), i32([150, 3, 0])
+
+    def make():
+        e, x = oa.extend_plan(counts, hq, hk, 400, lens, 64), oa.cross_plan(counts, hq, hk, 200, None, 64)
+        return e, oa.workspace_for(e.plan), x, oa.workspace_for(x.plan), torch.zeros(2, rows, hq * 128, dtype=torch.bfloat16, device="cuda")
+
+    def step(m, s=None):
+        oa.qwen3_extend_q8(m[0], q, c.kv, c.sc, pos, c.indptr, c.pages, 16, m[4][0], SCALE, m[1], s)
+        oa.cross_run(m[2], q, k, v, None, first, length, m[4][1], SCALE, m[3], s)
+
+    sets = [make() for _ in range(3)]
+    torch.cuda.synchronize()
+    graphs, s = [], torch.cuda.Stream()
+    for m in sets[1:]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            step(m)
+    for rep in range(12):
+        step(sets[0])
+        torch.cuda.synchronize()
+        for gr, m in zip(graphs, sets[1:]):
+            m[4].zero_()
+            gr.replay()
+        torch.cuda.synchronize()
+        for m in sets[1:]:
+            assert torch.equal(m[4], sets[0][4]), rep
+        pos += 2
+        length += i32([3, 7, 11])

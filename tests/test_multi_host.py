@@ -1,0 +1,161 @@
+"""Plans of extend and cross attention, and what the calls refuse before any launch (CPU)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import omni_attn as oa
+
+P = 4096  # stands for a device pointer: nothing is launched
+PLANS = [oa.extend_plan, oa.cross_plan]
+
+
+def groups_of(mp):
+    n0, n1 = mp.plan.groups
+    skip = mp.plan.work_bytes // 4 - 4 * (n0 + n1)
+    it = mp.work.numpy()[skip:skip + 4 * (n0 + n1)].reshape(-1, 4)
+    return it[:n0], it[n0:]
+
+
+@pytest.mark.parametrize("make", PLANS)
+@pytest.mark.parametrize("hq,hk", [(3, 1), (5, 1), (10, 2), (16, 1), (7, 7), (8, 2)])
+def test_groups_cover_every_row_once(make, hq, hk):
+    g = hq // hk
+    counts = [0, 1, 16 // g, 16 // g + 1, 32 // g, 2, 0, 3]
+    if g not in (1, 2, 4, 8):
+        counts += [32 // g + 1, 100]
+    mp = make(counts, hq, hk, 500, device="cpu")
+    starts = np.cumsum([0] + counts)
+    seen = np.zeros(sum(counts), int)
+    at = 0
+    for cols, list_ in zip((16, 32), groups_of(mp)):
+        for s, first, rows, ws in list_:
+            assert starts[s] <= first and first + rows <= starts[s + 1] and 1 <= rows and rows * g <= cols and ws == at
+            seen[first:first + rows] += 1
+            at += rows
+    assert (seen == 1).all() and mp.plan.group_rows == at == mp.plan.rows == sum(counts)
+
+
+@pytest.mark.parametrize("make", PLANS)
+def test_long_sequences_come_first(make):
+    mp = make([1, 1, 4, 1], 4, 4, 900, [5, 800, 20, 300], device="cpu")
+    assert groups_of(mp)[0][:, 0].tolist() == [1, 3, 2, 0]
+
+
+@pytest.mark.parametrize("make", PLANS)
+def test_plan_bounds(make):
+    for counts, keys, hq, hk, n, chunk, code in (
+            ([-1], None, 4, 2, 9, 0, oa.EINVAL), ([1], [-1], 4, 2, 9, 0, oa.EINVAL), ([1], [1, 2], 4, 2, 9, 0, oa.EINVAL),
+            ([1], None, 5, 2, 9, 0, oa.EINVAL), ([1], None, 0, 1, 9, 0, oa.EINVAL), ([1], None, 4, 0, 9, 0, oa.EINVAL),
+            ([1], None, 4, 2, 0, 0, oa.EINVAL), ([1], None, 4, 2, 9, 65, oa.EINVAL), ([1], None, 17, 1, 9, 0, oa.EUNSUPPORTED),
+            ([2**31 - 1, 2**31 - 1], None, 1, 1, 9, 0, oa.EUNSUPPORTED)):
+        with pytest.raises(oa.OmniAttnError) as e:
+            make(counts, hq, hk, n, keys, chunk, device="cpu")
+        assert e.value.code == code, (counts, hq, hk)
+    mp = make([], 4, 2, 9, device="cpu")
+    assert mp.plan.rows == 0 and mp.plan.work_bytes == 0 and mp.plan.workspace_bytes == 0
+
+
+@pytest.mark.parametrize("init", ["omni_attn_extend_plan_init", "omni_attn_cross_plan_init"])
+def test_plan_capacity(init):
+    f, plan = getattr(oa.load(), init), oa.MultiPlan()
+    counts, work = np.array([3, 1], np.int32), np.zeros(8, np.int32)
+    ptr = lambda a: a.ctypes.data_as(ctypes.c_void_p)
+    assert f(2, ptr(counts), None, 4, 2, 50, 0, ptr(work), 7, ctypes.byref(plan)) == oa.EWORKSPACE and plan.work_bytes == 32
+    assert f(2, ptr(counts), None, 4, 2, 50, 0, None, 99, ctypes.byref(plan)) == oa.EWORKSPACE
+    assert f(2, ptr(counts), None, 4, 2, 50, 0, ptr(work), 8, ctypes.byref(plan)) == oa.OK
+    assert f(2, None, None, 4, 2, 50, 0, ptr(work), 8, ctypes.byref(plan)) == oa.EINVAL
+    assert f(-1, ptr(counts), None, 4, 2, 50, 0, ptr(work), 8, ctypes.byref(plan)) == oa.EINVAL
+    assert f(2, ptr(counts), None, 4, 2, 50, 0, ptr(work), 8, None) == oa.EINVAL
+
+
+@pytest.mark.parametrize("make", PLANS)
+def test_splits_follow_the_chunk(make):
+    mp = make([1, 2], 4, 2, 1000, None, 128, device="cpu")
+    p = mp.plan
+    assert (p.chunk, p.splits) == (128, 8) and p.workspace_bytes == 3 * 4 * 8 * 129 * 4 + 4 * 2
+    assert make([1, 2], 4, 2, 1000, None, 1024, device="cpu").plan.workspace_bytes == 0
+
+
+def extend(plan=None, **k):
+    plan = plan or oa.extend_plan([3, 2], 4, 2, 100, chunk=128, device="cpu").plan
+    a = dict(plan=ctypes.byref(plan), q=P, stride=512, kv=P, scale=P, fmt=0, pos=P, indptr=P, pages=P, page=16, out=P, s=0.1, work=P, ws=None)
+    a.update(k)
+    return oa.load().omni_qwen3_extend_q8(*a.values(), None)
+
+
+def cross(plan=None, **k):
+    plan = plan or oa.cross_plan([3, 2], 4, 2, 100, chunk=128, device="cpu").plan
+    a = dict(plan=ctypes.byref(plan), q=P, stride=512, k=P, ks=256, v=P, vs=256, of=P, first=P, len=P, out=P, s=0.1, work=P, ws=None)
+    a.update(k)
+    return oa.load().omni_attn_cross_run(*a.values(), None)
+
+
+BAD = [dict(q=None), dict(out=None), dict(work=None), dict(q=P + 8), dict(out=P + 8), dict(work=P + 4), dict(stride=504), dict(stride=516),
+       dict(s=float("nan")), dict(s=3e38), dict(ws=P + 8), dict(plan=None)]
+
+
+@pytest.mark.parametrize("bad", BAD + [
+    dict(fmt=2), dict(fmt=-1), dict(kv=None), dict(scale=None), dict(pos=None), dict(indptr=None), dict(pages=None), dict(kv=P + 8), dict(page=0)])
+def test_extend_refusals(bad):
+    assert extend(**bad) == oa.EINVAL
+    assert b"extend" in oa.load().omni_attn_last_error()
+
+
+@pytest.mark.parametrize("bad", BAD + [
+    dict(k=None), dict(v=None), dict(first=None), dict(len=None), dict(k=P + 8), dict(v=P + 2), dict(ks=248), dict(vs=260), dict(ks=(1 << 22) + 8)])
+def test_cross_refusals(bad):
+    assert cross(**bad) == oa.EINVAL
+    assert b"cross" in oa.load().omni_attn_last_error()
+
+
+def test_other_codes():
+    assert extend(page=24) == oa.EUNSUPPORTED
+    split = oa.extend_plan([3, 2], 4, 2, 100, chunk=64, device="cpu").plan
+    assert extend(split) == oa.EWORKSPACE
+    split = oa.cross_plan([3, 2], 4, 2, 100, chunk=64, device="cpu").plan
+    assert cross(split) == oa.EWORKSPACE
+    none = oa.cross_plan([0], 4, 2, 100, device="cpu").plan
+    assert cross(none, q=None, k=None, out=None, work=None) == oa.OK
+    none = oa.extend_plan([0], 4, 2, 100, device="cpu").plan
+    assert extend(none, q=None, kv=None, out=None, work=None) == oa.OK
+    # Each call takes its own plans.
+    assert extend(oa.cross_plan([3], 4, 2, 100, device="cpu").plan) == oa.EINVAL
+    assert cross(oa.extend_plan([3], 4, 2, 100, device="cpu").plan) == oa.EINVAL
+
+
+@pytest.mark.parametrize("field,value", [
+    ("rows", -1), ("hq", 5), ("hq", 0), ("hk", 0), ("hq", 64), ("max_len", 0), ("max_len", 300), ("group_rows", -1), ("group_rows", 6), ("chunk", 0),
+    ("chunk", 65), ("splits", 2), ("splits", 0), ("tiles", -1), ("tiles", 1), ("tile_chunk", 0), ("tile_chunk", 64), ("tile_splits", 3), ("work_bytes", 0),
+    ("workspace_bytes", 16)])
+def test_plans_that_do_not_agree(field, value):
+    for make, call in ((oa.extend_plan, extend), (oa.cross_plan, cross)):
+        plan = make([3, 2], 4, 2, 100, chunk=128, device="cpu").plan
+        setattr(plan, field, value)
+        assert call(plan) == oa.EINVAL, field
+    for at in (0, 1):
+        plan = oa.cross_plan([3, 2], 4, 2, 100, chunk=128, device="cpu").plan
+        plan.groups[at] += 1
+        assert cross(plan) == oa.EINVAL
+        plan.groups[at] = -1
+        assert cross(plan) == oa.EINVAL
+
+
+def test_the_mirror_refuses_host_tensors_and_other_shapes():
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    z = torch.zeros(8, dtype=torch.int32)
+    kv, sc = oa.q8_cache(4, 16, 2, device="cpu")
+    e, x = oa.extend_plan([3], 4, 2, 50, device="cpu"), oa.cross_plan([3], 4, 2, 50, device="cpu")
+    for call in (lambda: oa.qwen3_extend_q8(e, b(3, 512), kv, sc, z, z, z, 16, b(3, 512), 0.1),
+                 lambda: oa.cross_run(x, b(3, 512), b(9, 256), b(9, 256), z, z, z, b(3, 512), 0.1)):
+        with pytest.raises(oa.OmniAttnError) as err:
+            call()
+        assert err.value.code == oa.EINVAL
+
+
+def test_launches_that_no_grid_holds():
+    for make in PLANS:
+        with pytest.raises(oa.OmniAttnError) as e:
+            make([1] * 3000, 128, 128, 64 * 100000, None, 64, device="cpu")
+        assert e.value.code == oa.EUNSUPPORTED
