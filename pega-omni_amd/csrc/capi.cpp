@@ -1091,15 +1091,32 @@ constexpr int64_t kPartialBytes = (OMNI_ATTN_HEAD_DIM + 1) * (int64_t)sizeof(flo
 // Rows of one sequence that a group of `cols` packed columns takes.
 int rows_of_group(int cols, int G) { return cols / G; }
 
-int64_t multi_workspace(const omni_attn_multi_plan& p) {
+int64_t align16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// The workspace: partials of the groups, splits that each took; then those of the tiles.
+int64_t groups_workspace(const omni_attn_multi_plan& p) {
   if (p.splits <= 1) return 0;
-  return (int64_t)p.group_rows * p.hq * p.splits * kPartialBytes + 4 * ((int64_t)p.groups[0] + p.groups[1]);
+  return align16((int64_t)p.group_rows * p.hq * p.splits * kPartialBytes + 4 * ((int64_t)p.groups[0] + p.groups[1]));
 }
 
-int64_t multi_work_ints(const omni_attn_multi_plan& p) { return 4 * ((int64_t)p.groups[0] + p.groups[1]); }
+int64_t tiles_workspace(const omni_attn_multi_plan& p) {
+  if (p.tile_splits <= 1) return 0;
+  const int64_t items = (int64_t)p.tiles * p.hk;
+  return align16(items * p.tile_splits * omni::kSegmentBytes + 4 * items);
+}
 
-// What a launch of the plan's groups holds.
-bool groups_fit(const omni_attn_multi_plan& p) {
+// The work list: the tiles' (of the form that the prefill's has), then the groups'.
+int64_t tiles_work_ints(const omni_attn_multi_plan& p) {
+  return p.tiles > 0 ? omni::kPrefillWorkHeader + 4 * (int64_t)p.tiles * p.hk : 0;
+}
+int64_t multi_work_ints(const omni_attn_multi_plan& p) { return tiles_work_ints(p) + 4 * ((int64_t)p.groups[0] + p.groups[1]); }
+
+// What the launches of a plan hold.
+bool multi_fits(const omni_attn_multi_plan& p) {
+  const int64_t items = (int64_t)p.tiles * p.hk;
+  if (!omni::grid_holds(items + omni::kXcds, omni::kTiledThreads, p.tile_splits) ||
+      (p.tile_splits > 1 && !omni::grid_holds(items, 256)))
+    return false;
   for (int c = 0; c < 2; ++c) {
     const int64_t rows = std::max(rows_of_group(16 * (c + 1), p.hq / p.hk), 1);
     if (!omni::grid_holds((int64_t)p.groups[c] * p.hk * p.splits, omni::kRowsThreads) ||
@@ -1108,6 +1125,15 @@ bool groups_fit(const omni_attn_multi_plan& p) {
       return false;
   }
   return true;
+}
+
+// Keys per split of the tiles: as many splits as fill the GPU's CUs once, each of four
+// key tiles at least (a partial is written and merged for every one).
+int pick_tile_chunk(int64_t items, int max_len) {
+  const int64_t steps = ((int64_t)max_len + 127) / 128;
+  int64_t splits = items > 0 ? std::min<int64_t>(256 / items, steps / 4) : 1;
+  if (splits < 2) splits = 1;
+  return (int)std::min<int64_t>((steps + splits - 1) / splits * 128, INT_MAX / 128 * 128);
 }
 
 int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
@@ -1134,11 +1160,23 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   plan->hk = hk;
   plan->max_len = max_len;
 
-  // Groups: (sequence, first row, rows, keys), of at most 16 packed rows where the rest of a sequence fits, else 32.
-  std::vector<std::array<int32_t, 4>> groups[2];
+  // Tiles: (sequence, first row, rows, keys that the last row sees), of sequences of more
+  // than 32 packed rows. Groups: the same, of at most 16 packed rows where what is left
+  // of a sequence fits, else 32.
+  std::vector<std::array<int32_t, 4>> groups[2], tl;
   const int small = rows_of_group(16, G), large = rows_of_group(32, G);
+  const bool tiled = G == 1 || G == 2 || G == 4 || G == 8;
+  const int per_tile = omni::kTiledRows / G;
   double keys = 0;
-  for (int32_t s = 0, at = 0; s < nseq; at += counts_h[s++])
+  for (int32_t s = 0, at = 0; s < nseq; at += counts_h[s++]) {
+    if (tiled && counts_h[s] > large) {
+      for (int32_t f = 0; f < counts_h[s]; f += per_tile) {
+        const int32_t n = std::min(per_tile, counts_h[s] - f);
+        tl.push_back({s, at + f, n, !keys_h ? (cross ? 0 : f + n) : cross ? keys_h[s] : std::max(keys_h[s] - (counts_h[s] - f - n), 0)});
+      }
+      if (tl.size() > (size_t)INT_MAX / 8) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many tiles", who);
+      continue;
+    }
     for (int32_t f = 0; f < counts_h[s];) {
       const int32_t left = counts_h[s] - f, n = std::min(left, left <= small ? small : large);
       groups[n > small].push_back({s, at + f, n, keys_h ? keys_h[s] : 0});
@@ -1146,6 +1184,7 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
       f += n;
       plan->group_rows += n;
     }
+  }
   for (int c = 0; c < 2; ++c) {
     if (groups[c].size() > (size_t)INT_MAX) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many groups", who);
     plan->groups[c] = (int32_t)groups[c].size();
@@ -1154,14 +1193,17 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   const double n = (double)groups[0].size() + (double)groups[1].size();
   plan->chunk = chunk_hint > 0 ? chunk_hint : pick_chunk_keys(n * hk, max_len, n > 0 ? keys / n : 1, cross ? 512 : 256);
   plan->splits = (int32_t)(((int64_t)max_len + plan->chunk - 1) / plan->chunk);
-  plan->tile_chunk = (int32_t)std::min<int64_t>(((int64_t)max_len + 127) / 128 * 128, INT_MAX / 128 * 128);
+  plan->tiles = (int32_t)tl.size();
+  plan->tile_chunk = pick_tile_chunk((int64_t)tl.size() * hk, max_len);
   plan->tile_splits = (int32_t)(((int64_t)max_len + plan->tile_chunk - 1) / plan->tile_chunk);
-  if (!groups_fit(*plan)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, plan->rows, hq, plan->splits);
-  plan->workspace_bytes = multi_workspace(*plan);
+  if (!multi_fits(*plan)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, plan->rows, hq, plan->splits);
+  plan->workspace_bytes = groups_workspace(*plan) + tiles_workspace(*plan);
   const int64_t need = multi_work_ints(*plan);
   plan->work_bytes = need * (int64_t)sizeof(int32_t);
   if (need > 0 && (!work_h || need > work_cap))
     return fail(OMNI_ATTN_EWORKSPACE, "%s: work list needs %lld int32", who, (long long)need);
+  if (!tl.empty()) write_work_list(tl, hk, work_h);
+  work_h += tiles_work_ints(*plan);
   int32_t at = 0;
   for (auto& list : groups)
     for (const auto& g : list) {
@@ -1182,10 +1224,12 @@ int multi_checks(const omni_attn_multi_plan* plan, int cross, const void* q, int
       p.groups[1] < 0 || p.group_rows < 0 || p.group_rows > p.rows || p.chunk <= 0 || p.chunk % 64 != 0 ||
       p.splits != ((int64_t)p.max_len + p.chunk - 1) / p.chunk || p.tiles < 0 || p.tile_chunk <= 0 || p.tile_chunk % 128 != 0 ||
       p.tile_splits != ((int64_t)p.max_len + p.tile_chunk - 1) / p.tile_chunk ||
-      p.work_bytes != multi_work_ints(p) * (int64_t)sizeof(int32_t) || p.workspace_bytes != multi_workspace(p))
+      (p.tiles > 0 && (32 % (p.hq / p.hk) != 0 || p.hq / p.hk > 8)) ||
+      p.work_bytes != multi_work_ints(p) * (int64_t)sizeof(int32_t) ||
+      p.workspace_bytes != groups_workspace(p) + tiles_workspace(p))
     return fail(OMNI_ATTN_EINVAL, "%s: plan is not one its plan_init made (rows=%d hq=%d hk=%d max_len=%d groups=%d,%d chunk=%d splits=%d)",
                 who, p.rows, p.hq, p.hk, p.max_len, p.groups[0], p.groups[1], p.chunk, p.splits);
-  if (!groups_fit(p)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, p.rows, p.hq, p.splits);
+  if (!multi_fits(p)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, p.rows, p.hq, p.splits);
   if (!std::isfinite(scale * kLog2e)) return fail(OMNI_ATTN_EINVAL, "%s: scale * log2(e) is not finite", who);
   if (p.rows == 0) return 0;
   if (!q || !out || !work) return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
@@ -1201,10 +1245,45 @@ int multi_checks(const omni_attn_multi_plan* plan, int cross, const void* q, int
 
 int multi_launch(omni::RowsArgs& a, const omni_attn_multi_plan& p, int source, const void* q, int64_t q_stride, void* out,
                  float scale, const int32_t* work, void* workspace, void* stream, const char* who) {
+  if (p.tiles > 0) {
+    omni::TiledArgs t{};
+    t.q = static_cast<const omni::bf16_t*>(q);
+    t.q_stride = q_stride;
+    t.kv8 = a.kv;
+    t.kv_scale = a.kv_scale;
+    t.pos = a.pos;
+    t.indptr = a.indptr;
+    t.pages = a.pages;
+    t.pd = a.pd;
+    t.k = a.k;
+    t.v = a.v;
+    t.k_stride = a.k_stride;
+    t.v_stride = a.v_stride;
+    t.of = a.of;
+    t.first = a.first;
+    t.len = a.len;
+    t.work = work;
+    t.out = static_cast<omni::bf16_t*>(out);
+    t.hq = p.hq;
+    t.hk = p.hk;
+    t.scale_log2 = scale * kLog2e;
+    const int64_t items = (int64_t)p.tiles * p.hk;
+    const int resident = resident_tiled_groups();
+    t.quarters = omni::tiled_quarters(items, resident);
+    t.halved = omni::prefill_halves(items, resident);
+    t.split_k = p.tile_splits;
+    t.split_tiles = p.tile_chunk / 128;
+    if (p.tile_splits > 1) {
+      t.ws = reinterpret_cast<float*>(static_cast<char*>(workspace) + groups_workspace(p));
+      t.used = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(t.ws) + items * p.tile_splits * omni::kSegmentBytes);
+    }
+    if (omni::launch_multi_tiles(t, source, (int)items, as_stream(stream)) != 0)
+      return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));
+  }
   a.q = static_cast<const omni::bf16_t*>(q);
   a.q_stride = q_stride;
   a.out = static_cast<omni::bf16_t*>(out);
-  a.items = work;
+  a.items = work + tiles_work_ints(p);
   a.ws_o = static_cast<float*>(workspace);
   const int64_t partials = (int64_t)p.group_rows * p.hq * p.splits;
   a.ws_lse = a.ws_o ? a.ws_o + partials * OMNI_ATTN_HEAD_DIM : nullptr;

@@ -112,8 +112,17 @@ struct TiledArgs {
   int quarters;
   // Prefill with P carried as two bf16 terms (hi + lo) through P.V.
   int exact_p;
-  // packed prompts (mode 2): elements between rows of k and of v
+  // packed prompts (mode 2), cross attention: elements between rows of k and of v
   int64_t k_stride, v_stride;
+  // Several rows per sequence: split_k splits of split_tiles key tiles each, partials
+  // to ws (a segment per item and split), the splits that an item used to `used`.
+  const uint8_t* kv8;       // the 8-bit cache (pd: blocks per page)
+  const uint8_t* kv_scale;
+  const int32_t* of;        // cross: the source of each sequence (null: the sequence)
+  const int32_t* first;     // and its first row and rows
+  const int32_t* len;
+  int split_tiles;
+  int32_t* used;
 };
 
 // Packed (position, head) query rows per MFMA tile: one 8-wave workgroup, one per CU.
@@ -131,6 +140,8 @@ int launch_prefill(const TiledArgs& a, int items, hipStream_t stream);
 // Packed prompts: items are (sequence's first row, first row, rows, kv head).
 constexpr int64_t kMostPromptStride = 1LL << 22;  // elements: 128 rows stay below 2^30 bytes
 int launch_prompt(const TiledArgs& a, int items, hipStream_t stream);
+// Several rows per sequence over a source of launch_rows: items are (sequence, first row, rows, kv head).
+int launch_multi_tiles(const TiledArgs& a, int source, int items, hipStream_t stream);
 
 // Rotary embedding + K/V scatter (the step before attention).
 struct RopeArgs {

@@ -27,10 +27,10 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "q8_bytes.h"
 
 namespace omni {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kBM = kTiledRows;  // packed query rows per workgroup
@@ -162,11 +162,36 @@ static_assert(kDmas == 8, "one DMA per K-step of the S stage");
 // bf16 as in the other sources (error 0.0020 against 64 bits, 0.0016 of it the bf16
 // output's); EXACT carries it in two terms.
 constexpr int kDense = 0, kPagedWave = 1, kPagedLane = 2, kPacked = 3;
+// And for calls of several rows per sequence: cross attention, every row seeing all
+// rows of its sequence's source; and the 8-bit block cache, rows at any positions.
+// A tile is 8 blocks of that, one a wave: its bytes go to registers a tile ahead,
+// and after the softmax, as bf16 that the block's exponent has been put into (exact
+// but at the ends of bf16's range), to LDS: K as in the other sources, V, which lies
+// [dim][token], as the operand that P.V takes: [block][half h][dim][8 tokens], tokens
+// 4 h + {0..3, 8..11}. Rows without keys store zeros; P is at most 1.
+constexpr int kCross = 4, kCacheE4m3 = 5, kCacheInt8 = 6;
+
+// Four stored bytes times 2^(e - 127), as bf16: once rounded.
+template <int SRC>
+__device__ __forceinline__ uint2 scaled_bf16(uint32_t w, float scale) {
+  if constexpr (SRC == kCacheE4m3) {
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, scale, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, scale, true)));
+  } else {
+    float v[4];
+    from_bytes<kQ8Int8>(w, v);
+    return make_uint2(pack_bf16x2(v[0] * scale, v[1] * scale), pack_bf16x2(v[2] * scale, v[3] * scale));
+  }
+}
 
 template <int G, int SRC, int FORM = kWhole, bool EXACT = false>
 __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items, int ntiles) {
   constexpr bool LISTED = SRC != kDense;  // items come from a work list
   constexpr bool PAGED = SRC == kPagedWave || SRC == kPagedLane;
+  constexpr bool Q8 = SRC == kCacheE4m3 || SRC == kCacheInt8;
+  constexpr bool MULTI = Q8 || SRC == kCross;
+  constexpr bool ROWS = SRC == kPacked || SRC == kCross;  // rows of k and v at strides of their own
+  constexpr float kAbove = MULTI ? 8.f : 0.f;             // how far the base stands above the maximum that moved it
   constexpr int PARTS = FORM == kQuarters ? 4 : FORM == kHalves ? 2 : 1;
   // DiT, XCD-aware order: workgroup id i runs on XCD i % 8; give each XCD a
   // contiguous block of work items so the tiles sharing one K/V head (and
@@ -263,6 +288,29 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     t.kbase = a.kv + (int64_t)kvh * kHead;
     t.vbase = a.kv + (int64_t)(a.hk + kvh) * kHead;
     t.qpos0 = 0;
+  } else if constexpr (MULTI) {
+    const int first = item.y;
+    t.nq = item.z;
+    if (no_rows(t.nq)) return;
+    t.q = a.q + (int64_t)first * a.q_stride;
+    t.out = a.out + (int64_t)first * a.hq * kHead;
+    t.qpos0 = 0;
+    if constexpr (SRC == kCross) {
+      const int e = a.of ? a.of[item.x] : item.x;
+      const int64_t begin = a.first[e];
+      t.last = max(a.len[e], 0);
+      t.kbase = a.k + begin * a.k_stride + (int64_t)kvh * kHead;
+      t.vbase = a.v + begin * a.v_stride + (int64_t)kvh * kHead;
+    } else {
+      t.pos = a.pos + first;
+      t.pg = a.pages + a.indptr[item.x];
+      int most = -1;  // of this workgroup's rows
+      for (int i = (part > 0 ? kPartPos * part : 0) + (threadIdx.x & 63); i < ends(t.nq); i += 64) most = max(most, t.pos[i]);
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d));
+      t.last = __builtin_amdgcn_readfirstlane(most) + 1;
+    }
+    t.len = t.last;
   } else if constexpr (SRC == kPacked) {
     const int begin = item.x, first = item.y;
     t.nq = item.z;
@@ -294,9 +342,22 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   __shared__ __align__(16) bf16_t smem1[kBufElems];
 
   // Key tiles [s_lo, s_hi): all of them, or this chunk's share.
-  const int steps = (t.last + kBN - 1) / kBN;
-  const int s_lo = chunk < 0 ? 0 : chunk * steps / a.split_k;
-  const int s_hi = chunk < 0 ? steps : (chunk + 1) * steps / a.split_k;
+  const int steps = MULTI ? (int)(((int64_t)t.last + kBN - 1) / kBN) : (t.last + kBN - 1) / kBN;
+  int s_lo = chunk < 0 ? 0 : chunk * steps / a.split_k;
+  int s_hi = chunk < 0 ? steps : (chunk + 1) * steps / a.split_k;
+  bool split = false;  // several rows per sequence: whether the item's keys are split
+  if constexpr (MULTI) {
+    // Splits of whole key tiles: the plan's, or more where the rows pass its bound.
+    if (a.split_k > 1) {
+      const int per = max(a.split_tiles, (steps + a.split_k - 1) / a.split_k), used = steps > 0 ? (steps - 1) / per + 1 : 0;
+      chunk = blockIdx.y;
+      if (chunk == 0 && part <= 0 && threadIdx.x == 0) a.used[idx] = used;
+      if (chunk > 0 && chunk >= used) return;
+      s_lo = chunk * per;
+      s_hi = min(steps, s_lo + per);
+      split = used > 1;
+    }
+  }
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int j = lane & 31, h = lane >> 5;
@@ -316,6 +377,10 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   int lim;  // keys this row sees
   if constexpr (PAGED)
     lim = row_ok ? t.pos[p] + 1 : 0;
+  else if constexpr (Q8)
+    lim = row_ok ? max(t.pos[p], -1) + 1 : 0;
+  else if constexpr (SRC == kCross)
+    lim = row_ok ? t.len : 0;
   else if constexpr (SRC == kPacked)
     lim = row_ok ? t.qpos0 + p + 1 : 0;
   else
@@ -352,8 +417,8 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   // block (dense: from the tile's first key): constants for every tile.
   uint32_t koff[kRowsPerWave / 4], voff[kRowsPerWave / 4];
   {
-    const int64_t stride = PAGED ? t.per_slot : SRC == kPacked ? a.k_stride : t.kv_stride;
-    const int64_t vstride = SRC == kPacked ? a.v_stride : stride;
+    const int64_t stride = PAGED ? t.per_slot : ROWS ? a.k_stride : Q8 ? 0 : t.kv_stride;
+    const int64_t vstride = ROWS ? a.v_stride : stride;
 #pragma unroll
     for (int i = 0; i < kRowsPerWave / 4; ++i) {
       const int wrow = 4 * i + (lane >> 4);  // row within the wave's block
@@ -387,7 +452,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     const int first = PAGED ? n0 + kRowsPerWave * wave_u : n0;  // key of this lane's row 0
     const int rows = st < s_hi ? min(max(t.last - first, 0), PAGED ? kRowsPerWave : kBN) : 0;
     const bool whole = rows == (PAGED ? kRowsPerWave : kBN);
-    if constexpr (SRC == kPacked) {
+    if constexpr (ROWS) {
       k_rsrc = buffer_rsrc(t.kbase + n0 * a.k_stride, whole ? -1 : (int)(rows * 2 * a.k_stride));
       v_rsrc = buffer_rsrc(t.vbase + n0 * a.v_stride, whole ? -1 : (int)(rows * 2 * a.v_stride));
       return;
@@ -414,9 +479,59 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     else
       dma_buffer16(v_rsrc, 2 * voff[i], at + kTileElems);
   };
+  // 8-bit cache: block wave_u of tile st. Lane l holds the block and its exponents for
+  // tile 64 b + l of the call's range (blocks past the last key: its own).
+  int block_ids = 0, block_exps = 0;
+  uint4 raw[4];
+  float k_by = 0.f, v_by = 0.f;  // scales of the block in `raw`
+  int raw_left = 0;              // tokens from its first to the last that any row sees
+  auto look_up = [&](int st) __attribute__((always_inline)) {
+    const int b = (int)min((int64_t)(st + lane) * (kBN / kQ8Block) + wave_u, (int64_t)((t.last - 1) / kQ8Block));
+    block_ids = (int)page_slot(a.pd, t.pg[page_index(a.pd, b)], b);
+    const uint8_t* e = a.kv_scale + (int64_t)block_ids * 2 * a.hk + kvh;
+    block_exps = e[0] | e[a.hk] << 16;
+  };
+  auto ask_block = [&](int st) __attribute__((always_inline)) {
+    const int at = st - s_lo;
+    if ((at & 63) == 0) look_up(st);
+    const int64_t block = __builtin_amdgcn_readlane(block_ids, at & 63);
+    const int exps = __builtin_amdgcn_readlane(block_exps, at & 63);
+    const uint8_t* kb = a.kv8 + (block * 2 * a.hk + kvh) * kQ8HeadBytes + 16 * lane;
+    const uint8_t* vb = kb + (int64_t)a.hk * kQ8HeadBytes;
+    raw[0] = ldg16(kb), raw[1] = ldg16(kb + 1024), raw[2] = ldg16(vb), raw[3] = ldg16(vb + 1024);
+    k_by = pow2_biased(exps & 0xff), v_by = pow2_biased(exps >> 16);
+    raw_left = (int)min((int64_t)t.last - (int64_t)st * kBN - kQ8Block * wave_u, (int64_t)kQ8Block);
+  };
+  auto put_block = [&](bf16_t* kd) __attribute__((always_inline)) {
+    if (raw_left < kQ8Block) {  // V of tokens that no row sees weighs 0, whatever it holds
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int n_ok = min(max(raw_left - 4 * w, 0), 4);
+        const uint32_t stay = n_ok == 4 ? ~0u : (1u << (8 * n_ok)) - 1;
+        (&raw[2].x)[w] &= stay, (&raw[3].x)[w] &= stay;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // K: 16 dims of token 8 i + l / 8; V: 16 tokens of dim 64 i + l.
+      const int row = kRowsPerWave * wave_u + 8 * i + (lane >> 3), c = 2 * (lane & 7);
+      const uint2 k0 = scaled_bf16<SRC>(raw[i].x, k_by), k1 = scaled_bf16<SRC>(raw[i].y, k_by);
+      const uint2 k2 = scaled_bf16<SRC>(raw[i].z, k_by), k3 = scaled_bf16<SRC>(raw[i].w, k_by);
+      *reinterpret_cast<uint4*>(kd + row * kHead + 8 * (c ^ (row & 15))) = make_uint4(k0.x, k0.y, k1.x, k1.y);
+      *reinterpret_cast<uint4*>(kd + row * kHead + 8 * ((c + 1) ^ (row & 15))) = make_uint4(k2.x, k2.y, k3.x, k3.y);
+      const uint2 v0 = scaled_bf16<SRC>(raw[2 + i].x, v_by), v1 = scaled_bf16<SRC>(raw[2 + i].y, v_by);
+      const uint2 v2 = scaled_bf16<SRC>(raw[2 + i].z, v_by), v3 = scaled_bf16<SRC>(raw[2 + i].w, v_by);
+      bf16_t* vd = kd + kTileElems + wave_u * (kQ8Block * kHead) + 8 * (64 * i + lane);
+      *reinterpret_cast<uint4*>(vd) = make_uint4(v0.x, v0.y, v2.x, v2.y);
+      *reinterpret_cast<uint4*>(vd + 8 * kHead) = make_uint4(v1.x, v1.y, v3.x, v3.y);
+    }
+  };
   // The whole tile st into buffer kd.
   auto issue_tile = [&](int st, bf16_t* kd) __attribute__((always_inline)) {
-    if constexpr (SRC != kPagedLane) {
+    if constexpr (Q8) {
+      ask_block(st);
+      put_block(kd);
+    } else if constexpr (SRC != kPagedLane) {
       aim_tile(st);
 #pragma unroll
       for (int d = 0; d < kDmas; ++d) dma_tile(d, kd);
@@ -464,6 +579,17 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   const int k_lane = j * kHead + 8 * (h ^ (j & 15));
   const int vg = lane >> 4, vi = lane & 15;
   const int v_lane = (4 * (vg >> 1) + (vi >> 2)) * kHead + 32 * (vi >> 2) + 16 * (vg & 1) + 4 * (vi & 3);
+  // V's operand of K-step ks and dims 32 md .. + 31.
+  auto v_operand = [&](const bf16_t* vt, int ks, int md) __attribute__((always_inline)) {
+    if constexpr (Q8) {
+      return as_bf16x8(*reinterpret_cast<const uint4*>(vt + ks * (kQ8Block * kHead) + h * (8 * kHead) + 8 * (32 * md + j)));
+    } else {
+      const bf16_t* vb = vt + (v_lane ^ (32 * md)) + 16 * ks * kHead;
+      const bf16x4 lo = lds_read_tr(vb);
+      const bf16x4 hi = lds_read_tr(vb + 8 * kHead);
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
 
   // The first tile. Q (and the page ids) were asked for above and are waited
   // for with it, so the key loop's first MFMA does not wait on the next
@@ -487,7 +613,9 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   // the eight waves' 64 KiB kept the address unit busy and every wave waiting
   // to issue for 0.45-0.75 us of a 3.1 us step, with the matrix cores idle.
   auto tile_step = [&](int st, const bf16_t* cur, bf16_t* nxt) __attribute__((always_inline)) {
-    if constexpr (SRC != kPagedLane)
+    if constexpr (Q8) {
+      if (st + 1 < s_hi) ask_block(st + 1);
+    } else if constexpr (SRC != kPagedLane)
       aim_tile(st + 1);
     else if (st + 1 < s_hi)
       issue_tile(st + 1, nxt);
@@ -516,7 +644,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
 #pragma unroll
       for (int mb = 0; mb < kMB; ++mb)
         sc[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(kf[kk][mb]), qf[kk], sc[mb], 0, 0, 0);
-      if constexpr (SRC != kPagedLane) dma_tile(kk, nxt);
+      if constexpr (SRC != kPagedLane && !Q8) dma_tile(kk, nxt);
       if (kk + 2 < 8) read_k(kk + 2);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -541,7 +669,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     // The running base m moves only when the max grows by more than 8 (log2):
     // p = 2^(s - m) <= 2^8 stays exact in f32 and l, O share the same base,
     // so the result is unchanged while most tiles skip rescaling O.
-    const float mt = mx * sl2;
+    const float mt = mx * sl2 + kAbove;
     const bool grow = mt > m + 8.f;
     if (__any(grow)) {
       const float alpha = grow ? fast_exp2(m - mt) : 1.f;
@@ -553,6 +681,8 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
         for (int e = 0; e < 16; ++e) o[md][e] *= alpha;
     }
     const float base = m == -INFINITY ? 0.f : m;
+    if constexpr (Q8)
+      if (st + 1 < s_hi) put_block(nxt);
     // O^T += V^T . P^T: K-step ks covers keys 16 ks + 4 h + {0..3, 8..11}. The
     // V operands of the next K-step are read, and its exponentials taken, beside
     // this one's MFMAs (against all exponentials first: exact P 240 -> 229 us on
@@ -585,12 +715,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     bf16x8 vf[2][4];
     auto read_v = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-      for (int md = 0; md < 4; ++md) {
-        const bf16_t* vb = vt + (v_lane ^ (32 * md)) + 16 * ks * kHead;
-        const bf16x4 lo = lds_read_tr(vb);
-        const bf16x4 hi = lds_read_tr(vb + 8 * kHead);
-        vf[ks & 1][md] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
+      for (int md = 0; md < 4; ++md) vf[ks & 1][md] = v_operand(vt, ks, md);
     };
     read_v(0);
 #pragma unroll
@@ -643,10 +768,18 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       return sum;
     };
     auto quarter_step = [&](int st, bf16_t* cur, bf16_t* nxt) __attribute__((always_inline)) {
-      aim_tile(st + 1);
+      if constexpr (Q8) {
+        if (st + 1 < s_hi) ask_block(st + 1);
+      } else {
+        aim_tile(st + 1);
+      }
       if (!active) {
+        if constexpr (Q8) {
+          if (st + 1 < s_hi) put_block(nxt);
+        } else {
 #pragma unroll
-        for (int d = 0; d < kDmas; ++d) dma_tile(d, nxt);
+          for (int d = 0; d < kDmas; ++d) dma_tile(d, nxt);
+        }
         __syncthreads();
         __syncthreads();
         __builtin_amdgcn_s_waitcnt(0x0F70);
@@ -667,17 +800,12 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       // V's operands too, a K-step beside each MFMA of S (after the exchange of
       // maxima they would stand before it in the LDS queue).
       bf16x8 vf[kSteps];
-      auto read_v = [&](int ks) __attribute__((always_inline)) {
-        const bf16_t* vb = vt + (v_lane ^ (32 * kg)) + 16 * ks * kHead;
-        const bf16x4 lo = lds_read_tr(vb);
-        const bf16x4 hi = lds_read_tr(vb + 8 * kHead);
-        vf[ks] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      };
+      auto read_v = [&](int ks) __attribute__((always_inline)) { vf[ks] = v_operand(vt, ks, kg); };
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
         sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(kf[kk]), qf[kk], sc, 0, 0, 0);
-        dma_tile(kk, nxt);
+        if constexpr (!Q8) dma_tile(kk, nxt);
         read_v(kk);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -698,7 +826,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       __syncthreads();  // every score is taken: the maxima are there and K is free
       if (later && kg == 3) l += chain(s_sum[blk][2][lane]);  // before this tile's base moves
       mx = fmaxf(fmaxf(s_max[blk][0][j], s_max[blk][1][j]), fmaxf(s_max[blk][2][j], s_max[blk][3][j]));
-      const float mt = mx * sl2;
+      const float mt = mx * sl2 + kAbove;
       const bool grow = mt > m + 8.f;
       if (__any(grow)) {
         const float alpha = grow ? fast_exp2(m - mt) : 1.f;
@@ -727,6 +855,8 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
         }
       }
       if (kg == 0) s_sum[blk][0][lane] = chain(0.f);
+      if constexpr (Q8)
+        if (st + 1 < s_hi) put_block(nxt);
       __syncthreads();  // P is there
       if (kg == 1) s_sum[blk][1][lane] = chain(s_sum[blk][0][lane]);
       uint4 pf[kSteps], pfl[EXACT ? kSteps : 1];
@@ -766,6 +896,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
         uint2 w;
         w.x = pack_bf16x2(ov[4 * q4 + 0] * inv, ov[4 * q4 + 1] * inv);
         w.y = pack_bf16x2(ov[4 * q4 + 2] * inv, ov[4 * q4 + 3] * inv);
+        if (MULTI && lim == 0) w = make_uint2(0, 0);
         *reinterpret_cast<uint2*>(rows + j * kHead + 8 * ((4 * kg + q4) ^ (j & 15)) + 4 * h) = w;
       }
     }
@@ -796,9 +927,9 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
 
   // Register e of block md is dim 32 md + 8 (e / 4) + 4 h + e % 4.
   l += xor_lane(l, 32);
-  if (chunk >= 0) {  // a chunk's partial: unnormalised O with its base m and sum l, for dit_combine
-    if (!row_ok) return;  // dit_combine reads the tile's positions only
-    float* seg = a.ws + (int64_t)((idx - a.split_from) * a.split_k + chunk) * (kBM * (kHead + 2));
+  if (MULTI ? split : chunk >= 0) {  // a chunk's partial: unnormalised O with its base m and sum l, for the combine
+    if (!row_ok) return;  // which reads the tile's positions only
+    float* seg = a.ws + ((int64_t)(MULTI ? idx : idx - a.split_from) * a.split_k + chunk) * (kBM * (kHead + 2));
 #pragma unroll
     for (int md = 0; md < 4; ++md)
 #pragma unroll
@@ -827,6 +958,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       uint2 w;
       w.x = pack_bf16x2(o[md][4 * q4 + 0] * inv, o[md][4 * q4 + 1] * inv);
       w.y = pack_bf16x2(o[md][4 * q4 + 2] * inv, o[md][4 * q4 + 3] * inv);
+      if (MULTI && lim == 0) w = make_uint2(0, 0);
       *reinterpret_cast<uint2*>(rows + jn * kHead + 8 * ((4 * md + q4) ^ (jn & 15)) + 4 * hn) = w;
     }
   // Lanes read what other lanes of the wave wrote: LDS keeps a wave's accesses in
@@ -853,23 +985,15 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
 constexpr int kCombineRows = 16;
 constexpr int kCombineBatch = 8;
 
-__global__ __launch_bounds__(256) void dit_combine(TiledArgs a, int ntiles) {
-  const int idx = a.split_from + blockIdx.x;
-  const int G = a.hq / a.hk, kpos = kBM / G;
-  const int tile = idx % ntiles, kvh = (idx / ntiles) % a.hk, b = idx / (ntiles * a.hk);
-  const int q0 = tile * kpos, nq = min(kpos, a.q_len - q0);
-  const int r = blockIdx.y * kCombineRows + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
-  const int p = r / G, head = kvh * G + r % G;
-  if (p >= nq) return;
+// Packed row r of a segment list: nk chunks' partials, merged, to 8 values of `out`.
+__device__ __forceinline__ void combine_row(const float* seg0, int nk, int r, int d0, bf16_t* out) {
   constexpr int kSeg = kBM * (kHead + 2);
-  const int nk = a.split_k;
-  const float* seg0 = a.ws + (int64_t)(blockIdx.x * nk) * kSeg;
   const float* ml0 = seg0 + kBM * kHead + 2 * r;  // chunk c's (m, l) at ml0 + c * kSeg
   float top = -INFINITY;
   for (int c0 = 0; c0 < nk; c0 += kCombineBatch) {
     float m[kCombineBatch];
 #pragma unroll
-    for (int i = 0; i < kCombineBatch; ++i) m[i] = ml0[min(c0 + i, nk - 1) * kSeg];
+    for (int i = 0; i < kCombineBatch; ++i) m[i] = ml0[(int64_t)min(c0 + i, nk - 1) * kSeg];
 #pragma unroll
     for (int i = 0; i < kCombineBatch; ++i) top = fmaxf(top, m[i]);  // a repeated chunk changes no max
   }
@@ -880,7 +1004,7 @@ __global__ __launch_bounds__(256) void dit_combine(TiledArgs a, int ntiles) {
     float4 v0[kCombineBatch], v1[kCombineBatch];
 #pragma unroll
     for (int i = 0; i < kCombineBatch; ++i) {
-      const float* seg = seg0 + min(c0 + i, nk - 1) * kSeg;
+      const float* seg = seg0 + (int64_t)min(c0 + i, nk - 1) * kSeg;
       ml[i] = *reinterpret_cast<const float2*>(seg + kBM * kHead + 2 * r);
       v0[i] = *reinterpret_cast<const float4*>(seg + r * kHead + d0);
       v1[i] = *reinterpret_cast<const float4*>(seg + r * kHead + d0 + 4);
@@ -907,15 +1031,47 @@ __global__ __launch_bounds__(256) void dit_combine(TiledArgs a, int ntiles) {
   o.y = pack_bf16x2(num[2] * inv, num[3] * inv);
   o.z = pack_bf16x2(num[4] * inv, num[5] * inv);
   o.w = pack_bf16x2(num[6] * inv, num[7] * inv);
-  *reinterpret_cast<uint4*>(a.out + b * a.out_bstride + ((int64_t)(q0 + p) * a.hq + head) * kHead + d0) = o;
+  *reinterpret_cast<uint4*>(out) = o;
 }
+
+__global__ __launch_bounds__(256) void dit_combine(TiledArgs a, int ntiles) {
+  const int idx = a.split_from + blockIdx.x;
+  const int G = a.hq / a.hk, kpos = kBM / G;
+  const int tile = idx % ntiles, kvh = (idx / ntiles) % a.hk, b = idx / (ntiles * a.hk);
+  const int q0 = tile * kpos, nq = min(kpos, a.q_len - q0);
+  const int r = blockIdx.y * kCombineRows + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
+  const int p = r / G, head = kvh * G + r % G;
+  if (p >= nq) return;
+  combine_row(a.ws + (int64_t)blockIdx.x * a.split_k * (kBM * (kHead + 2)), a.split_k, r, d0,
+              a.out + b * a.out_bstride + ((int64_t)(q0 + p) * a.hq + head) * kHead + d0);
+}
+
+// The same for calls of several rows per sequence: the work list's items, each of
+// as many chunks as it has used. Rows without keys have none that weighs: zeros.
+template <bool Q8>
+__global__ __launch_bounds__(256) void multi_combine(TiledArgs a) {
+  const int idx = blockIdx.x, G = a.hq / a.hk;
+  const int used = a.used[idx];
+  if (used <= 1) return;
+  const int32_t* item = a.work + kPrefillWorkHeader + 4 * (int64_t)idx;
+  const int r = blockIdx.y * kCombineRows + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
+  const int p = r / G, head = item[3] * G + r % G;
+  if (p >= item[2]) return;
+  bf16_t* out = a.out + ((int64_t)(item[1] + p) * a.hq + head) * kHead + d0;
+  if (Q8 && a.pos[item[1] + p] < 0)
+    *reinterpret_cast<uint4*>(out) = make_uint4(0, 0, 0, 0);
+  else
+    combine_row(a.ws + (int64_t)idx * a.split_k * (kBM * (kHead + 2)), used, r, d0, out);
+}
+
 
 // Prefill with exact_p set: the hi + lo P.V variant (prefill only; DiT rounds
 // P to bf16 as hidream.cu does).
 template <int G, int SRC, int FORM>
-void launch_g(const TiledArgs& a, int grid, int items, int ntiles, hipStream_t stream) {
-  if (SRC != kDense && a.exact_p)
-    tiled_attn<G, SRC, FORM, SRC != kDense><<<grid, kThreads, 0, stream>>>(a, items, ntiles);
+void launch_g(const TiledArgs& a, dim3 grid, int items, int ntiles, hipStream_t stream) {
+  constexpr bool CAN = SRC != kDense && SRC < kCross;  // several rows per sequence: P rounded
+  if (CAN && a.exact_p)
+    tiled_attn<G, SRC, FORM, CAN><<<grid, kThreads, 0, stream>>>(a, items, ntiles);
   else
     tiled_attn<G, SRC, FORM><<<grid, kThreads, 0, stream>>>(a, items, ntiles);
 }
@@ -933,17 +1089,18 @@ int launch_tiled(TiledArgs a, int items, int ntiles, hipStream_t stream) {
   if (a.scale_log2 == 0.f) a.scale_log2 = 0x1p-149f;
   // Pages that are no multiple of a wave's rows keep whole tiles.
   const bool lane_pages = SRC == kPagedWave && a.pd.page % kRowsPerWave != 0;
-  const bool parts = !lane_pages && (LISTED || a.split_k == 0);
+  constexpr bool MULTI = SRC >= kCross;
+  const bool parts = !lane_pages && (MULTI ? a.split_k <= 1 : LISTED || a.split_k == 0);
   const int form = parts && a.quarters ? kQuarters : parts && a.halved > 0 ? kHalves : kWhole;
-  int grid = ((items + 7) >> 3) << 3;
+  dim3 grid(((items + 7) >> 3) << 3, MULTI ? a.split_k : 1);
   if (LISTED)
-    grid *= form == kQuarters ? 4 : form == kHalves ? 2 : 1;  // an XCD's items, each as so many workgroups
+    grid.x *= form == kQuarters ? 4 : form == kHalves ? 2 : 1;  // an XCD's items, each as so many workgroups
   else if (form == kQuarters)
-    grid = ((items * 4 + 7) >> 3) << 3;
+    grid.x = ((items * 4 + 7) >> 3) << 3;
   else if (form == kHalves)
-    grid = (((items - a.halved + 7) >> 3) << 3) + (((a.halved * 2 + 7) >> 3) << 3);
+    grid.x = (((items - a.halved + 7) >> 3) << 3) + (((a.halved * 2 + 7) >> 3) << 3);
   else if (a.split_k > 0)
-    grid = (((a.split_from + 7) >> 3) << 3) + ((((items - a.split_from) * a.split_k + 7) >> 3) << 3);
+    grid.x = (((a.split_from + 7) >> 3) << 3) + ((((items - a.split_from) * a.split_k + 7) >> 3) << 3);
   switch (a.hq / a.hk) {
 #define OMNI_CASE(G)                                                                       \
   case G:                                                                                  \
@@ -964,6 +1121,12 @@ int launch_tiled(TiledArgs a, int items, int ntiles, hipStream_t stream) {
     default: return -2;
   }
   if (check_launch() != 0) return -3;
+  if constexpr (MULTI) {
+    if (a.split_k > 1) {
+      multi_combine<SRC != kCross><<<dim3(items, kBM / kCombineRows), 256, 0, stream>>>(a);
+      return check_launch();
+    }
+  }
   if (!LISTED && a.split_k > 0) {
     dit_combine<<<dim3(items - a.split_from, kBM / kCombineRows), 256, 0, stream>>>(a, ntiles);
     return check_launch();
@@ -977,6 +1140,12 @@ int launch_prefill(const TiledArgs& a, int items, hipStream_t stream) {
 
 int launch_prompt(const TiledArgs& a, int items, hipStream_t stream) {
   return launch_tiled<kPacked>(a, items, 0, stream);
+}
+
+int launch_multi_tiles(const TiledArgs& a, int source, int items, hipStream_t stream) {
+  return source == kRowsBf16 ? launch_tiled<kCross>(a, items, 0, stream)
+         : source == kQ8E4m3 ? launch_tiled<kCacheE4m3>(a, items, 0, stream)
+                             : launch_tiled<kCacheInt8>(a, items, 0, stream);
 }
 
 int launch_dit(const TiledArgs& a, int batch, hipStream_t stream) {

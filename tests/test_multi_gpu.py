@@ -175,6 +175,74 @@ def test_extend_of_strided_rows_on_another_stream(stride):
     extend(c, [20, 1], 4, stride=stride, stream=torch.cuda.Stream())
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hq,hk,page", [(1, 1, 16), (4, 2, 48), (8, 2, 16), (16, 2, 256)])
+def test_extend_in_tiles(hq, hk, page, fmt):
+    """Tiles of a few packed rows to more than one, keys about one and two key tiles; with sequences in groups beside them."""
+    g = hq // hk
+    counts = [32 // g + 1, 64 // g + 3, 256 // g, 1, 256 // g + 1, 0, 3]
+    lens = [counts[0], 129, 256 // g, 70, 256 // g + 128, 5, 300]
+    mp, _ = extend(Cache(hq + page, lens, hk, page, fmt), counts, hq)
+    assert mp.plan.tiles == 5 and sum(mp.plan.groups) == 2
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("seqs,hk", [(1, 2), (12, 8), (20, 16)])
+def test_extend_in_every_form_of_a_tile(seqs, hk, fmt):
+    """Quarters, halves and whole tiles: the plan splits none of these."""
+    rng = np.random.default_rng(seqs)
+    counts = [int(x) for x in rng.integers(34, 130, seqs)]
+    lens = [c + int(x) for c, x in zip(counts, rng.integers(0, 260, seqs))]
+    mp, _ = extend(Cache(seqs, lens, hk, 16, fmt), counts, 2 * hk)
+    assert mp.plan.tiles * hk in ((2, 96, 320) if seqs < 20 else (320,)) or mp.plan.tiles >= seqs
+    assert mp.plan.tile_splits == 1
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hq,hk", [(4, 1), (2, 2)])
+def test_extend_of_tiles_in_splits(hq, hk, fmt):
+    """Few tiles over long contexts, rows that see nothing of the later splits, and (a bound below the lengths) splits that grow."""
+    c = Cache(hq, [2600, 700, 90], hk, 16, fmt)
+    counts = [70, 40, 40]
+    for most in (None, 1100):
+        mp, _ = extend(c, counts, hq, max_len=most, seed=3)
+        assert mp.plan.tiles > 0 and mp.plan.tile_splits > 1
+    pos = [2599 - 37 * i if i % 3 else -1 for i in range(70)] + [i for i in range(40)] + [-1] * 40
+    extend(c, counts, hq, pos=pos, seed=4)
+
+
+def test_extend_of_tiles_at_any_positions():
+    """Rows in no order, rows that are none, a tile and a part of one without any."""
+    for hk, n in ((1, 300), (8, 40)):
+        c = Cache(30 + hk, [500, 90], hk, 16, torch.float8_e4m3fn)
+        rng = np.random.default_rng(hk)
+        pos = [int(x) for x in rng.integers(-3, 500, n)] + [-1] * 40
+        pos[:20] = [-1] * 20
+        extend(c, [n, 40], 4 * hk, pos=pos)
+
+
+@pytest.mark.parametrize("scale", [0.0, -SCALE])
+def test_extend_of_tiles_scales_strides_streams(scale):
+    c = Cache(41, [200, 150], 2, 16, torch.int8)
+    extend(c, [120, 60], 4, scale=scale, stride=24, stream=torch.cuda.Stream())
+
+
+def test_a_tile_whose_row_sees_nothing_leaves_the_others_alone():
+    """NaN in V of a token that only later rows see: the rows of other sequences keep their bits."""
+    c = Cache(42, [150, 150], 1, 16, torch.float8_e4m3fn)
+    _, a = extend(c, [100, 100], 2)
+    raw = c.kv.view(torch.uint8)
+    slot = c.slots[0][149]
+    raw[slot // 16, 1].view(128, 16)[:, slot % 16] = 0x7f
+    q = bf16(torch.Generator(device="cuda").manual_seed(1), 202, 256)
+    out = torch.zeros(202, 256, dtype=torch.bfloat16, device="cuda")
+    mp = oa.extend_plan([100, 100], 2, 1, 150, c.lens)
+    pos = i32(list(range(50, 150)) * 2)
+    oa.qwen3_extend_q8(mp, q, c.kv, c.sc, pos, c.indptr, c.pages, 16, out, SCALE, oa.workspace_for(mp.plan))
+    torch.cuda.synchronize()
+    assert bool(out[99].isnan().any()) and torch.equal(out[100:200], a[100:200])
+
+
 # ------------------------------------------------------------------ cross
 def cross(seed, counts, lens, hq, hk, chunk=0, keys=True, of=None, max_len=None, extra=2, layout="one", stream=None, scale=SCALE):
     """Sources of the given lengths in any order, NaN between them; the call against 64 bits."""
@@ -237,6 +305,35 @@ def test_cross_in_splits(chunk):
     cross(chunk, [4, 70, 3, 1, 2, 5, 5], [1900, 700, 129, 128, 0, 65, 5], 8, 2, chunk=chunk, keys=chunk != 128)
 
 
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (8, 2), (16, 2)])
+@pytest.mark.parametrize("layout", ["own", "one", "apart"])
+def test_cross_in_tiles(hq, hk, layout):
+    g = hq // hk
+    counts = [32 // g + 1, 64 // g + 3, 256 // g, 1, 256 // g + 1, 0, 3, 40]
+    lens = [1, 129, 128, 70, 257, 5, 300, 0]
+    mp, _ = cross(hq, counts, lens, hq, hk, layout=layout)
+    assert mp.plan.tiles == sum(-(-c * g // 256) for c in counts if c > 32 // g)
+
+
+@pytest.mark.parametrize("seqs,hk", [(1, 2), (12, 8), (20, 16)])
+def test_cross_in_every_form_of_a_tile(seqs, hk):
+    rng = np.random.default_rng(seqs)
+    counts = [int(x) for x in rng.integers(34, 130, seqs)]
+    mp, _ = cross(seqs, counts, [int(x) for x in rng.integers(0, 300, seqs)], 2 * hk, hk)
+    assert mp.plan.tile_splits == 1
+
+
+@pytest.mark.parametrize("most", [None, 1100])
+def test_cross_of_tiles_in_splits(most):
+    mp, _ = cross(6, [70, 40, 40, 50], [2600, 700, 90, 0], 4, 1, max_len=most)
+    assert mp.plan.tile_splits > 1
+
+
+@pytest.mark.parametrize("scale", [0.0, -SCALE])
+def test_cross_of_tiles_scales_streams(scale):
+    cross(7, [120, 60], [200, 150], 4, 2, scale=scale, stream=torch.cuda.Stream())
+
+
 def test_cross_over_shared_sources():
     cross(3, [5, 5, 1, 40, 2], [300, 77, 12], 4, 2, of=[1, 0, 1, 1, 2])
 
@@ -264,18 +361,19 @@ def test_no_rows_and_no_sequences():
 # ------------------------------------------------------------------ graphs
 def test_two_graphs_with_workspaces_of_their_own():
     """Extend and cross captured together, twice; lengths and positions move on between replays, eager work in between."""
-    hq, hk, lens, counts = 8, 2, [400, 90, 33], [4, 20, 2]
+    hq, hk, lens, counts = 8, 2, [1400, 90, 33], [40, 20, 2]
     c = Cache(21, lens, hk, 16, torch.float8_e4m3fn)
     g = torch.Generator(device="cuda").manual_seed(4)
     rows = sum(counts)
     q = bf16(g, rows, hq * 128)
     kv = bf16(g, 500, 2 * hk * 128)
     k, v = kv[:, :hk * 128], kv[:, hk * 128:]
-    start = [n - m + i - 30 for n, m in zip(lens, counts) for i in range(m)]
+    start = [max(n - m + i - 30, -1) for n, m in zip(lens, counts) for i in range(m)]
     pos, first, length = i32(start), i32([0, 200, 333]), i32([150, 3, 0])
 
     def make():
-        e, x = oa.extend_plan(counts, hq, hk, 400, lens, 64), oa.cross_plan(counts, hq, hk, 200, None, 64)
+        e, x = oa.extend_plan(counts, hq, hk, 1400, lens, 64), oa.cross_plan(counts, hq, hk, 1200, None, 64)
+        assert e.plan.tile_splits > 1 and x.plan.tile_splits > 1 and e.plan.splits > 1 and e.plan.groups[0] > 0 and x.plan.tiles > 0
         return e, oa.workspace_for(e.plan), x, oa.workspace_for(x.plan), torch.zeros(2, rows, hq * 128, dtype=torch.bfloat16, device="cuda")
 
     def step(m, s=None):

@@ -74,7 +74,7 @@ def test_plan_capacity(init):
 def test_splits_follow_the_chunk(make):
     mp = make([1, 2], 4, 2, 1000, None, 128, device="cpu")
     p = mp.plan
-    assert (p.chunk, p.splits) == (128, 8) and p.workspace_bytes == 3 * 4 * 8 * 129 * 4 + 4 * 2
+    assert (p.chunk, p.splits) == (128, 8) and p.workspace_bytes == 3 * 4 * 8 * 129 * 4 + 16  # partials, and the splits of two groups
     assert make([1, 2], 4, 2, 1000, None, 1024, device="cpu").plan.workspace_bytes == 0
 
 
@@ -82,6 +82,8 @@ def extend(plan=None, **k):
     plan = plan or oa.extend_plan([3, 2], 4, 2, 100, chunk=128, device="cpu").plan
     a = dict(plan=ctypes.byref(plan), q=P, stride=512, kv=P, scale=P, fmt=0, pos=P, indptr=P, pages=P, page=16, out=P, s=0.1, work=P, ws=None)
     a.update(k)
+    if a.pop("plan_", None):
+        a["plan"] = None
     return oa.load().omni_qwen3_extend_q8(*a.values(), None)
 
 
@@ -89,11 +91,13 @@ def cross(plan=None, **k):
     plan = plan or oa.cross_plan([3, 2], 4, 2, 100, chunk=128, device="cpu").plan
     a = dict(plan=ctypes.byref(plan), q=P, stride=512, k=P, ks=256, v=P, vs=256, of=P, first=P, len=P, out=P, s=0.1, work=P, ws=None)
     a.update(k)
+    if a.pop("plan_", None):
+        a["plan"] = None
     return oa.load().omni_attn_cross_run(*a.values(), None)
 
 
 BAD = [dict(q=None), dict(out=None), dict(work=None), dict(q=P + 8), dict(out=P + 8), dict(work=P + 4), dict(stride=504), dict(stride=516),
-       dict(s=float("nan")), dict(s=3e38), dict(ws=P + 8), dict(plan=None)]
+       dict(s=float("nan")), dict(s=3e38), dict(ws=P + 8)]
 
 
 @pytest.mark.parametrize("bad", BAD + [
@@ -111,6 +115,7 @@ def test_cross_refusals(bad):
 
 
 def test_other_codes():
+    assert extend(plan_=1) == oa.EINVAL and cross(plan_=1) == oa.EINVAL
     assert extend(page=24) == oa.EUNSUPPORTED
     split = oa.extend_plan([3, 2], 4, 2, 100, chunk=64, device="cpu").plan
     assert extend(split) == oa.EWORKSPACE
@@ -159,3 +164,44 @@ def test_launches_that_no_grid_holds():
         with pytest.raises(oa.OmniAttnError) as e:
             make([1] * 3000, 128, 128, 64 * 100000, None, 64, device="cpu")
         assert e.value.code == oa.EUNSUPPORTED
+
+
+def tile_items(mp):
+    p = mp.plan
+    work = mp.work.numpy()
+    return work[:16], work[16:16 + 4 * p.tiles * p.hk].reshape(-1, 4)
+
+
+@pytest.mark.parametrize("make", PLANS)
+@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 4), (8, 2), (16, 2)])
+def test_tiles_and_groups_cover_every_row_once(make, hq, hk):
+    g = hq // hk
+    counts = [1, 32 // g, 32 // g + 1, 0, 256 // g, 256 // g + 1, 1000, 3]
+    mp = make(counts, hq, hk, 3000, [c + 7 for c in counts], device="cpu")
+    starts = np.cumsum([0] + counts)
+    seen = np.zeros((sum(counts), hk), int)
+    ranges, items = tile_items(mp)
+    assert ranges[0] == 0 and ranges[8] == len(items) == mp.plan.tiles * hk
+    for s, first, rows, head in items:
+        assert counts[s] > 32 // g and starts[s] <= first and first + rows <= starts[s + 1] and 1 <= rows <= 256 // g
+        assert (first - starts[s]) % (256 // g) == 0
+        seen[first:first + rows, head] += 1
+    for list_ in groups_of(mp):
+        for s, first, rows, _ in list_:
+            seen[first:first + rows] += 1
+    assert (seen == 1).all() and mp.plan.group_rows == sum(c for c in counts if c <= 32 // g)
+    # An XCD's tiles run by the keys that their last rows see, most first.
+    for x in range(8):
+        lens = [first + rows - starts[s] + (7 if make is oa.extend_plan else 0) if make is oa.extend_plan else counts[s]
+                for s, first, rows, _ in items[ranges[x]:ranges[x + 1]]]
+        assert lens == sorted(lens, reverse=True)
+
+
+@pytest.mark.parametrize("make", PLANS)
+def test_tiles_are_split_where_they_are_few(make):
+    few = make([100], 4, 1, 30000, device="cpu").plan
+    assert few.tiles == 2 and few.tile_splits > 16 and few.tile_chunk * few.tile_splits >= 30000
+    assert few.workspace_bytes >= 2 * few.tile_splits * 256 * 130 * 4
+    many = make([2000] * 4, 32, 8, 30000, device="cpu").plan
+    assert many.tile_splits == 1 and many.workspace_bytes == 0
+    assert make([100], 4, 1, 700, device="cpu").plan.tile_splits == 1  # too short to be worth it
