@@ -503,7 +503,9 @@ typedef struct omni_attn_multi_plan {
   int32_t group_rows; /* rows in them */
   int32_t chunk, splits; /* keys per split of a group's rows (a multiple of 64), ceil(max_len / chunk) */
   int32_t tiles;      /* tiles of 256 packed rows (each runs once per kv head) */
-  int32_t tile_chunk, tile_splits; /* keys per split of a tile (a multiple of 128), ceil(max_len / tile_chunk) */
+  int32_t tile_chunk; /* keys per split of a tile (a multiple of 128) */
+  int32_t tile_units; /* splits of all tiles (each runs once per kv head) */
+  int32_t split_tiles, tile_segments; /* tiles in more than one split, and their splits */
   int64_t work_bytes; /* bytes of the int32 work list that the caller uploads */
   int64_t workspace_bytes; /* device scratch of a run (split partials), 16-byte aligned */
 } omni_attn_multi_plan;

@@ -12,6 +12,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <functional>
 #include <new>
 #include <vector>
 
@@ -778,8 +779,8 @@ namespace {
 // 29.3; 5 of 20,000-90,000 1536 keys 111 / 108 (2048); 4 of 100,000-130,000 4096 keys
 // 162 / 153 (8192, which rows of unlike lengths cannot fill); 2 of 60,000, hk = 2,
 // 1024 keys 22.4 / 22.4; 1 of 40,000, hk = 1, 768 keys 15.7 / 14.8 (512).
-int pick_chunk_keys(double units, int max_len, double mean_len, int key_bytes) {
-  const double read = units * mean_len * key_bytes / 6.2e6;
+int pick_chunk_q8(int rows, int hk, int max_len) {
+  const double units = (double)rows * hk, read = units * max_len * 0.6 * 256 / 6.2e6;
   int best = 0;
   double least = 0;
   for (int chunk : {128, 256, 384, 512, 768, 1024, 1536, 2048, 4096, 8192, 16384, 32768, 0}) {
@@ -791,10 +792,6 @@ int pick_chunk_keys(double units, int max_len, double mean_len, int key_bytes) {
     if (chunk >= max_len) break;
   }
   return best;
-}
-
-int pick_chunk_q8(int rows, int hk, int max_len) {
-  return pick_chunk_keys((double)rows * hk, max_len, max_len * 0.6, 256);
 }
 
 constexpr float kLog2e = 1.4426950408889634f;  // the kernels take exponentials to base 2
@@ -1100,22 +1097,20 @@ int64_t groups_workspace(const omni_attn_multi_plan& p) {
 }
 
 int64_t tiles_workspace(const omni_attn_multi_plan& p) {
-  if (p.tile_splits <= 1) return 0;
-  const int64_t items = (int64_t)p.tiles * p.hk;
-  return align16(items * p.tile_splits * omni::kSegmentBytes + 4 * items);
+  return align16((int64_t)p.tile_segments * p.hk * omni::kSegmentBytes + 4 * (int64_t)p.split_tiles * p.hk);
 }
 
-// The work list: the tiles' (of the form that the prefill's has), then the groups'.
-int64_t tiles_work_ints(const omni_attn_multi_plan& p) {
-  return p.tiles > 0 ? omni::kPrefillWorkHeader + 4 * (int64_t)p.tiles * p.hk : 0;
+// The work list: the tiles' splits behind a header (as the prefill's), the split tiles, the groups.
+int64_t units_work_ints(const omni_attn_multi_plan& p) {
+  return p.tile_units > 0 ? omni::kPrefillWorkHeader + omni::kMultiItem * (int64_t)p.tile_units * p.hk : 0;
 }
+int64_t tiles_work_ints(const omni_attn_multi_plan& p) { return units_work_ints(p) + 4 * (int64_t)p.split_tiles * p.hk; }
 int64_t multi_work_ints(const omni_attn_multi_plan& p) { return tiles_work_ints(p) + 4 * ((int64_t)p.groups[0] + p.groups[1]); }
 
 // What the launches of a plan hold.
 bool multi_fits(const omni_attn_multi_plan& p) {
-  const int64_t items = (int64_t)p.tiles * p.hk;
-  if (!omni::grid_holds(items + omni::kXcds, omni::kTiledThreads, p.tile_splits) ||
-      (p.tile_splits > 1 && !omni::grid_holds(items, 256)))
+  if (!omni::grid_holds((int64_t)p.tile_units * p.hk + omni::kXcds, omni::kTiledThreads) ||
+      !omni::grid_holds((int64_t)p.split_tiles * p.hk, 256) || (int64_t)p.tile_segments * p.hk > INT_MAX)
     return false;
   for (int c = 0; c < 2; ++c) {
     const int64_t rows = std::max(rows_of_group(16 * (c + 1), p.hq / p.hk), 1);
@@ -1127,14 +1122,133 @@ bool multi_fits(const omni_attn_multi_plan& p) {
   return true;
 }
 
-// Keys per split of the tiles: as many splits as fill the GPU's CUs once, each of four
-// key tiles at least (a partial is written and merged for every one).
-int pick_tile_chunk(int64_t items, int max_len) {
-  const int64_t steps = ((int64_t)max_len + 127) / 128;
-  int64_t splits = items > 0 ? std::min<int64_t>(256 / items, steps / 4) : 1;
-  if (splits < 2) splits = 1;
-  return (int)std::min<int64_t>((steps + splits - 1) / splits * 128, INT_MAX / 128 * 128);
+// Key tiles per split of the tiles: the size with the least estimated time, us. Each kv
+// head has 256 / hk CUs; these take the splits, longest first, as they come free:
+//   3.9 for each 128 keys, 2.4 where at most 128 packed rows keep half the waves;
+//   12 for a workgroup's first loads and last stores, 5 more to write a partial;
+//   with splits, 8 for the merge's launch and the partials, written and read, at 4.5 TB/s.
+// Fitted to sweeps of 19 shapes (1 to 230 tiles, 600 to 60,000 keys) over 20 sizes.
+int pick_tile_steps(const std::vector<std::array<int32_t, 4>>& tl, int G, int hk, int max_len) {
+  const size_t machines = (size_t)std::max(256 / hk, 1);
+  const auto steps_of = [&](const std::array<int32_t, 4>& t) { return (int)((std::min((int64_t)t[3], (int64_t)max_len) + 127) / 128); };
+  int most = 1;
+  for (const auto& t : tl) most = std::max(most, steps_of(t));
+  if (tl.size() * 2 > 3 * machines) return most;  // enough of them to share the CUs evenly
+  int best = most, last = 0;
+  double least = 0;
+  std::vector<double> cost, free_at;
+  for (int n = 1; n <= most; ++n) {
+    const int per = (most + n - 1) / n;
+    if (per == last) continue;
+    last = per;
+    cost.clear();
+    double partials = 0;
+    for (const auto& t : tl) {
+      const int steps = std::max(steps_of(t), 1), used = (steps + per - 1) / per, packed = t[2] * G;
+      if (used > 1) partials += (double)used * hk * packed * 2 * kPartialBytes;
+      for (int k = 0; k < used; ++k)
+        cost.push_back((packed <= 128 ? 2.4 : 3.9) * std::min(per, steps - k * per) + (used > 1 ? 17 : 12));
+    }
+    if (n > 1 && cost.size() > 3 * machines) break;
+    std::sort(cost.begin(), cost.end(), std::greater<double>());
+    free_at.assign(machines, 0);  // a heap: the CU that comes free first in front
+    for (const double c : cost) {
+      std::pop_heap(free_at.begin(), free_at.end(), std::greater<double>());
+      free_at.back() += c;
+      std::push_heap(free_at.begin(), free_at.end(), std::greater<double>());
+    }
+    const double t = *std::max_element(free_at.begin(), free_at.end()) + (partials > 0 ? 8 + partials / 4.5e6 : 0);
+    if (n == 1 || t < least) best = per, least = t;
+  }
+  return best;
 }
+
+// The tiles' part of the work list. In workgroup order the splits run longest first,
+// each with its hk kv heads (an XCD sees the same kv heads, as in write_work_list).
+void write_tile_list(const std::vector<std::array<int32_t, 4>>& tl, int G, const omni_attn_multi_plan& p, int32_t* work_h) {
+  struct Unit {
+    int32_t tile, split, splits, segment, which;
+    double cost;
+  };
+  std::vector<Unit> units;
+  units.reserve((size_t)p.tile_units);
+  int32_t* items = work_h + units_work_ints(p);
+  int32_t segment = 0, which = 0;
+  for (size_t t = 0; t < tl.size(); ++t) {
+    const int steps = (int)std::max<int64_t>(((int64_t)std::min(tl[t][3], p.max_len) + 127) / 128, 1), per = p.tile_chunk / 128;
+    const int32_t n = (steps + per - 1) / per;
+    for (int32_t k = 0; k < n; ++k)
+      units.push_back({(int32_t)t, k, n, segment + k, which, (tl[t][2] * G <= 128 ? 2.4 : 3.9) * std::min(per, steps - k * per)});
+    if (n == 1) continue;
+    for (int32_t h = 0; h < p.hk; ++h) {
+      *items++ = tl[t][1], *items++ = tl[t][2], *items++ = h;
+      *items++ = segment * p.hk + h * n;
+    }
+    segment += n, ++which;
+  }
+  std::stable_sort(units.begin(), units.end(), [](const Unit& x, const Unit& y) { return x.cost > y.cost; });
+  const int64_t total = (int64_t)units.size() * p.hk;
+  for (int k = 0; k < omni::kPrefillWorkHeader; ++k) work_h[k] = 0;
+  int32_t* it = work_h + omni::kPrefillWorkHeader;
+  int64_t at = 0;
+  for (int x = 0; x < omni::kXcds; ++x) {
+    work_h[x] = (int32_t)at;
+    for (int64_t k = x; k < total; k += omni::kXcds, ++at) {
+      const Unit& u = units[(size_t)(k / p.hk)];
+      const auto& t = tl[(size_t)u.tile];
+      const int32_t h = (int32_t)(k % p.hk);
+      *it++ = t[0], *it++ = t[1], *it++ = t[2], *it++ = h, *it++ = u.split, *it++ = u.splits;
+      *it++ = (u.segment - u.split) * p.hk + h * u.splits + u.split, *it++ = u.which * p.hk + h;
+    }
+  }
+  work_h[omni::kXcds] = (int32_t)total;
+}
+
+// Split size of the groups: the one with the least estimated time, us, fitted to sweeps
+// of 27 shapes (1 to 128 groups, 1 to 16 K/V heads, 100 to 60,000 keys) over 34 sizes:
+//   the keys' bytes at 9 TB/s, or a wave's walk through the tiles of its quarter of a
+//   split, 0.86 for each 32 keys (bf16 1.4), whichever is longer, and 0.1 of the walk;
+//   the partials, written and read, at 12 TB/s;
+//   0.35 for each 1024 workgroups, those that find nothing to do too;
+//   with splits, 5.7 for the merge's launch and 1.6 for every 16 splits of a row.
+// Measured at the choice / at the best of the sweep: 1.8% apart in the mean; 5 rows
+// behind 2400 keys of 16q/8kv, 192 keys 12.1 / 12.1; 4 rows of 8 behind 20,000-60,000 of
+// 32q/8kv, 3584 keys 75.4 / 75.2; 5 candidates of 48 sources of 100-1500 none 33.0 / 33.0;
+// 20 rows over 30,000-60,000 bf16 keys of 16 heads 4096 keys 143 / 143.
+int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, int hk, int max_len, bool known, bool cross) {
+  const int64_t n = (int64_t)(groups[0].size() + groups[1].size());
+  const int64_t whole = std::min<int64_t>(((int64_t)max_len + 63) / 64 * 64, INT_MAX / 64 * 64);
+  if (n == 0) return (int)whole;
+  const int64_t step = (n + 255) / 256;  // of many groups, as many as 256 stand for all
+  const double key_bytes = cross ? 512 : 256;
+  double keys = 0, longest = 1;
+  std::vector<std::array<double, 2>> some;  // keys, packed rows
+  for (int64_t i = 0, at = 0; i < 2; at -= (int64_t)groups[i++].size())
+    for (; at < (int64_t)groups[i].size(); at += step) {
+      const double len = known ? std::min(groups[i][at][3], max_len) : max_len;
+      some.push_back({len, (double)groups[i][at][2] * G});
+      keys += known ? len : 0.6 * len;
+      longest = std::max(longest, len);
+    }
+  const double each = (double)n / some.size() * hk, read = keys * each * key_bytes / 9e6;
+  int best = 0;
+  double least = 0;
+  for (int64_t chunk = 64;; chunk = chunk < 768 ? chunk + 64 : chunk * 9 / 8 / 64 * 64) {
+    chunk = std::min(chunk, whole);
+    double part = 0;
+    for (const auto& g : some)
+      if (g[0] > chunk) part += std::ceil(g[0] / chunk) * g[1];
+    const double splits = std::ceil((double)max_len / chunk), most = std::ceil(longest / chunk);
+    const double walk = (cross ? 1.4 : 0.86) * std::min<double>(chunk, longest) / 128;
+    const double t = std::max(read, walk) + 0.1 * walk + part * each * 2 * kPartialBytes / 12e6 + 0.35 * n * hk * splits / 1024 +
+                     (splits > 1 ? 5.7 + 1.6 * std::ceil(most / 16) : 0);
+    if (best == 0 || t < least) best = (int)chunk, least = t;
+    if (chunk >= whole) return best;
+  }
+}
+
+// Workgroups of a group kernel that a CU holds: by its registers, or (bf16) LDS.
+int groups_a_cu(int cross, bool large) { return cross || large ? 2 : 4; }
 
 int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
                     int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan, const char* who) try {
@@ -1167,12 +1281,11 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   const int small = rows_of_group(16, G), large = rows_of_group(32, G);
   const bool tiled = G == 1 || G == 2 || G == 4 || G == 8;
   const int per_tile = omni::kTiledRows / G;
-  double keys = 0;
   for (int32_t s = 0, at = 0; s < nseq; at += counts_h[s++]) {
     if (tiled && counts_h[s] > large) {
       for (int32_t f = 0; f < counts_h[s]; f += per_tile) {
         const int32_t n = std::min(per_tile, counts_h[s] - f);
-        tl.push_back({s, at + f, n, !keys_h ? (cross ? 0 : f + n) : cross ? keys_h[s] : std::max(keys_h[s] - (counts_h[s] - f - n), 0)});
+        tl.push_back({s, at + f, n, std::max((keys_h ? keys_h[s] : max_len) - (cross ? 0 : counts_h[s] - f - n), 0)});
       }
       if (tl.size() > (size_t)INT_MAX / 8) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many tiles", who);
       continue;
@@ -1180,7 +1293,6 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
     for (int32_t f = 0; f < counts_h[s];) {
       const int32_t left = counts_h[s] - f, n = std::min(left, left <= small ? small : large);
       groups[n > small].push_back({s, at + f, n, keys_h ? keys_h[s] : 0});
-      keys += keys_h ? std::min(keys_h[s], max_len) : 0.6 * max_len;
       f += n;
       plan->group_rows += n;
     }
@@ -1190,19 +1302,32 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
     plan->groups[c] = (int32_t)groups[c].size();
     std::stable_sort(groups[c].begin(), groups[c].end(), [](const auto& x, const auto& y) { return x[3] > y[3]; });
   }
-  const double n = (double)groups[0].size() + (double)groups[1].size();
-  plan->chunk = chunk_hint > 0 ? chunk_hint : pick_chunk_keys(n * hk, max_len, n > 0 ? keys / n : 1, cross ? 512 : 256);
+  plan->chunk = chunk_hint > 0 ? chunk_hint : pick_chunk_groups(groups, G, hk, max_len, keys_h != nullptr, cross);
   plan->splits = (int32_t)(((int64_t)max_len + plan->chunk - 1) / plan->chunk);
   plan->tiles = (int32_t)tl.size();
-  plan->tile_chunk = pick_tile_chunk((int64_t)tl.size() * hk, max_len);
-  plan->tile_splits = (int32_t)(((int64_t)max_len + plan->tile_chunk - 1) / plan->tile_chunk);
+  plan->tile_chunk = 128 * std::min(pick_tile_steps(tl, G, hk, max_len), INT_MAX / 128);
+  int64_t units = 0, segments = 0;
+  for (const auto& t : tl) {
+    const int64_t n = std::max<int64_t>(((int64_t)std::min(t[3], max_len) + plan->tile_chunk - 1) / plan->tile_chunk, 1);
+    units += n;
+    if (n > 1) segments += n, ++plan->split_tiles;
+  }
+  if (units > INT_MAX) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many tiles", who);
+  plan->tile_units = (int32_t)units;
+  plan->tile_segments = (int32_t)segments;
   if (!multi_fits(*plan)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, plan->rows, hq, plan->splits);
   plan->workspace_bytes = groups_workspace(*plan) + tiles_workspace(*plan);
   const int64_t need = multi_work_ints(*plan);
   plan->work_bytes = need * (int64_t)sizeof(int32_t);
   if (need > 0 && (!work_h || need > work_cap))
     return fail(OMNI_ATTN_EWORKSPACE, "%s: work list needs %lld int32", who, (long long)need);
-  if (!tl.empty()) write_work_list(tl, hk, work_h);
+  // Unsplit groups that the GPU takes all at once: every other round of workgroups (one a
+  // CU) backwards, so that a CU's keys add up to much the same.
+  const size_t round = (size_t)std::max(256 / hk, 1);
+  for (auto& list : groups)
+    if (plan->splits == 1 && (int64_t)list.size() * hk <= 256 * groups_a_cu(cross, &list != groups))
+      for (size_t r = round; r < list.size(); r += 2 * round) std::reverse(list.begin() + r, list.begin() + std::min(r + round, list.size()));
+  if (!tl.empty()) write_tile_list(tl, G, *plan, work_h);
   work_h += tiles_work_ints(*plan);
   int32_t at = 0;
   for (auto& list : groups)
@@ -1223,7 +1348,8 @@ int multi_checks(const omni_attn_multi_plan* plan, int cross, const void* q, int
   if (p.rows < 0 || p.hk <= 0 || p.hq <= 0 || p.hq % p.hk != 0 || p.hq / p.hk > 16 || p.max_len <= 0 || p.groups[0] < 0 ||
       p.groups[1] < 0 || p.group_rows < 0 || p.group_rows > p.rows || p.chunk <= 0 || p.chunk % 64 != 0 ||
       p.splits != ((int64_t)p.max_len + p.chunk - 1) / p.chunk || p.tiles < 0 || p.tile_chunk <= 0 || p.tile_chunk % 128 != 0 ||
-      p.tile_splits != ((int64_t)p.max_len + p.tile_chunk - 1) / p.tile_chunk ||
+      p.split_tiles < 0 || p.split_tiles > p.tiles || p.tile_segments < 2 * (int64_t)p.split_tiles ||
+      p.tile_units != (int64_t)p.tiles - p.split_tiles + p.tile_segments || (p.split_tiles == 0 && p.tile_segments > 0) ||
       (p.tiles > 0 && (32 % (p.hq / p.hk) != 0 || p.hq / p.hk > 8)) ||
       p.work_bytes != multi_work_ints(p) * (int64_t)sizeof(int32_t) ||
       p.workspace_bytes != groups_workspace(p) + tiles_workspace(p))
@@ -1267,15 +1393,16 @@ int multi_launch(omni::RowsArgs& a, const omni_attn_multi_plan& p, int source, c
     t.hq = p.hq;
     t.hk = p.hk;
     t.scale_log2 = scale * kLog2e;
-    const int64_t items = (int64_t)p.tiles * p.hk;
+    const int64_t items = (int64_t)p.tile_units * p.hk;
     const int resident = resident_tiled_groups();
     t.quarters = omni::tiled_quarters(items, resident);
     t.halved = omni::prefill_halves(items, resident);
-    t.split_k = p.tile_splits;
     t.split_tiles = p.tile_chunk / 128;
-    if (p.tile_splits > 1) {
+    t.splits_listed = p.split_tiles * p.hk;
+    if (p.split_tiles > 0) {
+      t.split_items = work + units_work_ints(p);
       t.ws = reinterpret_cast<float*>(static_cast<char*>(workspace) + groups_workspace(p));
-      t.used = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(t.ws) + items * p.tile_splits * omni::kSegmentBytes);
+      t.used = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(t.ws) + (int64_t)p.tile_segments * p.hk * omni::kSegmentBytes);
     }
     if (omni::launch_multi_tiles(t, source, (int)items, as_stream(stream)) != 0)
       return fail(OMNI_ATTN_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(omni::g_launch_status));

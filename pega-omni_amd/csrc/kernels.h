@@ -114,16 +114,20 @@ struct TiledArgs {
   int exact_p;
   // packed prompts (mode 2), cross attention: elements between rows of k and of v
   int64_t k_stride, v_stride;
-  // Several rows per sequence: split_k splits of split_tiles key tiles each, partials
-  // to ws (a segment per item and split), the splits that an item used to `used`.
+  // Several rows per sequence: an item is (sequence, first row, rows, kv head, split,
+  // splits, segment of ws, split tile); splits are of split_tiles key tiles, and of a
+  // split tile's, how many it used goes to `used`.
   const uint8_t* kv8;       // the 8-bit cache (pd: blocks per page)
   const uint8_t* kv_scale;
   const int32_t* of;        // cross: the source of each sequence (null: the sequence)
   const int32_t* first;     // and its first row and rows
   const int32_t* len;
   int split_tiles;
+  int splits_listed;          // (tile, kv head) pairs that are split
+  const int32_t* split_items; // (first row, rows, kv head, first segment) of each
   int32_t* used;
 };
+constexpr int kMultiItem = 8;  // int32 per item
 
 // Packed (position, head) query rows per MFMA tile: one 8-wave workgroup, one per CU.
 constexpr int kTiledRows = 256;
@@ -348,6 +352,7 @@ struct RowsArgs {
   float* ws_lse;     // [workspace rows][hq][splits]
   int32_t* ws_used;  // splits that each group takes
   int hq, hk;
+  int g16;  // set by the launch: divides a packed column by hq / hk
   int chunk, splits;
   float scale_log2;
 };

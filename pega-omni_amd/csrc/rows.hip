@@ -28,8 +28,7 @@ namespace omni {
 
 namespace {
 
-constexpr int kThreads = kRowsThreads;
-constexpr int kWaves = kThreads / 64;
+constexpr int kThreads = kRowsThreads, kWaves = kThreads / 64;
 constexpr int kTile = 32;  // keys per step: two blocks of the cache
 constexpr int kBlocksPerTile = kTile / kQ8Block;
 constexpr int kIds = 64 / kBlocksPerTile;  // tiles whose blocks a wave looks up at once
@@ -44,27 +43,48 @@ __device__ __forceinline__ bf16x4 lds_read_tr(const bf16_t* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p));
 }
 
-// Orders a wave's LDS accesses with its own of other lanes' data (LDS keeps a wave's
-// order; this keeps the compiler's).
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+constexpr int kBufferFlags = 0x00020000;  // resource word 3 of raw buffer loads
+
+// A raw buffer over a wave-uniform base, `bytes` long: what lies past that is read as zeros.
+__device__ __forceinline__ i32x4 buffer_rsrc(const void* base, int bytes) {
+  const uint64_t b = (uint64_t)base;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32)),
+               __builtin_amdgcn_readfirstlane(bytes), kBufferFlags};
+}
+// Sixteen bytes at offset off of a buffer, read once: nontemporal (bit 1 of the last operand).
+__device__ __forceinline__ uint4 ldb16_stream(i32x4 rsrc, int off) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)(uint32_t)rsrc[0] | (uint64_t)(uint32_t)rsrc[1] << 32), 0, rsrc[2], rsrc[3]);
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 2));
+}
+// The same to LDS, lane l's to lds + 16 l (lds wave-uniform). The compiler does not
+// see these loads, nor M0's and the resource's hazards: s_nop 4 covers those, and
+// the wave waits for the loads by itself.
+__device__ __forceinline__ void dma16_stream(i32x4 rsrc, int off, const void* lds) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
+               :
+               : "v"(off), "s"(rsrc), "{m0}"((uint32_t)(uintptr_t)(lds_void*)lds)
+               : "memory");
 }
 
-// The larger of v over the 16 lanes of a DPP row, and the smaller.
+// The larger of v over the 16 lanes of a DPP row.
+template <int CTRL>
+__device__ __forceinline__ int dpp_max(int v) {
+  return max(v, __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false));
+}
 __device__ __forceinline__ int row16_max(int v) {
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) v = max(v, __shfl_xor(v, d));
-  return v;
+  return dpp_max<kRowMirror>(dpp_max<kRowHalfMirror>(dpp_max<kQuadSwap2>(dpp_max<kQuadSwap1>(v))));
 }
-__device__ __forceinline__ int row16_min(int v) {
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) v = min(v, __shfl_xor(v, d));
-  return v;
-}
+
+// c / G for packed columns: 0 <= c < 32, 1 <= G <= 16 (g16 = 65536 / G + 1).
+__device__ __forceinline__ int row_of_column(int c, int g16) { return c * g16 >> 16; }
+
+// Waves per SIMD that a kernel's registers (bf16: its LDS) leave room for.
+constexpr int room(int src, int nc) { return nc == 2 || src == kBf16 ? 2 : 4; }
 
 template <int SRC, int NC>
-__global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) void rows_attn(RowsArgs a) {
+__global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a) {
   constexpr bool Q8 = SRC != kBf16;
   constexpr int FMT = Q8 ? SRC : kQ8E4m3;
   const int slot = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
@@ -84,24 +104,24 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
     const int e = a.of ? a.of[item.x] : item.x;
     src0 = a.first[e], src_len = max(a.len[e], 0);
   }
-  int lim[NC], most = 0, least = INT_MAX;
+  int lim[NC], most = 0, not_least = -INT_MAX;
   bf16x8 q[NC][4];  // product step kk holds dims 64 (kk / 2) + 16 g + 8 (kk % 2) .. + 7
 #pragma unroll
   for (int b = 0; b < NC; ++b) {
-    const int c = 16 * b + col, i = c / G;
+    const int c = 16 * b + col, i = row_of_column(c, a.g16);
     const bool mine = i < nrows;
     lim[b] = -1;
     if (mine) {
       lim[b] = Q8 ? max(a.pos[item.y + i], -1) + 1 : src_len;
-      most = max(most, lim[b]), least = min(least, lim[b]);
+      most = max(most, lim[b]), not_least = max(not_least, -lim[b]);
     }
-    const bf16_t* qp = a.q + (int64_t)(item.y + (mine ? i : 0)) * a.q_stride + (int64_t)(kh * G + c % G) * kHead;
+    const bf16_t* qp = a.q + (int64_t)(item.y + (mine ? i : 0)) * a.q_stride + (int64_t)(kh * G + c - i * G) * kHead;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
       q[b][kk] = __builtin_bit_cast(bf16x8, ldg16(qp + 64 * (kk >> 1) + 16 * grp + 8 * (kk & 1)));
   }
   most = __builtin_amdgcn_readfirstlane(row16_max(most));
-  least = __builtin_amdgcn_readfirstlane(row16_min(least));
+  const int least = -__builtin_amdgcn_readfirstlane(row16_max(not_least));
 
   const int split_len = most > 0 ? split_len_of(a.chunk, a.splits, most) : 0;
   const int used = most > 0 ? (most - 1) / split_len + 1 : 0;
@@ -130,7 +150,21 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
     const uint8_t* e = a.kv_scale + ids * row_blocks + kh;
     exps = e[0] | e[a.hk] << 16;
   };
-  uint4 kr[Q8 ? 2 : 4][2], vr[Q8 ? 4 : 8];
+  // One buffer for the waves' tiles of V (bf16: two each, of 8 KiB) and, in the end,
+  // their parts of a block of columns (8.25 KiB each).
+  constexpr int kPart = 16 * (kHead + 4), kVTile = kTile * kHead;
+  __shared__ __align__(16) float s_buf[kWaves * (Q8 ? kPart : kVTile)];
+  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+  bf16_t* v_lds = reinterpret_cast<bf16_t*>(s_buf) + wave * (2 * kVTile);
+
+  // bf16: a tile's rows from a scalar base, each lane's first one at a constant offset
+  // (bytes); those past the last key are read as zeros.
+  const int k_off = Q8 ? 0 : (2 * (col & 4) + (col & 3)) * 2 * (int)a.k_stride + 32 * grp + 2 * (col & 8);
+  auto tile_rows = [&](const bf16_t* base, int64_t stride, int k) __attribute__((always_inline)) {
+    const int n0 = t0 + (wave + kWaves * k) * kTile, rows = min(t1 - n0, kTile);
+    return buffer_rsrc(base + (src0 + n0) * stride + (int64_t)kh * kHead, (rows - 1) * 2 * (int)stride + 2 * kHead);
+  };
+  uint4 kr[Q8 ? 2 : 4][2], vr[Q8 ? 4 : 1];
   auto load_k = [&](int k) __attribute__((always_inline)) {
     if constexpr (Q8) {
       const uint8_t* kb = a.kv + kh * kQ8HeadBytes + (2 * (col & 4) + (col & 3)) * kHead + 16 * grp + 8 * (col & 8);
@@ -141,14 +175,15 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
         for (int j = 0; j < 2; ++j) kr[j][b] = ldg16_stream(kb + block * row_blocks * kQ8HeadBytes + 4 * j * kHead);
       }
     } else {
-      const int n0 = t0 + (wave + kWaves * k) * kTile;
+      // Rows 0-7 of the product, then 8-15, whole lines of 128 bytes, eight lanes a key; columns n and n + 8 trade halves.
+      const auto rsrc = tile_rows(a.k, a.k_stride, k);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int key = min(n0 + 8 * (col >> 2) + 4 * j + (col & 3), t1 - 1);
-        const bf16_t* kp = a.k + (src0 + key) * a.k_stride + (int64_t)kh * kHead + 16 * grp;
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) kr[2 * j + (kk >> 1)][kk & 1] = ldg16_stream(kp + 64 * (kk >> 1) + 8 * (kk & 1));
-      }
+        for (int i = 0; i < 2; ++i) {
+          const int at = k_off + (16 * i + 4 * j) * 2 * (int)a.k_stride;
+          kr[2 * j][i] = ldb16_stream(rsrc, at), kr[2 * j + 1][i] = ldb16_stream(rsrc, at + 128);
+        }
     }
   };
   auto load_v = [&](int k) __attribute__((always_inline)) {
@@ -157,13 +192,15 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
       const uint8_t* vb = a.kv + (block * row_blocks + a.hk + kh) * kQ8HeadBytes + (16 * (grp & 1) + col) * kQ8Block;
 #pragma unroll
       for (int i = 0; i < 4; ++i) vr[i] = ldg16_stream(vb + i * 32 * kQ8Block);
-    } else {  // rows 4 i + g of the tile, 16-byte chunk col
-      const int n0 = t0 + (wave + kWaves * k) * kTile;
+    } else {
+      // To LDS, four rows a load. 32-byte unit u of row r lies in unit u ^ (r % 4 + 4 (r / 8 % 2)):
+      // the 8 rows x 32 bytes that 32 lanes of a transposing read take are disjoint banks.
+      const auto rsrc = tile_rows(a.v, a.v_stride, k);
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the tile before has been read
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = min(n0 + 4 * i + grp, t1 - 1);
-        vr[i] = ldg16_stream(a.v + (src0 + key) * a.v_stride + (int64_t)kh * kHead + 8 * col);
-      }
+      for (int i = 0; i < 8; ++i)
+        dma16_stream(rsrc, (4 * i + grp) * 2 * (int)a.v_stride + 32 * ((col >> 1) ^ (grp | (i >> 1 & 1) << 2)) + 16 * (col & 1),
+                     v_lds + (k & 1) * kVTile + 4 * i * kHead);
     }
   };
 
@@ -175,20 +212,18 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
     for (int i = 0; i < 8; ++i) o[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     m[b] = -INFINITY, l[b] = 0.f;
   }
-  // One buffer for the waves' tiles of V (bf16) and, in the end, their parts of a block of columns.
-  constexpr int kPart = 16 * (kHead + 4);
-  constexpr int kLdsFloats = kWaves * kPart;  // 33 KiB, a wave's tile of V being 8
-  __shared__ __align__(16) float s_buf[kLdsFloats];
-  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
-  bf16_t* v_lds = reinterpret_cast<bf16_t*>(s_buf) + wave * (kTile * kHead);
-
   if (mine > 0) {
-    if constexpr (Q8) next_blocks(0);
+    if constexpr (Q8)
+      next_blocks(0);
+    else
+      load_v(0);
     load_k(0);
   }
   for (int k = 0; k < mine; ++k) {
-    // V of this tile, then (when its scores are taken) K of the next: one of the two is always in flight.
-    load_v(k);
+    // 8-bit: V of this tile, then (when its scores are taken) K of the next: one of the
+    // two is always in flight. bf16: V and K of the next tile when this one's scores are
+    // taken; V, whose loads the compiler does not see, is waited for below.
+    if constexpr (Q8) load_v(k);
     int e2 = 0;
     if constexpr (Q8) e2 = from_lane(exps, 2 * (k & (kIds - 1)) + (grp >> 1));
     const int n0 = t0 + (wave + kWaves * k) * kTile, left = t1 - n0;  // keys from this tile on
@@ -198,7 +233,10 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
       f32x4 d[NC];
 #pragma unroll
       for (int b = 0; b < NC; ++b) d[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (Q8) trade_halves(kr[j][0], kr[j][1]);
+      if constexpr (Q8)
+        trade_halves(kr[j][0], kr[j][1]);
+      else
+        trade_halves(kr[2 * j][0], kr[2 * j][1]), trade_halves(kr[2 * j + 1][0], kr[2 * j + 1][1]);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         bf16x8 ka;
@@ -216,8 +254,13 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[b][4 * j + r] = d[b][r];
     }
+    if constexpr (!Q8) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): V of this tile; K has been used, so that nothing younger is in flight
+      asm volatile("" ::: "memory");       // V's reads stay behind it
+    }
     if (k + 1 < mine) {
       if (Q8 && ((k + 1) & (kIds - 1)) == 0) next_blocks(k + 1);
+      if constexpr (!Q8) load_v(k + 1);
       load_k(k + 1);
     }
     const float ks = Q8 ? pow2_biased(e2 & 0xff) * a.scale_log2 : a.scale_log2, vs = Q8 ? pow2_biased(e2 >> 16) : 1.f;
@@ -232,8 +275,8 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
         for (int t = 0; t < 8; ++t)
           if (n0 + 8 * grp + t >= lim[b]) s[b][t] = -INFINITY;
     }
-    if (left < kTile) {  // nothing past the last key that any row sees counts, whatever it holds
-      if constexpr (Q8) {
+    if constexpr (Q8) {
+      if (left < kTile) {  // nothing past the last key that any row sees counts, whatever it holds
         const int tokens = left - kQ8Block * (grp >> 1);  // of this lane's block
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -242,10 +285,6 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
 #pragma unroll
           for (int i = 0; i < 4; ++i) (&vr[i].x)[w] &= stay;
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (4 * i + grp >= left) vr[i] = make_uint4(0, 0, 0, 0);
       }
     }
     bf16x8 ph[NC], pl[NC];
@@ -294,22 +333,14 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
         weigh(2 * i + 1, bf16_of<FMT>(a0[1], a1[1]));
       }
     } else {
-      // 32-byte unit u of row r lies in unit u ^ (r % 4 + 4 (r / 8 % 2)): the 8 rows x
-      // 32 bytes that 32 lanes of a transposing read take are disjoint banks.
-      wave_lds_fence();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + grp, f = (r & 3) | (r >> 3 & 1) << 2;
-        *reinterpret_cast<uint4*>(v_lds + r * kHead + 16 * ((col >> 1) ^ f) + 8 * (col & 1)) = vr[i];
-      }
-      wave_lds_fence();
+      const bf16_t* vt = v_lds + (k & 1) * kVTile;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         bf16x4 part[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = 8 * grp + 4 * h + (col >> 2), f = (r & 3) | (r >> 3 & 1) << 2;
-          part[h] = lds_read_tr(v_lds + r * kHead + 16 * (i ^ f) + 4 * (col & 3));
+          part[h] = lds_read_tr(vt + r * kHead + 16 * (i ^ f) + 4 * (col & 3));
         }
         weigh(i, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
       }
@@ -329,8 +360,9 @@ __global__ __launch_bounds__(kThreads, NC == 1 ? (SRC == kBf16 ? 3 : 4) : 2) voi
       *reinterpret_cast<f32x4*>(s_buf + wave * kPart + col * (kHead + 4) + 16 * i + 4 * grp) = o[b][i];
     if (grp == 0) s_m[wave][col] = m[b], s_l[wave][col] = l[b];
     __syncthreads();
-    for (int i = tid; i < min(packed - 16 * b, 16) * kHead; i += kThreads) {
-      const int g = i / kHead, d = i % kHead, c = 16 * b + g, row = c / G, head = kh * G + c % G;
+    const int d = tid & (kHead - 1);
+    for (int g = wave >> 1; g < min(packed - 16 * b, 16); g += kThreads / kHead) {
+      const int c = 16 * b + g, row = row_of_column(c, a.g16), head = kh * G + c - row * G;
       float top = s_m[0][g];
       for (int w = 1; w < waves; ++w) top = fmaxf(top, s_m[w][g]);
       const float base = top == -INFINITY ? 0.f : top;
@@ -362,53 +394,56 @@ constexpr int kMergeBatch = 16;
 template <bool Q8>
 __global__ __launch_bounds__(kThreads) void rows_merge(RowsArgs a, int parts) {
   const int group = blockIdx.x / parts;
-  const int used = a.ws_used[group];
-  if (used <= 1) return;
-  const int4 item = reinterpret_cast<const int4*>(a.items)[group];
   const int x = (blockIdx.x % parts) * kMergeRows + (threadIdx.x >> 5), row = x / a.hq, head = x % a.hq;
+  const int used = a.ws_used[group];
+  const int4 item = reinterpret_cast<const int4*>(a.items)[group];
   if (row >= item.z) return;
+  const bool none = Q8 && a.pos[item.y + row] < 0;
   const int lane = threadIdx.x & 31;
   const int64_t h = (int64_t)(item.w + row) * a.hq + head;
   const float* lse = a.ws_lse + h * a.splits;
   const float* part = a.ws_o + h * a.splits * kHead + 4 * lane;
   f32x4 num = {0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, den = 0.f;
-  for (int i0 = 0; i0 < used; i0 += kMergeBatch) {
+  for (int i0 = 0; i0 < used || i0 == 0; i0 += kMergeBatch) {
     f32x4 o[kMergeBatch];
     float e[kMergeBatch];
 #pragma unroll
     for (int j = 0; j < kMergeBatch; ++j) {
-      const int i = min(i0 + j, used - 1);
+      const int i = min(i0 + j, (i0 == 0 ? a.splits : used) - 1);  // the first are asked for before it is known how many count
       e[j] = lse[i];
       o[j] = *reinterpret_cast<const f32x4*>(part + (int64_t)i * kHead);
     }
+    if (i0 == 0 && used <= 1) return;
     float mx = top;
 #pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j) mx = fmaxf(mx, e[j]);  // one seen twice changes no maximum
+    for (int j = 0; j < kMergeBatch; ++j) mx = i0 + j < used ? fmaxf(mx, e[j]) : mx;
     const float base = mx == -INFINITY ? 0.f : mx, alpha = fast_exp2(top - base);
     top = mx;
     num *= alpha, den *= alpha;
 #pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j) {
-      const float w = i0 + j < used ? fast_exp2(e[j] - base) : 0.f;
-      num += o[j] * w, den += w;
-    }
+    for (int j = 0; j < kMergeBatch; ++j)
+      if (i0 + j < used) {  // what was asked for beyond may be anything
+        const float w = fast_exp2(e[j] - base);
+        num += o[j] * w, den += w;
+      }
   }
   uint2 w = make_uint2(pack_bf16x2(num[0] / den, num[1] / den), pack_bf16x2(num[2] / den, num[3] / den));
-  if (Q8 && a.pos[item.y + row] < 0) w = make_uint2(0, 0);
+  if (none) w = make_uint2(0, 0);
   *reinterpret_cast<uint2*>(a.out + ((int64_t)(item.y + row) * a.hq + head) * kHead + 4 * lane) = w;
 }
 
 template <int SRC>
-int launch(RowsArgs a, const int* groups, hipStream_t stream) {
+int launch(const RowsArgs& a, const int* groups, hipStream_t stream) {
   RowsArgs x = a;
+  x.g16 = 65536 / (a.hq / a.hk) + 1;
   for (int c = 0; c < 2; ++c) {
     if (groups[c] == 0) continue;
-    const unsigned grid = (unsigned)((int64_t)groups[c] * a.hk * a.splits);
+    const int64_t grid = (int64_t)groups[c] * a.hk * a.splits;
     if (c == 0)
-      rows_attn<SRC, 1><<<grid, kThreads, 0, stream>>>(x);
+      rows_attn<SRC, 1><<<(unsigned)grid, kThreads, 0, stream>>>(x);
     else
-      rows_attn<SRC, 2><<<grid, kThreads, 0, stream>>>(x);
+      rows_attn<SRC, 2><<<(unsigned)grid, kThreads, 0, stream>>>(x);
     if (check_launch() != 0) return -3;
     if (a.splits > 1) {
       const int rows = std::max((c + 1) * 16 / (a.hq / a.hk), 1), parts = (rows * a.hq + kMergeRows - 1) / kMergeRows;

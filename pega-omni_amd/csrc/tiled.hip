@@ -207,13 +207,15 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   // chunks.
   int idx, chunk = -1, part = -1;
   int4 item{};  // prefill: sequence (packed: its first row), first row, rows, kv head
+  int4 unit{};  // several rows per sequence: split, splits, its segment of the workspace, (tile, kv head)
   if constexpr (LISTED) {
     // XCD x's items are those from header entry x to entry x + 1. The plan puts
     // its range at x (items / 8) + min(x, items % 8), so the item is read there
     // beside the header, in one round trip, and once more only if the list's
     // header says otherwise (the chain item -> sequence -> page ids -> K follows).
     const auto at = [&](int i) {
-      const int32_t* it = a.work + kPrefillWorkHeader + 4 * (int64_t)i;
+      const int32_t* it = a.work + kPrefillWorkHeader + (MULTI ? kMultiItem : 4) * (int64_t)i;
+      if constexpr (MULTI) unit = int4{it[4], it[5], it[6], it[7]};
       return int4{it[0], it[1], it[2], it[3]};
     };
     const int x = blockIdx.x & 7, k = blockIdx.x >> 3, nth = k / PARTS;
@@ -348,10 +350,10 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   bool split = false;  // several rows per sequence: whether the item's keys are split
   if constexpr (MULTI) {
     // Splits of whole key tiles: the plan's, or more where the rows pass its bound.
-    if (a.split_k > 1) {
-      const int per = max(a.split_tiles, (steps + a.split_k - 1) / a.split_k), used = steps > 0 ? (steps - 1) / per + 1 : 0;
-      chunk = blockIdx.y;
-      if (chunk == 0 && part <= 0 && threadIdx.x == 0) a.used[idx] = used;
+    if (unit.y > 1) {
+      const int per = max(a.split_tiles, (steps + unit.y - 1) / unit.y), used = steps > 0 ? (steps - 1) / per + 1 : 0;
+      chunk = unit.x;
+      if (chunk == 0 && threadIdx.x == 0) a.used[unit.w] = used;
       if (chunk > 0 && chunk >= used) return;
       s_lo = chunk * per;
       s_hi = min(steps, s_lo + per);
@@ -929,7 +931,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   l += xor_lane(l, 32);
   if (MULTI ? split : chunk >= 0) {  // a chunk's partial: unnormalised O with its base m and sum l, for the combine
     if (!row_ok) return;  // which reads the tile's positions only
-    float* seg = a.ws + ((int64_t)(MULTI ? idx : idx - a.split_from) * a.split_k + chunk) * (kBM * (kHead + 2));
+    float* seg = a.ws + (MULTI ? (int64_t)unit.z : (int64_t)(idx - a.split_from) * a.split_k + chunk) * (kBM * (kHead + 2));
 #pragma unroll
     for (int md = 0; md < 4; ++md)
 #pragma unroll
@@ -1046,29 +1048,29 @@ __global__ __launch_bounds__(256) void dit_combine(TiledArgs a, int ntiles) {
               a.out + b * a.out_bstride + ((int64_t)(q0 + p) * a.hq + head) * kHead + d0);
 }
 
-// The same for calls of several rows per sequence: the work list's items, each of
-// as many chunks as it has used. Rows without keys have none that weighs: zeros.
+// The same for calls of several rows per sequence, over the work list's split tiles
+// (first row, rows, kv head and first segment; the segments of a tile's splits follow
+// one another). Rows without keys have none that weighs: zeros.
 template <bool Q8>
 __global__ __launch_bounds__(256) void multi_combine(TiledArgs a) {
   const int idx = blockIdx.x, G = a.hq / a.hk;
   const int used = a.used[idx];
+  const int4 item = reinterpret_cast<const int4*>(a.split_items)[idx];
   if (used <= 1) return;
-  const int32_t* item = a.work + kPrefillWorkHeader + 4 * (int64_t)idx;
   const int r = blockIdx.y * kCombineRows + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
-  const int p = r / G, head = item[3] * G + r % G;
-  if (p >= item[2]) return;
-  bf16_t* out = a.out + ((int64_t)(item[1] + p) * a.hq + head) * kHead + d0;
-  if (Q8 && a.pos[item[1] + p] < 0)
+  const int p = r / G, head = item.z * G + r % G;
+  if (p >= item.y) return;
+  bf16_t* out = a.out + ((int64_t)(item.x + p) * a.hq + head) * kHead + d0;
+  if (Q8 && a.pos[item.x + p] < 0)
     *reinterpret_cast<uint4*>(out) = make_uint4(0, 0, 0, 0);
   else
-    combine_row(a.ws + (int64_t)idx * a.split_k * (kBM * (kHead + 2)), used, r, d0, out);
+    combine_row(a.ws + (int64_t)item.w * (kBM * (kHead + 2)), used, r, d0, out);
 }
-
 
 // Prefill with exact_p set: the hi + lo P.V variant (prefill only; DiT rounds
 // P to bf16 as hidream.cu does).
 template <int G, int SRC, int FORM>
-void launch_g(const TiledArgs& a, dim3 grid, int items, int ntiles, hipStream_t stream) {
+void launch_g(const TiledArgs& a, int grid, int items, int ntiles, hipStream_t stream) {
   constexpr bool CAN = SRC != kDense && SRC < kCross;  // several rows per sequence: P rounded
   if (CAN && a.exact_p)
     tiled_attn<G, SRC, FORM, CAN><<<grid, kThreads, 0, stream>>>(a, items, ntiles);
@@ -1090,17 +1092,17 @@ int launch_tiled(TiledArgs a, int items, int ntiles, hipStream_t stream) {
   // Pages that are no multiple of a wave's rows keep whole tiles.
   const bool lane_pages = SRC == kPagedWave && a.pd.page % kRowsPerWave != 0;
   constexpr bool MULTI = SRC >= kCross;
-  const bool parts = !lane_pages && (MULTI ? a.split_k <= 1 : LISTED || a.split_k == 0);
+  const bool parts = !lane_pages && (MULTI ? a.splits_listed == 0 : LISTED || a.split_k == 0);
   const int form = parts && a.quarters ? kQuarters : parts && a.halved > 0 ? kHalves : kWhole;
-  dim3 grid(((items + 7) >> 3) << 3, MULTI ? a.split_k : 1);
+  int grid = ((items + 7) >> 3) << 3;
   if (LISTED)
-    grid.x *= form == kQuarters ? 4 : form == kHalves ? 2 : 1;  // an XCD's items, each as so many workgroups
+    grid *= form == kQuarters ? 4 : form == kHalves ? 2 : 1;  // an XCD's items, each as so many workgroups
   else if (form == kQuarters)
-    grid.x = ((items * 4 + 7) >> 3) << 3;
+    grid = ((items * 4 + 7) >> 3) << 3;
   else if (form == kHalves)
-    grid.x = (((items - a.halved + 7) >> 3) << 3) + (((a.halved * 2 + 7) >> 3) << 3);
+    grid = (((items - a.halved + 7) >> 3) << 3) + (((a.halved * 2 + 7) >> 3) << 3);
   else if (a.split_k > 0)
-    grid.x = (((a.split_from + 7) >> 3) << 3) + ((((items - a.split_from) * a.split_k + 7) >> 3) << 3);
+    grid = (((a.split_from + 7) >> 3) << 3) + ((((items - a.split_from) * a.split_k + 7) >> 3) << 3);
   switch (a.hq / a.hk) {
 #define OMNI_CASE(G)                                                                       \
   case G:                                                                                  \
@@ -1122,10 +1124,8 @@ int launch_tiled(TiledArgs a, int items, int ntiles, hipStream_t stream) {
   }
   if (check_launch() != 0) return -3;
   if constexpr (MULTI) {
-    if (a.split_k > 1) {
-      multi_combine<SRC != kCross><<<dim3(items, kBM / kCombineRows), 256, 0, stream>>>(a);
-      return check_launch();
-    }
+    if (a.splits_listed > 0) multi_combine<SRC != kCross><<<dim3(a.splits_listed, kBM / kCombineRows), 256, 0, stream>>>(a);
+    return check_launch();
   }
   if (!LISTED && a.split_k > 0) {
     dit_combine<<<dim3(items - a.split_from, kBM / kCombineRows), 256, 0, stream>>>(a, ntiles);

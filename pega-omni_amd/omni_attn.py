@@ -146,7 +146,9 @@ class MultiPlan(ctypes.Structure):
         ("splits", ctypes.c_int32),
         ("tiles", ctypes.c_int32),
         ("tile_chunk", ctypes.c_int32),
-        ("tile_splits", ctypes.c_int32),
+        ("tile_units", ctypes.c_int32),
+        ("split_tiles", ctypes.c_int32),
+        ("tile_segments", ctypes.c_int32),
         ("work_bytes", ctypes.c_int64),
         ("workspace_bytes", ctypes.c_int64),
     ]

@@ -195,7 +195,7 @@ def test_extend_in_every_form_of_a_tile(seqs, hk, fmt):
     lens = [c + int(x) for c, x in zip(counts, rng.integers(0, 260, seqs))]
     mp, _ = extend(Cache(seqs, lens, hk, 16, fmt), counts, 2 * hk)
     assert mp.plan.tiles * hk in ((2, 96, 320) if seqs < 20 else (320,)) or mp.plan.tiles >= seqs
-    assert mp.plan.tile_splits == 1
+    assert mp.plan.split_tiles == 0
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -206,7 +206,7 @@ def test_extend_of_tiles_in_splits(hq, hk, fmt):
     counts = [70, 40, 40]
     for most in (None, 1100):
         mp, _ = extend(c, counts, hq, max_len=most, seed=3)
-        assert mp.plan.tiles > 0 and mp.plan.tile_splits > 1
+        assert mp.plan.split_tiles > 0
     pos = [2599 - 37 * i if i % 3 else -1 for i in range(70)] + [i for i in range(40)] + [-1] * 40
     extend(c, counts, hq, pos=pos, seed=4)
 
@@ -320,13 +320,13 @@ def test_cross_in_every_form_of_a_tile(seqs, hk):
     rng = np.random.default_rng(seqs)
     counts = [int(x) for x in rng.integers(34, 130, seqs)]
     mp, _ = cross(seqs, counts, [int(x) for x in rng.integers(0, 300, seqs)], 2 * hk, hk)
-    assert mp.plan.tile_splits == 1
+    assert mp.plan.split_tiles == 0
 
 
 @pytest.mark.parametrize("most", [None, 1100])
 def test_cross_of_tiles_in_splits(most):
     mp, _ = cross(6, [70, 40, 40, 50], [2600, 700, 90, 0], 4, 1, max_len=most)
-    assert mp.plan.tile_splits > 1
+    assert mp.plan.split_tiles > 0
 
 
 @pytest.mark.parametrize("scale", [0.0, -SCALE])
@@ -373,7 +373,7 @@ def test_two_graphs_with_workspaces_of_their_own():
 
     def make():
         e, x = oa.extend_plan(counts, hq, hk, 1400, lens, 64), oa.cross_plan(counts, hq, hk, 1200, None, 64)
-        assert e.plan.tile_splits > 1 and x.plan.tile_splits > 1 and e.plan.splits > 1 and e.plan.groups[0] > 0 and x.plan.tiles > 0
+        assert e.plan.split_tiles > 0 and x.plan.split_tiles > 0 and e.plan.splits > 1 and e.plan.groups[0] > 0 and x.plan.tiles > 0
         return e, oa.workspace_for(e.plan), x, oa.workspace_for(x.plan), torch.zeros(2, rows, hq * 128, dtype=torch.bfloat16, device="cuda")
 
     def step(m, s=None):

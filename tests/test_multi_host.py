@@ -132,7 +132,7 @@ def test_other_codes():
 
 @pytest.mark.parametrize("field,value", [
     ("rows", -1), ("hq", 5), ("hq", 0), ("hk", 0), ("hq", 64), ("max_len", 0), ("max_len", 300), ("group_rows", -1), ("group_rows", 6), ("chunk", 0),
-    ("chunk", 65), ("splits", 2), ("splits", 0), ("tiles", -1), ("tiles", 1), ("tile_chunk", 0), ("tile_chunk", 64), ("tile_splits", 3), ("work_bytes", 0),
+    ("chunk", 65), ("splits", 2), ("splits", 0), ("tiles", -1), ("tiles", 1), ("tile_chunk", 0), ("tile_chunk", 64), ("tile_units", 3), ("split_tiles", 1), ("tile_segments", 2), ("work_bytes", 0),
     ("workspace_bytes", 16)])
 def test_plans_that_do_not_agree(field, value):
     for make, call in ((oa.extend_plan, extend), (oa.cross_plan, cross)):
@@ -169,39 +169,81 @@ def test_launches_that_no_grid_holds():
 def tile_items(mp):
     p = mp.plan
     work = mp.work.numpy()
-    return work[:16], work[16:16 + 4 * p.tiles * p.hk].reshape(-1, 4)
+    n = 16 + 8 * p.tile_units * p.hk
+    return work[:16], work[16:n].reshape(-1, 8), work[n:n + 4 * p.split_tiles * p.hk].reshape(-1, 4)
+
+
+def check_tiles(mp, counts, keys, causal):
+    """Every row of a sequence in tiles once for each split of its tile and each head; segments and the combine's list agree."""
+    p = mp.plan
+    g = p.hq // p.hk
+    starts = np.cumsum([0] + counts)
+    ranges, items, split = tile_items(mp)
+    assert ranges[0] == 0 and ranges[8] == len(items) == p.tile_units * p.hk and np.ptp(np.diff(ranges[:9])) <= 1
+    seen, segments, which = {}, {}, {}
+    for s, first, rows, head, k, n, seg, at in items:
+        assert counts[s] > 32 // g and starts[s] <= first and first + rows <= starts[s + 1] and 1 <= rows <= 256 // g
+        assert (first - starts[s]) % (256 // g) == 0 and 0 <= k < n
+        last = min(max(keys[s] - (starts[s + 1] - first - rows if causal else 0), 0), p.max_len)
+        assert n == max(1, -(-last // p.tile_chunk))
+        seen.setdefault((first, rows, head, n), []).append(k)
+        if n > 1:
+            assert segments.setdefault(seg, (first, head, k)) == (first, head, k) and 0 <= seg < p.tile_segments * p.hk
+            assert tuple(split[at]) == (first, rows, head, seg - k)
+            which[at] = True
+    assert all(sorted(ks) == list(range(n)) for (_, _, _, n), ks in seen.items())
+    covered = np.zeros((sum(counts), p.hk), int)
+    for first, rows, head, _ in seen:
+        covered[first:first + rows, head] += 1
+    for list_ in groups_of(mp):
+        for s, first, rows, _ in list_:
+            covered[first:first + rows] += 1
+    assert (covered == 1).all() and len(segments) == p.tile_segments * p.hk and len(which) == p.split_tiles * p.hk
+    # An XCD's splits run longest first.
+    for x in range(8):
+        def cost(i):
+            s, first, rows, _, k, n = i[:6]
+            last = min(max(keys[s] - (starts[s + 1] - first - rows if causal else 0), 0), p.max_len)
+            steps = max(1, -(-last // 128))
+            return (2.4 if rows * g <= 128 else 3.9) * min(p.tile_chunk // 128, steps - k * (p.tile_chunk // 128))
+        costs = [cost(i) for i in items[ranges[x]:ranges[x + 1]]]
+        assert costs == sorted(costs, reverse=True)
 
 
 @pytest.mark.parametrize("make", PLANS)
-@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 4), (8, 2), (16, 2)])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 4), (8, 2), (16, 2), (3, 3)])
 def test_tiles_and_groups_cover_every_row_once(make, hq, hk):
     g = hq // hk
     counts = [1, 32 // g, 32 // g + 1, 0, 256 // g, 256 // g + 1, 1000, 3]
-    mp = make(counts, hq, hk, 3000, [c + 7 for c in counts], device="cpu")
-    starts = np.cumsum([0] + counts)
-    seen = np.zeros((sum(counts), hk), int)
-    ranges, items = tile_items(mp)
-    assert ranges[0] == 0 and ranges[8] == len(items) == mp.plan.tiles * hk
-    for s, first, rows, head in items:
-        assert counts[s] > 32 // g and starts[s] <= first and first + rows <= starts[s + 1] and 1 <= rows <= 256 // g
-        assert (first - starts[s]) % (256 // g) == 0
-        seen[first:first + rows, head] += 1
-    for list_ in groups_of(mp):
-        for s, first, rows, _ in list_:
-            seen[first:first + rows] += 1
-    assert (seen == 1).all() and mp.plan.group_rows == sum(c for c in counts if c <= 32 // g)
-    # An XCD's tiles run by the keys that their last rows see, most first.
-    for x in range(8):
-        lens = [first + rows - starts[s] + (7 if make is oa.extend_plan else 0) if make is oa.extend_plan else counts[s]
-                for s, first, rows, _ in items[ranges[x]:ranges[x + 1]]]
-        assert lens == sorted(lens, reverse=True)
+    for reach in (7, 9000):
+        keys = [c + reach + 13 * i for i, c in enumerate(counts)]
+        mp = make(counts, hq, hk, max(keys) - 5, keys, device="cpu")
+        check_tiles(mp, counts, keys, make is oa.extend_plan)
+        assert mp.plan.group_rows == sum(c for c in counts if c <= 32 // g)
+        assert mp.plan.tiles == sum(-(-c // (256 // g)) for c in counts if c > 32 // g)
+        mp = make(counts, hq, hk, 500, device="cpu")  # lengths not known: the longest
+        check_tiles(mp, counts, [500] * len(counts), make is oa.extend_plan)
 
 
 @pytest.mark.parametrize("make", PLANS)
 def test_tiles_are_split_where_they_are_few(make):
     few = make([100], 4, 1, 30000, device="cpu").plan
-    assert few.tiles == 2 and few.tile_splits > 16 and few.tile_chunk * few.tile_splits >= 30000
-    assert few.workspace_bytes >= 2 * few.tile_splits * 256 * 130 * 4
-    many = make([2000] * 4, 32, 8, 30000, device="cpu").plan
-    assert many.tile_splits == 1 and many.workspace_bytes == 0
-    assert make([100], 4, 1, 700, device="cpu").plan.tile_splits == 1  # too short to be worth it
+    assert few.tiles == few.split_tiles == 2 and few.tile_units > 32 and few.tile_segments == few.tile_units
+    assert few.workspace_bytes >= few.tile_units * 256 * 130 * 4
+    many = make([2000] * 8, 32, 8, 30000, device="cpu").plan
+    assert many.tile_units == many.tiles and many.split_tiles == many.workspace_bytes == 0
+    short = make([100], 4, 1, 200, device="cpu").plan
+    assert short.split_tiles == 0  # not worth it
+    # Tiles of unlike lengths: the long ones are split.
+    p = make([60, 60, 60], 4, 4, 20000, [20000, 300, 0], device="cpu").plan
+    assert 1 <= p.split_tiles < p.tiles
+
+
+@pytest.mark.parametrize("field,by", [("tile_units", 1), ("tile_units", -1), ("split_tiles", 1), ("split_tiles", -1), ("tile_segments", 1),
+                                      ("tile_segments", -1), ("tile_chunk", 64), ("workspace_bytes", -16), ("work_bytes", 4)])
+def test_plans_of_tiles_that_do_not_agree(field, by):
+    for make, call in ((oa.extend_plan, extend), (oa.cross_plan, cross)):
+        plan = make([100, 3], 4, 2, 30000, device="cpu").plan
+        assert plan.split_tiles > 0
+        setattr(plan, field, getattr(plan, field) + by)
+        assert call(plan, ws=P) == oa.EINVAL
