@@ -1204,17 +1204,21 @@ void write_tile_list(const std::vector<std::array<int32_t, 4>>& tl, int G, const
   work_h[omni::kXcds] = (int32_t)total;
 }
 
+// Workgroups of a group kernel that a CU holds: by its registers, or (bf16) LDS.
+int groups_a_cu(int cross, bool large) { return cross || large ? 2 : 4; }
+
 // Split size of the groups: the one with the least estimated time, us, fitted to sweeps
-// of 27 shapes (1 to 128 groups, 1 to 16 K/V heads, 100 to 60,000 keys) over 34 sizes:
-//   the keys' bytes at 9 TB/s, or a wave's walk through the tiles of its quarter of a
-//   split, 0.86 for each 32 keys (bf16 1.4), whichever is longer, and 0.1 of the walk;
-//   the partials, written and read, at 12 TB/s;
-//   0.35 for each 1024 workgroups, those that find nothing to do too;
-//   with splits, 5.7 for the merge's launch and 1.6 for every 16 splits of a row.
-// Measured at the choice / at the best of the sweep: 1.8% apart in the mean; 5 rows
-// behind 2400 keys of 16q/8kv, 192 keys 12.1 / 12.1; 4 rows of 8 behind 20,000-60,000 of
-// 32q/8kv, 3584 keys 75.4 / 75.2; 5 candidates of 48 sources of 100-1500 none 33.0 / 33.0;
-// 20 rows over 30,000-60,000 bf16 keys of 16 heads 4096 keys 143 / 143.
+// of 33 shapes (1 to 128 groups, 1 to 16 K/V heads, 100 to 60,000 keys) over 34 sizes:
+//   the keys' bytes at 7.6 TB/s, or a wave's walk through the tiles of its quarter of a
+//   split, 0.82 for each 32 keys (bf16 2; 1.14 times that with 32 columns), whichever is
+//   longer; and of the walk 0.19, or 0.35 where not all workgroups run at once;
+//   the partials, written and read, at 6.4 TB/s;
+//   0.6 for each 1024 workgroups, those that find nothing to do too;
+//   with splits, 7.2 for the merge's launch and 1.1 for every 16 splits of a row.
+// Measured at the choice / at the best of the sweep: 0.3% apart in the mean; 5 rows
+// behind 2400 keys of 16q/8kv, 192 keys 9.9 / 9.9; 4 x 8 rows behind 20,000-60,000 of
+// 32q/8kv, 3584 keys 67.2 / 67.2; 5 candidates of 48 sources of 100-1500 none 31.3 / 31.3;
+// 2 x 20 rows over 30,000-60,000 bf16 keys of 16 heads, 3200 keys 145 / 139 (3584).
 int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, int hk, int max_len, bool known, bool cross) {
   const int64_t n = (int64_t)(groups[0].size() + groups[1].size());
   const int64_t whole = std::min<int64_t>(((int64_t)max_len + 63) / 64 * 64, INT_MAX / 64 * 64);
@@ -1230,25 +1234,27 @@ int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, 
       keys += known ? len : 0.6 * len;
       longest = std::max(longest, len);
     }
-  const double each = (double)n / some.size() * hk, read = keys * each * key_bytes / 9e6;
+  const double each = (double)n / some.size() * hk, read = keys * each * key_bytes / 7.6e6;
+  const double tile = (cross ? 2.0 : 0.82) * (groups[1].empty() ? 1 : 1.14);
   int best = 0;
   double least = 0;
   for (int64_t chunk = 64;; chunk = chunk < 768 ? chunk + 64 : chunk * 9 / 8 / 64 * 64) {
     chunk = std::min(chunk, whole);
-    double part = 0;
-    for (const auto& g : some)
-      if (g[0] > chunk) part += std::ceil(g[0] / chunk) * g[1];
+    double part = 0, wgs = 0;
+    for (const auto& g : some) {
+      const double used = std::ceil(g[0] / chunk);
+      wgs += used;
+      if (used > 1) part += used * g[1];
+    }
+    const bool at_once = wgs * each <= 256 * groups_a_cu(cross, !groups[1].empty());
     const double splits = std::ceil((double)max_len / chunk), most = std::ceil(longest / chunk);
-    const double walk = (cross ? 1.4 : 0.86) * std::min<double>(chunk, longest) / 128;
-    const double t = std::max(read, walk) + 0.1 * walk + part * each * 2 * kPartialBytes / 12e6 + 0.35 * n * hk * splits / 1024 +
-                     (splits > 1 ? 5.7 + 1.6 * std::ceil(most / 16) : 0);
+    const double walk = tile * std::min<double>(chunk, longest) / 128;
+    const double t = std::max(read, walk) + (at_once ? 0.19 : 0.35) * walk + part * each * 2 * kPartialBytes / 6.4e6 +
+                     0.6 * n * hk * splits / 1024 + (splits > 1 ? 7.2 + 1.1 * std::ceil(most / 16) : 0);
     if (best == 0 || t < least) best = (int)chunk, least = t;
     if (chunk >= whole) return best;
   }
 }
-
-// Workgroups of a group kernel that a CU holds: by its registers, or (bf16) LDS.
-int groups_a_cu(int cross, bool large) { return cross || large ? 2 : 4; }
 
 int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
                     int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan, const char* who) try {

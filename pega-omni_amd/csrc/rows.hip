@@ -347,8 +347,8 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
     }
   }
 
-  // The waves' parts, merged, a block of columns at a time: O rows [column][dim], then (m, l).
-  const int waves = min(tiles, kWaves);
+  // The waves' parts, merged, a block of columns at a time: O rows [column][dim], then
+  // (m, l). A wave without a tile has m = -inf and zeros.
 #pragma unroll
   for (int b = 0; b < NC; ++b) {
     if (16 * b >= packed) break;
@@ -360,25 +360,31 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
       *reinterpret_cast<f32x4*>(s_buf + wave * kPart + col * (kHead + 4) + 16 * i + 4 * grp) = o[b][i];
     if (grp == 0) s_m[wave][col] = m[b], s_l[wave][col] = l[b];
     __syncthreads();
-    const int d = tid & (kHead - 1);
-    for (int g = wave >> 1; g < min(packed - 16 * b, 16); g += kThreads / kHead) {
-      const int c = 16 * b + g, row = row_of_column(c, a.g16), head = kh * G + c - row * G;
-      float top = s_m[0][g];
-      for (int w = 1; w < waves; ++w) top = fmaxf(top, s_m[w][g]);
+#pragma unroll
+    for (int it = 0; it < 16 * kHead / 4 / kThreads; ++it) {  // four dims of a column a thread
+      const int x = tid + it * kThreads, g = x / (kHead / 4), d = 4 * (x & (kHead / 4 - 1)), c = 16 * b + g;
+      if (c >= packed) break;
+      float wm[kWaves], top = -INFINITY, den = 0.f;
+      f32x4 num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) wm[w] = s_m[w][g], top = fmaxf(top, wm[w]);
       const float base = top == -INFINITY ? 0.f : top;
-      float num = 0.f, den = 0.f;
-      for (int w = 0; w < waves; ++w) {
-        const float e = fast_exp2(s_m[w][g] - base);
-        num = fmaf(s_buf[w * kPart + g * (kHead + 4) + d], e, num);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float e = fast_exp2(wm[w] - base);
+        num += *reinterpret_cast<const f32x4*>(s_buf + w * kPart + g * (kHead + 4) + d) * e;
         den = fmaf(s_l[w][g], e, den);
       }
+      const int row = row_of_column(c, a.g16), head = kh * G + c - row * G;
+      const int64_t h = (int64_t)(item.y + row) * a.hq + head;
       if (used == 1) {
-        const bool none = Q8 && a.pos[item.y + row] < 0;  // among rows that see keys
-        a.out[((int64_t)(item.y + row) * a.hq + head) * kHead + d] = none ? 0 : (bf16_t)f2bf(num / den);
+        uint2 w = make_uint2(pack_bf16x2(num[0] / den, num[1] / den), pack_bf16x2(num[2] / den, num[3] / den));
+        if (Q8 && a.pos[item.y + row] < 0) w = make_uint2(0, 0);  // a row that is none, among rows that see keys
+        *reinterpret_cast<uint2*>(a.out + h * kHead + d) = w;
       } else {
         // den = 0: the row sees nothing of this split (or every score is -inf): it weighs nothing beside the others.
         const int64_t at = ((int64_t)(item.w + row) * a.hq + head) * a.splits + split;
-        a.ws_o[at * kHead + d] = den == 0.f ? 0.f : num / den;
+        *reinterpret_cast<f32x4*>(a.ws_o + at * kHead + d) = den == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : num / den;
         if (d == 0) a.ws_lse[at] = base + __log2f(den);
       }
     }
