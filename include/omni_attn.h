@@ -576,7 +576,7 @@ int omni_attn_cross_run(const omni_attn_multi_plan* plan, const void* q, int64_t
  *   OMNI_ATTN_PAGES_UNHELD      (pages_free) more pages came back than were in use:
  *                               shares, table and queue do not agree. The holders
  *                               are counted down, and the queue stays
- * Tables have at most 2^18 lines, pools that are compacted at most 2^20 pages. Page
+ * Tables have at most 2^18 lines, pools that are compacted at most 2^19 pages. Page
  * ids of a line that are outside the pool are passed over. Calls that share a
  * table, a queue or shares follow one another on a stream. */
 #define OMNI_ATTN_PAGES_UNHELD 6

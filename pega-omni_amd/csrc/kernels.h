@@ -218,7 +218,7 @@ int launch_tables(const TablesArgs& a, hipStream_t stream);
 
 // Pages of a cache (pages.hip): forked, given back, compacted, copied.
 constexpr int kMostLines = 1 << 18;  // of a table: a bit each in LDS
-constexpr int kMostPool = 1 << 20;   // pages of a pool that is compacted: likewise
+constexpr int kMostPool = 1 << 19;   // pages of a pool that is compacted: likewise, and a sum for 32
 
 struct PagesArgs {
   const int32_t* parents;  // fork: [n] table lines

@@ -54,9 +54,31 @@ struct Looked {
 // one after the other (224 forks of up to 250 pages move 0.5 MB).
 constexpr int kForkThreads = 256;
 
+// What a workgroup's own entry is, and (asked for before it is known whether the call
+// can be made) its thread's first page.
+struct Mine {
+  int tokens, held;
+  const int32_t* line;
+  int id0;
+};
+
+__device__ __forceinline__ Mine mine_of(const PagesArgs& a, const int32_t* lines) {
+  const int me = blockIdx.x;
+  Mine m{-1, 0, a.table, -1};
+  if (me >= a.n) return m;
+  m.tokens = a.tokens[me];
+  const int line = lines[me];
+  if (m.tokens <= 0 || line < 0 || line >= a.num_lines) return m;
+  m.held = page_index(a.pd, m.tokens - 1) + 1;
+  m.line = a.table + (int64_t)line * a.table_ld;
+  if ((int)threadIdx.x < m.held && m.held <= a.table_ld) m.id0 = m.line[threadIdx.x];
+  return m;
+}
+
 __global__ __launch_bounds__(kForkThreads) void pages_fork(PagesArgs a) {
   const int tid = threadIdx.x, me = blockIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ Looked<kForkThreads> s;
+  const Mine mine = mine_of(a, a.parents);
   for (int i = tid; i < (a.num_lines + 31) / 32; i += kForkThreads) s.marked[i] = 0;
   const int head = a.free_state[0], avail = a.free_state[1];
   __syncthreads();
@@ -105,38 +127,34 @@ __global__ __launch_bounds__(kForkThreads) void pages_fork(PagesArgs a) {
     a.status[4] = code ? avail : avail - part;
   }
   if (me >= a.n) return;
-  const int tokens = a.tokens[me];
-  if (code || tokens < 0) {
+  if (code || mine.tokens < 0) {
     if (tid == 0) a.src[me] = a.dst[me] = -1;
     return;
   }
-  const int32_t* from = a.table + (int64_t)a.parents[me] * a.table_ld;
   int32_t* to = a.table_out + (int64_t)a.lines[me] * a.table_ld;
-  const int full = page_index(a.pd, tokens);
+  const int full = page_index(a.pd, mine.tokens);
   for (int j = tid; j < full; j += kForkThreads) {
-    const int id = from[j];
+    const int id = j == tid ? mine.id0 : mine.line[j];
     to[j] = id;
     if (id >= 0 && id < a.num_pages) atomicAdd(a.shares + id, 1);
   }
   if (tid == 0) {
-    const bool has_part = tokens > full * a.pd.page;
+    const bool has_part = mine.held > full;
     const int id = has_part ? a.free_pages[queue_at(head, before, a.num_pages)] : -1;
     if (has_part) to[full] = id;
-    a.src[me] = has_part ? from[full] : -1;
+    a.src[me] = has_part ? mine.line[full] : -1;
     a.dst[me] = id;
   }
 }
 
-// Ended lines, a workgroup each: every page of theirs loses a holder. A page that had
-// none beside this one is at -1 afterwards, which pages_gather looks for.
-__global__ __launch_bounds__(kForkThreads) void pages_drop(PagesArgs a) {
-  const int tid = threadIdx.x, me = blockIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ Looked<kForkThreads> s;
-  for (int i = tid; i < (a.num_lines + 31) / 32; i += kForkThreads) s.marked[i] = 0;
-  const int head = a.free_state[0], avail = a.free_state[1];
+// Whether lines can be given back: the code, the same in every thread.
+template <int THREADS>
+__device__ __forceinline__ int free_code(const PagesArgs& a, Looked<THREADS>& s, int head, int avail) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < (a.num_lines + 31) / 32; i += THREADS) s.marked[i] = 0;
   __syncthreads();
   int codes = bad_state(head, avail, a.num_pages) ? 1 << kBad : 0, pages = 0;
-  for (int i = tid; i < a.n; i += kForkThreads) {
+  for (int i = tid; i < a.n; i += THREADS) {
     const int tokens = a.tokens[i], c = a.lines[i];
     if (tokens < 0) continue;
     if (c < 0 || c >= a.num_lines) {
@@ -157,49 +175,62 @@ __global__ __launch_bounds__(kForkThreads) void pages_drop(PagesArgs a) {
   __syncthreads();
   codes = pages = 0;
 #pragma unroll
-  for (int w = 0; w < kForkThreads / 64; ++w) {
+  for (int w = 0; w < THREADS / 64; ++w) {
     codes |= s.codes[w];
     pages = (int)min((uint32_t)pages + (uint32_t)s.pages[w], 0x7fffffffu);
   }
   const int code = codes ? __ffs(codes) - 1 : 0;
-  if (me == 0 && tid == 0) a.status[0] = code, a.status[2] = code ? 0 : pages;
-  if (code || me >= a.n || a.tokens[me] <= 0) return;
-  const int32_t* line = a.table + (int64_t)a.lines[me] * a.table_ld;
-  const int held = page_index(a.pd, a.tokens[me] - 1) + 1;
-  for (int j = tid; j < held; j += kForkThreads) {
-    const int id = line[j];
+  if (blockIdx.x == 0 && tid == 0) a.status[0] = code, a.status[2] = code ? 0 : pages;
+  return code;
+}
+
+// Ended lines, a workgroup each: every page of theirs loses a holder. A page that had
+// none beside this one is at -1 afterwards, which gather() looks for.
+__global__ __launch_bounds__(kForkThreads) void pages_drop(PagesArgs a) {
+  __shared__ Looked<kForkThreads> s;
+  const Mine mine = mine_of(a, a.lines);
+  if (free_code(a, s, a.free_state[0], a.free_state[1])) return;
+  for (int j = threadIdx.x; j < mine.held; j += kForkThreads) {
+    const int id = j == (int)threadIdx.x ? mine.id0 : mine.line[j];
     if (id >= 0 && id < a.num_pages) atomicSub(a.shares + id, 1);
   }
 }
 
 // The pages without a holder, in ascending order, to the queue's end. One workgroup,
-// a wave for each sixteenth of the pool: counted, then written.
+// a wave for each sixteenth of the pool: counted, then written. SAME: the launch that
+// dropped them, so that the counts are read where its atomics work, past the caches.
 constexpr int kGatherThreads = 1024;
 
-__global__ __launch_bounds__(kGatherThreads) void pages_gather(PagesArgs a) {
+template <bool SAME>
+__device__ __forceinline__ void gather(const PagesArgs& a, int code, int head, int avail) {
   constexpr int kWaves = kGatherThreads / 64, kAhead = 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int head = a.free_state[0], avail = a.free_state[1];
-  if (a.status[0]) {
-    if (tid == 0) a.status[1] = 0, a.status[3] = head, a.status[4] = avail;
-    return;
-  }
   __shared__ int s_count[kWaves];
   // Rounds of 64 pages; the first `rounds % kWaves` waves have one more.
   const int rounds = (a.num_pages + 63) / 64;
   const int r0 = wave * (rounds / kWaves) + min(wave, rounds % kWaves), r1 = r0 + rounds / kWaves + (wave < rounds % kWaves ? 1 : 0);
-  // f(round, this lane's page, those of the round without a holder)
-  const auto each = [&](auto f) {
-    for (int r = r0; r < r1; r += kAhead) {
-      int v[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) v[i] = r + i < r1 && 64 * (r + i) + lane < a.num_pages ? a.shares[64 * (r + i) + lane] : 0;
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) f(64 * (r + i) + lane, __ballot(v[i] < 0));
-    }
+  const auto holders = [&](int p) {
+    return SAME ? __hip_atomic_load(a.shares + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : a.shares[p];
   };
+  // The pages of kAhead rounds from r on without a holder.
+  const auto look = [&](int r, uint64_t* free) __attribute__((always_inline)) {
+    int v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) v[i] = r + i < r1 && 64 * (r + i) + lane < a.num_pages ? holders(64 * (r + i) + lane) : 0;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) free[i] = __ballot(v[i] < 0);
+  };
+  uint64_t free[kAhead] = {};
   int count = 0;
-  each([&](int, uint64_t free) { count += __popcll(free); });
+  for (int r = r0; r < r1; r += kAhead) {
+    look(r, free);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) count += __popcll(free[i]);
+  }
+  if (code) {  // nothing was dropped
+    if (tid == 0) a.status[1] = 0, a.status[3] = head, a.status[4] = avail;
+    return;
+  }
   if (lane == 0) s_count[wave] = count;
   __syncthreads();
   int at = 0, total = 0;
@@ -216,38 +247,64 @@ __global__ __launch_bounds__(kGatherThreads) void pages_gather(PagesArgs a) {
     a.status[4] = fits ? avail + total : avail;
   }
   if (count == 0) return;
-  each([&](int p, uint64_t free) {
-    if (free >> lane & 1) {
-      a.shares[p] = 0;
-      if (fits) a.free_pages[queue_at(head, avail + at + __popcll(free & ((1ull << lane) - 1)), a.num_pages)] = p;
+  for (int r = r0; r < r1; r += kAhead) {
+    if (r1 - r0 > kAhead) look(r, free);  // else they are the ones at hand
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int p = 64 * (r + i) + lane;
+      if (free[i] >> lane & 1) {
+        a.shares[p] = 0;
+        if (fits) a.free_pages[queue_at(head, avail + at + __popcll(free[i] & ((1ull << lane) - 1)), a.num_pages)] = p;
+      }
+      at += __popcll(free[i]);
     }
-    at += __popcll(free);
-  });
+  }
+}
+
+__global__ __launch_bounds__(kGatherThreads) void pages_gather(PagesArgs a) {
+  gather<false>(a, a.status[0], a.free_state[0], a.free_state[1]);
+}
+
+// Both for a few short lines, a wave each, in one workgroup and launch: 8 lines of 12
+// pages 3.0 + 2.4 us apart.
+__global__ __launch_bounds__(kGatherThreads) void pages_end(PagesArgs a) {
+  __shared__ Looked<kGatherThreads> s;
+  const int head = a.free_state[0], avail = a.free_state[1];
+  const int code = free_code(a, s, head, avail);
+  if (!code) {
+    for (int i = threadIdx.x >> 6; i < a.n; i += kGatherThreads / 64) {
+      const int tokens = a.tokens[i], held = tokens > 0 ? page_index(a.pd, tokens - 1) + 1 : 0;
+      const int32_t* line = a.table + (held > 0 ? (int64_t)a.lines[i] * a.table_ld : 0);
+      for (int j = threadIdx.x & 63; j < held; j += 64) {
+        const int id = line[j];
+        if (id >= 0 && id < a.num_pages) atomicSub(a.shares + id, 1);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the counts are down before the barrier (a device fence took 3 us more)
+  }
+  __syncthreads();
+  gather<true>(a, code, head, avail);
 }
 
 // ------------------------------------------------------------------ compact
 
-// The free pages as bits, and how many are free below each run of kRun.
-constexpr int kRun = 256;
-
+// The free pages as bits, 32 a word, and how many are free below each word.
 struct FreeBits {
   uint32_t bits[kMostPool / 32];
-  int below[kMostPool / kRun + 1];
+  int below[kMostPool / 32 + 1];
   int sums[16];
   int code;
 };
 
 // Free pages with an id below p.
 __device__ __forceinline__ int free_below(const FreeBits& s, int p) {
-  int c = s.below[p / kRun];
-  for (int w = p / kRun * (kRun / 32); w < p / 32; ++w) c += __popc(s.bits[w]);
-  return (p & 31) ? c + __popc(s.bits[p >> 5] & ((1u << (p & 31)) - 1)) : c;
+  return (p & 31) ? s.below[p >> 5] + __popc(s.bits[p >> 5] & ((1u << (p & 31)) - 1)) : s.below[p >> 5];
 }
 
 // The k-th free page (k from 0; there is one).
-__device__ __forceinline__ int nth_free(const FreeBits& s, int k, int runs) {
-  int lo = 0, hi = runs - 1;
-  while (lo < hi) {  // the last run with at most k free pages before it
+__device__ __forceinline__ int nth_free(const FreeBits& s, int k, int words) {
+  int lo = 0, hi = words - 1;
+  while (lo < hi) {  // the last word with at most k free pages before it
     const int mid = (lo + hi + 1) >> 1;
     if (s.below[mid] <= k)
       lo = mid;
@@ -255,45 +312,56 @@ __device__ __forceinline__ int nth_free(const FreeBits& s, int k, int runs) {
       hi = mid - 1;
   }
   k -= s.below[lo];
-  int w = lo * (kRun / 32);
-  for (int c = __popc(s.bits[w]); k >= c; c = __popc(s.bits[w])) k -= c, ++w;
-  uint32_t b = s.bits[w];
-  for (; k > 0; --k) b &= b - 1;
-  return 32 * w + __ffs(b) - 1;
+  const uint32_t b = s.bits[lo];
+  int at = 0;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {  // the lower half holds the k-th bit, or it is that many bits on in the upper
+    const int c = __popc(b >> at & ((1u << d) - 1));
+    if (k >= c) k -= c, at += d;
+  }
+  return 32 * lo + at;
 }
 
 // The k-th page in use from `limit` on moves to the k-th free page below it. Every
 // workgroup reads the free queue into bits of its own, and then maps its share of the
-// table, the holders and the queue: one launch.
+// table, the holders and the queue: one launch, bound by its chain (state, queue, bits,
+// sums, search). With the sums by 256 pages in place of 32, a pool of 41,000 pages
+// took 15 us.
 constexpr int kCompactThreads = 1024;
 
 __global__ __launch_bounds__(kCompactThreads) void pages_compact(CompactArgs a) {
+  constexpr int kAhead = 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t first = (int64_t)blockIdx.x * kCompactThreads + tid, step = (int64_t)gridDim.x * kCompactThreads;
   __shared__ FreeBits s;
-  const int runs = (a.num_pages + kRun - 1) / kRun, words = runs * (kRun / 32);
+  const int words = (a.num_pages + 31) / 32;
   const int head = a.free_state[0], avail = a.free_state[1];
+  // This thread's first page and cell, needed last: asked for now.
+  const int held0 = first < a.num_pages ? a.shares[first] : 0, cell0 = first < a.cells ? a.table[first] : 0;
   for (int i = tid; i < words; i += kCompactThreads) s.bits[i] = 0;
   if (tid == 0) s.code = 0;
   __syncthreads();
   bool bad = bad_state(head, avail, a.num_pages);
   if (!bad)
-    for (int k = tid; k < avail; k += kCompactThreads) {
-      const int id = a.free_pages[queue_at(head, k, a.num_pages)];
-      if (id < 0 || id >= a.num_pages || (atomicOr(&s.bits[id >> 5], 1u << (id & 31)) >> (id & 31) & 1)) bad = true;
+    for (int k0 = tid; k0 < avail; k0 += kAhead * kCompactThreads) {
+      int id[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int k = k0 + i * kCompactThreads;
+        id[i] = k < avail ? a.free_pages[queue_at(head, k, a.num_pages)] : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (k0 + i * kCompactThreads >= avail) break;
+        if (id[i] < 0 || id[i] >= a.num_pages || (atomicOr(&s.bits[id[i] >> 5], 1u << (id[i] & 31)) >> (id[i] & 31) & 1)) bad = true;
+      }
     }
   if (bad) s.code = kBad;
   __syncthreads();
-  // Free pages before each run: four runs a thread, 4096 in all.
-  int c[4], sum = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 4 * tid + i;
-    c[i] = 0;
-    if (r < runs)
-      for (int w = 0; w < kRun / 32; ++w) c[i] += __popc(s.bits[r * (kRun / 32) + w]);
-    sum += c[i];
-  }
+  // Free pages before each word: so many words a thread.
+  const int per = (words + kCompactThreads - 1) / kCompactThreads, w0 = tid * per, w1 = min(w0 + per, words);
+  int sum = 0;
+  for (int w = w0; w < w1; ++w) sum += __popc(s.bits[w]);
   int at = sum;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -303,13 +371,13 @@ __global__ __launch_bounds__(kCompactThreads) void pages_compact(CompactArgs a) 
   if (lane == 63) s.sums[wave] = at;
   __syncthreads();
   at -= sum;
-  for (int w = 0; w < wave; ++w) at += s.sums[w];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (4 * tid + i <= runs) s.below[4 * tid + i] = at;
-    at += c[i];
+  for (int w = 0; w < kCompactThreads / 64; ++w) at += w < wave ? s.sums[w] : 0;
+  for (int w = w0; w < w1; ++w) {
+    s.below[w] = at;
+    at += __popc(s.bits[w]);
   }
-  if (tid == kCompactThreads - 1 && runs == 4 * kCompactThreads) s.below[runs] = at;
+  if (w0 < words && w1 == words) s.below[words] = at;
   __syncthreads();
 
   const int holes = free_below(s, a.limit);
@@ -326,7 +394,7 @@ __global__ __launch_bounds__(kCompactThreads) void pages_compact(CompactArgs a) 
   }
   const auto is_free = [&](int p) { return s.bits[p >> 5] >> (p & 31) & 1; };
   // Where page p, in use, is afterwards.
-  const auto moved = [&](int p) { return p < a.limit ? p : nth_free(s, p - a.limit - (free_below(s, p) - holes), runs); };
+  const auto moved = [&](int p) { return p < a.limit ? p : nth_free(s, p - a.limit - (free_below(s, p) - holes), words); };
   for (int64_t i = (code ? 0 : moves) + first; i < a.cap; i += step) a.src[i] = a.dst[i] = -1;
   if (code) return;
   for (int64_t i = first; i < a.num_pages; i += step) {
@@ -344,7 +412,7 @@ __global__ __launch_bounds__(kCompactThreads) void pages_compact(CompactArgs a) 
     } else {
       const int to = moved(p);
       a.new_ids[p] = to;
-      a.shares_out[to] = a.shares[p];
+      a.shares_out[to] = i == first ? held0 : a.shares[p];
       if (p >= a.limit) {
         a.src[p - a.limit - (free_below(s, p) - holes)] = p;
         a.free_out[holes - moves + (p - a.limit)] = p, a.shares_out[p] = 0;
@@ -353,7 +421,7 @@ __global__ __launch_bounds__(kCompactThreads) void pages_compact(CompactArgs a) 
   }
   for (int64_t i = avail + first; i < a.num_pages; i += step) a.free_out[i] = -1;
   for (int64_t i = first; i < a.cells; i += step) {
-    const int id = a.table[i];
+    const int id = i == first ? cell0 : a.table[i];
     a.table_out[i] = id >= a.limit && id < a.num_pages && !is_free(id) ? moved(id) : id;
   }
 }
@@ -399,7 +467,14 @@ int launch_pages_fork(const PagesArgs& a, hipStream_t stream) {
   return check_launch();
 }
 
+// Entries (of all lines, at most) that one workgroup takes back by itself.
+constexpr int64_t kFewEntries = 4096;
+
 int launch_pages_free(const PagesArgs& a, hipStream_t stream) {
+  if ((int64_t)a.n * a.table_ld <= kFewEntries) {
+    pages_end<<<1, kGatherThreads, 0, stream>>>(a);
+    return check_launch();
+  }
   pages_drop<<<dim3((unsigned)std::max(a.n, 1)), kForkThreads, 0, stream>>>(a);
   if (check_launch() != 0) return -3;
   pages_gather<<<1, kGatherThreads, 0, stream>>>(a);

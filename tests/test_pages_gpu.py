@@ -213,9 +213,9 @@ def test_compact(total, keep):
 
 
 def test_compact_of_a_pool_as_large_as_one_may_be():
-    """2^20 pages: every bit of the map is in use."""
+    """2^19 pages: every bit of the map is in use."""
     rng = np.random.default_rng(8)
-    total = 1 << 20
+    total = 1 << 19
     pool = Pool(rng, [total // 2], 1, total - total // 2, 0)
     pool.upload()
     assert compact(pool, total // 2 + 1000, total // 2)[0][0] == 0

@@ -62,7 +62,7 @@ def test_compact_refusals(bad):
 
 
 def test_compact_limits():
-    assert compact(num_pages=(1 << 20) + 1) == oa.EUNSUPPORTED
+    assert compact(num_pages=(1 << 19) + 1) == oa.EUNSUPPORTED
 
 
 def copy(**k):
