@@ -1181,7 +1181,7 @@ void write_tile_list(const std::vector<std::array<int32_t, 4>>& tl, int G, const
       units.push_back({(int32_t)t, k, n, segment + k, which, (tl[t][2] * G <= 128 ? 2.4 : 3.9) * std::min(per, steps - k * per)});
     if (n == 1) continue;
     for (int32_t h = 0; h < p.hk; ++h) {
-      *items++ = tl[t][1], *items++ = tl[t][2], *items++ = h;
+      *items++ = tl[t][1], *items++ = (int32_t)((uint32_t)n << 9 | (uint32_t)tl[t][2]), *items++ = h;
       *items++ = segment * p.hk + h * n;
     }
     segment += n, ++which;
@@ -1318,7 +1318,7 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
     units += n;
     if (n > 1) segments += n, ++plan->split_tiles;
   }
-  if (units > INT_MAX) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many tiles", who);
+  if (units > INT_MAX || plan->max_len / plan->tile_chunk >= 1 << 22) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many tiles", who);
   plan->tile_units = (int32_t)units;
   plan->tile_segments = (int32_t)segments;
   if (!multi_fits(*plan)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, plan->rows, hq, plan->splits);

@@ -987,15 +987,23 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
 constexpr int kCombineRows = 16;
 constexpr int kCombineBatch = 8;
 
-// Packed row r of a segment list: nk chunks' partials, merged, to 8 values of `out`.
-__device__ __forceinline__ void combine_row(const float* seg0, int nk, int r, int d0, bf16_t* out) {
+__global__ __launch_bounds__(256) void dit_combine(TiledArgs a, int ntiles) {
+  const int idx = a.split_from + blockIdx.x;
+  const int G = a.hq / a.hk, kpos = kBM / G;
+  const int tile = idx % ntiles, kvh = (idx / ntiles) % a.hk, b = idx / (ntiles * a.hk);
+  const int q0 = tile * kpos, nq = min(kpos, a.q_len - q0);
+  const int r = blockIdx.y * kCombineRows + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
+  const int p = r / G, head = kvh * G + r % G;
+  if (p >= nq) return;
   constexpr int kSeg = kBM * (kHead + 2);
+  const int nk = a.split_k;
+  const float* seg0 = a.ws + (int64_t)(blockIdx.x * nk) * kSeg;
   const float* ml0 = seg0 + kBM * kHead + 2 * r;  // chunk c's (m, l) at ml0 + c * kSeg
   float top = -INFINITY;
   for (int c0 = 0; c0 < nk; c0 += kCombineBatch) {
     float m[kCombineBatch];
 #pragma unroll
-    for (int i = 0; i < kCombineBatch; ++i) m[i] = ml0[(int64_t)min(c0 + i, nk - 1) * kSeg];
+    for (int i = 0; i < kCombineBatch; ++i) m[i] = ml0[min(c0 + i, nk - 1) * kSeg];
 #pragma unroll
     for (int i = 0; i < kCombineBatch; ++i) top = fmaxf(top, m[i]);  // a repeated chunk changes no max
   }
@@ -1006,7 +1014,7 @@ __device__ __forceinline__ void combine_row(const float* seg0, int nk, int r, in
     float4 v0[kCombineBatch], v1[kCombineBatch];
 #pragma unroll
     for (int i = 0; i < kCombineBatch; ++i) {
-      const float* seg = seg0 + (int64_t)min(c0 + i, nk - 1) * kSeg;
+      const float* seg = seg0 + min(c0 + i, nk - 1) * kSeg;
       ml[i] = *reinterpret_cast<const float2*>(seg + kBM * kHead + 2 * r);
       v0[i] = *reinterpret_cast<const float4*>(seg + r * kHead + d0);
       v1[i] = *reinterpret_cast<const float4*>(seg + r * kHead + d0 + 4);
@@ -1033,38 +1041,65 @@ __device__ __forceinline__ void combine_row(const float* seg0, int nk, int r, in
   o.y = pack_bf16x2(num[2] * inv, num[3] * inv);
   o.z = pack_bf16x2(num[4] * inv, num[5] * inv);
   o.w = pack_bf16x2(num[6] * inv, num[7] * inv);
-  *reinterpret_cast<uint4*>(out) = o;
+  *reinterpret_cast<uint4*>(a.out + b * a.out_bstride + ((int64_t)(q0 + p) * a.hq + head) * kHead + d0) = o;
 }
 
-__global__ __launch_bounds__(256) void dit_combine(TiledArgs a, int ntiles) {
-  const int idx = a.split_from + blockIdx.x;
-  const int G = a.hq / a.hk, kpos = kBM / G;
-  const int tile = idx % ntiles, kvh = (idx / ntiles) % a.hk, b = idx / (ntiles * a.hk);
-  const int q0 = tile * kpos, nq = min(kpos, a.q_len - q0);
-  const int r = blockIdx.y * kCombineRows + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
-  const int p = r / G, head = kvh * G + r % G;
-  if (p >= nq) return;
-  combine_row(a.ws + (int64_t)blockIdx.x * a.split_k * (kBM * (kHead + 2)), a.split_k, r, d0,
-              a.out + b * a.out_bstride + ((int64_t)(q0 + p) * a.hq + head) * kHead + d0);
-}
-
-// The same for calls of several rows per sequence, over the work list's split tiles
-// (first row, rows, kv head and first segment; the segments of a tile's splits follow
-// one another). Rows without keys have none that weighs: zeros.
+// The splits of tiles of several rows per sequence, merged: workgroups, rows and dims
+// as in dit_combine, over the work list's split tiles (first row, rows and splits, kv
+// head, first segment; the segments of a tile's splits follow one another). One pass
+// with a running base, the first batch asked for before it is known how many splits
+// were used. Rows without keys have none that weighs: zeros.
 template <bool Q8>
 __global__ __launch_bounds__(256) void multi_combine(TiledArgs a) {
+  constexpr int kSeg = kBM * (kHead + 2);
   const int idx = blockIdx.x, G = a.hq / a.hk;
   const int used = a.used[idx];
   const int4 item = reinterpret_cast<const int4*>(a.split_items)[idx];
-  if (used <= 1) return;
+  const int rows = item.y & 0x1ff, splits = (int)((uint32_t)item.y >> 9);
   const int r = blockIdx.y * kCombineRows + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
   const int p = r / G, head = item.z * G + r % G;
-  if (p >= item.y) return;
-  bf16_t* out = a.out + ((int64_t)(item.x + p) * a.hq + head) * kHead + d0;
-  if (Q8 && a.pos[item.x + p] < 0)
-    *reinterpret_cast<uint4*>(out) = make_uint4(0, 0, 0, 0);
-  else
-    combine_row(a.ws + (int64_t)item.w * (kBM * (kHead + 2)), used, r, d0, out);
+  if (p >= rows) return;
+  const bool none = Q8 && a.pos[item.x + p] < 0;
+  const float* seg0 = a.ws + (int64_t)item.w * kSeg;
+  float num[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float den = 0.f, top = -INFINITY;
+  for (int c0 = 0; c0 < used || c0 == 0; c0 += kCombineBatch) {
+    float2 ml[kCombineBatch];
+    float4 v[kCombineBatch][2];
+#pragma unroll
+    for (int i = 0; i < kCombineBatch; ++i) {
+      if (c0 + i >= splits) continue;  // uniform
+      const float* seg = seg0 + (int64_t)(c0 + i) * kSeg;
+      ml[i] = *reinterpret_cast<const float2*>(seg + kBM * kHead + 2 * r);
+      v[i][0] = *reinterpret_cast<const float4*>(seg + r * kHead + d0);
+      v[i][1] = *reinterpret_cast<const float4*>(seg + r * kHead + d0 + 4);
+    }
+    if (c0 == 0 && used <= 1) return;
+    float mx = top;
+#pragma unroll
+    for (int i = 0; i < kCombineBatch; ++i) mx = c0 + i < used ? fmaxf(mx, ml[i].x) : mx;
+    const float base = mx == -INFINITY ? 0.f : mx, alpha = fast_exp2(top - base);
+    top = mx;
+    den *= alpha;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) num[e] *= alpha;
+#pragma unroll
+    for (int i = 0; i < kCombineBatch; ++i)
+      if (c0 + i < used) {  // what was asked for beyond may be anything
+        const float w = fast_exp2(ml[i].x - base);
+        den = fmaf(ml[i].y, w, den);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) num[e] = fmaf((&v[i][e >> 2].x)[e & 3], w, num[e]);
+      }
+  }
+  const float inv = 1.f / den;
+  uint4 o;
+  o.x = pack_bf16x2(num[0] * inv, num[1] * inv);
+  o.y = pack_bf16x2(num[2] * inv, num[3] * inv);
+  o.z = pack_bf16x2(num[4] * inv, num[5] * inv);
+  o.w = pack_bf16x2(num[6] * inv, num[7] * inv);
+  if (none) o = make_uint4(0, 0, 0, 0);
+  *reinterpret_cast<uint4*>(a.out + ((int64_t)(item.x + p) * a.hq + head) * kHead + d0) = o;
 }
 
 // Prefill with exact_p set: the hi + lo P.V variant (prefill only; DiT rounds

@@ -189,7 +189,7 @@ def check_tiles(mp, counts, keys, causal):
         seen.setdefault((first, rows, head, n), []).append(k)
         if n > 1:
             assert segments.setdefault(seg, (first, head, k)) == (first, head, k) and 0 <= seg < p.tile_segments * p.hk
-            assert tuple(split[at]) == (first, rows, head, seg - k)
+            assert tuple(split[at]) == (first, rows + 512 * n, head, seg - k)
             which[at] = True
     assert all(sorted(ks) == list(range(n)) for (_, _, _, n), ks in seen.items())
     covered = np.zeros((sum(counts), p.hk), int)
