@@ -1266,13 +1266,20 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   if (G > 16) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: hq/hk=%d above 16", who, G);
   if (max_len <= 0) return fail(OMNI_ATTN_EINVAL, "%s: max_len=%d", who, max_len);
   if (chunk_hint > 0 && chunk_hint % 64 != 0) return fail(OMNI_ATTN_EINVAL, "%s: chunk=%d is not a multiple of 64", who, chunk_hint);
-  int64_t rows = 0;
+  const int small = rows_of_group(16, G), large = rows_of_group(32, G), per_tile = omni::kTiledRows / G;
+  const bool tiled = G == 1 || G == 2 || G == 4 || G == 8;
+  int64_t rows = 0, group_count = 0, tile_count = 0;
   for (int s = 0; s < nseq; ++s) {
     if (counts_h[s] < 0) return fail(OMNI_ATTN_EINVAL, "%s: %d rows of sequence %d", who, counts_h[s], s);
     if (keys_h && keys_h[s] < 0) return fail(OMNI_ATTN_EINVAL, "%s: %d keys of sequence %d", who, keys_h[s], s);
     rows += counts_h[s];
+    if (tiled && counts_h[s] > large)
+      tile_count += ((int64_t)counts_h[s] + per_tile - 1) / per_tile;
+    else
+      group_count += ((int64_t)counts_h[s] + large - 1) / large;
   }
-  if (rows > INT_MAX || rows * hq > (int64_t)INT_MAX * 8) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many rows", who);
+  if (rows > INT_MAX || !omni::grid_holds(group_count * hk, omni::kRowsThreads) || !omni::grid_holds(tile_count * hk, omni::kTiledThreads))
+    return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many rows", who);
   plan->cross = cross;
   plan->nseq = nseq;
   plan->rows = (int32_t)rows;
@@ -1284,16 +1291,12 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   // than 32 packed rows. Groups: the same, of at most 16 packed rows where what is left
   // of a sequence fits, else 32.
   std::vector<std::array<int32_t, 4>> groups[2], tl;
-  const int small = rows_of_group(16, G), large = rows_of_group(32, G);
-  const bool tiled = G == 1 || G == 2 || G == 4 || G == 8;
-  const int per_tile = omni::kTiledRows / G;
   for (int32_t s = 0, at = 0; s < nseq; at += counts_h[s++]) {
     if (tiled && counts_h[s] > large) {
       for (int32_t f = 0; f < counts_h[s]; f += per_tile) {
         const int32_t n = std::min(per_tile, counts_h[s] - f);
         tl.push_back({s, at + f, n, std::max((keys_h ? keys_h[s] : max_len) - (cross ? 0 : counts_h[s] - f - n), 0)});
       }
-      if (tl.size() > (size_t)INT_MAX / 8) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many tiles", who);
       continue;
     }
     for (int32_t f = 0; f < counts_h[s];) {
@@ -1304,7 +1307,6 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
     }
   }
   for (int c = 0; c < 2; ++c) {
-    if (groups[c].size() > (size_t)INT_MAX) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many groups", who);
     plan->groups[c] = (int32_t)groups[c].size();
     std::stable_sort(groups[c].begin(), groups[c].end(), [](const auto& x, const auto& y) { return x[3] > y[3]; });
   }

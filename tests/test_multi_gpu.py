@@ -348,6 +348,34 @@ def test_cross_scales_on_another_stream(scale):
     cross(5, [3, 20], [200, 40], 2, 1, scale=scale, stream=torch.cuda.Stream())
 
 
+def test_the_mirror_refuses_what_the_kernels_do_not_take():
+    hq, hk = 4, 2
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")
+    kv, sc = oa.q8_cache(4, 16, hk)
+    z = i32([0] * 8)
+
+    def refused(f, *a):
+        with pytest.raises(oa.OmniAttnError):
+            f(*a)
+
+    e, x = oa.extend_plan([2, 1], hq, hk, 300, chunk=64), oa.cross_plan([2, 1], hq, hk, 300, chunk=64)
+    ws = oa.workspace_for(e.plan)
+    good = [e, b(3, 512), kv, sc, z[:3], z[:3], z, 16, b(3, 512), SCALE, ws]
+    oa.qwen3_extend_q8(*good)
+    for at, bad in ((0, x), (1, b(2, 512)), (1, b(3, 256)), (1, b(3, 512).float()), (2, kv.view(torch.uint8)), (2, kv[:, :2]), (3, sc[:3]),
+                    (3, sc.cpu()), (4, z[:2]), (5, z[:2]), (5, z[:3].long()), (7, 24), (8, b(2, 512)), (8, b(512, 3).t()), (10, ws[:-1]), (10, None),
+                    (10, ws.cpu()), (0, oa.Multi(e.plan, e.work[:4])), (1, b(3, 516)[:, 2:514])):
+        refused(oa.qwen3_extend_q8, *good[:at], bad, *good[at + 1:])
+    ws = oa.workspace_for(x.plan)
+    good = [x, b(3, 512), b(9, 256), b(9, 256), z[:2], z[:5], z[:5], b(3, 512), SCALE, ws]
+    oa.cross_run(*good)
+    for at, bad in ((0, e), (1, b(2, 512)), (2, b(9, 128)), (3, b(9, 256).float()), (2, b(256, 9).t()), (4, z[:1]), (5, z[:5].float()), (6, z[:4]),
+                    (7, b(3, 256)), (9, ws[:-1]), (9, None), (0, oa.Multi(x.plan, x.work[:4])), (3, b(9, 260)[:, 2:258])):
+        refused(oa.cross_run, *good[:at], bad, *good[at + 1:])
+    refused(oa.cross_run, x, b(3, 512), b(9, 256), b(9, 256), None, z[:1], z[:5], b(3, 512), SCALE, ws)  # a source for each sequence
+    torch.cuda.synchronize()
+
+
 def test_no_rows_and_no_sequences():
     for counts in ([], [0, 0]):
         mp = oa.cross_plan(counts, 4, 2, 10)
@@ -356,6 +384,57 @@ def test_no_rows_and_no_sequences():
         oa.cross_run(mp, q, k, k, None, i32([0, 0]), i32([0, 0]), out, SCALE)
         torch.cuda.synchronize()
         assert bool((out == 7).all())
+
+
+# ------------------------------------------------------------------ odd heads, far offsets
+@pytest.mark.parametrize("hq,hk", [(3, 3), (10, 5), (22, 11)])
+def test_kv_heads_that_are_no_power_of_two(hq, hk):
+    """Few rows and tiles, split and not."""
+    extend(Cache(50 + hk, [900, 200, 70], hk, 16, torch.int8), [3, 70, 40], hq)
+    extend(Cache(51 + hk, [2600, 700], hk, 16, torch.float8_e4m3fn), [40, 3], hq)
+    cross(52 + hk, [3, 70, 40], [900, 200, 70], hq, hk)
+    cross(53 + hk, [40, 3], [2600, 700], hq, hk)
+
+
+def test_extend_past_32_bits():
+    """Blocks at the end of a cache of 4.5 GiB."""
+    hk, blocks = 8, 147_500
+    kv = torch.zeros(blocks, 2 * hk, 2048, dtype=torch.int8, device="cuda")
+    sc = torch.full((blocks, 2 * hk), 120, dtype=torch.uint8, device="cuda")
+    n = 12
+    g = torch.Generator(device="cuda").manual_seed(3)
+    kv[-n:] = torch.randint(-127, 128, kv[-n:].shape, dtype=torch.int8, device="cuda", generator=g)
+    small_kv, small_sc = kv[-n:].clone(), sc[-n:].clone()
+    q = bf16(g, 40, 16 * 128)
+    for counts, lens in (([3, 2], [100, 90]), ([37, 3], [100, 90])):
+        rows = sum(counts)
+        pos = i32([l - c + i for l, c in zip(lens, counts) for i in range(c)])
+        out = torch.zeros(2, rows, 16 * 128, dtype=torch.bfloat16, device="cuda")
+        for i, (k, s, first) in enumerate(((kv, sc, blocks - n), (small_kv, small_sc, 0))):
+            mp = oa.extend_plan(counts, 16, hk, 100, lens)
+            pages = i32([first + x for x in (7, 3, 11, 0, 9, 1, 2, 4, 5, 6, 8, 10, 11)])
+            oa.qwen3_extend_q8(mp, q, k, s, pos, i32([0, 7, 13]), pages, 16, out[i], SCALE, oa.workspace_for(mp.plan))
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], out[1]) and bool(out[0].any())
+
+
+def test_cross_past_32_bits():
+    """Sources behind 5 GiB of k and v rows."""
+    hk, total, n = 8, 1_250_000, 300
+    kv = torch.zeros(total, 2 * hk * 128, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    kv[-n:] = bf16(g, n, 2 * hk * 128)
+    small = kv[-n:].clone()
+    q = bf16(g, 40, 16 * 128)
+    for counts in ([3, 2], [37, 3]):
+        rows = sum(counts)
+        out = torch.zeros(2, rows, 16 * 128, dtype=torch.bfloat16, device="cuda")
+        for i, (x, first) in enumerate(((kv, total - n), (small, 0))):
+            mp = oa.cross_plan(counts, 16, hk, 200, [200, 100])
+            oa.cross_run(mp, q, x[:, :hk * 128], x[:, hk * 128:], None, i32([first, first + 200]), i32([200, 100]), out[i], SCALE,
+                         oa.workspace_for(mp.plan))
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], out[1]) and bool(out[0].any())
 
 
 # ------------------------------------------------------------------ graphs

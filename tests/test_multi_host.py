@@ -1,5 +1,8 @@
 """Plans of extend and cross attention, and what the calls refuse before any launch (CPU)."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -247,3 +250,36 @@ def test_plans_of_tiles_that_do_not_agree(field, by):
         assert plan.split_tiles > 0
         setattr(plan, field, getattr(plan, field) + by)
         assert call(plan, ws=P) == oa.EINVAL
+
+
+NO_MEMORY = """
+import ctypes, resource, sys
+import numpy as np
+import omni_attn as oa
+L = oa.load()
+p = lambda a: a.ctypes.data_as(ctypes.c_void_p)
+f = getattr(L, "omni_attn_%s_plan_init" % sys.argv[1])
+counts, plan = np.full(1 << 21, 3, np.int32), oa.MultiPlan()
+work = np.zeros(4 << 21, np.int32)
+size = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize() + (4 << 20)
+resource.setrlimit(resource.RLIMIT_AS, (size, size))
+rc = f(len(counts), p(counts), None, 3, 1, 100, 0, p(work), len(work), ctypes.byref(plan))
+assert rc == oa.EUNSUPPORTED and b"memory" in L.omni_attn_last_error(), rc
+print("refused")
+"""
+
+
+@pytest.mark.parametrize("which", ["extend", "cross"])
+def test_plans_without_host_memory_return_an_error(which):
+    """The groups of two million sequences (32 MiB) are host memory; where there is none the C call says so, and throws nothing."""
+    here = os.path.dirname(oa.__file__)
+    r = subprocess.run([sys.executable, "-c", NO_MEMORY, which], capture_output=True, text=True, env={**os.environ, "PYTHONPATH": here})
+    assert r.returncode == 0 and "refused" in r.stdout, (r.returncode, r.stderr[-500:])
+
+
+@pytest.mark.parametrize("make", PLANS)
+def test_counts_that_no_grid_holds_are_refused_before_their_lists_are_made(make):
+    for counts, hq, hk in (([2**31 - 1], 3, 1), ([2**31 - 1], 4, 4), ([10**8], 16, 1), ([1] * 70000, 512, 512)):
+        with pytest.raises(oa.OmniAttnError) as e:
+            make(counts, hq, hk, 100, device="cpu")
+        assert e.value.code == oa.EUNSUPPORTED
