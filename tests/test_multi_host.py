@@ -283,3 +283,15 @@ def test_counts_that_no_grid_holds_are_refused_before_their_lists_are_made(make)
         with pytest.raises(oa.OmniAttnError) as e:
             make(counts, hq, hk, 100, device="cpu")
         assert e.value.code == oa.EUNSUPPORTED
+
+
+def test_the_mirrors_plan_is_the_headers(tmp_path):
+    fields = [f[0] for f in oa.MultiPlan._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "omni_attn.h"\nint main(void) {\n  printf("%zu", sizeof(omni_attn_multi_plan));\n'
+                   + "".join(f'  printf(" %zu", offsetof(omni_attn_multi_plan, {f}));\n' for f in fields) + "  return 0;\n}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    exe = str(tmp_path / "layout")
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-I" + include, str(src), "-o", exe], check=True)
+    got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [ctypes.sizeof(oa.MultiPlan)] + [getattr(oa.MultiPlan, f).offset for f in fields]
