@@ -1256,6 +1256,23 @@ int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, 
   }
 }
 
+// Which kernel takes a sequence. By itself, one of up to 16 packed rows is a group of one
+// column block, up to 32 a group of two, more are tiles. But each of the three is a launch
+// of its own, whose first 5-10 us no other fills, so a call that would mix them runs in
+// one of them where that is faster. Over 500 drawn calls, against three launches:
+//   - groups of 32 alone, where a CU gets one of them at most and they have up to 1024
+//     keys: 4 % less over 63 calls that had tiles (58 sequences of 3-20 rows over 173-1039
+//     keys, 8 heads over 2: 27 -> 17.6 us); with more keys or groups the tiles win, which
+//     read a sequence's keys once for 256 packed rows.
+//   - tiles alone, where the groups' keys are at most kFewKeyBytes (26 us of them) and a CU
+//     gets one tile at most: the 43 us of 13 sequences of 1-10 rows over 650 keys -> 15.
+//   - groups of 32 alone, where nothing is for the tiles and the groups' keys are as few.
+// Together: 141 calls of 500 differ, 0.72 of the time in the mean, the worst 1.11 (7.8 us).
+// A caller who gives a chunk keeps every sequence where its own rows send it.
+constexpr double kFewKeyBytes = 128e6;
+constexpr int kShortKeys = 1024;
+constexpr int kCus = 256;
+
 int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
                     int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan, const char* who) try {
   if (!plan) return fail(OMNI_ATTN_EINVAL, "%s: null plan", who);
@@ -1267,17 +1284,35 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   if (max_len <= 0) return fail(OMNI_ATTN_EINVAL, "%s: max_len=%d", who, max_len);
   if (chunk_hint > 0 && chunk_hint % 64 != 0) return fail(OMNI_ATTN_EINVAL, "%s: chunk=%d is not a multiple of 64", who, chunk_hint);
   const int small = rows_of_group(16, G), large = rows_of_group(32, G), per_tile = omni::kTiledRows / G;
-  const bool tiled = G == 1 || G == 2 || G == 4 || G == 8;
-  int64_t rows = 0, group_count = 0, tile_count = 0;
+  const bool may_tile = G == 1 || G == 2 || G == 4 || G == 8;
+  int64_t rows = 0, group_count = 0, tile_count = 0, if_grouped = 0;
+  double group_keys = 0;
+  int reach = 0;
+  bool large_groups = false;
   for (int s = 0; s < nseq; ++s) {
     if (counts_h[s] < 0) return fail(OMNI_ATTN_EINVAL, "%s: %d rows of sequence %d", who, counts_h[s], s);
     if (keys_h && keys_h[s] < 0) return fail(OMNI_ATTN_EINVAL, "%s: %d keys of sequence %d", who, keys_h[s], s);
     rows += counts_h[s];
-    if (tiled && counts_h[s] > large)
+    const int64_t n = ((int64_t)counts_h[s] + large - 1) / large;
+    const int32_t keys = keys_h ? std::min(keys_h[s], max_len) : max_len;
+    if_grouped += n;
+    if (n > 0) reach = std::max(reach, keys);
+    if (may_tile && counts_h[s] > large) {
       tile_count += ((int64_t)counts_h[s] + per_tile - 1) / per_tile;
-    else
-      group_count += ((int64_t)counts_h[s] + large - 1) / large;
+    } else {
+      group_count += n;
+      group_keys += (double)n * keys;
+      large_groups |= n > 1 || counts_h[s] > small;
+    }
   }
+  const bool may_mix = chunk_hint <= 0;
+  const bool grouped = may_mix && tile_count > 0 && if_grouped * hk <= kCus && reach <= kShortKeys;
+  const bool few_keys = may_mix && group_keys * hk * (cross ? 512 : 256) <= kFewKeyBytes;
+  const bool all_tiles = !grouped && few_keys && tile_count > 0 && (tile_count + group_count) * hk <= kCus;
+  const bool one_size = grouped || (few_keys && large_groups);
+  const int grouped_rows = all_tiles ? 0 : may_tile && !grouped ? large : INT_MAX;
+  if (grouped) group_count = if_grouped, tile_count = 0;
+  if (all_tiles) tile_count += group_count, group_count = 0;
   if (rows > INT_MAX || !omni::grid_holds(group_count * hk, omni::kRowsThreads) || !omni::grid_holds(tile_count * hk, omni::kTiledThreads))
     return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many rows", who);
   plan->cross = cross;
@@ -1287,12 +1322,10 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   plan->hk = hk;
   plan->max_len = max_len;
 
-  // Tiles: (sequence, first row, rows, keys that the last row sees), of sequences of more
-  // than 32 packed rows. Groups: the same, of at most 16 packed rows where what is left
-  // of a sequence fits, else 32.
+  // Tiles: (sequence, first row, rows, keys that the last row sees). Groups: the same.
   std::vector<std::array<int32_t, 4>> groups[2], tl;
   for (int32_t s = 0, at = 0; s < nseq; at += counts_h[s++]) {
-    if (tiled && counts_h[s] > large) {
+    if (counts_h[s] > grouped_rows) {
       for (int32_t f = 0; f < counts_h[s]; f += per_tile) {
         const int32_t n = std::min(per_tile, counts_h[s] - f);
         tl.push_back({s, at + f, n, std::max((keys_h ? keys_h[s] : max_len) - (cross ? 0 : counts_h[s] - f - n), 0)});
@@ -1301,7 +1334,7 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
     }
     for (int32_t f = 0; f < counts_h[s];) {
       const int32_t left = counts_h[s] - f, n = std::min(left, left <= small ? small : large);
-      groups[n > small].push_back({s, at + f, n, keys_h ? keys_h[s] : 0});
+      groups[n > small || one_size].push_back({s, at + f, n, keys_h ? keys_h[s] : 0});
       f += n;
       plan->group_rows += n;
     }

@@ -15,6 +15,7 @@ pytestmark = pytest.mark.gpu
 
 FORMATS = [torch.float8_e4m3fn, torch.int8]
 SCALE = 128 ** -0.5
+APART = 1 << 14  # a chunk: groups unsplit, and sequences of more than 32 packed rows in tiles
 
 
 def i32(a):
@@ -182,7 +183,7 @@ def test_extend_in_tiles(hq, hk, page, fmt):
     g = hq // hk
     counts = [32 // g + 1, 64 // g + 3, 256 // g, 1, 256 // g + 1, 0, 3]
     lens = [counts[0], 129, 256 // g, 70, 256 // g + 128, 5, 300]
-    mp, _ = extend(Cache(hq + page, lens, hk, page, fmt), counts, hq)
+    mp, _ = extend(Cache(hq + page, lens, hk, page, fmt), counts, hq, chunk=APART)
     assert mp.plan.tiles == 5 and sum(mp.plan.groups) == 2
 
 
@@ -193,7 +194,7 @@ def test_extend_in_every_form_of_a_tile(seqs, hk, fmt):
     rng = np.random.default_rng(seqs)
     counts = [int(x) for x in rng.integers(34, 130, seqs)]
     lens = [c + int(x) for c, x in zip(counts, rng.integers(0, 260, seqs))]
-    mp, _ = extend(Cache(seqs, lens, hk, 16, fmt), counts, 2 * hk)
+    mp, _ = extend(Cache(seqs, lens, hk, 16, fmt), counts, 2 * hk, chunk=APART)
     assert mp.plan.tiles * hk in ((2, 96, 320) if seqs < 20 else (320,)) or mp.plan.tiles >= seqs
     assert mp.plan.split_tiles == 0
 
@@ -205,9 +206,10 @@ def test_extend_of_tiles_in_splits(hq, hk, fmt):
     c = Cache(hq, [2600, 700, 90], hk, 16, fmt)
     counts = [70, 40, 40]
     for most in (None, 1100):
-        mp, _ = extend(c, counts, hq, max_len=most, seed=3)
+        mp, _ = extend(c, counts, hq, max_len=most, seed=3, chunk=APART)
         assert mp.plan.split_tiles > 0
     pos = [2599 - 37 * i if i % 3 else -1 for i in range(70)] + [i for i in range(40)] + [-1] * 40
+    extend(c, counts, hq, pos=pos, seed=4, chunk=APART)
     extend(c, counts, hq, pos=pos, seed=4)
 
 
@@ -218,25 +220,27 @@ def test_extend_of_tiles_at_any_positions():
         rng = np.random.default_rng(hk)
         pos = [int(x) for x in rng.integers(-3, 500, n)] + [-1] * 40
         pos[:20] = [-1] * 20
+        extend(c, [n, 40], 4 * hk, pos=pos, chunk=APART)
         extend(c, [n, 40], 4 * hk, pos=pos)
 
 
 @pytest.mark.parametrize("scale", [0.0, -SCALE])
 def test_extend_of_tiles_scales_strides_streams(scale):
     c = Cache(41, [200, 150], 2, 16, torch.int8)
-    extend(c, [120, 60], 4, scale=scale, stride=24, stream=torch.cuda.Stream())
+    extend(c, [120, 60], 4, scale=scale, stride=24, stream=torch.cuda.Stream(), chunk=APART)
 
 
 def test_a_tile_whose_row_sees_nothing_leaves_the_others_alone():
     """NaN in V of a token that only later rows see: the rows of other sequences keep their bits."""
     c = Cache(42, [150, 150], 1, 16, torch.float8_e4m3fn)
-    _, a = extend(c, [100, 100], 2)
+    _, a = extend(c, [100, 100], 2, chunk=APART)
     raw = c.kv.view(torch.uint8)
     slot = c.slots[0][149]
     raw[slot // 16, 1].view(128, 16)[:, slot % 16] = 0x7f
     q = bf16(torch.Generator(device="cuda").manual_seed(1), 202, 256)
     out = torch.zeros(202, 256, dtype=torch.bfloat16, device="cuda")
-    mp = oa.extend_plan([100, 100], 2, 1, 150, c.lens)
+    mp = oa.extend_plan([100, 100], 2, 1, 150, c.lens, APART)
+    assert mp.plan.tiles > 0
     pos = i32(list(range(50, 150)) * 2)
     oa.qwen3_extend_q8(mp, q, c.kv, c.sc, pos, c.indptr, c.pages, 16, out, SCALE, oa.workspace_for(mp.plan))
     torch.cuda.synchronize()
@@ -311,7 +315,7 @@ def test_cross_in_tiles(hq, hk, layout):
     g = hq // hk
     counts = [32 // g + 1, 64 // g + 3, 256 // g, 1, 256 // g + 1, 0, 3, 40]
     lens = [1, 129, 128, 70, 257, 5, 300, 0]
-    mp, _ = cross(hq, counts, lens, hq, hk, layout=layout)
+    mp, _ = cross(hq, counts, lens, hq, hk, layout=layout, chunk=APART)
     assert mp.plan.tiles == sum(-(-c * g // 256) for c in counts if c > 32 // g)
 
 
@@ -319,19 +323,19 @@ def test_cross_in_tiles(hq, hk, layout):
 def test_cross_in_every_form_of_a_tile(seqs, hk):
     rng = np.random.default_rng(seqs)
     counts = [int(x) for x in rng.integers(34, 130, seqs)]
-    mp, _ = cross(seqs, counts, [int(x) for x in rng.integers(0, 300, seqs)], 2 * hk, hk)
+    mp, _ = cross(seqs, counts, [int(x) for x in rng.integers(0, 300, seqs)], 2 * hk, hk, chunk=APART)
     assert mp.plan.split_tiles == 0
 
 
 @pytest.mark.parametrize("most", [None, 1100])
 def test_cross_of_tiles_in_splits(most):
-    mp, _ = cross(6, [70, 40, 40, 50], [2600, 700, 90, 0], 4, 1, max_len=most)
+    mp, _ = cross(6, [70, 40, 40, 50], [2600, 700, 90, 0], 4, 1, max_len=most, chunk=APART)
     assert mp.plan.split_tiles > 0
 
 
 @pytest.mark.parametrize("scale", [0.0, -SCALE])
 def test_cross_of_tiles_scales_streams(scale):
-    cross(7, [120, 60], [200, 150], 4, 2, scale=scale, stream=torch.cuda.Stream())
+    cross(7, [120, 60], [200, 150], 4, 2, scale=scale, stream=torch.cuda.Stream(), chunk=APART)
 
 
 def test_cross_over_shared_sources():
@@ -386,14 +390,33 @@ def test_no_rows_and_no_sequences():
         assert bool((out == 7).all())
 
 
+# ------------------------------------------------------------------ all sequences in one kernel
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (3, 1), (8, 2), (16, 2), (16, 1)])
+def test_small_calls_run_in_one_kernel(hq, hk, fmt):
+    """A row, what one and two column blocks of groups hold, and more: all as groups over 900 and 60 keys, as tiles over 1100 if more is
+    there, as groups in splits if not."""
+    g = hq // hk
+    for longest, last in ((900, 64 // g + 3), (60, 64 // g + 3), (1100, 64 // g + 3), (6000, 2)):
+        counts = [1, 16 // g, 0, 16 // g + 1, 32 // g, last, 2]
+        lens = [max(n, c) for n, c in zip((longest, 33, 7, 41, 64, longest - 7, 16), counts)]
+        tiles = longest == 1100 and g in (1, 2, 4, 8)
+        e, _ = extend(Cache(hq + longest, lens, hk, 16, fmt), counts, hq)
+        x, _ = cross(hq + longest, counts, lens, hq, hk)
+        for p in (e.plan, x.plan):
+            assert (p.tiles > 0, p.group_rows) == ((True, 0) if tiles else (False, sum(counts))) and p.groups[0] == 0
+            assert p.splits > 1 or longest < 6000
+
+
 # ------------------------------------------------------------------ odd heads, far offsets
 @pytest.mark.parametrize("hq,hk", [(3, 3), (10, 5), (22, 11)])
 def test_kv_heads_that_are_no_power_of_two(hq, hk):
-    """Few rows and tiles, split and not."""
-    extend(Cache(50 + hk, [900, 200, 70], hk, 16, torch.int8), [3, 70, 40], hq)
-    extend(Cache(51 + hk, [2600, 700], hk, 16, torch.float8_e4m3fn), [40, 3], hq)
-    cross(52 + hk, [3, 70, 40], [900, 200, 70], hq, hk)
-    cross(53 + hk, [40, 3], [2600, 700], hq, hk)
+    """Few rows and tiles, split and not, apart and together."""
+    for chunk in (64, 0):
+        extend(Cache(50 + hk, [900, 200, 70], hk, 16, torch.int8), [3, 70, 40], hq, chunk=chunk)
+        extend(Cache(51 + hk, [2600, 700], hk, 16, torch.float8_e4m3fn), [40, 3], hq, chunk=chunk)
+        cross(52 + hk, [3, 70, 40], [900, 200, 70], hq, hk, chunk=chunk)
+        cross(53 + hk, [40, 3], [2600, 700], hq, hk, chunk=chunk)
 
 
 def test_extend_past_32_bits():
@@ -411,7 +434,7 @@ def test_extend_past_32_bits():
         pos = i32([l - c + i for l, c in zip(lens, counts) for i in range(c)])
         out = torch.zeros(2, rows, 16 * 128, dtype=torch.bfloat16, device="cuda")
         for i, (k, s, first) in enumerate(((kv, sc, blocks - n), (small_kv, small_sc, 0))):
-            mp = oa.extend_plan(counts, 16, hk, 100, lens)
+            mp = oa.extend_plan(counts, 16, hk, 100, lens, 64)
             pages = i32([first + x for x in (7, 3, 11, 0, 9, 1, 2, 4, 5, 6, 8, 10, 11)])
             oa.qwen3_extend_q8(mp, q, k, s, pos, i32([0, 7, 13]), pages, 16, out[i], SCALE, oa.workspace_for(mp.plan))
         torch.cuda.synchronize()
@@ -430,7 +453,7 @@ def test_cross_past_32_bits():
         rows = sum(counts)
         out = torch.zeros(2, rows, 16 * 128, dtype=torch.bfloat16, device="cuda")
         for i, (x, first) in enumerate(((kv, total - n), (small, 0))):
-            mp = oa.cross_plan(counts, 16, hk, 200, [200, 100])
+            mp = oa.cross_plan(counts, 16, hk, 200, [200, 100], 64)
             oa.cross_run(mp, q, x[:, :hk * 128], x[:, hk * 128:], None, i32([first, first + 200]), i32([200, 100]), out[i], SCALE,
                          oa.workspace_for(mp.plan))
         torch.cuda.synchronize()

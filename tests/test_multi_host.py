@@ -181,11 +181,14 @@ def check_tiles(mp, counts, keys, causal):
     p = mp.plan
     g = p.hq // p.hk
     starts = np.cumsum([0] + counts)
-    ranges, items, split = tile_items(mp)
+    if p.tiles == 0:
+        ranges, items, split = [0] * 9, [], []
+    else:
+        ranges, items, split = tile_items(mp)
     assert ranges[0] == 0 and ranges[8] == len(items) == p.tile_units * p.hk and np.ptp(np.diff(ranges[:9])) <= 1
     seen, segments, which = {}, {}, {}
     for s, first, rows, head, k, n, seg, at in items:
-        assert counts[s] > 32 // g and starts[s] <= first and first + rows <= starts[s + 1] and 1 <= rows <= 256 // g
+        assert (counts[s] > 32 // g or p.group_rows == 0) and starts[s] <= first and first + rows <= starts[s + 1] and 1 <= rows <= 256 // g
         assert (first - starts[s]) % (256 // g) == 0 and 0 <= k < n
         last = min(max(keys[s] - (starts[s + 1] - first - rows if causal else 0), 0), p.max_len)
         assert n == max(1, -(-last // p.tile_chunk))
@@ -222,10 +225,38 @@ def test_tiles_and_groups_cover_every_row_once(make, hq, hk):
         keys = [c + reach + 13 * i for i, c in enumerate(counts)]
         mp = make(counts, hq, hk, max(keys) - 5, keys, device="cpu")
         check_tiles(mp, counts, keys, make is oa.extend_plan)
-        assert mp.plan.group_rows == sum(c for c in counts if c <= 32 // g)
+        assert mp.plan.group_rows == 0 and mp.plan.tiles == sum(-(-c // (256 // g)) for c in counts)  # few keys: all of them tiles
+        for chunk in (0, 512):
+            mp = make(counts, hq, hk, 500, None, chunk, device="cpu")  # lengths not known: the longest
+            check_tiles(mp, counts, [500] * len(counts), make is oa.extend_plan)
+        # With a chunk, by their rows.
+        assert mp.plan.group_rows == sum(c for c in counts if c <= 32 // g) and min(mp.plan.groups) > 0
         assert mp.plan.tiles == sum(-(-c // (256 // g)) for c in counts if c > 32 // g)
-        mp = make(counts, hq, hk, 500, device="cpu")  # lengths not known: the longest
-        check_tiles(mp, counts, [500] * len(counts), make is oa.extend_plan)
+
+
+@pytest.mark.parametrize("make", PLANS)
+@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 2), (16, 2)])
+def test_calls_that_mix_run_in_one_kernel_where_keys_are_few(make, hq, hk):
+    g = hq // hk
+    small, large, tall = 16 // g, 32 // g, 32 // g + 1
+    tiles = lambda counts: sum(-(-c // (256 // g)) for c in counts)
+
+    def plan(counts, reach):
+        keys = [max(reach - 3 * (i % 5), 0) for i in range(len(counts))]
+        mp = make(counts, hq, hk, reach, keys, device="cpu")
+        check_tiles(mp, counts, keys, make is oa.extend_plan)
+        return mp.plan.tiles, list(mp.plan.groups)
+
+    mixed = [small, large, 0, tall, 1]
+    assert plan(mixed, 1024) == (0, [0, 5])                                  # groups of 32: a CU gets one at most
+    assert plan(mixed, 1025) == (4, [0, 0])                                  # tiles
+    assert plan([300 * 32 // g] + mixed, 1024) == (tiles([300 * 32 // g] + mixed), [0, 0])  # more groups than CUs
+    assert plan([257 * 256 // g] + mixed, 1025) == (tiles([257 * 256 // g, tall]), [0, 3])  # more tiles than CUs
+    assert plan([small, large], 1025) == (0, [0, 2])
+    assert plan([small, 1], 1025) == (0, [2, 0])
+    # Many keys: each by itself.
+    reach = 128_000_000 // (256 * 3 * hk)
+    assert plan(mixed, reach + 100) == (1, [2, 1])
 
 
 @pytest.mark.parametrize("make", PLANS)
