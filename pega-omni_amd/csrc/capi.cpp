@@ -1305,6 +1305,7 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
       large_groups |= n > 1 || counts_h[s] > small;
     }
   }
+  if (rows > INT_MAX) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many rows", who);
   const bool may_mix = chunk_hint <= 0;
   const bool grouped = may_mix && tile_count > 0 && if_grouped * hk <= kCus && reach <= kShortKeys;
   const bool few_keys = may_mix && group_keys * hk * (cross ? 512 : 256) <= kFewKeyBytes;
@@ -1313,7 +1314,7 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   const int grouped_rows = all_tiles ? 0 : may_tile && !grouped ? large : INT_MAX;
   if (grouped) group_count = if_grouped, tile_count = 0;
   if (all_tiles) tile_count += group_count, group_count = 0;
-  if (rows > INT_MAX || !omni::grid_holds(group_count * hk, omni::kRowsThreads) || !omni::grid_holds(tile_count * hk, omni::kTiledThreads))
+  if (!omni::grid_holds(group_count * hk, omni::kRowsThreads) || !omni::grid_holds(tile_count * hk, omni::kTiledThreads))
     return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many rows", who);
   plan->cross = cross;
   plan->nseq = nseq;
@@ -1614,6 +1615,8 @@ int omni_attn_pages_compact(const int32_t* table, int64_t table_ld, int num_line
   if ((free_out + num_pages > free_pages && free_out < free_pages + num_pages) ||
       (shares_out + num_pages > shares && shares_out < shares + num_pages))
     return fail(OMNI_ATTN_EINVAL, "%s: free_out and shares_out are buffers of their own", who);
+  if (cells > 0 && table_out != table && table_out + cells > table && table_out < table + cells)
+    return fail(OMNI_ATTN_EINVAL, "%s: table_out is the table or a buffer of its own", who);
   omni::CompactArgs a{};
   a.table = table;
   a.table_out = table_out;

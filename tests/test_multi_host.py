@@ -52,7 +52,8 @@ def test_plan_bounds(make):
             ([-1], None, 4, 2, 9, 0, oa.EINVAL), ([1], [-1], 4, 2, 9, 0, oa.EINVAL), ([1], [1, 2], 4, 2, 9, 0, oa.EINVAL),
             ([1], None, 5, 2, 9, 0, oa.EINVAL), ([1], None, 0, 1, 9, 0, oa.EINVAL), ([1], None, 4, 0, 9, 0, oa.EINVAL),
             ([1], None, 4, 2, 0, 0, oa.EINVAL), ([1], None, 4, 2, 9, 65, oa.EINVAL), ([1], None, 17, 1, 9, 0, oa.EUNSUPPORTED),
-            ([2**31 - 1, 2**31 - 1], None, 1, 1, 9, 0, oa.EUNSUPPORTED)):
+            ([2**31 - 1, 2**31 - 1], None, 1, 1, 9, 0, oa.EUNSUPPORTED),
+            ([2**31 - 1] * 3, None, 2**31 - 1, 2**31 - 1, 9, 0, oa.EUNSUPPORTED)):
         with pytest.raises(oa.OmniAttnError) as e:
             make(counts, hq, hk, n, keys, chunk, device="cpu")
         assert e.value.code == code, (counts, hq, hk)

@@ -55,7 +55,8 @@ def compact(**k):
 @pytest.mark.parametrize("bad", [
     dict(ld=-1), dict(ld=2**31), dict(num_lines=-1), dict(num_pages=0), dict(limit=-1), dict(limit=10), dict(cap=-1), dict(table=None),
     dict(table_out=None), dict(free=None), dict(state=None), dict(shares=None), dict(free_out=None), dict(shares_out=None), dict(ids=None),
-    dict(src=None), dict(dst=None), dict(status=None), dict(state=P + 16), dict(free_out=P), dict(free_out=P + 32), dict(shares_out=P + 4096)])
+    dict(src=None), dict(dst=None), dict(status=None), dict(state=P + 16), dict(free_out=P), dict(free_out=P + 32), dict(shares_out=P + 4096),
+    dict(table_out=P + 4), dict(table=P + 28)])
 def test_compact_refusals(bad):
     assert compact(**bad) == oa.EINVAL
     assert b"pages_compact" in oa.load().omni_attn_last_error()
