@@ -1284,7 +1284,7 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   if (max_len <= 0) return fail(OMNI_ATTN_EINVAL, "%s: max_len=%d", who, max_len);
   if (chunk_hint > 0 && chunk_hint % 64 != 0) return fail(OMNI_ATTN_EINVAL, "%s: chunk=%d is not a multiple of 64", who, chunk_hint);
   const int small = rows_of_group(16, G), large = rows_of_group(32, G), per_tile = omni::kTiledRows / G;
-  const bool may_tile = G == 1 || G == 2 || G == 4 || G == 8;
+  const bool may_tile = omni::multi_tiles_hold(G);
   int64_t rows = 0, group_count = 0, tile_count = 0, if_grouped = 0;
   double group_keys = 0;
   int reach = 0;
@@ -1392,7 +1392,7 @@ int multi_checks(const omni_attn_multi_plan* plan, int cross, const void* q, int
       p.splits != ((int64_t)p.max_len + p.chunk - 1) / p.chunk || p.tiles < 0 || p.tile_chunk <= 0 || p.tile_chunk % 128 != 0 ||
       p.split_tiles < 0 || p.split_tiles > p.tiles || p.tile_segments < 2 * (int64_t)p.split_tiles ||
       p.tile_units != (int64_t)p.tiles - p.split_tiles + p.tile_segments || (p.split_tiles == 0 && p.tile_segments > 0) ||
-      (p.tiles > 0 && (32 % (p.hq / p.hk) != 0 || p.hq / p.hk > 8)) ||
+      (p.tiles > 0 && !omni::multi_tiles_hold(p.hq / p.hk)) ||
       p.work_bytes != multi_work_ints(p) * (int64_t)sizeof(int32_t) ||
       p.workspace_bytes != groups_workspace(p) + tiles_workspace(p))
     return fail(OMNI_ATTN_EINVAL, "%s: plan is not one its plan_init made (rows=%d hq=%d hk=%d max_len=%d groups=%d,%d chunk=%d splits=%d)",

@@ -128,6 +128,8 @@ struct TiledArgs {
   int32_t* used;
 };
 constexpr int kMultiItem = 8;  // int32 per item
+// Query heads of a K/V head that such tiles are built for.
+constexpr bool multi_tiles_hold(int G) { return (G >= 1 && G <= 8) || G == 16; }
 
 // Packed (position, head) query rows per MFMA tile: one 8-wave workgroup, one per CU.
 constexpr int kTiledRows = 256;

@@ -1127,7 +1127,7 @@ int launch_tiled(TiledArgs a, int items, int ntiles, hipStream_t stream) {
   // Pages that are no multiple of a wave's rows keep whole tiles.
   const bool lane_pages = SRC == kPagedWave && a.pd.page % kRowsPerWave != 0;
   constexpr bool MULTI = SRC >= kCross;
-  const bool parts = !lane_pages && (MULTI ? a.splits_listed == 0 : LISTED || a.split_k == 0);
+  const bool parts = !lane_pages && kBM % (a.hq / a.hk) == 0 && (MULTI ? a.splits_listed == 0 : LISTED || a.split_k == 0);
   const int form = parts && a.quarters ? kQuarters : parts && a.halved > 0 ? kHalves : kWhole;
   int grid = ((items + 7) >> 3) << 3;
   if (LISTED)
@@ -1154,8 +1154,21 @@ int launch_tiled(TiledArgs a, int items, int ntiles, hipStream_t stream) {
     OMNI_CASE(2)
     OMNI_CASE(4)
     OMNI_CASE(8)
+    default:
+      if constexpr (MULTI) {
+        switch (a.hq / a.hk) {
+          OMNI_CASE(16)
+          // Whole tiles alone, of 252 to 255 packed rows: a part of one would end inside a position.
+          case 3: launch_g<3, SRC, kWhole>(a, grid, items, ntiles, stream); break;
+          case 5: launch_g<5, SRC, kWhole>(a, grid, items, ntiles, stream); break;
+          case 6: launch_g<6, SRC, kWhole>(a, grid, items, ntiles, stream); break;
+          case 7: launch_g<7, SRC, kWhole>(a, grid, items, ntiles, stream); break;
+          default: return -2;
+        }
+        break;
+      }
+      return -2;
 #undef OMNI_CASE
-    default: return -2;
   }
   if (check_launch() != 0) return -3;
   if constexpr (MULTI) {

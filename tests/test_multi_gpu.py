@@ -177,11 +177,11 @@ def test_extend_of_strided_rows_on_another_stream(stride):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("hq,hk,page", [(1, 1, 16), (4, 2, 48), (8, 2, 16), (16, 2, 256)])
+@pytest.mark.parametrize("hq,hk,page", [(1, 1, 16), (4, 2, 48), (8, 2, 16), (16, 2, 256), (3, 1, 16), (10, 2, 16), (6, 1, 32), (14, 2, 16), (16, 1, 16)])
 def test_extend_in_tiles(hq, hk, page, fmt):
     """Tiles of a few packed rows to more than one, keys about one and two key tiles; with sequences in groups beside them."""
     g = hq // hk
-    counts = [32 // g + 1, 64 // g + 3, 256 // g, 1, 256 // g + 1, 0, 3]
+    counts = [32 // g + 1, 64 // g + 3, 256 // g, 1, 256 // g + 1, 0, 2]
     lens = [counts[0], 129, 256 // g, 70, 256 // g + 128, 5, 300]
     mp, _ = extend(Cache(hq + page, lens, hk, page, fmt), counts, hq, chunk=APART)
     assert mp.plan.tiles == 5 and sum(mp.plan.groups) == 2
@@ -200,7 +200,7 @@ def test_extend_in_every_form_of_a_tile(seqs, hk, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("hq,hk", [(4, 1), (2, 2)])
+@pytest.mark.parametrize("hq,hk", [(4, 1), (2, 2), (5, 1), (16, 1)])
 def test_extend_of_tiles_in_splits(hq, hk, fmt):
     """Few tiles over long contexts, rows that see nothing of the later splits, and (a bound below the lengths) splits that grow."""
     c = Cache(hq, [2600, 700, 90], hk, 16, fmt)
@@ -309,14 +309,14 @@ def test_cross_in_splits(chunk):
     cross(chunk, [4, 70, 3, 1, 2, 5, 5], [1900, 700, 129, 128, 0, 65, 5], 8, 2, chunk=chunk, keys=chunk != 128)
 
 
-@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (8, 2), (16, 2)])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (8, 2), (16, 2), (3, 1), (10, 2), (6, 1), (14, 2), (16, 1)])
 @pytest.mark.parametrize("layout", ["own", "one", "apart"])
 def test_cross_in_tiles(hq, hk, layout):
     g = hq // hk
-    counts = [32 // g + 1, 64 // g + 3, 256 // g, 1, 256 // g + 1, 0, 3, 40]
+    counts = [32 // g + 1, 64 // g + 3, 256 // g, 1, 256 // g + 1, 0, 2, 40]
     lens = [1, 129, 128, 70, 257, 5, 300, 0]
     mp, _ = cross(hq, counts, lens, hq, hk, layout=layout, chunk=APART)
-    assert mp.plan.tiles == sum(-(-c * g // 256) for c in counts if c > 32 // g)
+    assert mp.plan.tiles == sum(-(-c // (256 // g)) for c in counts if c > 32 // g)
 
 
 @pytest.mark.parametrize("seqs,hk", [(1, 2), (12, 8), (20, 16)])
@@ -327,9 +327,20 @@ def test_cross_in_every_form_of_a_tile(seqs, hk):
     assert mp.plan.split_tiles == 0
 
 
+@pytest.mark.parametrize("seqs,hk,g", [(1, 1, 16), (4, 4, 16), (12, 8, 16), (1, 1, 5), (6, 4, 3), (6, 8, 7)])
+def test_every_form_of_other_head_layouts(seqs, hk, g):
+    rng = np.random.default_rng(seqs + g)
+    counts = [int(x) for x in rng.integers(34, 130, seqs)]
+    lens = [c + int(x) for c, x in zip(counts, rng.integers(0, 260, seqs))]
+    e, _ = extend(Cache(seqs, lens, hk, 16, torch.float8_e4m3fn), counts, g * hk, chunk=APART)
+    x, _ = cross(seqs, counts, lens, g * hk, hk, chunk=APART)
+    assert e.plan.tiles == x.plan.tiles == sum(-(-c // (256 // g)) for c in counts) and e.plan.split_tiles == x.plan.split_tiles == 0
+
+
 @pytest.mark.parametrize("most", [None, 1100])
-def test_cross_of_tiles_in_splits(most):
-    mp, _ = cross(6, [70, 40, 40, 50], [2600, 700, 90, 0], 4, 1, max_len=most, chunk=APART)
+@pytest.mark.parametrize("hq", [4, 7, 16])
+def test_cross_of_tiles_in_splits(hq, most):
+    mp, _ = cross(6, [70, 40, 40, 50], [2600, 700, 90, 0], hq, 1, max_len=most, chunk=APART)
     assert mp.plan.split_tiles > 0
 
 
@@ -400,7 +411,7 @@ def test_small_calls_run_in_one_kernel(hq, hk, fmt):
     for longest, last in ((900, 64 // g + 3), (60, 64 // g + 3), (1100, 64 // g + 3), (6000, 2)):
         counts = [1, 16 // g, 0, 16 // g + 1, 32 // g, last, 2]
         lens = [max(n, c) for n, c in zip((longest, 33, 7, 41, 64, longest - 7, 16), counts)]
-        tiles = longest == 1100 and g in (1, 2, 4, 8)
+        tiles = longest == 1100
         e, _ = extend(Cache(hq + longest, lens, hk, 16, fmt), counts, hq)
         x, _ = cross(hq + longest, counts, lens, hq, hk)
         for p in (e.plan, x.plan):
