@@ -1260,7 +1260,7 @@ int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, 
 // column block, up to 32 a group of two, more are tiles. But each of the three is a launch
 // of its own, whose first 5-10 us no other fills, so a call that would mix them runs in
 // one of them where that is faster. Over 500 drawn calls, against three launches:
-//   - groups of 32 alone, where a CU gets one of them at most and they have up to 1024
+//   - groups of 32 alone, where a CU gets one of them at most and they have up to 1152
 //     keys: 4 % less over 63 calls that had tiles (58 sequences of 3-20 rows over 173-1039
 //     keys, 8 heads over 2: 27 -> 17.6 us); with more keys or groups the tiles win, which
 //     read a sequence's keys once for 256 packed rows.
@@ -1270,7 +1270,7 @@ int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, 
 // Together: 141 calls of 500 differ, 0.72 of the time in the mean, the worst 1.11 (7.8 us).
 // A caller who gives a chunk keeps every sequence where its own rows send it.
 constexpr double kFewKeyBytes = 128e6;
-constexpr int kShortKeys = 1024;
+constexpr int kShortKeys = 1152;
 constexpr int kCus = 256;
 
 int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,

@@ -405,13 +405,13 @@ def test_no_rows_and_no_sequences():
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (3, 1), (8, 2), (16, 2), (16, 1)])
 def test_small_calls_run_in_one_kernel(hq, hk, fmt):
-    """A row, what one and two column blocks of groups hold, and more: all as groups over 900 and 60 keys, as tiles over 1100 if more is
+    """A row, what one and two column blocks of groups hold, and more: all as groups over 900 and 60 keys, as tiles over 1200 if more is
     there, as groups in splits if not."""
     g = hq // hk
-    for longest, last in ((900, 64 // g + 3), (60, 64 // g + 3), (1100, 64 // g + 3), (6000, 2)):
+    for longest, last in ((900, 64 // g + 3), (60, 64 // g + 3), (1200, 64 // g + 3), (6000, 2)):
         counts = [1, 16 // g, 0, 16 // g + 1, 32 // g, last, 2]
         lens = [max(n, c) for n, c in zip((longest, 33, 7, 41, 64, longest - 7, 16), counts)]
-        tiles = longest == 1100
+        tiles = longest == 1200
         e, _ = extend(Cache(hq + longest, lens, hk, 16, fmt), counts, hq)
         x, _ = cross(hq + longest, counts, lens, hq, hk)
         for p in (e.plan, x.plan):

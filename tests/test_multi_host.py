@@ -222,7 +222,7 @@ def check_tiles(mp, counts, keys, causal):
 def test_tiles_and_groups_cover_every_row_once(make, hq, hk):
     g = hq // hk
     counts = [1, 32 // g, 32 // g + 1, 0, 256 // g, 256 // g + 1, 1000, 2]
-    for reach in (7, 9000):
+    for reach in (160, 9000):
         keys = [c + reach + 13 * i for i, c in enumerate(counts)]
         mp = make(counts, hq, hk, max(keys) - 5, keys, device="cpu")
         check_tiles(mp, counts, keys, make is oa.extend_plan)
@@ -249,12 +249,12 @@ def test_calls_that_mix_run_in_one_kernel_where_keys_are_few(make, hq, hk):
         return mp.plan.tiles, list(mp.plan.groups)
 
     mixed = [small, large, 0, tall, 1]
-    assert plan(mixed, 1024) == (0, [0, 5])                                  # groups of 32: a CU gets one at most
-    assert plan(mixed, 1025) == (4, [0, 0])                                  # tiles
-    assert plan([300 * 32 // g] + mixed, 1024) == (tiles([300 * 32 // g] + mixed), [0, 0])  # more groups than CUs
-    assert plan([257 * 256 // g] + mixed, 1025) == (tiles([257 * 256 // g, tall]), [0, 3])  # more tiles than CUs
-    assert plan([small, large], 1025) == (0, [0, 2])
-    assert plan([small, 1], 1025) == (0, [2, 0])
+    assert plan(mixed, 1152) == (0, [0, 5])                                  # groups of 32: a CU gets one at most
+    assert plan(mixed, 1153) == (4, [0, 0])                                  # tiles
+    assert plan([300 * 32 // g] + mixed, 1152) == (tiles([300 * 32 // g] + mixed), [0, 0])  # more groups than CUs
+    assert plan([257 * 256 // g] + mixed, 1153) == (tiles([257 * 256 // g, tall]), [0, 3])  # more tiles than CUs
+    assert plan([small, large], 1153) == (0, [0, 2])
+    assert plan([small, 1], 1153) == (0, [2, 0])
     # Many keys: each by itself.
     reach = 128_000_000 // (256 * 3 * hk)
     assert plan(mixed, reach + 100) == (1, [2, 1])
