@@ -168,7 +168,11 @@ constexpr int kDense = 0, kPagedWave = 1, kPagedLane = 2, kPacked = 3;
 // and after the softmax, as bf16 that the block's exponent has been put into (exact
 // but at the ends of bf16's range), to LDS: K as in the other sources, V, which lies
 // [dim][token], as the operand that P.V takes: [block][half h][dim][8 tokens], tokens
-// 4 h + {0..3, 8..11}. Rows without keys store zeros; P is at most 1.
+// 4 h + {0..3, 8..11}. Rows without keys store zeros; P is at most 1. The loop is bound
+// as in the other sources, and a step's conversions hide behind its products: 12 chunks
+// of 512-4096 rows behind up to 1024 cached tokens of 32q/8kv, E4M3, 0.79 ms, 1.0
+// PFLOP/s; 12 x 187-4000 rows over 300-2400 bf16 rows 0.54 ms, 1.0 PFLOP/s. 128 keys
+// take 3.9 us, or 2.4 where at most half the waves have rows.
 constexpr int kCross = 4, kCacheE4m3 = 5, kCacheInt8 = 6;
 
 // Four stored bytes times 2^(e - 127), as bf16: once rounded.
