@@ -512,12 +512,13 @@ typedef struct omni_attn_multi_plan {
 
 /* Host: counts (zero allowed) to a work list. hq / hk from 1 to 16. keys_h (NULL:
  * not known): how many keys each sequence's last row sees when the plan is made,
- * for the order of the work and the size of the splits alone; the lengths of a run
- * are read on the device. chunk_hint, a multiple of 64 (<= 0 picks from the
- * shape), is the split of the groups, and keeps sequences apart by their rows alone:
- * up to 16 packed rows, up to 32, and the rest in tiles where hq / hk is at most 8,
- * or 16. Without one, a small call runs all of them in one kernel. OMNI_ATTN_EWORKSPACE
- * with plan->work_bytes set when work_h is too small. */
+ * for the choice of kernels, the order of the work and the size of the splits alone;
+ * the lengths of a run are read on the device. chunk_hint, a multiple of 64 (<= 0
+ * picks from the shape), is the split of the groups, and keeps sequences apart by
+ * their rows alone: up to 16 packed rows, up to 32, and the rest in tiles where hq /
+ * hk is at most 8, or 16. Without one they run in one kernel or two, and which one
+ * takes a row, and so its rounding, may depend on the call's other sequences.
+ * OMNI_ATTN_EWORKSPACE with plan->work_bytes set when work_h is too small. */
 int omni_attn_extend_plan_init(int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,
                                int chunk_hint, int32_t* work_h, int64_t work_cap, omni_attn_multi_plan* plan);
 int omni_attn_cross_plan_init(int nseq, const int32_t* counts_h, const int32_t* keys_h, int hq, int hk, int max_len,

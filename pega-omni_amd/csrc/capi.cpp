@@ -1264,12 +1264,16 @@ int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, 
 //     keys: 4 % less over 63 calls that had tiles (58 sequences of 3-20 rows over 173-1039
 //     keys, 8 heads over 2: 27 -> 17.6 us); with more keys or groups the tiles win, which
 //     read a sequence's keys once for 256 packed rows.
-//   - tiles alone, where the groups' keys are at most kFewKeyBytes (26 us of them) and a CU
-//     gets one tile at most: the 43 us of 13 sequences of 1-10 rows over 650 keys -> 15.
-//   - groups of 32 alone, where nothing is for the tiles and the groups' keys are as few.
-// Together: 141 calls of 500 differ, 0.72 of the time in the mean, the worst 1.11 (7.8 us).
-// A caller who gives a chunk keeps every sequence where its own rows send it.
-constexpr double kFewKeyBytes = 128e6;
+//   - tiles alone, where a CU gets one of them at most and the groups' keys are few: up to
+//     kFewKeyBytes, as a tile of few rows takes 8-bit keys at 3.5 TB/s and a group at 5.5,
+//     or kFewStateBytes (bf16: 7 and 5.5). The 43 us of 13 sequences of 1-10 rows over 650
+//     keys -> 15; 32 and 58 rows over 57,812 and 39,270 bf16 keys of 16 heads 164 -> 154.
+//   - else groups of 32 for all that are no tiles, if any is: the second block costs less
+//     than a launch (13 sources of up to 5387 keys, 3-21 rows, 8 heads: 47 -> 33 us).
+// 141 calls of 500 differ, 0.72 of the time in the mean, the worst 1.11 (7.8 us); at 128 MB
+// to 2 GB of keys 24 of 2500 more, 0.67-0.96. A caller who gives a chunk keeps every
+// sequence where its own rows send it.
+constexpr double kFewKeyBytes = 128e6, kFewStateBytes = 2e9;
 constexpr int kShortKeys = 1152;
 constexpr int kCus = 256;
 
@@ -1308,9 +1312,9 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
   if (rows > INT_MAX) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many rows", who);
   const bool may_mix = chunk_hint <= 0;
   const bool grouped = may_mix && tile_count > 0 && if_grouped * hk <= kCus && reach <= kShortKeys;
-  const bool few_keys = may_mix && group_keys * hk * (cross ? 512 : 256) <= kFewKeyBytes;
-  const bool all_tiles = !grouped && few_keys && tile_count > 0 && (tile_count + group_count) * hk <= kCus;
-  const bool one_size = grouped || (few_keys && large_groups);
+  const bool few_keys = group_keys * hk * (cross ? 512 : 256) <= (cross ? kFewStateBytes : kFewKeyBytes);
+  const bool all_tiles = may_mix && !grouped && few_keys && tile_count > 0 && (tile_count + group_count) * hk <= kCus;
+  const bool one_size = grouped || (may_mix && large_groups);
   const int grouped_rows = all_tiles ? 0 : may_tile && !grouped ? large : INT_MAX;
   if (grouped) group_count = if_grouped, tile_count = 0;
   if (all_tiles) tile_count += group_count, group_count = 0;

@@ -255,9 +255,11 @@ def test_calls_that_mix_run_in_one_kernel_where_keys_are_few(make, hq, hk):
     assert plan([257 * 256 // g] + mixed, 1153) == (tiles([257 * 256 // g, tall]), [0, 3])  # more tiles than CUs
     assert plan([small, large], 1153) == (0, [0, 2])
     assert plan([small, 1], 1153) == (0, [2, 0])
-    # Many keys: each by itself.
-    reach = 128_000_000 // (256 * 3 * hk)
-    assert plan(mixed, reach + 100) == (1, [2, 1])
+    # Many keys: what is no tile as groups.
+    limit = 128_000_000 // 256 if make is oa.extend_plan else 2_000_000_000 // 512
+    assert plan(mixed, limit // (3 * hk) - 100) == (4, [0, 0])
+    assert plan(mixed, limit // (3 * hk) + 100) == (1, [0, 3])
+    assert plan([small, 1], limit // hk) == (0, [2, 0])
 
 
 @pytest.mark.parametrize("make", PLANS)
