@@ -771,8 +771,8 @@ def _multi_plan(init, counts, keys, hq, hk, max_len, chunk, device) -> Multi:
 def extend_plan(counts, hq, hk, max_len, keys=None, chunk=0, device="cuda") -> Multi:
     """Host plan of qwen3_extend_q8 for ``counts[s]`` rows of each sequence;
     uploads the work list. ``keys``: how many keys each sequence's last row sees
-    now, if known (order and split sizes alone); the workspace is
-    ``workspace_for(plan.plan)``."""
+    now, if known (for the choice of kernels, the order and the split sizes alone);
+    the workspace is ``workspace_for(plan.plan)``."""
     return _multi_plan(load().omni_attn_extend_plan_init, counts, keys, hq, hk, max_len, chunk, device)
 
 
