@@ -1126,10 +1126,9 @@ bool multi_fits(const omni_attn_multi_plan& p) {
 // head has 256 / hk CUs; these take the splits, longest first, as they come free:
 //   3.9 for each 128 keys, 2.4 where at most 128 packed rows keep half the waves;
 //   12 for a workgroup's first loads and last stores, 5 more to write a partial;
-//   with splits, 8 for the merge's launch, 0.14 for each split of the tile that has most
-//   (a merging thread takes them in turn), and the partials, written and read, at 4.5 TB/s.
-// Fitted to sweeps of 34 shapes (1 to 230 tiles, 600 to 60,000 keys) over 20 sizes; without
-// the 0.14, 8 rows over 27,779 keys of 8q/1kv took 218 splits and 45.5 us, with it 24.
+//   with splits, 8 for the merge's launch, 0.05 for each split of the tile that has most
+//   (a merging wave takes them in turn), and the partials, written and read, at 4.5 TB/s.
+// Fitted to sweeps of 40 shapes (1 to 230 tiles, 600 to 60,000 keys) over 10 to 20 sizes.
 int pick_tile_steps(const std::vector<std::array<int32_t, 4>>& tl, int G, int hk, int max_len) {
   const size_t machines = (size_t)std::max(256 / hk, 1);
   const auto steps_of = [&](const std::array<int32_t, 4>& t) { return (int)((std::min((int64_t)t[3], (int64_t)max_len) + 127) / 128); };
@@ -1161,7 +1160,7 @@ int pick_tile_steps(const std::vector<std::array<int32_t, 4>>& tl, int G, int hk
       free_at.back() += c;
       std::push_heap(free_at.begin(), free_at.end(), std::greater<double>());
     }
-    const double t = *std::max_element(free_at.begin(), free_at.end()) + (partials > 0 ? 8 + 0.14 * most_used + partials / 4.5e6 : 0);
+    const double t = *std::max_element(free_at.begin(), free_at.end()) + (partials > 0 ? 8 + 0.05 * most_used + partials / 4.5e6 : 0);
     if (n == 1 || t < least) best = per, least = t;
   }
   return best;
@@ -1449,6 +1448,7 @@ int multi_launch(omni::RowsArgs& a, const omni_attn_multi_plan& p, int source, c
     t.halved = omni::prefill_halves(items, resident);
     t.split_tiles = p.tile_chunk / 128;
     t.splits_listed = p.split_tiles * p.hk;
+    t.segments = (int64_t)p.tile_segments * p.hk;
     if (p.split_tiles > 0) {
       t.split_items = work + units_work_ints(p);
       t.ws = reinterpret_cast<float*>(static_cast<char*>(workspace) + groups_workspace(p));

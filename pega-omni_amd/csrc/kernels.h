@@ -124,6 +124,7 @@ struct TiledArgs {
   const int32_t* len;
   int split_tiles;
   int splits_listed;          // (tile, kv head) pairs that are split
+  int64_t segments;           // their splits
   const int32_t* split_items; // (first row, rows + 2^9 splits, kv head, first segment) of each
   int32_t* used;
 };

@@ -1048,47 +1048,55 @@ __global__ __launch_bounds__(256) void dit_combine(TiledArgs a, int ntiles) {
   *reinterpret_cast<uint4*>(a.out + b * a.out_bstride + ((int64_t)(q0 + p) * a.hq + head) * kHead + d0) = o;
 }
 
-// The splits of tiles of several rows per sequence, merged: workgroups, rows and dims
-// as in dit_combine, over the work list's split tiles (first row, rows and splits, kv
-// head, first segment; the segments of a tile's splits follow one another). One pass
-// with a running base, the first batch asked for before it is known how many splits
-// were used. Rows without keys have none that weighs: zeros.
-template <bool Q8>
-__global__ __launch_bounds__(256) void multi_combine(TiledArgs a) {
+// The splits of tiles of several rows per sequence, merged, over the work list's split
+// tiles (first row, rows and splits, kv head, first segment; the segments of a tile's
+// splits follow one another). A workgroup takes four packed rows, 16 threads of 8 dims
+// each; its WAVES waves take batches of splits in turn, in one pass with a running base,
+// the first batch asked for before it is known how many splits were used, and wave 0
+// joins them. Bound by a round trip a batch, so that four waves are faster where tiles
+// have more splits than one batch holds, and slower by their idle threads where not. The
+// whole call, us, with one and four: one tile of 64 packed rows in 55 splits 21.6 / 18.2,
+// two in 60 each 22.3 / 17.3; 15 tiles x 8 K/V heads in 2 118 / 132. (16 rows a workgroup,
+// one wave for four of them, took 24.2, 23.7 and 121; batches of 16 a quarter more.) Rows
+// without keys have no split that weighs: zeros.
+constexpr int kMultiBatch = 8, kMultiRows = 4;
+
+template <bool Q8, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void multi_combine(TiledArgs a) {
   constexpr int kSeg = kBM * (kHead + 2);
   const int idx = blockIdx.x, G = a.hq / a.hk;
   const int used = a.used[idx];
   const int4 item = reinterpret_cast<const int4*>(a.split_items)[idx];
   const int rows = item.y & 0x1ff, splits = (int)((uint32_t)item.y >> 9);
-  const int r = blockIdx.y * kCombineRows + (threadIdx.x >> 4), d0 = 8 * (threadIdx.x & 15);
+  if ((int)blockIdx.y * kMultiRows >= rows * G) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = min((int)blockIdx.y * kMultiRows + (lane >> 4), rows * G - 1), d0 = 8 * (lane & 15);
   const int p = r / G, head = item.z * G + r % G;
-  if (p >= rows) return;
-  const bool none = Q8 && a.pos[item.x + p] < 0;
   const float* seg0 = a.ws + (int64_t)item.w * kSeg;
   float num[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float den = 0.f, top = -INFINITY;
-  for (int c0 = 0; c0 < used || c0 == 0; c0 += kCombineBatch) {
-    float2 ml[kCombineBatch];
-    float4 v[kCombineBatch][2];
+  for (int c0 = kMultiBatch * wave, first = 1; c0 < used || first; c0 += kMultiBatch * WAVES, first = 0) {
+    float2 ml[kMultiBatch];
+    float4 v[kMultiBatch][2];
 #pragma unroll
-    for (int i = 0; i < kCombineBatch; ++i) {
+    for (int i = 0; i < kMultiBatch; ++i) {
       if (c0 + i >= splits) continue;  // uniform
       const float* seg = seg0 + (int64_t)(c0 + i) * kSeg;
       ml[i] = *reinterpret_cast<const float2*>(seg + kBM * kHead + 2 * r);
       v[i][0] = *reinterpret_cast<const float4*>(seg + r * kHead + d0);
       v[i][1] = *reinterpret_cast<const float4*>(seg + r * kHead + d0 + 4);
     }
-    if (c0 == 0 && used <= 1) return;
+    if (used <= 1) return;
     float mx = top;
 #pragma unroll
-    for (int i = 0; i < kCombineBatch; ++i) mx = c0 + i < used ? fmaxf(mx, ml[i].x) : mx;
+    for (int i = 0; i < kMultiBatch; ++i) mx = c0 + i < used ? fmaxf(mx, ml[i].x) : mx;
     const float base = mx == -INFINITY ? 0.f : mx, alpha = fast_exp2(top - base);
     top = mx;
     den *= alpha;
 #pragma unroll
     for (int e = 0; e < 8; ++e) num[e] *= alpha;
 #pragma unroll
-    for (int i = 0; i < kCombineBatch; ++i)
+    for (int i = 0; i < kMultiBatch; ++i)
       if (c0 + i < used) {  // what was asked for beyond may be anything
         const float w = fast_exp2(ml[i].x - base);
         den = fmaf(ml[i].y, w, den);
@@ -1096,6 +1104,31 @@ __global__ __launch_bounds__(256) void multi_combine(TiledArgs a) {
         for (int e = 0; e < 8; ++e) num[e] = fmaf((&v[i][e >> 2].x)[e & 3], w, num[e]);
       }
   }
+  if (WAVES > 1 && used > kMultiBatch) {  // else wave 0 had them all
+    __shared__ float s_part[WAVES > 1 ? WAVES - 1 : 1][10][64];
+    if (wave > 0) {
+      s_part[wave - 1][8][lane] = den, s_part[wave - 1][9][lane] = top;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_part[wave - 1][e][lane] = num[e];
+    }
+    __syncthreads();
+    float mx = top;
+#pragma unroll
+    for (int w = 0; w < WAVES - 1; ++w) mx = fmaxf(mx, s_part[w][9][lane]);
+    const float base = mx == -INFINITY ? 0.f : mx, own = fast_exp2(top - base);
+    den *= own;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) num[e] *= own;
+#pragma unroll
+    for (int w = 0; w < WAVES - 1; ++w) {
+      const float x = fast_exp2(s_part[w][9][lane] - base);
+      den = fmaf(s_part[w][8][lane], x, den);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) num[e] = fmaf(s_part[w][e][lane], x, num[e]);
+    }
+  }
+  if (wave > 0 || (int)blockIdx.y * kMultiRows + (lane >> 4) >= rows * G) return;
+  const bool none = Q8 && a.pos[item.x + p] < 0;
   const float inv = 1.f / den;
   uint4 o;
   o.x = pack_bf16x2(num[0] * inv, num[1] * inv);
@@ -1176,7 +1209,11 @@ int launch_tiled(TiledArgs a, int items, int ntiles, hipStream_t stream) {
   }
   if (check_launch() != 0) return -3;
   if constexpr (MULTI) {
-    if (a.splits_listed > 0) multi_combine<SRC != kCross><<<dim3(a.splits_listed, kBM / kCombineRows), 256, 0, stream>>>(a);
+    const dim3 rows(std::max(a.splits_listed, 0), kBM / kMultiRows);
+    if (a.splits_listed > 0 && a.segments > (int64_t)kMultiBatch * a.splits_listed)
+      multi_combine<SRC != kCross, 4><<<rows, 256, 0, stream>>>(a);
+    else if (a.splits_listed > 0)
+      multi_combine<SRC != kCross, 1><<<rows, 64, 0, stream>>>(a);
     return check_launch();
   }
   if (!LISTED && a.split_k > 0) {
