@@ -401,6 +401,22 @@ def test_no_rows_and_no_sequences():
         assert bool((out == 7).all())
 
 
+@pytest.mark.parametrize("hq,hk", [(1, 1), (3, 1), (14, 2), (16, 1)])
+def test_one_tile_in_many_splits(hq, hk):
+    """Waves share a row's splits: all of them, as many as one wave takes at once, one, none; rows that see only the first; rows * G that
+    are no multiple of four."""
+    g = hq // hk
+    rows = 32 // g + 1
+    c = Cache(hq, [9000], hk, 16, torch.int8)
+    for last in (8999, 1900, 1000, 129, 60, -1):
+        pos = [max(last - 3 * i, -1) if i % 4 else min(last, 5) for i in range(rows)]
+        mp, _ = extend(c, [rows], hq, pos=pos)
+        assert mp.plan.tile_segments > 8 * mp.plan.split_tiles > 0
+    for n in (9000, 1900, 1000, 129, 60, 0):
+        mp, _ = cross(hq, [rows], [n], hq, hk, max_len=9000, keys=False)
+        assert mp.plan.tile_segments > 8 * mp.plan.split_tiles > 0
+
+
 # ------------------------------------------------------------------ all sequences in one kernel
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (3, 1), (8, 2), (16, 2), (16, 1)])
