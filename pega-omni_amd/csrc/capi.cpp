@@ -1113,10 +1113,10 @@ bool multi_fits(const omni_attn_multi_plan& p) {
       !omni::grid_holds((int64_t)p.split_tiles * p.hk, 256) || (int64_t)p.tile_segments * p.hk > INT_MAX)
     return false;
   for (int c = 0; c < 2; ++c) {
-    const int64_t rows = std::max(rows_of_group(16 * (c + 1), p.hq / p.hk), 1);
+    const int64_t rows = std::max(rows_of_group(16 * (c + 1), p.hq / p.hk), 1), merged = omni::rows_merged(p.splits);
     if (!omni::grid_holds((int64_t)p.groups[c] * p.hk * p.splits, omni::kRowsThreads) ||
         (int64_t)p.groups[c] * p.hk * p.splits > INT_MAX ||
-        (p.splits > 1 && !omni::grid_holds((int64_t)p.groups[c] * ((rows * p.hq + 7) / 8), omni::kRowsThreads)))
+        (p.splits > 1 && !omni::grid_holds((int64_t)p.groups[c] * ((rows * p.hq + merged - 1) / merged), omni::kRowsThreads)))
       return false;
   }
   return true;
@@ -1217,7 +1217,8 @@ int groups_a_cu(int cross, bool large) { return cross || large ? 2 : 4; }
 //   longer; and of the walk 0.19, or 0.35 where not all workgroups run at once;
 //   the partials, written and read, at 6.4 TB/s;
 //   0.6 for each 1024 workgroups, those that find nothing to do too;
-//   with splits, 7.2 for the merge's launch and 1.1 for every 16 splits of a row.
+//   with splits, 7.2 for the merge's launch and 1.1 for each batch of a row's splits: of
+//   16, or (behind two) of 64.
 // Measured at the choice / at the best of the sweep: 0.3% apart in the mean; 5 rows
 // behind 2400 keys of 16q/8kv, 192 keys 9.9 / 9.9; 4 x 8 rows behind 20,000-60,000 of
 // 32q/8kv, 3584 keys 67.2 / 67.2; 5 candidates of 48 sources of 100-1500 none 31.3 / 31.3;
@@ -1253,7 +1254,7 @@ int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, 
     const double splits = std::ceil((double)max_len / chunk), most = std::ceil(longest / chunk);
     const double walk = tile * std::min<double>(chunk, longest) / 128;
     const double t = std::max(read, walk) + (at_once ? 0.19 : 0.35) * walk + part * each * 2 * kPartialBytes / 6.4e6 +
-                     0.6 * n * hk * splits / 1024 + (splits > 1 ? 7.2 + 1.1 * std::ceil(most / 16) : 0);
+                     0.6 * n * hk * splits / 1024 + (splits > 1 ? 7.2 + 1.1 * std::min(std::ceil(most / 16), 2 + std::ceil(most / 64)) : 0);
     if (best == 0 || t < least) best = (int)chunk, least = t;
     if (chunk >= whole) return best;
   }

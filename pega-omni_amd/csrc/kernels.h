@@ -330,6 +330,10 @@ int launch_decode_q8(DecodeQ8Args a, int rows, hipStream_t stream);
 // Groups of rows that see the same keys (rows.hip): an item is (sequence, first row,
 // rows, its first row in the workspace).
 constexpr int kRowsThreads = 256;
+// (row, head) pairs that a workgroup of rows_merge takes: with many splits its four waves
+// share them.
+constexpr int kRowsMergeMany = 32;
+constexpr int rows_merged(int splits) { return splits > kRowsMergeMany ? 2 : 8; }
 constexpr int kRowsBf16 = 2;  // source: bf16 rows, beside kQ8E4m3 and kQ8Int8
 
 struct RowsArgs {

@@ -417,6 +417,20 @@ def test_one_tile_in_many_splits(hq, hk):
         assert mp.plan.tile_segments > 8 * mp.plan.split_tiles > 0
 
 
+@pytest.mark.parametrize("hq,hk,rows", [(1, 1, 1), (3, 1, 5), (14, 2, 4), (16, 1, 2), (9, 3, 7)])
+def test_groups_in_many_splits(hq, hk, rows):
+    """Waves share a row's splits: all of them, a batch more than one wave takes at once, one batch, two splits, one, none; a row alone in
+    its workgroup."""
+    c = Cache(hq, [9000, 40], hk, 16, torch.float8_e4m3fn)
+    for last in (8999, 2100, 1000, 100, 60, -1):
+        pos = [max(last - 3 * i, -1) if i % 4 < 3 else min(last, 5) for i in range(rows)] + [39]
+        mp, _ = extend(c, [rows, 1], hq, pos=pos, chunk=64)
+        assert mp.plan.splits > 32 and mp.plan.tiles == 0
+    for n in (9000, 2100, 1000, 100, 60, 0):
+        mp, _ = cross(hq, [rows, 1], [n, 33], hq, hk, max_len=9000, keys=False, chunk=64)
+        assert mp.plan.splits > 32 and mp.plan.tiles == 0
+
+
 # ------------------------------------------------------------------ all sequences in one kernel
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2), (3, 1), (8, 2), (16, 2), (16, 1)])
