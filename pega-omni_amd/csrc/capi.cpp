@@ -1362,7 +1362,7 @@ int multi_plan_init(int cross, int nseq, const int32_t* counts_h, const int32_t*
     units += n;
     if (n > 1) segments += n, ++plan->split_tiles;
   }
-  if (units > INT_MAX || plan->max_len / plan->tile_chunk >= 1 << 22) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many tiles", who);
+  if (units > INT_MAX || (!tl.empty() && plan->max_len / plan->tile_chunk >= 1 << 22)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: too many tiles", who);
   plan->tile_units = (int32_t)units;
   plan->tile_segments = (int32_t)segments;
   if (!multi_fits(*plan)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, plan->rows, hq, plan->splits);

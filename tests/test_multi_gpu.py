@@ -417,6 +417,13 @@ def test_one_tile_in_many_splits(hq, hk):
         assert mp.plan.tile_segments > 8 * mp.plan.split_tiles > 0
 
 
+@pytest.mark.parametrize("counts", [[3, 1], [40, 1]])
+def test_a_bound_that_bounds_nothing(counts):
+    c = Cache(3, [700, 90], 1, 16, torch.int8)
+    extend(c, counts, 4, max_len=2**31 - 1, keys=False)
+    cross(3, counts, [700, 90], 4, 1, max_len=2**31 - 1, keys=False)
+
+
 @pytest.mark.parametrize("hq,hk,rows", [(1, 1, 1), (3, 1, 5), (14, 2, 4), (16, 1, 2), (9, 3, 7)])
 def test_groups_in_many_splits(hq, hk, rows):
     """Waves share a row's splits: all of them, a batch more than one wave takes at once, one batch, two splits, one, none; a row alone in

@@ -61,6 +61,13 @@ def test_plan_bounds(make):
     assert mp.plan.rows == 0 and mp.plan.work_bytes == 0 and mp.plan.workspace_bytes == 0
 
 
+@pytest.mark.parametrize("make", PLANS)
+def test_a_bound_that_bounds_nothing(make):
+    for counts in ([1], [1, 0, 8], [40], [300, 2]):
+        p = make(counts, 4, 1, 2**31 - 1, device="cpu").plan
+        assert p.rows == sum(counts) and p.splits >= 1 and p.tile_chunk > 0
+
+
 @pytest.mark.parametrize("init", ["omni_attn_extend_plan_init", "omni_attn_cross_plan_init"])
 def test_plan_capacity(init):
     f, plan = getattr(oa.load(), init), oa.MultiPlan()
