@@ -506,6 +506,9 @@ typedef struct omni_attn_multi_plan {
   int32_t tile_chunk; /* keys per split of a tile (a multiple of 128) */
   int32_t tile_units; /* splits of all tiles (each runs once per kv head) */
   int32_t split_tiles, tile_segments; /* tiles in more than one split, and their splits */
+  int32_t exact_p;    /* as in omni_attn_prefill_plan, for the rows in tiles (at up to 1.35x
+                         the time); groups carry P in 16 bits in any case, so that with 1
+                         every row of a call does */
   int64_t work_bytes; /* bytes of the int32 work list that the caller uploads */
   int64_t workspace_bytes; /* device scratch of a run (split partials), 16-byte aligned */
 } omni_attn_multi_plan;
@@ -531,8 +534,8 @@ int omni_attn_cross_plan_init(int nseq, const int32_t* counts_h, const int32_t* 
  * < 0 stores zeros. The rows of a sequence may have any positions. indptr has nseq +
  * 1 entries. q rows [hq][128] of stride q_stride (a multiple of 8), out rows
  * [hq][128]; rows past the plan's are left as they were.
- * P is carried in 16 bits in groups and rounded to bf16 in tiles, which also take K
- * and V as bf16 (exact, but for values that bf16 does not hold: 2^128, which
+ * P is carried in 16 bits in groups and, unless the plan's exact_p is set, rounded to
+ * bf16 in tiles, which also take K and V as bf16 (exact, but for values that bf16 does not hold: 2^128, which
  * rounding to 8 bits can make, and what lies below 2^-126). P is at most 1 on the
  * way, as in omni_qwen3_attend_q8. Tokens past the last key that a row of the group
  * or tile sees may hold anything; among their own keys, an infinity or NaN in V

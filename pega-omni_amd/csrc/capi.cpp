@@ -1400,11 +1400,12 @@ int multi_checks(const omni_attn_multi_plan* plan, int cross, const void* q, int
       p.splits != ((int64_t)p.max_len + p.chunk - 1) / p.chunk || p.tiles < 0 || p.tile_chunk <= 0 || p.tile_chunk % 128 != 0 ||
       p.split_tiles < 0 || p.split_tiles > p.tiles || p.tile_segments < 2 * (int64_t)p.split_tiles ||
       p.tile_units != (int64_t)p.tiles - p.split_tiles + p.tile_segments || (p.split_tiles == 0 && p.tile_segments > 0) ||
-      (p.tiles > 0 && !omni::multi_tiles_hold(p.hq / p.hk)) ||
+      (p.tiles > 0 && !omni::multi_tiles_hold(p.hq / p.hk)) || (p.exact_p != 0 && p.exact_p != 1) ||
       p.work_bytes != multi_work_ints(p) * (int64_t)sizeof(int32_t) ||
       p.workspace_bytes != groups_workspace(p) + tiles_workspace(p))
-    return fail(OMNI_ATTN_EINVAL, "%s: plan is not one its plan_init made (rows=%d hq=%d hk=%d max_len=%d groups=%d,%d chunk=%d splits=%d)",
-                who, p.rows, p.hq, p.hk, p.max_len, p.groups[0], p.groups[1], p.chunk, p.splits);
+    return fail(OMNI_ATTN_EINVAL,
+                "%s: plan is not one its plan_init made (rows=%d hq=%d hk=%d max_len=%d groups=%d,%d chunk=%d splits=%d exact_p=%d)", who,
+                p.rows, p.hq, p.hk, p.max_len, p.groups[0], p.groups[1], p.chunk, p.splits, p.exact_p);
   if (!multi_fits(p)) return fail(OMNI_ATTN_EUNSUPPORTED, "%s: %d rows of %d heads in %d splits", who, p.rows, p.hq, p.splits);
   if (!std::isfinite(scale * kLog2e)) return fail(OMNI_ATTN_EINVAL, "%s: scale * log2(e) is not finite", who);
   if (p.rows == 0) return 0;
@@ -1447,6 +1448,7 @@ int multi_launch(omni::RowsArgs& a, const omni_attn_multi_plan& p, int source, c
     const int resident = resident_tiled_groups();
     t.quarters = omni::tiled_quarters(items, resident);
     t.halved = omni::prefill_halves(items, resident);
+    t.exact_p = p.exact_p;
     t.split_tiles = p.tile_chunk / 128;
     t.splits_listed = p.split_tiles * p.hk;
     t.segments = (int64_t)p.tile_segments * p.hk;

@@ -110,7 +110,7 @@ struct TiledArgs {
   int halved;
   // All items run as four workgroups of a quarter of the rows each (no split).
   int quarters;
-  // Prefill with P carried as two bf16 terms (hi + lo) through P.V.
+  // All but DiT: P carried as two bf16 terms (hi + lo) through P.V.
   int exact_p;
   // packed prompts (mode 2), cross attention: elements between rows of k and of v
   int64_t k_stride, v_stride;
@@ -147,7 +147,7 @@ int launch_prefill(const TiledArgs& a, int items, hipStream_t stream);
 // Packed prompts: items are (sequence's first row, first row, rows, kv head).
 constexpr int64_t kMostPromptStride = 1LL << 22;  // elements: 128 rows stay below 2^30 bytes
 int launch_prompt(const TiledArgs& a, int items, hipStream_t stream);
-// Several rows per sequence over a source of launch_rows: items are (sequence, first row, rows, kv head).
+// Several rows per sequence over a source of launch_rows: items of kMultiItem fields, as TiledArgs has them.
 int launch_multi_tiles(const TiledArgs& a, int source, int items, hipStream_t stream);
 
 // Rotary embedding + K/V scatter (the step before attention).

@@ -171,8 +171,8 @@ constexpr int kDense = 0, kPagedWave = 1, kPagedLane = 2, kPacked = 3;
 // 4 h + {0..3, 8..11}. Rows without keys store zeros; P is at most 1. The loop is bound
 // as in the other sources, and a step's conversions hide behind its products: 12 chunks
 // of 512-4096 rows behind up to 1024 cached tokens of 32q/8kv, E4M3, 0.79 ms, 1.0
-// PFLOP/s; 12 x 187-4000 rows over 300-2400 bf16 rows 0.54 ms, 1.0 PFLOP/s. 128 keys
-// take 3.9 us, or 2.4 where at most half the waves have rows.
+// PFLOP/s; 12 x 187-4000 rows over 300-2400 bf16 rows 0.54 ms, 1.0 PFLOP/s (EXACT: 1.03
+// and 0.71 ms). 128 keys take 3.9 us, or 2.4 where at most half the waves have rows.
 constexpr int kCross = 4, kCacheE4m3 = 5, kCacheInt8 = 6;
 
 // Four stored bytes times 2^(e - 127), as bf16: once rounded.
@@ -1139,13 +1139,12 @@ __global__ __launch_bounds__(64 * WAVES) void multi_combine(TiledArgs a) {
   *reinterpret_cast<uint4*>(a.out + ((int64_t)(item.x + p) * a.hq + head) * kHead + d0) = o;
 }
 
-// Prefill with exact_p set: the hi + lo P.V variant (prefill only; DiT rounds
-// P to bf16 as hidream.cu does).
+// A plan's exact_p: the hi + lo P.V variant (not DiT, which rounds P to bf16 as
+// hidream.cu does).
 template <int G, int SRC, int FORM>
 void launch_g(const TiledArgs& a, int grid, int items, int ntiles, hipStream_t stream) {
-  constexpr bool CAN = SRC != kDense && SRC < kCross;  // several rows per sequence: P rounded
-  if (CAN && a.exact_p)
-    tiled_attn<G, SRC, FORM, CAN><<<grid, kThreads, 0, stream>>>(a, items, ntiles);
+  if (SRC != kDense && a.exact_p)
+    tiled_attn<G, SRC, FORM, SRC != kDense><<<grid, kThreads, 0, stream>>>(a, items, ntiles);
   else
     tiled_attn<G, SRC, FORM><<<grid, kThreads, 0, stream>>>(a, items, ntiles);
 }

@@ -149,6 +149,7 @@ class MultiPlan(ctypes.Structure):
         ("tile_units", ctypes.c_int32),
         ("split_tiles", ctypes.c_int32),
         ("tile_segments", ctypes.c_int32),
+        ("exact_p", ctypes.c_int32),
         ("work_bytes", ctypes.c_int64),
         ("workspace_bytes", ctypes.c_int64),
     ]
@@ -751,7 +752,7 @@ class Multi:
     work: object  # device int32 tensor
 
 
-def _multi_plan(init, counts, keys, hq, hk, max_len, chunk, device) -> Multi:
+def _multi_plan(init, counts, keys, hq, hk, max_len, chunk, device, exact_p) -> Multi:
     import numpy as np
 
     counts_a = np.ascontiguousarray(counts, dtype=np.int32)
@@ -765,20 +766,22 @@ def _multi_plan(init, counts, keys, hq, hk, max_len, chunk, device) -> Multi:
         _check(rc)
     work_h = np.zeros(max(4, int(plan.work_bytes) // 4), dtype=np.int32)
     _check(init(len(counts_a), ptr(counts_a), ptr(keys_a), hq, hk, max_len, chunk, ptr(work_h), len(work_h), ctypes.byref(plan)))
+    plan.exact_p = 1 if exact_p else 0
     return Multi(plan, _torch.from_numpy(work_h).to(device))
 
 
-def extend_plan(counts, hq, hk, max_len, keys=None, chunk=0, device="cuda") -> Multi:
+def extend_plan(counts, hq, hk, max_len, keys=None, chunk=0, device="cuda", exact_p=False) -> Multi:
     """Host plan of qwen3_extend_q8 for ``counts[s]`` rows of each sequence;
     uploads the work list. ``keys``: how many keys each sequence's last row sees
     now, if known (for the choice of kernels, the order and the split sizes alone);
-    the workspace is ``workspace_for(plan.plan)``."""
-    return _multi_plan(load().omni_attn_extend_plan_init, counts, keys, hq, hk, max_len, chunk, device)
+    exact_p: P in 16 bits in every row (else rounded to bf16 in rows that run in
+    tiles); the workspace is ``workspace_for(plan.plan)``."""
+    return _multi_plan(load().omni_attn_extend_plan_init, counts, keys, hq, hk, max_len, chunk, device, exact_p)
 
 
-def cross_plan(counts, hq, hk, max_len, keys=None, chunk=0, device="cuda") -> Multi:
+def cross_plan(counts, hq, hk, max_len, keys=None, chunk=0, device="cuda", exact_p=False) -> Multi:
     """Host plan of cross_run for ``counts[s]`` rows over each source, as extend_plan."""
-    return _multi_plan(load().omni_attn_cross_plan_init, counts, keys, hq, hk, max_len, chunk, device)
+    return _multi_plan(load().omni_attn_cross_plan_init, counts, keys, hq, hk, max_len, chunk, device, exact_p)
 
 
 def _multi_ws(plan, workspace, d):
