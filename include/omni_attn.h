@@ -579,9 +579,14 @@ int omni_attn_cross_run(const omni_attn_multi_plan* plan, const void* q, int64_t
  *   OMNI_ATTN_TABLES_PAGES      more moves than src and dst hold
  *   OMNI_ATTN_TABLES_LINE       an entry has more than table_ld pages
  *   OMNI_ATTN_TABLES_EXHAUSTED  fewer free pages than are needed
- *   OMNI_ATTN_PAGES_UNHELD      (pages_free) more pages came back than were in use:
+ *   OMNI_ATTN_PAGES_UNHELD      (pages_free) pages came back that nobody held, being
+ *                               in the queue already, or more than were in use:
  *                               shares, table and queue do not agree. The holders
- *                               are counted down, and the queue stays
+ *                               are counted down to none at least, and the queue
+ *                               stays, without any page of the call. So a line that
+ *                               is given back twice is found while one of its pages
+ *                               is free; once others have taken them all, it is not,
+ *                               and they lose theirs
  * Tables have at most 2^18 lines, pools that are compacted at most 2^19 pages. Page
  * ids of a line that are outside the pool are passed over. Calls that share a
  * table, a queue or shares follow one another on a stream. */

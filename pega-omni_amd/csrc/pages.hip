@@ -197,51 +197,109 @@ __global__ __launch_bounds__(kForkThreads) void pages_drop(PagesArgs a) {
 }
 
 // The pages without a holder, in ascending order, to the queue's end. One workgroup,
-// a wave for each sixteenth of the pool: counted, then written. SAME: the launch that
-// dropped them, so that the counts are read where its atomics work, past the caches.
-// Bound by a round trip for the counts, eight rounds of a wave's at a time, and the
-// exchange between waves: 4.6 us, behind 4.2 of drops, for 224 lines of 100-4000 tokens.
+// a wave for each sixteenth of the pool: counted, then written, from bits in LDS. A page
+// that is in the queue already was held by nobody: the queue is looked through for those
+// before anything joins it. SAME: the launch that dropped them, so that the counts are
+// read where its atomics work, past the caches.
+// Bound by round trips, a batch's under way while the one before is looked at: for the
+// counts, eight rounds of a wave's, and the queue, 8192 entries, of which a thread's first
+// is asked for beforehand. A fork of a few lines and their end, us: pools of 4600 pages
+// with 600 in the queue 14.6, 31,000 with 30,930 21, 524,288 with 511,788 197 (287 when
+// the counts were read twice, one batch after the other, and the queue not at all). All of
+// the array asked for at the start, which needs no head, and 16 at a time were slower: the
+// instructions of sixteen waves, 0.1 us for two dozen, count as much as a round trip.
 constexpr int kGatherThreads = 1024;
 
+struct Returned {
+  uint64_t bits[kMostPool / 64];  // pages without a holder, where the pool has so many at most
+  int count[kGatherThreads / 64];
+  int twice;
+};
+
+// A thread's entries of the queue from entry k0 on, the last one again past its end.
+constexpr int kQueueAhead = 8;
+struct Queued {
+  int id[kQueueAhead];
+};
+__device__ __forceinline__ int queued_at(const PagesArgs& a, uint32_t k, int head, int avail) {
+  return a.free_pages[queue_at(head, (int)min(k, (uint32_t)avail - 1), a.num_pages)];
+}
+__device__ __forceinline__ Queued queued_from(const PagesArgs& a, uint32_t k0, int head, int avail) {
+  Queued q;
+#pragma unroll
+  for (int i = 0; i < kQueueAhead; ++i) q.id[i] = queued_at(a, k0 + i * kGatherThreads + threadIdx.x, head, avail);
+  return q;
+}
+// Its first entry, to be asked for early; none where the state is bad.
+__device__ __forceinline__ int queued_first(const PagesArgs& a, int head, int avail) {
+  return avail > 0 && !bad_state(head, avail, a.num_pages) ? queued_at(a, threadIdx.x, head, avail) : -1;
+}
+
 template <bool SAME>
-__device__ __forceinline__ void gather(const PagesArgs& a, int code, int head, int avail) {
+__device__ __forceinline__ void gather(const PagesArgs& a, int code, int head, int avail, int queued0) {
   constexpr int kWaves = kGatherThreads / 64, kAhead = 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ int s_count[kWaves];
+  __shared__ Returned s;
+  const bool kept = a.num_pages <= kMostPool;
   // Rounds of 64 pages; the first `rounds % kWaves` waves have one more.
   const int rounds = (a.num_pages + 63) / 64;
   const int r0 = wave * (rounds / kWaves) + min(wave, rounds % kWaves), r1 = r0 + rounds / kWaves + (wave < rounds % kWaves ? 1 : 0);
   const auto holders = [&](int p) {
     return SAME ? __hip_atomic_load(a.shares + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : a.shares[p];
   };
-  // The pages of kAhead rounds from r on without a holder.
-  const auto look = [&](int r, uint64_t* free) __attribute__((always_inline)) {
-    int v[kAhead];
+  // The holders of kAhead rounds' pages from r on.
+  const auto ask = [&](int r, int* v) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) v[i] = r + i < r1 && 64 * (r + i) + lane < a.num_pages ? holders(64 * (r + i) + lane) : 0;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) free[i] = __ballot(v[i] < 0);
   };
   uint64_t free[kAhead] = {};
   int count = 0;
+  if (kept)
+    for (int r = r0 + lane; r < r1; r += 64) s.bits[r] = 0;
+  int v[kAhead], next[kAhead] = {};
+  ask(r0, v);
   for (int r = r0; r < r1; r += kAhead) {
-    look(r, free);
+    if (r + kAhead < r1) ask(r + kAhead, next);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) count += __popcll(free[i]);
+    for (int i = 0; i < kAhead; ++i) free[i] = __ballot(v[i] < 0), v[i] = next[i];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (free[i] == 0) continue;  // uniform
+      count += __popcll(free[i]);
+      if (kept && lane == 0) s.bits[r + i] = free[i];
+    }
   }
   if (code) {  // nothing was dropped
     if (tid == 0) a.status[1] = 0, a.status[3] = head, a.status[4] = avail;
     return;
   }
-  if (lane == 0) s_count[wave] = count;
+  if (lane == 0) s.count[wave] = count;
+  if (tid == 0) s.twice = 0;
   __syncthreads();
   int at = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) at += s_count[w];
-    total += s_count[w];
+    if (w < wave) at += s.count[w];
+    total += s.count[w];
   }
-  const bool fits = total <= a.num_pages - avail;  // else pages were given back that nobody held
+  bool twice = false;
+  const auto back = [&](int id) {
+    return id >= 0 && id < a.num_pages && (kept ? (s.bits[id >> 6] >> (id & 63) & 1) != 0 : holders(id) < 0);
+  };
+  if (total > 0) twice = back(queued0);
+  if (total > 0 && avail > kGatherThreads) {
+    Queued q = queued_from(a, kGatherThreads, head, avail);
+    for (uint32_t k0 = kGatherThreads; k0 < (uint32_t)avail; k0 += kQueueAhead * kGatherThreads) {
+      const Queued next = queued_from(a, k0 + kQueueAhead * kGatherThreads, head, avail);
+#pragma unroll
+      for (int i = 0; i < kQueueAhead; ++i) twice |= back(q.id[i]);
+      q = next;
+    }
+  }
+  if (twice) s.twice = 1;
+  __syncthreads();
+  // Else pages were given back that nobody held: they are in the queue, or there are more than were in use.
+  const bool fits = !s.twice && total <= a.num_pages - avail;
   if (tid == 0) {
     if (!fits) a.status[0] = kUnheld;
     a.status[1] = fits ? total : 0;
@@ -250,7 +308,16 @@ __device__ __forceinline__ void gather(const PagesArgs& a, int code, int head, i
   }
   if (count == 0) return;
   for (int r = r0; r < r1; r += kAhead) {
-    if (r1 - r0 > kAhead) look(r, free);  // else they are the ones at hand
+    if (r1 - r0 > kAhead) {  // else they are the ones at hand
+      if (kept) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) free[i] = r + i < r1 ? s.bits[r + i] : 0;
+      } else {
+        ask(r, v);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) free[i] = __ballot(v[i] < 0);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int p = 64 * (r + i) + lane;
@@ -264,7 +331,8 @@ __device__ __forceinline__ void gather(const PagesArgs& a, int code, int head, i
 }
 
 __global__ __launch_bounds__(kGatherThreads) void pages_gather(PagesArgs a) {
-  gather<false>(a, a.status[0], a.free_state[0], a.free_state[1]);
+  const int head = a.free_state[0], avail = a.free_state[1];
+  gather<false>(a, a.status[0], head, avail, queued_first(a, head, avail));
 }
 
 // Both for a few short lines, a wave each, in one workgroup and launch: 8 lines of 12
@@ -272,6 +340,7 @@ __global__ __launch_bounds__(kGatherThreads) void pages_gather(PagesArgs a) {
 __global__ __launch_bounds__(kGatherThreads) void pages_end(PagesArgs a) {
   __shared__ Looked<kGatherThreads> s;
   const int head = a.free_state[0], avail = a.free_state[1];
+  const int queued0 = queued_first(a, head, avail);
   const int code = free_code(a, s, head, avail);
   if (!code) {
     for (int i = threadIdx.x >> 6; i < a.n; i += kGatherThreads / 64) {
@@ -285,7 +354,7 @@ __global__ __launch_bounds__(kGatherThreads) void pages_end(PagesArgs a) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the counts are down before the barrier (a device fence took 3 us more)
   }
   __syncthreads();
-  gather<true>(a, code, head, avail);
+  gather<true>(a, code, head, avail, queued0);
 }
 
 // ------------------------------------------------------------------ compact
