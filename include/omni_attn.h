@@ -588,8 +588,9 @@ int omni_attn_cross_run(const omni_attn_multi_plan* plan, const void* q, int64_t
  *                               is free; once others have taken them all, it is not,
  *                               and they lose theirs
  * Tables have at most 2^18 lines, pools that are compacted at most 2^19 pages. Page
- * ids of a line that are outside the pool are passed over. Calls that share a
- * table, a queue or shares follow one another on a stream. */
+ * ids of a line that are outside the pool are passed over. What a call writes lies
+ * apart from all else that it is given. Calls that share a table, a queue or shares
+ * follow one another on a stream. */
 #define OMNI_ATTN_PAGES_UNHELD 6
 
 /* Fork i: line children[i] begins with the first tokens[i] tokens of line
@@ -622,7 +623,7 @@ int omni_attn_pages_free(const int32_t* lines, const int32_t* tokens, int n, int
  * below the limit first), -1 past the last. status = {code, moves, free pages below
  * the limit, 0, free pages}: to shrink the pool, go on with num_pages = limit and
  * status[2] free entries from head 0; to keep it, with &status[3].
- * table_out may be the table; the other outputs are buffers of their own. Page
+ * table_out may be the table, which is then changed in place. Page
  * lists that omni_attn_step_tables made before are out of date. */
 int omni_attn_pages_compact(const int32_t* table, int64_t table_ld, int num_lines, const int32_t* free_pages,
                             int num_pages, const int32_t* free_state, const int32_t* shares, int limit,

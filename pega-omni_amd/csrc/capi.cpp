@@ -13,6 +13,7 @@
 #include <cstdio>
 #include <cstring>
 #include <functional>
+#include <iterator>
 #include <new>
 #include <vector>
 
@@ -1541,6 +1542,28 @@ int omni_attn_cross_run(const omni_attn_multi_plan* plan, const void* q, int64_t
 
 namespace {
 
+// int32 entries that a call is given, and whether it writes them.
+struct Span {
+  const char* name;
+  const int32_t* at;
+  int64_t n;
+  bool written;
+};
+
+// Workgroups read lists, state, table, counts and queue while others write: nothing that
+// is written overlaps anything else.
+int apart(const Span* spans, int count, const char* who) {
+  const auto begin = [](const Span& s) { return (uint64_t)(uintptr_t)s.at; };
+  const auto end = [&](const Span& s) { return begin(s) + 4 * (uint64_t)s.n; };
+  for (int i = 0; i < count; ++i)
+    for (int j = 0; j < i; ++j) {
+      const Span &x = spans[j], &y = spans[i];
+      if ((x.written || y.written) && x.n > 0 && y.n > 0 && begin(x) < end(y) && begin(y) < end(x))
+        return fail(OMNI_ATTN_EINVAL, "%s: %s and %s overlap", who, x.name, y.name);
+    }
+  return 0;
+}
+
 // What fork and free have in common.
 int pages_common(omni::PagesArgs& a, int page, const char* who) {
   if (a.n < 0 || page <= 0 || a.table_ld < 0 || a.num_lines < 0 || a.num_pages <= 0)
@@ -1555,6 +1578,8 @@ int pages_common(omni::PagesArgs& a, int page, const char* who) {
   a.pd = omni::make_page_div(page);
   return 0;
 }
+
+int64_t table_cells(const omni::PagesArgs& a) { return a.n > 0 ? std::min<int64_t>(a.table_ld, 1LL << 40) * a.num_lines : 0; }
 
 }  // namespace
 
@@ -1580,6 +1605,11 @@ int omni_attn_pages_fork(const int32_t* parents, const int32_t* children, const 
   a.status = status;
   if (int rc = pages_common(a, page, "pages_fork")) return rc;
   if (n > 0 && (!parents || !src || !dst)) return fail(OMNI_ATTN_EINVAL, "pages_fork: null device pointer");
+  const Span spans[] = {{"parents", parents, n, false},         {"children", children, n, false}, {"tokens", tokens, n, false},
+                        {"free_pages", free_pages, num_pages, false}, {"free_state", free_state, 2, false}, {"table", table, table_cells(a), true},
+                        {"shares", shares, num_pages, true},    {"src", src, n, true},            {"dst", dst, n, true},
+                        {"status", status, 5, true}};
+  if (int rc = apart(spans, (int)std::size(spans), "pages_fork")) return rc;
   if (omni::launch_pages_fork(a, as_stream(stream)) != 0)
     return fail(OMNI_ATTN_ELAUNCH, "pages_fork: launch failed: %s", hipGetErrorString(omni::g_launch_status));
   return ok();
@@ -1601,6 +1631,10 @@ int omni_attn_pages_free(const int32_t* lines, const int32_t* tokens, int n, int
   a.shares = shares;
   a.status = status;
   if (int rc = pages_common(a, page, "pages_free")) return rc;
+  const Span spans[] = {{"lines", lines, n, false},           {"tokens", tokens, n, false},          {"table", table, table_cells(a), false},
+                        {"free_state", free_state, 2, false}, {"free_pages", free_pages, num_pages, true}, {"shares", shares, num_pages, true},
+                        {"status", status, 5, true}};
+  if (int rc = apart(spans, (int)std::size(spans), "pages_free")) return rc;
   if (omni::launch_pages_free(a, as_stream(stream)) != 0)
     return fail(OMNI_ATTN_ELAUNCH, "pages_free: launch failed: %s", hipGetErrorString(omni::g_launch_status));
   return ok();
@@ -1622,12 +1656,12 @@ int omni_attn_pages_compact(const int32_t* table, int64_t table_ld, int num_line
     return fail(OMNI_ATTN_EINVAL, "%s: null device pointer", who);
   if (free_state + 2 > status && free_state < status + 5)
     return fail(OMNI_ATTN_EINVAL, "%s: free_state lies in status (two status buffers take turns)", who);
-  // Workgroups read all of the queue and any page's holders while others write.
-  if ((free_out + num_pages > free_pages && free_out < free_pages + num_pages) ||
-      (shares_out + num_pages > shares && shares_out < shares + num_pages))
-    return fail(OMNI_ATTN_EINVAL, "%s: free_out and shares_out are buffers of their own", who);
-  if (cells > 0 && table_out != table && table_out + cells > table && table_out < table + cells)
-    return fail(OMNI_ATTN_EINVAL, "%s: table_out is the table or a buffer of its own", who);
+  const bool in_place = table_out == table;
+  const Span spans[] = {{"table", table, cells, in_place},            {"free_pages", free_pages, num_pages, false}, {"free_state", free_state, 2, false},
+                        {"shares", shares, num_pages, false},         {"table_out", table_out, in_place ? 0 : cells, true}, {"free_out", free_out, num_pages, true},
+                        {"shares_out", shares_out, num_pages, true},  {"new_ids", new_ids, num_pages, true},        {"src", src, move_cap, true},
+                        {"dst", dst, move_cap, true},                 {"status", status, 5, true}};
+  if (int rc = apart(spans, (int)std::size(spans), who)) return rc;
   omni::CompactArgs a{};
   a.table = table;
   a.table_out = table_out;
