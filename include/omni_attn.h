@@ -383,7 +383,8 @@ int64_t omni_hidream_workspace_bytes(void);
  * token a sequence. omni_qwen3_attend, the prefill and the calls over the 8-bit
  * cache (omni_qwen3_rope_q8, omni_qwen3_attend_q8) know no ring: they see keys
  * 0..pos, and past the ring would look up pages that the sequence does not
- * list. They take tables made with ring = 0 only.
+ * list. They take tables made with ring = 0 only. So do lines that share pages
+ * (omni_attn_pages_fork): a ring would write to pages that others read.
  *
  * Pages come from the free queue: entries head, head + 1, .. (modulo num_pages)
  * of free_pages [num_pages], num_pages being the pool's pages, with free_state =
@@ -568,7 +569,15 @@ int omni_attn_cross_run(const omni_attn_multi_plan* plan, const void* q, int64_t
  * the start, and for every free page. omni_attn_step_tables knows nothing of it: a
  * request that shares pages ends with omni_attn_pages_free, not with count < 0
  * (one that shares none may end either way). New rows are written behind a line's
- * last token, so never to a shared page.
+ * last token, so never to a shared page, as long as the line only grows:
+ *  - A line that shares pages, parent or child, does not come round a ring: position
+ *    p is written at p % ring, in a page that others read, and by all of them. Its
+ *    tables are made with ring = 0 for as long as it lives (or the ring is longer
+ *    than it will ever be). No call can see that; a line that a ring takes round is
+ *    copied (omni_attn_pages_copy to pages of its own), not forked. pages_free takes
+ *    such a line with at most ring tokens: it holds no more pages.
+ *  - It does not go back to fewer tokens than a fork of it shares: one that proposes
+ *    tokens and takes them back is forked at what stays.
  *
  * Lists of n entries are looked over before anything is written; an entry with
  * tokens < 0 is none (the padding of a captured call). status int32[5] = {code,

@@ -839,7 +839,8 @@ def pages_fork(parents, children, tokens, table, free_pages, free_state, shares,
     beside the first), the part-filled one a page of its own from the free queue,
     to be copied by ``pages_copy(.., src, dst)``. ``status`` = [code, pages taken,
     pages shared, head, free entries]; ``status[3:5]`` is the next call's free_state.
-    tokens < 0: no fork."""
+    tokens < 0: no fork. Lines that share pages take tables without a ring, whose
+    rows would come round to the shared pages."""
     d = _current_device() if parents.is_cuda else -1
     n, (lines, ld), pool = parents.numel(), _table_shape(table), free_pages.numel()
     (p_par, p_chi, p_tok, p_table, p_free, p_state, p_shares, p_src, p_dst, p_status) = _take(
