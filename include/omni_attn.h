@@ -538,9 +538,9 @@ int omni_attn_cross_plan_init(int nseq, const int32_t* counts_h, const int32_t* 
  * P is carried in 16 bits in groups and, unless the plan's exact_p is set, rounded to
  * bf16 in tiles, which also take K and V as bf16 (exact, but for values that bf16 does not hold: 2^128, which
  * rounding to 8 bits can make, and what lies below 2^-126). P is at most 1 on the
- * way, as in omni_qwen3_attend_q8. Tokens past the last key that a row of the group
- * or tile sees may hold anything; among their own keys, an infinity or NaN in V
- * reaches the rows of its group or tile that see earlier keys only.
+ * way, as in omni_qwen3_attend_q8. Tokens past a row's position may hold anything,
+ * but that in tiles an infinity or NaN in V, among the keys that some row of the
+ * tile sees, reaches its rows that see earlier keys only.
  * A workspace serves one call at a time: two captured graphs that may run at once
  * need one each. `work` is the device copy of this plan's work list. */
 int omni_qwen3_extend_q8(const omni_attn_multi_plan* plan, const void* q, int64_t q_stride, const void* kv,

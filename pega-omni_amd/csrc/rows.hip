@@ -16,7 +16,10 @@
 //     reads take eight keys of a dim.
 // K and V operands are made once a tile and serve NC columns blocks. P is carried as
 // two bf16 terms (hi + lo, 16 bits) and is at most 1 on the way: the running base
-// stands 8 (log2) above the maximum that moved it.
+// stands 8 (log2) above the maximum that moved it. What a row's later keys hold does
+// not reach it: their scores go, and as 0 times a NaN of V is NaN, those count as 0 in
+// the tiles that not all rows see whole, and come back in the end for the rows that see
+// them (0.25 us of the 31 below).
 //
 // The keys' bytes bound it where groups are many: 64 sequences of 4 rows over 200-2400
 // tokens of 16q/8kv, E4M3, 31.0 us, 5.5 TB/s (a row per workgroup, each reading the keys
@@ -88,6 +91,12 @@ __device__ __forceinline__ int row16_max(int v) {
 
 // c / G for packed columns: 0 <= c < 32, 1 <= G <= 16 (g16 = 65536 / G + 1).
 __device__ __forceinline__ int row_of_column(int c, int g16) { return c * g16 >> 16; }
+
+// v, so that what follows from it is worked out here and not held in registers through a loop.
+__device__ __forceinline__ int here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 
 // Waves per SIMD that a kernel's registers (bf16: its LDS) leave room for.
 constexpr int room(int src, int nc) { return nc == 2 || src == kBf16 ? 2 : 4; }
@@ -164,6 +173,11 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
   constexpr int kPart = 16 * (kHead + 4), kVTile = kTile * kHead;
   __shared__ __align__(16) float s_buf[kWaves * (Q8 ? kPart : kVTile)];
   __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+  // E4M3: of each wave, the first key that holds a NaN in dim d of V among the keys that
+  // not all rows see, and whether there is one at all.
+  constexpr bool NANS = Q8 && FMT == kQ8E4m3;
+  __shared__ int s_nan[NANS ? kWaves : 1][kHead], s_bad[kWaves];
+  int bad = 0;
   bf16_t* v_lds = reinterpret_cast<bf16_t*>(s_buf) + wave * (2 * kVTile);
 
   // bf16: a tile's rows from a scalar base, each lane's first one at a constant offset
@@ -278,15 +292,16 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
 #pragma unroll
       for (int t = 0; t < 8; ++t) s[b][t] *= ks;
     if (n0 + kTile > least) {  // keys that some row does not see
+      const int key = n0 + 8 * (here(lane) >> 4);
 #pragma unroll
       for (int b = 0; b < NC; ++b)
 #pragma unroll
         for (int t = 0; t < 8; ++t)
-          if (n0 + 8 * grp + t >= lim[b]) s[b][t] = -INFINITY;
+          if (key + t >= lim[b]) s[b][t] = -INFINITY;
     }
     if constexpr (Q8) {
       if (left < kTile) {  // nothing past the last key that any row sees counts, whatever it holds
-        const int tokens = left - kQ8Block * (grp >> 1);  // of this lane's block
+        const int tokens = left - kQ8Block * (here(lane) >> 5);  // of this lane's block
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int n_ok = min(max(tokens - 4 * w, 0), 4);
@@ -324,6 +339,35 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
 #pragma unroll
       for (int t = 0; t < 8; ++t) rest[t] = s[b][t] - rest[t];
       ph[b] = __builtin_bit_cast(bf16x8, hi), pl[b] = __builtin_bit_cast(bf16x8, pack8(rest));
+    }
+    if constexpr (NANS) {
+      // A NaN times the weight 0 of a row that does not see its key is NaN: where such
+      // rows are it counts as 0 here, and the rows that do see it get it in the end.
+      if (n0 + kTile > least) {
+        const auto nan_bits = [](uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };  // 0x80 in a byte of 0x7f or 0xff
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) any |= nan_bits((&vr[i].x)[w]);
+        if (__any(any != 0)) {
+          const int ln = here(lane);
+          if (!bad) s_nan[wave][ln] = s_nan[wave][ln + 64] = INT_MAX;
+          bad = 1;
+          const int dim = ln & 31, key = n0 + (ln & 32) / (32 / kQ8Block);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            int first = INT_MAX;
+#pragma unroll
+            for (int w = 3; w >= 0; --w) {
+              const uint32_t x = (&vr[i].x)[w], nan = nan_bits(x);
+              if (nan) first = key + 4 * w + (__ffs(nan) - 8) / 8;
+              (&vr[i].x)[w] = x & ~((nan >> 7) * 0xffu);
+            }
+            atomicMin(&s_nan[wave][32 * i + dim], first);
+          }
+        }
+      }
     }
     const auto weigh = [&](int i, const bf16x8& v) __attribute__((always_inline)) {
 #pragma unroll
@@ -368,6 +412,7 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
     for (int i = 0; i < 8; ++i)
       *reinterpret_cast<f32x4*>(s_buf + wave * kPart + col * (kHead + 4) + 16 * i + 4 * grp) = o[b][i];
     if (grp == 0) s_m[wave][col] = m[b], s_l[wave][col] = l[b];
+    if (NANS && lane == 0) s_bad[wave] = bad;
     __syncthreads();
 #pragma unroll
     for (int it = 0; it < 16 * kHead / 4 / kThreads; ++it) {  // four dims of a column a thread
@@ -386,6 +431,14 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
       }
       const int row = row_of_column(c, a.g16), head = kh * G + c - row * G;
       const int64_t h = (int64_t)(item.y + row) * a.hq + head;
+      if (NANS && (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3])) {
+        const int last = a.pos[item.y + row];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (s_bad[w] && s_nan[w][d + e] <= last) num[e] = NAN;
+      }
       if (used == 1) {
         uint2 w = make_uint2(pack_bf16x2(num[0] / den, num[1] / den), pack_bf16x2(num[2] / den, num[3] / den));
         if (Q8 && a.pos[item.y + row] < 0) w = make_uint2(0, 0);  // a row that is none, among rows that see keys
