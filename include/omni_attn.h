@@ -536,11 +536,10 @@ int omni_attn_cross_plan_init(int nseq, const int32_t* counts_h, const int32_t* 
  * 1 entries. q rows [hq][128] of stride q_stride (a multiple of 8), out rows
  * [hq][128]; rows past the plan's are left as they were.
  * P is carried in 16 bits in groups and, unless the plan's exact_p is set, rounded to
- * bf16 in tiles, which also take K and V as bf16 (exact, but for values that bf16 does not hold: 2^128, which
- * rounding to 8 bits can make, and what lies below 2^-126). P is at most 1 on the
- * way, as in omni_qwen3_attend_q8. Tokens past a row's position may hold anything,
- * but that in tiles an infinity or NaN in V, among the keys that some row of the
- * tile sees, reaches its rows that see earlier keys only.
+ * bf16 in tiles, which also take K and V as bf16: exact, but for what lies below
+ * 2^-126, and 2^128, which rounding to E4M3 can make and which counts as the largest
+ * bf16 value. P is at most 1 on the way, as in omni_qwen3_attend_q8. Tokens past a
+ * row's position may hold anything, NaN among them, whatever other rows see of them.
  * A workspace serves one call at a time: two captured graphs that may run at once
  * need one each. `work` is the device copy of this plan's work list. */
 int omni_qwen3_extend_q8(const omni_attn_multi_plan* plan, const void* q, int64_t q_stride, const void* kv,

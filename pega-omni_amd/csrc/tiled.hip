@@ -129,6 +129,7 @@ struct Tile {
   int nq;             // positions in the tile (<= 128 / G)
   int len;            // keys of the source
   int last;           // keys any row of the tile sees
+  int apart;          // 8-bit cache: of those, keys that not all rows see
   int qpos0;          // DiT: position of row 0 (causal rule n sees 0..n)
   const int32_t* pos; // prefill: positions of the tile's rows
   // key sources
@@ -186,6 +187,15 @@ __device__ __forceinline__ uint2 scaled_bf16(uint32_t w, float scale) {
     from_bytes<kQ8Int8>(w, v);
     return make_uint2(pack_bf16x2(v[0] * scale, v[1] * scale), pack_bf16x2(v[2] * scale, v[3] * scale));
   }
+}
+
+// E4M3 blocks of this scale hold 2^128 where a bf16 value was rounded up to it, past bf16's
+// range: taken as its largest value (2^-8 less), not as an infinity, which 0 does not weigh
+// out. (Integers: 127 2^121 is below.)
+constexpr float kReachesInf = 0x1p120f;
+__device__ __forceinline__ void finite(uint32_t& w) {
+  if ((w & 0x7fffu) == 0x7f80u) w -= 1u;
+  if ((w & 0x7fff0000u) == 0x7f800000u) w -= 0x10000u;
 }
 
 template <int G, int SRC, int FORM = kWhole, bool EXACT = false>
@@ -310,11 +320,15 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     } else {
       t.pos = a.pos + first;
       t.pg = a.pages + a.indptr[item.x];
-      int most = -1;  // of this workgroup's rows
-      for (int i = (part > 0 ? kPartPos * part : 0) + (threadIdx.x & 63); i < ends(t.nq); i += 64) most = max(most, t.pos[i]);
+      int most = -1, not_least = INT_MIN;  // of this workgroup's rows
+      for (int i = (part > 0 ? kPartPos * part : 0) + (threadIdx.x & 63); i < ends(t.nq); i += 64) {
+        const int pos = max(t.pos[i], -1);
+        most = max(most, pos), not_least = max(not_least, ~pos);
+      }
 #pragma unroll
-      for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d));
+      for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d)), not_least = max(not_least, __shfl_xor(not_least, d));
       t.last = __builtin_amdgcn_readfirstlane(most) + 1;
+      t.apart = t.last + __builtin_amdgcn_readfirstlane(not_least);
     }
     t.len = t.last;
   } else if constexpr (SRC == kPacked) {
@@ -491,6 +505,12 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   uint4 raw[4];
   float k_by = 0.f, v_by = 0.f;  // scales of the block in `raw`
   int raw_left = 0;              // tokens from its first to the last that any row sees
+  // E4M3: of each wave's blocks, the first key that holds a NaN in dim d of V among the
+  // keys that not all rows see, and whether there is one at all.
+  constexpr bool NANS = SRC == kCacheE4m3;
+  __shared__ int s_nan[NANS ? kThreads / 64 : 1][kHead], s_bad[kThreads / 64];
+  int bad = 0;
+  if (NANS && lane == 0) s_bad[wave_u] = 0;
   auto look_up = [&](int st) __attribute__((always_inline)) {
     const int b = (int)min((int64_t)(st + lane) * (kBN / kQ8Block) + wave_u, (int64_t)((t.last - 1) / kQ8Block));
     block_ids = (int)page_slot(a.pd, t.pg[page_index(a.pd, b)], b);
@@ -506,7 +526,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     const uint8_t* vb = kb + (int64_t)a.hk * kQ8HeadBytes;
     raw[0] = ldg16(kb), raw[1] = ldg16(kb + 1024), raw[2] = ldg16(vb), raw[3] = ldg16(vb + 1024);
     k_by = pow2_biased(exps & 0xff), v_by = pow2_biased(exps >> 16);
-    raw_left = (int)min((int64_t)t.last - (int64_t)st * kBN - kQ8Block * wave_u, (int64_t)kQ8Block);
+    raw_left = (int)((int64_t)t.last - (int64_t)st * kBN - kQ8Block * wave_u);
   };
   auto put_block = [&](bf16_t* kd) __attribute__((always_inline)) {
     if (raw_left < kQ8Block) {  // V of tokens that no row sees weighs 0, whatever it holds
@@ -515,6 +535,36 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
         const int n_ok = min(max(raw_left - 4 * w, 0), 4);
         const uint32_t stay = n_ok == 4 ? ~0u : (1u << (8 * n_ok)) - 1;
         (&raw[2].x)[w] &= stay, (&raw[3].x)[w] &= stay;
+      }
+    }
+    if constexpr (NANS) {
+      // A NaN times the weight 0 of a row that does not see its key is NaN: where such
+      // rows are it counts as 0 here, and the rows that do see it get it in the end.
+      if (raw_left < t.apart + kQ8Block) {
+        const auto nan_bits = [](uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };  // 0x80 in a byte of 0x7f or 0xff
+        uint32_t any = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) any |= nan_bits((&raw[2].x)[w]) | nan_bits((&raw[3].x)[w]);
+        if (__builtin_expect(__any(any != 0), 0)) {
+          int ln = lane;
+          asm volatile("" : "+v"(ln));  // worked out here, not held in registers through the key loop
+          if (!bad) {
+            s_nan[wave_u][ln] = s_nan[wave_u][ln + 64] = INT_MAX;
+            if (ln == 0) s_bad[wave_u] = 1;
+          }
+          bad = 1;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            int first = INT_MAX;
+#pragma unroll
+            for (int w = 3; w >= 0; --w) {
+              const uint32_t x = (&raw[2 + i].x)[w], nan = nan_bits(x);
+              if (nan) first = t.last - raw_left + 4 * w + ((__ffs(nan) - 8) >> 3);
+              (&raw[2 + i].x)[w] = x & ~((nan >> 7) * 0xffu);
+            }
+            s_nan[wave_u][ln + 64 * i] = min(s_nan[wave_u][ln + 64 * i], first);  // the lane's own
+          }
+        }
       }
     }
 #pragma unroll
@@ -532,11 +582,24 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       *reinterpret_cast<uint4*>(vd + 8 * kHead) = make_uint4(v1.x, v1.y, v3.x, v3.y);
     }
   };
+  // What put_block wrote, before the barrier that shows it to others: no infinities.
+  auto check_block = [&](bf16_t* kd) __attribute__((always_inline)) {
+    if (SRC != kCacheE4m3 || __builtin_expect(k_by < kReachesInf && v_by < kReachesInf, 1)) return;
+    wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint4* at = reinterpret_cast<uint4*>(kd + (i < 4 ? 0 : kTileElems) + wave_u * (kQ8Block * kHead)) + 64 * (i & 3) + lane;
+      uint4 u = *at;
+      finite(u.x), finite(u.y), finite(u.z), finite(u.w);
+      *at = u;
+    }
+  };
   // The whole tile st into buffer kd.
   auto issue_tile = [&](int st, bf16_t* kd) __attribute__((always_inline)) {
     if constexpr (Q8) {
       ask_block(st);
       put_block(kd);
+      check_block(kd);
     } else if constexpr (SRC != kPagedLane) {
       aim_tile(st);
 #pragma unroll
@@ -564,6 +627,29 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
         dma_global16(t.vbase + voffs[i], vd + lrow);
       }
     }
+  };
+
+  // NaN to dims 32 md .. + 31 of a row (registers as in o below) where a key that it sees
+  // has one; after the loop's last barrier, with 128 bytes of the wave's own.
+  auto any_nans = [&]() {
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) any |= s_bad[w];
+    return any != 0;
+  };
+  auto give_nans = [&](f32x16* v, int md, int* by_dim) __attribute__((always_inline)) {
+    wave_lds_fence();
+    if (lane < 32) {
+      int first = INT_MAX;
+      for (int w = 0; w < kThreads / 64; ++w)
+        if (s_bad[w]) first = min(first, s_nan[w][32 * md + lane]);
+      by_dim[lane] = first;
+    }
+    wave_lds_fence();
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (by_dim[8 * (e >> 2) + 4 * h + (e & 3)] < lim) (*v)[e] = NAN;
+    wave_lds_fence();
   };
 
   f32x16 o[4];
@@ -745,6 +831,8 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       if constexpr (EXACT) pfl = pnl;
     }
     l += psum;
+    if constexpr (Q8)
+      if (st + 1 < s_hi) check_block(nxt);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();
   };
@@ -781,7 +869,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
       }
       if (!active) {
         if constexpr (Q8) {
-          if (st + 1 < s_hi) put_block(nxt);
+          if (st + 1 < s_hi) put_block(nxt), check_block(nxt);
         } else {
 #pragma unroll
           for (int d = 0; d < kDmas; ++d) dma_tile(d, nxt);
@@ -877,6 +965,8 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
         ov = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks], as_bf16x8(pf[ks]), ov, 0, 0, 0);
         if constexpr (EXACT) ov = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks], as_bf16x8(pfl[ks]), ov, 0, 0, 0);
       }
+      if constexpr (Q8)
+        if (st + 1 < s_hi) check_block(nxt);
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
       __syncthreads();
     };
@@ -896,6 +986,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     __syncthreads();
     bf16_t* rows = smem0 + blk * 32 * kHead;
     if (active) {
+      if (NANS && __builtin_expect(any_nans(), 0)) give_nans(&ov, kg, reinterpret_cast<int*>(smem1) + wave_u * 32);
       const float inv = s_inv[blk][lane];
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
@@ -932,6 +1023,11 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   }
 
   // Register e of block md is dim 32 md + 8 (e / 4) + 4 h + e % 4.
+  if (NANS && __builtin_expect(any_nans(), 0)) {
+    int* by_dim = reinterpret_cast<int*>((wave_u < 4 ? smem0 : smem1) + (wave_u & 3) * 32 * kHead);
+#pragma unroll
+    for (int md = 0; md < 4; ++md) give_nans(&o[md], md, by_dim);
+  }
   l += xor_lane(l, 32);
   if (MULTI ? split : chunk >= 0) {  // a chunk's partial: unnormalised O with its base m and sum l, for the combine
     if (!row_ok) return;  // which reads the tile's positions only
