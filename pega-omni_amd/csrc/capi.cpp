@@ -1133,14 +1133,25 @@ bool multi_fits(const omni_attn_multi_plan& p) {
 int pick_tile_steps(const std::vector<std::array<int32_t, 4>>& tl, int G, int hk, int max_len) {
   const size_t machines = (size_t)std::max(256 / hk, 1);
   const auto steps_of = [&](const std::array<int32_t, 4>& t) { return (int)((std::min((int64_t)t[3], (int64_t)max_len) + 127) / 128); };
+  const auto step_cost = [&](const std::array<int32_t, 4>& t) { return t[2] * G <= 128 ? 2.4 : 3.9; };
   int most = 1;
-  for (const auto& t : tl) most = std::max(most, steps_of(t));
-  if (tl.size() * 2 > 3 * machines) return most;  // enough of them to share the CUs evenly
+  double longest = 0, total = 0;
+  for (const auto& t : tl) {
+    most = std::max(most, steps_of(t));
+    const double c = step_cost(t) * std::max(steps_of(t), 1) + 12;
+    longest = std::max(longest, c), total += c;
+  }
+  // Many tiles share the CUs evenly as they are, unless one is long beside all others (48
+  // tiles of 40 rows over 200 keys and one of 120 over 60,000, 16q/8kv: 1541 us whole, 104
+  // with its keys in 22 splits).
+  const bool many = tl.size() * 2 > 3 * machines;
+  if (many && longest <= 1.5 * total / machines) return most;
+  const size_t limit = 3 * machines + (many ? tl.size() : 0);
   int best = most, last = 0;
   double least = 0;
   std::vector<double> cost, free_at;
-  for (int n = 1; n <= most; ++n) {
-    const int per = (most + n - 1) / n;
+  for (int64_t n = 1; n <= most; n = many ? std::max(n + 1, n * 5 / 4) : n + 1) {
+    const int per = (int)((most + n - 1) / n);
     if (per == last) continue;
     last = per;
     cost.clear();
@@ -1151,9 +1162,9 @@ int pick_tile_steps(const std::vector<std::array<int32_t, 4>>& tl, int G, int hk
       most_used = std::max(most_used, used);
       if (used > 1) partials += (double)used * hk * packed * 2 * kPartialBytes;
       for (int k = 0; k < used; ++k)
-        cost.push_back((packed <= 128 ? 2.4 : 3.9) * std::min(per, steps - k * per) + (used > 1 ? 17 : 12));
+        cost.push_back(step_cost(t) * std::min(per, steps - k * per) + (used > 1 ? 17 : 12));
     }
-    if (n > 1 && cost.size() > 3 * machines) break;
+    if (n > 1 && cost.size() > limit) break;
     std::sort(cost.begin(), cost.end(), std::greater<double>());
     free_at.assign(machines, 0);  // a heap: the CU that comes free first in front
     for (const double c : cost) {
