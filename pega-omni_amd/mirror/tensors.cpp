@@ -11,7 +11,7 @@
 //   b tensor, least           the same of bf16                       -> pointer
 //   r tensor, rows, width     bf16 [>= rows][width], elements of a row adjacent -> pointer, row stride
 //   c kv, kv_scale, 2 hk      the 8-bit cache and its exponents      -> pointer, pointer, format
-//   p kv, kv_scale, page      a cache of one layer or several, 8-bit or (kv_scale None) bf16 slots
+//   p kv, kv_scale, page      a cache of one layer or several, 8-bit or (kv_scale None) bf16 slots or bytes [slots][bytes of one]
 //                             -> pointer, pointer, layers, blocks (slots), bytes and exponents of one, and how many a page has
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -101,11 +101,23 @@ int take_one(char kind, PyObject* const* a, Py_ssize_t left, int64_t device, Ans
     const int64_t page = int_of(a[2]);
     const bool slots = a[1] == Py_None;
     const auto type = t.scalar_type();
+    if (slots && type == at::kByte) {  // FP8 slots, or any of so many bytes
+      if (t.dim() != 2 && t.dim() != 3) throw Bad{" must be uint8 slots [slots][bytes], or layers of them"};
+      const int64_t layers = t.dim() == 3 ? t.size(0) : 1, units = t.size(t.dim() - 2);
+      if (page <= 0) throw Bad{": page=" + std::to_string(page)};
+      if (units % page != 0) throw Bad{" must hold whole pages"};
+      if (!t.is_contiguous()) throw Bad{" must be contiguous"};
+      check_device(t, device);
+      out.put_ptr(t);
+      out.put(Py_NewRef(Py_None));
+      for (const int64_t v : {layers, units, t.size(t.dim() - 1), (int64_t)0, page}) out.put(PyLong_FromLongLong(v));
+      return args;
+    }
     const int64_t lead = t.dim() - 3;  // layers before the blocks
     const bool shaped = (lead == 0 || lead == 1) && t.size(lead + 1) > 0 && t.size(lead + 1) % 2 == 0;
     if (slots ? type != at::kBFloat16 || !shaped || t.size(lead + 2) != 128
               : (type != at::kFloat8_e4m3fn && type != at::kChar) || !shaped || t.size(lead + 2) != 2048)
-      throw Bad{slots ? " must be bf16 slots [slots][2 hk][128], or layers of them"
+      throw Bad{slots ? " must be bf16 slots [slots][2 hk][128] or uint8 slots [slots][bytes], or layers of them"
                       : " must be float8_e4m3fn or int8 [blocks][2 hk][2048], or layers of it"};
     const int64_t units = t.size(lead), heads = t.size(lead + 1), layers = lead ? t.size(0) : 1;
     if (page <= 0 || (!slots && page % 16 != 0)) throw Bad{": page=" + std::to_string(page)};

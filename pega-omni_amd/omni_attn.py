@@ -887,7 +887,8 @@ def pages_copy(kv, kv_scale, src, dst, page=16, count=None, stream=None):
     """Page ``dst[k]`` takes the bytes of page ``src[k]`` in every layer (ids outside
     the pool: no copy; ``count``: a device int32, how many pairs count). kv and
     kv_scale: the 8-bit cache, [blocks][2 hk][2048] and [blocks][2 hk]; kv_scale None:
-    bf16 slots [slots][2 hk][128]; either may have a dimension of layers before."""
+    bf16 slots [slots][2 hk][128], or uint8 slots [slots][bytes] (FP8 slots, of a
+    multiple of 16 bytes a page); each may have a dimension of layers before."""
     d = _current_device() if kv.is_cuda else -1
     n = src.numel()
     p_kv, p_scale, layers, units, width, scales, per, p_src, p_dst, p_count = _take(
