@@ -517,7 +517,9 @@ typedef struct omni_attn_multi_plan {
 /* Host: counts (zero allowed) to a work list. hq / hk from 1 to 16. keys_h (NULL:
  * not known): how many keys each sequence's last row sees when the plan is made,
  * for the choice of kernels, the order of the work and the size of the splits alone;
- * the lengths of a run are read on the device. chunk_hint, a multiple of 64 (<= 0
+ * the lengths of a run are read on the device. They fix the splits, so that a plan
+ * which serves sequences as they grow (a captured call) is given none, or the most
+ * that it will see. chunk_hint, a multiple of 64 (<= 0
  * picks from the shape), is the split of the groups, and keeps sequences apart by
  * their rows alone: up to 16 packed rows, up to 32, and the rest in tiles where hq /
  * hk is at most 8, or 16. Without one they run in one kernel or two, and which one

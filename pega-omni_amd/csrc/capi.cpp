@@ -1231,8 +1231,7 @@ int groups_a_cu(int cross, bool large) { return cross || large ? 2 : 4; }
 //   0.6 for each 1024 workgroups, those that find nothing to do too;
 //   with splits, 7.2 for the merge's launch and 1.1 for each batch of a row's splits: of
 //   16, or (behind two) of 64.
-// Measured at the choice / at the best of the sweep: 0.3% apart in the mean; 5 rows
-// behind 2400 keys of 16q/8kv, 192 keys 9.9 / 9.9; 4 x 8 rows behind 20,000-60,000 of
+// Measured at the choice / at the best of the sweep: 5 rows behind 2400 keys of 16q/8kv, 192 keys 9.9 / 9.9; 4 x 8 rows behind 20,000-60,000 of
 // 32q/8kv, 3584 keys 67.2 / 67.2; 5 candidates of 48 sources of 100-1500 none 31.3 / 31.3;
 // 2 x 20 rows over 30,000-60,000 bf16 keys of 16 heads, 3200 keys 145 / 139 (3584).
 int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, int hk, int max_len, bool known, bool cross) {
@@ -1275,20 +1274,18 @@ int pick_chunk_groups(const std::vector<std::array<int32_t, 4>>* groups, int G, 
 // Which kernel takes a sequence. By itself, one of up to 16 packed rows is a group of one
 // column block, up to 32 a group of two, more are tiles. But each of the three is a launch
 // of its own, whose first 5-10 us no other fills, so a call that would mix them runs in
-// one of them where that is faster. Over 500 drawn calls, against three launches:
+// one of them where that is faster than three launches:
 //   - groups of 32 alone, where a CU gets one of them at most and they have up to 1152
-//     keys: 4 % less over 63 calls that had tiles (58 sequences of 3-20 rows over 173-1039
-//     keys, 8 heads over 2: 27 -> 17.6 us); with more keys or groups the tiles win, which
-//     read a sequence's keys once for 256 packed rows.
+//     keys (58 sequences of 3-20 rows over 173-1039 keys, 8 heads over 2: 27 -> 17.6 us);
+//     with more keys or groups the tiles win, which read a sequence's keys once for 256
+//     packed rows.
 //   - tiles alone, where a CU gets one of them at most and the groups' keys are few: up to
 //     kFewKeyBytes, as a tile of few rows takes 8-bit keys at 3.5 TB/s and a group at 5.5,
 //     or kFewStateBytes (bf16: 7 and 5.5). The 43 us of 13 sequences of 1-10 rows over 650
 //     keys -> 15; 32 and 58 rows over 57,812 and 39,270 bf16 keys of 16 heads 164 -> 154.
 //   - else groups of 32 for all that are no tiles, if any is: the second block costs less
 //     than a launch (13 sources of up to 5387 keys, 3-21 rows, 8 heads: 47 -> 33 us).
-// 141 calls of 500 differ, 0.72 of the time in the mean, the worst 1.11 (7.8 us); at 128 MB
-// to 2 GB of keys 24 of 2500 more, 0.67-0.96. A caller who gives a chunk keeps every
-// sequence where its own rows send it.
+// A caller who gives a chunk keeps every sequence where its own rows send it.
 constexpr double kFewKeyBytes = 128e6, kFewStateBytes = 2e9;
 constexpr int kShortKeys = 1152;
 constexpr int kCus = 256;

@@ -172,7 +172,7 @@ constexpr int kDense = 0, kPagedWave = 1, kPagedLane = 2, kPacked = 3;
 // 4 h + {0..3, 8..11}. Rows without keys store zeros; P is at most 1. The loop is bound
 // as in the other sources, and a step's conversions hide behind its products: 12 chunks
 // of 512-4096 rows behind up to 1024 cached tokens of 32q/8kv, E4M3, 0.79 ms, 1.0
-// PFLOP/s; 12 x 187-4000 rows over 300-2400 bf16 rows 0.54 ms, 1.0 PFLOP/s (EXACT: 1.03
+// PFLOP/s; 12 x 187-4000 rows over 300-2400 bf16 rows 0.54 ms, 1.0 PFLOP/s (EXACT: 1.01
 // and 0.71 ms). 128 keys take 3.9 us, or 2.4 where at most half the waves have rows.
 constexpr int kCross = 4, kCacheE4m3 = 5, kCacheInt8 = 6;
 
