@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
 #pragma unroll
       for (int t = 0; t < 8; ++t) s[b][t] *= ks;
     if (n0 + kTile > least) {  // keys that some row does not see
-      const int key = n0 + 8 * (here(lane) >> 4);
+      const int key = n0 + 8 * ((NANS ? here(lane) : lane) >> 4);
 #pragma unroll
       for (int b = 0; b < NC; ++b)
 #pragma unroll
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
     }
     if constexpr (Q8) {
       if (left < kTile) {  // nothing past the last key that any row sees counts, whatever it holds
-        const int tokens = left - kQ8Block * (here(lane) >> 5);  // of this lane's block
+        const int tokens = left - kQ8Block * ((NANS ? here(lane) : lane) >> 5);  // of this lane's block
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int n_ok = min(max(tokens - 4 * w, 0), 4);
@@ -343,14 +343,16 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
     if constexpr (NANS) {
       // A NaN times the weight 0 of a row that does not see its key is NaN: where such
       // rows are it counts as 0 here, and the rows that do see it get it in the end.
-      if (n0 + kTile > least) {
-        const auto nan_bits = [](uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };  // 0x80 in a byte of 0x7f or 0xff
+      if (__builtin_expect(n0 + kTile > least, 1)) {
+        uint32_t low = 0x7f7f7f7fu, one = 0x01010101u;  // in registers: half the bytes of code, which a small call waits for
+        asm volatile("" : "+s"(low), "+s"(one));
+        const auto nans = [&](uint32_t x) { return (x & low) + one; };  // bit 7 of a byte of 0x7f or 0xff
         uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) any |= nan_bits((&vr[i].x)[w]);
-        if (__builtin_expect(__any(any != 0), 0)) {
+          for (int w = 0; w < 4; ++w) any |= nans((&vr[i].x)[w]);
+        if (__builtin_expect(__any((any & 0x80808080u) != 0), 0)) {
           const int ln = here(lane);
           if (!bad) s_nan[wave][ln] = s_nan[wave][ln + 64] = INT_MAX;
           bad = true;
@@ -360,7 +362,7 @@ __global__ __launch_bounds__(kThreads, room(SRC, NC)) void rows_attn(RowsArgs a)
             int first = INT_MAX;
 #pragma unroll
             for (int w = 3; w >= 0; --w) {
-              const uint32_t x = (&vr[i].x)[w], nan = nan_bits(x);
+              const uint32_t x = (uint32_t)here((int)(&vr[i].x)[w]), nan = nans(x) & 0x80808080u;
               if (nan) first = key + 4 * w + ((__ffs(nan) - 8) >> 3);
               (&vr[i].x)[w] = x & ~((nan >> 7) * 0xffu);
             }

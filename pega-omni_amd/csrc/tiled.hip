@@ -290,6 +290,7 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   const auto ends = [&](int nq) { return part < 0 ? nq : min(nq, kPartPos * (part + 1)); };
 
   Tile t;
+  int not_least = INT_MIN;  // 8-bit cache: ~ the least position of this lane's share of the rows
   if constexpr (PAGED) {
     const int s = item.x, first = item.y;
     t.nq = item.z;
@@ -320,15 +321,14 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
     } else {
       t.pos = a.pos + first;
       t.pg = a.pages + a.indptr[item.x];
-      int most = -1, not_least = INT_MIN;  // of this workgroup's rows
+      int most = -1;  // of this workgroup's rows
       for (int i = (part > 0 ? kPartPos * part : 0) + (threadIdx.x & 63); i < ends(t.nq); i += 64) {
         const int pos = max(t.pos[i], -1);
         most = max(most, pos), not_least = max(not_least, ~pos);
       }
 #pragma unroll
-      for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d)), not_least = max(not_least, __shfl_xor(not_least, d));
+      for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d));
       t.last = __builtin_amdgcn_readfirstlane(most) + 1;
-      t.apart = t.last + __builtin_amdgcn_readfirstlane(not_least);
     }
     t.len = t.last;
   } else if constexpr (SRC == kPacked) {
@@ -687,7 +687,20 @@ __global__ __launch_bounds__(kThreads, 1) void tiled_attn(TiledArgs a, int items
   // for with it, so the key loop's first MFMA does not wait on the next
   // tile's loads.
   if (SRC == kPagedWave && s_hi > s_lo) pids = wave_pages(s_lo);
-  if (s_hi > s_lo) issue_tile(s_lo, smem0);
+  if constexpr (Q8) {
+    if (s_hi > s_lo) {
+      ask_block(s_lo);
+      if constexpr (NANS) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) not_least = max(not_least, __shfl_xor(not_least, d));
+        t.apart = t.last + __builtin_amdgcn_readfirstlane(not_least);
+      }
+      put_block(smem0);
+      check_block(smem0);
+    }
+  } else if (s_hi > s_lo) {
+    issue_tile(s_lo, smem0);
+  }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), other counters free
   asm volatile("" ::: "memory");       // the reads of Q stay after the wait
   // Q^T: K-step kk holds dims 16 kk + 8 h .. + 7 of row r.
