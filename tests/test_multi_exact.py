@@ -100,3 +100,48 @@ def test_rows_of_groups_keep_their_bits():
         torch.cuda.synchronize()
         outs.append(out)
     assert torch.equal(*outs)
+
+
+@pytest.mark.gpu
+def test_in_graphs_beside_a_plan_that_rounds():
+    """Extend and cross with exact_p captured, with groups and split tiles, replayed as positions move on, beside eager calls of both kinds
+    on other streams with workspaces of their own."""
+    hq, hk, lens, counts = 8, 2, [1400, 90, 33], [40, 20, 2]
+    c = T.Cache(21, lens, hk, 16, torch.float8_e4m3fn)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rows = sum(counts)
+    q, kv = T.bf16(g, rows, hq * 128), T.bf16(g, 500, 2 * hk * 128)
+    k, v = kv[:, :hk * 128], kv[:, hk * 128:]
+    pos = T.i32([max(n - m + i - 30, -1) for n, m in zip(lens, counts) for i in range(m)])
+    first, length = T.i32([0, 200, 333]), T.i32([150, 3, 0])
+
+    def make(exact):
+        e, x = (f(counts, hq, hk, 1400, None, 64, exact_p=exact) for f in (oa.extend_plan, oa.cross_plan))
+        assert e.plan.split_tiles > 0 and x.plan.split_tiles > 0 and e.plan.group_rows > 0
+        return e, oa.workspace_for(e.plan), x, oa.workspace_for(x.plan), torch.zeros(2, rows, hq * 128, dtype=torch.bfloat16, device="cuda")
+
+    def step(m, s=None):
+        oa.qwen3_extend_q8(m[0], q, c.kv, c.sc, pos, c.indptr, c.pages, 16, m[4][0], T.SCALE, m[1], s)
+        oa.cross_run(m[2], q, k, v, None, first, length, m[4][1], T.SCALE, m[3], s)
+
+    eager, captured, rounded, other = make(True), make(True), make(False), make(False)
+    torch.cuda.synchronize()
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        step(captured)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for rep in range(8):
+        step(eager)
+        step(rounded)
+        torch.cuda.synchronize()
+        for m in (captured, other):
+            m[4].zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        step(other, streams[0])
+        step(eager, streams[1])
+        torch.cuda.synchronize()
+        assert torch.equal(captured[4], eager[4]) and torch.equal(other[4], rounded[4]), rep
+        assert not torch.equal(captured[4], rounded[4])
+        pos += 2
+        length += T.i32([3, 7, 11])
